@@ -38,7 +38,8 @@ typedef enum {
   MCOP_F16 = 1,
   MCOP_F32 = 2,
   MCOP_I8 = 3,
-  MCOP_FP8_E4M3FN = 4
+  MCOP_FP8_E4M3FN = 4,
+  MCOP_MXFP4 = 5 /* blocks of 32 4-bit codes with a scale byte; kv_cache entry points only */
 } mcop_dtype;
 
 enum {
@@ -248,6 +249,87 @@ int mcop_fused_add_rms_norm_dynamic_per_token_quant_padding_output(
     int8_t* output, void* output_rms, int8_t* output_quant_int8, float* out_scales,
     const void* input, void* residual, const void* weight, int64_t num_tokens,
     int64_t hidden_size, int64_t pad_size, float epsilon, void* stream);
+
+/* 4-bit operands (OCP MXFP4). A row of `hidden_size` values, a multiple of 32, is hidden_size / 2
+ * bytes of codes and hidden_size / 32 scale bytes. A code (E2M1) is a sign and one of 0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6; value 2i of the row is the low half of byte i. A scale byte e (E8M0) stands for
+ * 2^(e - 127), 255 for NaN. Per block of 32 consecutive values, A = max|x|:
+ *   e = max(floor(log2 A) - 2 + 127, 0), 0 for A = 0, 255 where a value is NaN or infinite;
+ *   code = e2m1(x * 2^(127 - e)), to nearest, ties to even, at most 6 (0 where e = 255).
+ * The reference has no counterpart of these operators. */
+
+/* Codes [num_tokens, hidden_size / 2] and scales [num_tokens, hidden_size / 32] of `input`, whose rows
+ * are input_row_stride elements apart. No counterpart in the reference. */
+int mcop_mxfp4_quant(uint8_t* out, uint8_t* scales, const void* input, int64_t num_tokens,
+                     int64_t hidden_size, int64_t input_row_stride, mcop_dtype in_dtype,
+                     void* stream);
+
+/* The values of such codes, rounded once to out_dtype (bf16, fp16, fp32). No counterpart in the
+ * reference. */
+int mcop_mxfp4_dequant(void* out, mcop_dtype out_dtype, const uint8_t* codes,
+                       const uint8_t* scales, int64_t num_tokens, int64_t hidden_size,
+                       void* stream);
+
+/* (Residual add +) RMSNorm + 4-bit codes: a = input (+ residual, read only); after_res <- round(a);
+ *   rho = 1/sqrt(sum(a^2)/H + eps); y = round(round(a * rho) * weight); out, scales <- blocks of y.
+ * residual and after_res are both given or both NULL; after_res may be the residual's or the input's
+ * own buffer. input, weight, residual and after_res share in_dtype. The 4-bit sibling of
+ * mcop_rms_norm_dynamic_per_token_quant; the reference has none. */
+int mcop_rms_norm_mxfp4_quant(uint8_t* out, uint8_t* scales, const void* input, const void* weight,
+                              const void* residual, void* after_res, int64_t num_tokens,
+                              int64_t hidden_size, mcop_dtype in_dtype, float epsilon,
+                              void* stream);
+
+/* Product of two such operands: out[m, n] = round(sum_k a[m, k] * b[n, k] (+ bias[n])), summed in
+ * fp32. a: codes [M, K / 2], scales [M, K / 32]; b: [N, K / 2], [N, K / 32]; all contiguous, codes
+ * aligned to 16 bytes. out [M, N] and bias [N] (or NULL) are out_dtype (bf16, fp16, fp32). K is a
+ * multiple of 32. Needs no workspace. A NaN scale makes its row (of a) or column (of b) NaN. The order
+ * of the sum depends on M, N and K only. No counterpart in the reference. */
+int mcop_mxfp4_scaled_mm(void* out, mcop_dtype out_dtype, const uint8_t* a,
+                         const uint8_t* a_scales, const uint8_t* b, const uint8_t* b_scales,
+                         const void* bias, int64_t M, int64_t N, int64_t K, void* stream);
+
+/* Keys or values of a paged cache of quantized vectors: one vector of head_size (1..1024) elements a
+ * token and head. `plain` is the tensor [num_tokens, num_heads, head_size] that is written from or
+ * read to (strides in elements); the cache has num_pages pages of page_size tokens (a slot is page *
+ * page_size + token), its codes addressed with strides in bytes, its scales in elements. A vector's
+ * own elements are contiguous. */
+typedef struct {
+  void* plain;
+  int64_t token_stride, head_stride;
+  void* codes;
+  int64_t code_page_stride, code_token_stride, code_head_stride;
+  void* scales; /* fp32, one a vector; MCOP_MXFP4: head_size / 32 bytes a vector */
+  int64_t scale_page_stride, scale_token_stride, scale_head_stride;
+  int64_t head_size;
+} mcop_kv_side;
+
+/* Quantizes the vectors of num_tokens tokens into the slots that slot_mapping [num_tokens] gives;
+ * tokens whose slot is negative (padding) or past the cache are not written. Per vector, A = max|x|:
+ *   MCOP_I8          s = A / 127, q = sat[-127,127](rne(x * (127 / A)))
+ *   MCOP_FP8_E4M3FN  s = max(A / 448, 1 / (448 * 512)), q = e4m3fn(clamp(x / s, -448, 448))
+ *   MCOP_MXFP4       blocks of 32 as above (head sizes multiples of 32)
+ * (the arithmetic of mcop_dynamic_scaled_int8_quant and mcop_dynamic_per_token_scaled_fp8_quant).
+ * Slots that are given must differ from each other: two tokens of one slot leave it with parts of
+ * either. num_pages * page_size is below 2^31. No counterpart in the reference's path. */
+int mcop_kv_cache_write_quant(const mcop_kv_side* key, const mcop_kv_side* value,
+                              mcop_dtype cache_dtype, int64_t num_pages, int64_t page_size,
+                              int64_t num_heads, const int64_t* slot_mapping, int64_t num_tokens,
+                              mcop_dtype in_dtype, void* stream);
+
+/* Reads sequences back: row t of the plain tensors, for cu_seqlens[s] <= t < cu_seqlens[s + 1], is
+ * position t - cu_seqlens[s] + seq_starts[s] (seq_starts NULL: 0) of sequence s, whose page i is
+ * block_table[s * table_row_stride + i]; each value is q * s in fp32 (exact for MCOP_MXFP4), rounded to
+ * out_dtype. Rows from cu_seqlens[num_sequences] on are left as they are. A position that the table has no page for (past
+ * its columns, or a page outside the cache) reads as NaN. cu_seqlens is non-decreasing from 0. No
+ * counterpart in the reference's path. */
+int mcop_kv_cache_read_dequant(const mcop_kv_side* key, const mcop_kv_side* value,
+                               mcop_dtype cache_dtype, int64_t num_pages, int64_t page_size,
+                               int64_t num_heads, const int32_t* block_table,
+                               int64_t table_row_stride, int64_t table_columns,
+                               const int32_t* cu_seqlens, const int32_t* seq_starts,
+                               int64_t num_sequences, int64_t num_tokens, mcop_dtype out_dtype,
+                               void* stream);
 
 /* Message of the last failed call on this host thread ("" if none). Stands in for the
  * reference's TORCH_CHECK messages (c10::Error text), which its entry points raise directly. */

@@ -19,7 +19,19 @@ LIB_PATH = Path(__file__).resolve().parent / "libmcop_norm.so"
 ABI_VERSION = 2
 
 # mcop_dtype codes (include/mcop_norm.h)
-BF16, F16, F32, I8, FP8_E4M3FN = 0, 1, 2, 3, 4
+BF16, F16, F32, I8, FP8_E4M3FN, MXFP4 = 0, 1, 2, 3, 4, 5
+
+
+class KvSide(ctypes.Structure):
+    """mcop_kv_side (include/mcop_norm.h)."""
+
+    _fields_ = ([("plain", ctypes.c_void_p), ("token_stride", ctypes.c_int64),
+                 ("head_stride", ctypes.c_int64)]
+                + [(f"{what}{tail}", kind) for what in ("code", "scale")
+                   for tail, kind in (("s", ctypes.c_void_p), ("_page_stride", ctypes.c_int64),
+                                      ("_token_stride", ctypes.c_int64),
+                                      ("_head_stride", ctypes.c_int64))]
+                + [("head_size", ctypes.c_int64)])
 
 
 def _load() -> ctypes.CDLL:
@@ -47,6 +59,14 @@ def _load() -> ctypes.CDLL:
     lib.mcop_vllm_rms_norm.argtypes = [P, P, P, I64, I64, I, I64, I64, I64, I64, I64, I, F, P]
     lib.mcop_rms_norm_dynamic_per_token_quant_custom.argtypes = [P, P, P, P, P, P, I64, I64, I,
                                                                   F, P]
+    lib.mcop_mxfp4_quant.argtypes = [P, P, P, I64, I64, I64, I, P]
+    lib.mcop_mxfp4_dequant.argtypes = [P, I, P, P, I64, I64, P]
+    lib.mcop_rms_norm_mxfp4_quant.argtypes = [P, P, P, P, P, P, I64, I64, I, F, P]
+    lib.mcop_mxfp4_scaled_mm.argtypes = [P, I, P, P, P, P, P, I64, I64, I64, P]
+    side = ctypes.POINTER(KvSide)
+    lib.mcop_kv_cache_write_quant.argtypes = [side, side, I, I64, I64, I64, P, I64, I, P]
+    lib.mcop_kv_cache_read_dequant.argtypes = [side, side, I, I64, I64, I64, P, I64, I64, P, P, I64,
+                                               I64, I, P]
     lib.mcop_check_row_scalars.argtypes = [P, ctypes.c_uint32, I64, I, F, P]
     lib.mcop_debug_set_launch_override.argtypes = [I, I]
     lib.mcop_debug_set_split_rows.argtypes = [I]
@@ -60,7 +80,10 @@ def _load() -> ctypes.CDLL:
                "mcop_dynamic_scaled_int8_quant", "mcop_dynamic_per_token_scaled_fp8_quant",
                "mcop_fused_add_rms_norm_dynamic_per_token_quant_padding_output",
                "mcop_rms_norm_per_block_quant", "mcop_rms_norm", "mcop_head_rms_norm",
-               "mcop_vllm_rms_norm", "mcop_rms_norm_dynamic_per_token_quant_custom"):
+               "mcop_vllm_rms_norm", "mcop_rms_norm_dynamic_per_token_quant_custom",
+               "mcop_mxfp4_quant", "mcop_mxfp4_dequant", "mcop_rms_norm_mxfp4_quant",
+               "mcop_mxfp4_scaled_mm", "mcop_kv_cache_write_quant",
+               "mcop_kv_cache_read_dequant"):
         getattr(lib, fn).restype = I
     lib.mcop_last_error.restype = ctypes.c_char_p
     lib.mcop_last_error.argtypes = []

@@ -1,0 +1,477 @@
+// kv_cache.hip -- keys and values quantized as they are written to a paged cache, and read back.
+//
+// A vector is one token's key (or value) of one head: D elements with a scale of their own, by the
+// arithmetic of the framework's per-token quantizers (per_token_quant.hip) or as 4-bit blocks
+// (mxfp4.h):
+//   int8   s = A / 127,                    q = sat[-127,127](rne(x * (127 / A))), A = max|x|
+//   fp8    s = max(A / 448, 1/(448*512)),  q = e4m3fn(clamp(x / s, +-448))
+//   mxfp4  a scale byte and 32 codes a block
+// and reads back as q * s in fp32 (exact for 4-bit blocks), rounded to the output's type.
+//
+// Both directions are bound by HBM (three bytes an element of a 16-bit type).  A vector takes the
+// fewest lanes (a power of two) that hold it at eight elements a lane, so that a wave's loads are 1 KiB
+// in a row where heads and tokens lie next to each other; its absmax is a few register moves.
+// Workgroups of blockIdx.y = 0 do the keys, 1 the values.
+#include <hip/hip_runtime.h>
+
+#include "../../include/mcop_norm.h"
+#include "mxfp4.h"
+
+namespace mcop {
+
+constexpr int kKvLanes = 256;
+constexpr int kKvMostDim = 1024;
+
+enum KvFormat { KV_INT8 = 0, KV_FP8 = 1, KV_MXFP4 = 2 };
+
+// One side (keys or values) of a launch.  Strides of the cache are in bytes for codes, in elements for
+// scales; those of the plain tensor in elements.
+struct KvSide {
+  void* plain;
+  uint8_t* codes;
+  void* scales;
+  int64_t p_token, p_head;
+  int64_t c_page, c_token, c_head;
+  int64_t s_page, s_token, s_head;
+  int dim, lanes;
+};
+struct KvSides {
+  KvSide side[2];
+  int heads;
+  Divisor by_heads, by_page;
+};
+
+// The eight (or, past the vector's end, fewer) elements of unit j.
+template <class E, bool WHOLE>
+__device__ __forceinline__ Pack<typename E::S, 8> load_unit(const typename E::S* p, int n) {
+  if constexpr (WHOLE) {
+    return load8<typename E::S, false>(p);
+  } else {
+    Pack<typename E::S, 8> v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v.v[e] = e < n ? p[e] : typename E::S(0);
+    return v;
+  }
+}
+template <class T, bool WHOLE>
+__device__ __forceinline__ void store_unit(T* p, const Pack<T, 8>& v, int n) {
+  if constexpr (WHOLE) {
+    if constexpr (sizeof(T) == 1) st_nt<T, 8>(p, v);
+    else store8<T, false>(p, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (e < n) p[e] = v.v[e];
+    }
+  }
+}
+// A dword of codes, in bytes where the cache is not aligned to it.
+template <bool WHOLE>
+__device__ __forceinline__ void store_dword(uint8_t* p, uint32_t v) {
+  if constexpr (WHOLE) *reinterpret_cast<uint32_t*>(p) = v;
+  else __builtin_memcpy(p, &v, 4);
+}
+template <bool WHOLE>
+__device__ __forceinline__ uint32_t load_dword(const uint8_t* p) {
+  uint32_t v;
+  if constexpr (WHOLE) v = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+  else __builtin_memcpy(&v, p, 4);
+  return v;
+}
+
+// WHOLE: vectors are whole units, and every tensor's vectors are aligned to theirs.  NU: units a lane.
+template <class E, int FMT, bool WHOLE, int NU>
+__global__ void __launch_bounds__(kKvLanes)
+k_kv_cache_write(KvSides a, const int64_t* __restrict__ slots, uint32_t vectors, int64_t num_slots,
+                 int page_size) {
+  using S = typename E::S;
+  const KvSide& k = a.side[blockIdx.y];
+  const int sh = 31 - __builtin_clz((unsigned)k.lanes);
+  const uint32_t i = blockIdx.x * (uint32_t)(kKvLanes >> sh) + (threadIdx.x >> sh);
+  const int j = (int)threadIdx.x & (k.lanes - 1);
+  const bool live = i < vectors;
+  const uint32_t token = a.by_heads.quotient(live ? i : vectors - 1);
+  const uint32_t head = (live ? i : vectors - 1) - token * (uint32_t)a.heads;
+  const S* src = static_cast<const S*>(k.plain) + token * k.p_token + head * k.p_head;
+  Pack<S, 8> v[NU];
+  int left[NU];  // elements of the unit inside the vector
+#pragma unroll
+  for (int n = 0; n < NU; ++n) {
+    const int at = (j + n * k.lanes) * 8;
+    left[n] = k.dim - at;
+    if constexpr (WHOLE) {
+      v[n] = load_unit<E, true>(src + (left[n] > 0 ? at : 0), 8);
+    } else {
+      v[n] = load_unit<E, false>(src + at, left[n]);
+    }
+  }
+  const int64_t slot = slots[token];
+  const bool store = live && slot >= 0 && slot < num_slots;
+  const uint32_t page = a.by_page.quotient(store ? (uint32_t)slot : 0u);
+  const uint32_t off = (store ? (uint32_t)slot : 0u) - page * (uint32_t)page_size;
+  uint8_t* dst = k.codes + page * k.c_page + off * k.c_token + head * k.c_head;
+  const int64_t s_at = page * k.s_page + off * k.s_token + head * k.s_head;
+  if constexpr (FMT == KV_MXFP4) {
+    uint8_t* sd = static_cast<uint8_t*>(k.scales) + s_at;
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      const int unit = j + n * k.lanes;
+      // vectors are whole blocks: a block's four lanes are all inside or all past the end
+      const uint32_t e = mx_scale(lanes_max(absmax8<E>(v[n]), 4));
+      if (!store || left[n] <= 0) continue;
+      store_dword<WHOLE>(dst + unit * 4, mx_codes8<E>(v[n], e));
+      if ((unit & 3) == 0) sd[unit >> 2] = (uint8_t)e;
+    }
+  } else {
+    float f[NU][8], m = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      widen<E, 8>(f[n], v[n]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float t = __builtin_fabsf(f[n][e]);
+        // a unit past the end holds copies of the first; NaN is ignored, as in a row's absmax
+        m = __builtin_fmaxf(m, t);
+      }
+    }
+    const float A = __builtin_bit_cast(float, lanes_max(__builtin_bit_cast(uint32_t, m), k.lanes));
+    float s, inv;
+    if constexpr (FMT == KV_INT8) {
+      s = row_div<127>(A);
+      inv = row_ratio(127.0f, A);
+    } else {
+      s = __builtin_fmaxf(div_floored<448>(A), 1.0f / 229376.0f);
+      inv = row_rcp(s);
+    }
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      const int at = (j + n * k.lanes) * 8;
+      Codes<8> q;
+      if constexpr (FMT == KV_INT8) q = i8_codes<-127, 8>(f[n], inv);
+      else q = fp8_quotient_codes<8>(f[n], s, inv, mcop_divisor_ok(s), s <= 0x1p100f);
+      if (store && left[n] > 0) {
+        store_unit<uint8_t, WHOLE>(dst + at, __builtin_bit_cast(Pack<uint8_t, 8>, q), left[n]);
+      }
+    }
+    if (store && j == 0) static_cast<float*>(k.scales)[s_at] = s;
+  }
+}
+
+// Four e4m3fn codes times s.
+__device__ __forceinline__ void widen_fp8(float* f, uint32_t w, float s) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  const f2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  f[0] = a[0] * s, f[1] = a[1] * s, f[2] = b[0] * s, f[3] = b[1] * s;
+}
+
+// The sequence that holds token t: how many of cu[1..n] are <= t (the wave counts together).
+__device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int n, int64_t t) {
+  int s = 0;
+  for (int i = 0; i < n; i += 64) {
+    const int at = i + (int)(threadIdx.x & 63);
+    const bool below = at < n && cu[at + 1] <= t;
+    s += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(below));
+  }
+  return s;
+}
+
+template <class E, int FMT, bool WHOLE, int NU, int R>
+__global__ void __launch_bounds__(kKvLanes)
+k_kv_cache_read(KvSides a, const int32_t* __restrict__ table, int64_t table_stride, int columns,
+                const int32_t* __restrict__ cu, const int32_t* __restrict__ starts, int sequences,
+                uint32_t vectors, int64_t pages, int page_size) {
+  using S = typename E::S;
+  const KvSide& k = a.side[blockIdx.y];
+  const int sh = 31 - __builtin_clz((unsigned)k.lanes);
+  const uint32_t per = kKvLanes >> sh;
+  const uint32_t i0 = blockIdx.x * (per * R);
+  if (i0 >= vectors) return;
+  const int j = (int)threadIdx.x & (k.lanes - 1);
+  const int s0 = sequence_of(cu, sequences, a.by_heads.quotient(i0));
+  const uint8_t* src[R];
+  int64_t s_at[R];
+  S* dst[R];
+  int state[R];  // 0: nothing to write, 1: a value, 2: no such page
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const uint32_t i = i0 + r * per + (threadIdx.x >> sh);
+    const uint32_t token = a.by_heads.quotient(i < vectors ? i : vectors - 1);
+    const uint32_t head = (i < vectors ? i : vectors - 1) - token * (uint32_t)a.heads;
+    int s = s0;
+    while (s < sequences && cu[s + 1] <= (int64_t)token) ++s;
+    dst[r] = static_cast<S*>(k.plain) + token * k.p_token + head * k.p_head;
+    state[r] = i < vectors && s < sequences ? 2 : 0;
+    uint32_t page = 0, off = 0;
+    if (state[r] != 0) {
+      const int64_t p = (int64_t)token - cu[s] + (starts != nullptr ? starts[s] : 0);
+      if (p >= 0 && p <= INT32_MAX) {
+        const uint32_t column = a.by_page.quotient((uint32_t)p);
+        if (column < (uint32_t)columns) {
+          const int32_t g = table[s * table_stride + column];
+          if (g >= 0 && g < pages) {
+            page = (uint32_t)g;
+            off = (uint32_t)p - column * (uint32_t)page_size;
+            state[r] = 1;
+          }
+        }
+      }
+    }
+    src[r] = k.codes + page * k.c_page + off * k.c_token + head * k.c_head;
+    s_at[r] = page * k.s_page + off * k.s_token + head * k.s_head;
+  }
+#pragma unroll
+  for (int n = 0; n < NU; ++n) {
+    const int unit = j + n * k.lanes, at = unit * 8, left = k.dim - at;
+    if (left <= 0) continue;
+    Pack<uint8_t, 8> q[R];
+    uint32_t c[R];
+    float s[R];
+    uint32_t e[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (state[r] != 1) continue;
+      if constexpr (FMT == KV_MXFP4) {
+        c[r] = load_dword<WHOLE>(src[r] + unit * 4);
+        e[r] = static_cast<const uint8_t*>(k.scales)[s_at[r] + (unit >> 2)];
+      } else {
+        if constexpr (WHOLE) {
+          q[r] = ld_nt<uint8_t, 8>(src[r] + at);
+        } else {
+#pragma unroll
+          for (int b = 0; b < 8; ++b) q[r].v[b] = b < left ? src[r][at + b] : 0;
+        }
+        s[r] = static_cast<const float*>(k.scales)[s_at[r]];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (state[r] == 0) continue;
+      float f[8];
+      if constexpr (FMT == KV_MXFP4) {
+        mx_widen8(f, c[r], e[r]);
+      } else if constexpr (FMT == KV_INT8) {
+#pragma unroll
+        for (int b = 0; b < 8; ++b) f[b] = (float)(int8_t)q[r].v[b] * s[r];
+      } else {
+        const Pack<uint32_t, 2> w = __builtin_bit_cast(Pack<uint32_t, 2>, q[r]);
+        widen_fp8(f, w.v[0], s[r]);
+        widen_fp8(f + 4, w.v[1], s[r]);
+      }
+      Pack<S, 8> o;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        o.v[b] = E::from_f(state[r] == 2 ? __builtin_nanf("") : f[b]);
+      }
+      store_unit<S, WHOLE>(dst[r] + at, o, left);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side.
+
+namespace {
+
+// The checks that both directions share of one side, and its form for the kernels.
+int side_of(const char* name, const char* what, const mcop_kv_side& in, int fmt, int64_t pages,
+            int64_t page_size, int64_t heads, int64_t tokens, KvSide* out) {
+  if (in.head_size <= 0 || in.head_size > kKvMostDim) {
+    return set_error(MCOP_E_INVALID, "%s: %s head_size %lld is not in 1..%d", name, what,
+                     (long long)in.head_size, kKvMostDim);
+  }
+  if (fmt == KV_MXFP4 && in.head_size % kMxBlock != 0) {
+    return set_error(MCOP_E_INVALID, "%s: %s head_size %lld is not a multiple of the block of 32",
+                     name, what, (long long)in.head_size);
+  }
+  if (!in.plain || (pages > 0 && (!in.codes || !in.scales))) {
+    return set_error(MCOP_E_INVALID, "%s: null pointer", name);
+  }
+  // element offsets of the last vector, which the kernels form in 64 bits
+  const int64_t n[8] = {pages, page_size, heads, pages, page_size, heads, tokens, heads};
+  const int64_t s[8] = {in.code_page_stride, in.code_token_stride, in.code_head_stride,
+                        in.scale_page_stride, in.scale_token_stride, in.scale_head_stride,
+                        in.token_stride, in.head_stride};
+  for (int d = 0; d < 8; ++d) {
+    if (s[d] < 0 || (n[d] > 0 && s[d] > INT64_MAX / 64 / n[d])) {
+      return set_error(MCOP_E_INVALID, "%s: bad %s stride %lld", name, what, (long long)s[d]);
+    }
+  }
+  int lanes = 4;
+  while (lanes < 64 && lanes * 8 < in.head_size) lanes *= 2;
+  *out = KvSide{in.plain, static_cast<uint8_t*>(in.codes), in.scales, in.token_stride,
+                in.head_stride, in.code_page_stride, in.code_token_stride, in.code_head_stride,
+                in.scale_page_stride, in.scale_token_stride, in.scale_head_stride,
+                (int)in.head_size, lanes};
+  return MCOP_OK;
+}
+
+int format_of(mcop_dtype t) {
+  return t == MCOP_I8 ? KV_INT8 : t == MCOP_FP8_E4M3FN ? KV_FP8 : t == MCOP_MXFP4 ? KV_MXFP4 : -1;
+}
+
+// Whether a side's vectors are whole units aligned to 16 bytes (plain) and to a unit's codes.
+bool whole_units(const KvSide& k, int fmt, int elem) {
+  const int64_t c = fmt == KV_MXFP4 ? 4 : 8;
+  return k.dim % 8 == 0 && aligned(16, k.plain) && aligned((int)c, k.codes) &&
+         k.p_token * elem % 16 == 0 && k.p_head * elem % 16 == 0 && k.c_page % c == 0 &&
+         k.c_token % c == 0 && k.c_head % c == 0;
+}
+
+int kv_sides(const char* name, const mcop_kv_side* key, const mcop_kv_side* value,
+             mcop_dtype cache_dtype, mcop_dtype dtype, int64_t pages, int64_t page_size,
+             int64_t heads, int64_t tokens, KvSides* a, int* fmt, bool* whole) {
+  *fmt = format_of(cache_dtype);
+  if (*fmt < 0) {
+    return set_error(MCOP_E_INVALID, "%s: cache dtype %d is not int8, fp8_e4m3fn or mxfp4", name,
+                     (int)cache_dtype);
+  }
+  if (dtype != MCOP_BF16 && dtype != MCOP_F16 && dtype != MCOP_F32) {
+    return set_error(MCOP_E_INVALID, "%s: dtype %d is not bf16/fp16/fp32", name, (int)dtype);
+  }
+  if (!key || !value) return set_error(MCOP_E_INVALID, "%s: null pointer", name);
+  if (tokens < 0 || heads <= 0 || pages < 0 || page_size <= 0 || page_size > INT32_MAX ||
+      heads > INT32_MAX || pages > INT32_MAX || pages * page_size > INT32_MAX) {
+    return set_error(MCOP_E_INVALID,
+                     "%s: bad shape num_tokens=%lld num_heads=%lld num_pages=%lld page_size=%lld "
+                     "(at most 2^31 - 1 slots)", name, (long long)tokens, (long long)heads,
+                     (long long)pages, (long long)page_size);
+  }
+  if (tokens > (INT32_MAX - 65536) / heads) {
+    return set_error(MCOP_E_UNSUPPORTED, "%s: %lld tokens of %lld heads are 2^31 vectors or more",
+                     name, (long long)tokens, (long long)heads);
+  }
+  if (int rc = side_of(name, "key", *key, *fmt, pages, page_size, heads, tokens, &a->side[0])) {
+    return rc;
+  }
+  if (int rc = side_of(name, "value", *value, *fmt, pages, page_size, heads, tokens,
+                       &a->side[1])) {
+    return rc;
+  }
+  a->heads = (int)heads;
+  a->by_heads = Divisor((uint32_t)heads);
+  a->by_page = Divisor((uint32_t)page_size);
+  const int elem = dtype == MCOP_F32 ? 4 : 2;
+  *whole = whole_units(a->side[0], *fmt, elem) && whole_units(a->side[1], *fmt, elem);
+  return MCOP_OK;
+}
+
+// Workgroups for `vectors` vectors at `r` rounds a workgroup, of the side that needs more.
+unsigned kv_blocks(const KvSides& a, int64_t vectors, int r) {
+  const int lanes = a.side[0].lanes > a.side[1].lanes ? a.side[0].lanes : a.side[1].lanes;
+  const int64_t per = (int64_t)kKvLanes / lanes * r;
+  return (unsigned)((vectors + per - 1) / per);
+}
+
+bool two_units(const KvSides& a) { return a.side[0].dim > 512 || a.side[1].dim > 512; }
+
+template <class E, int FMT, bool WHOLE>
+void write_of(const KvSides& a, const int64_t* slots, int64_t vectors, int64_t num_slots,
+              int page_size, hipStream_t st) {
+  const dim3 grid(kv_blocks(a, vectors, 1), 2), block(kKvLanes);
+  if (two_units(a)) {
+    hipLaunchKernelGGL((k_kv_cache_write<E, FMT, WHOLE, 2>), grid, block, 0, st, a, slots,
+                       (uint32_t)vectors, num_slots, page_size);
+  } else {
+    hipLaunchKernelGGL((k_kv_cache_write<E, FMT, WHOLE, 1>), grid, block, 0, st, a, slots,
+                       (uint32_t)vectors, num_slots, page_size);
+  }
+}
+
+template <class E, int FMT, bool WHOLE>
+void read_of(const KvSides& a, const int32_t* table, int64_t table_stride, int columns,
+             const int32_t* cu, const int32_t* starts, int sequences, int64_t vectors,
+             int64_t pages, int page_size, hipStream_t st) {
+  const dim3 block(kKvLanes);
+  if (two_units(a)) {
+    hipLaunchKernelGGL((k_kv_cache_read<E, FMT, WHOLE, 2, 1>), dim3(kv_blocks(a, vectors, 1), 2),
+                       block, 0, st, a, table, table_stride, columns, cu, starts, sequences,
+                       (uint32_t)vectors, pages, page_size);
+  } else {
+    hipLaunchKernelGGL((k_kv_cache_read<E, FMT, WHOLE, 1, 4>), dim3(kv_blocks(a, vectors, 4), 2),
+                       block, 0, st, a, table, table_stride, columns, cu, starts, sequences,
+                       (uint32_t)vectors, pages, page_size);
+  }
+}
+
+// f.template operator()<E, FMT, WHOLE>() for the launch's types.
+template <class F>
+void for_types(mcop_dtype dtype, int fmt, bool whole, F f) {
+  auto by_form = [&](auto e, auto m) {
+    if (whole) f(e, m, std::true_type());
+    else f(e, m, std::false_type());
+  };
+  auto by_format = [&](auto e) {
+    if (fmt == KV_INT8) by_form(e, std::integral_constant<int, KV_INT8>());
+    else if (fmt == KV_FP8) by_form(e, std::integral_constant<int, KV_FP8>());
+    else by_form(e, std::integral_constant<int, KV_MXFP4>());
+  };
+  if (dtype == MCOP_BF16) by_format(BF16());
+  else if (dtype == MCOP_F16) by_format(F16());
+  else by_format(F32());
+}
+
+}  // namespace
+
+}  // namespace mcop
+
+extern "C" int mcop_kv_cache_write_quant(const mcop_kv_side* key, const mcop_kv_side* value,
+                                         mcop_dtype cache_dtype, int64_t num_pages,
+                                         int64_t page_size, int64_t num_heads,
+                                         const int64_t* slot_mapping, int64_t num_tokens,
+                                         mcop_dtype in_dtype, void* stream) {
+  using namespace mcop;
+  const char* name = "kv_cache_write_quant";
+  KvSides a;
+  int fmt;
+  bool whole;
+  if (num_tokens == 0) return MCOP_OK;
+  if (int rc = kv_sides(name, key, value, cache_dtype, in_dtype, num_pages, page_size, num_heads,
+                        num_tokens, &a, &fmt, &whole)) {
+    return rc;
+  }
+  if (!slot_mapping) return set_error(MCOP_E_INVALID, "%s: null pointer", name);
+  if (num_pages == 0) return MCOP_OK;  // no slot to write to
+  auto st = static_cast<hipStream_t>(stream);
+  for_types(in_dtype, fmt, whole, [&](auto e, auto m, auto w) {
+    write_of<decltype(e), decltype(m)::value, decltype(w)::value>(
+        a, slot_mapping, num_tokens * num_heads, num_pages * page_size, (int)page_size, st);
+  });
+  return check_launch(name);
+}
+
+extern "C" int mcop_kv_cache_read_dequant(const mcop_kv_side* key, const mcop_kv_side* value,
+                                          mcop_dtype cache_dtype, int64_t num_pages,
+                                          int64_t page_size, int64_t num_heads,
+                                          const int32_t* block_table, int64_t table_row_stride,
+                                          int64_t table_columns, const int32_t* cu_seqlens,
+                                          const int32_t* seq_starts, int64_t num_sequences,
+                                          int64_t num_tokens, mcop_dtype out_dtype,
+                                          void* stream) {
+  using namespace mcop;
+  const char* name = "kv_cache_read_dequant";
+  KvSides a;
+  int fmt;
+  bool whole;
+  if (num_tokens == 0 || num_sequences == 0) return MCOP_OK;
+  if (int rc = kv_sides(name, key, value, cache_dtype, out_dtype, num_pages, page_size, num_heads,
+                        num_tokens, &a, &fmt, &whole)) {
+    return rc;
+  }
+  if (num_sequences < 0 || num_sequences > INT32_MAX || table_columns < 0 ||
+      table_columns > INT32_MAX || table_row_stride < 0 ||
+      table_row_stride > INT64_MAX / 8 / num_sequences) {
+    return set_error(MCOP_E_INVALID, "%s: bad block table: %lld sequences of %lld pages", name,
+                     (long long)num_sequences, (long long)table_columns);
+  }
+  if (!cu_seqlens || (!block_table && table_columns > 0)) {
+    return set_error(MCOP_E_INVALID, "%s: null pointer", name);
+  }
+  auto st = static_cast<hipStream_t>(stream);
+  for_types(out_dtype, fmt, whole, [&](auto e, auto m, auto w) {
+    read_of<decltype(e), decltype(m)::value, decltype(w)::value>(
+        a, block_table, table_row_stride, (int)table_columns, cu_seqlens, seq_starts,
+        (int)num_sequences, num_tokens * num_heads, num_pages, (int)page_size, st);
+  });
+  return check_launch(name);
+}

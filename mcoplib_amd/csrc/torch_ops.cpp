@@ -8,13 +8,17 @@
 //   - torch.ops._C (TORCH_LIBRARY, op/vllm/torch_bindings.cpp:155-164, 216-229, 359-364,
 //     374-379): rms_norm, fused_add_rms_norm, rms_norm_dynamic_per_token_quant,
 //     rms_norm_per_block_quant, dynamic_scaled_int8_quant, dynamic_per_token_scaled_fp8_quant,
-//     registered by register_vllm_ops() for the CUDA (HIP) key, plus a no-op Meta kernel.
+//     registered by register_vllm_ops() for the CUDA (HIP) key, plus a no-op Meta kernel;
+//     and, of the same kind without a counterpart in the reference, the 4-bit operators
+//     (mxfp4_quant, mxfp4_dequant, rms_norm_mxfp4_quant, mxfp4_scaled_mm) and the quantized
+//     key/value cache (kv_cache_write_quant, kv_cache_read_dequant).
 // Every function checks its arguments as the reference does (TORCH_CHECK with the reference's
 // condition text) and, beyond the reference, that every tensor is on the device and that element
 // counts match (the kernels trust them); then it makes the input's device current and enqueues
 // one kernel on torch's current stream of that device.  Nothing synchronizes.
 #include <torch/extension.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/HIPContext.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <torch/library.h>
@@ -577,6 +581,330 @@ void c_fp8_quant(Tensor& result, const Tensor& input, Tensor& scale, const OptTe
       H, in_stride, out_stride, code_of(input.scalar_type()), stream_of(input)));
 }
 
+// ------------------------------------------------- 4-bit operators, quantized key/value cache
+// (no counterpart in the reference; shapes and dtypes are checked before devices)
+
+constexpr int64_t kMxBlock = 32;
+
+bool is_codes4(at::ScalarType t) { return t == at::kByte || t == at::kFloat4_e2m1fn_x2; }
+bool is_scale8(at::ScalarType t) { return t == at::kByte || t == at::kFloat8_e8m0fnu; }
+
+// Codes and scales of rows of H values: [..., H / 2] and [..., H / 32], contiguous.
+void mx_check(const char* name, const char* what, const Tensor& codes, const Tensor& scale,
+              int64_t T, int64_t H) {
+  TORCH_CHECK(H % kMxBlock == 0, name, ": the last dimension, ", H,
+              " values, is not a multiple of the block of 32");
+  TORCH_CHECK(is_codes4(codes.scalar_type()), name, ": ", what,
+              " must be uint8 or float4_e2m1fn_x2, got ", codes.scalar_type());
+  TORCH_CHECK(is_scale8(scale.scalar_type()), name, ": the scale of ", what,
+              " must be uint8 or float8_e8m0fnu, got ", scale.scalar_type());
+  TORCH_CHECK(codes.dim() > 0 && codes.size(-1) == H / 2 && codes.numel() == T * (H / 2), name,
+              ": ", what, " has shape ", codes.sizes(), ", expected ", T, " rows of ", H / 2);
+  TORCH_CHECK(scale.dim() > 0 && scale.size(-1) == H / kMxBlock &&
+                  scale.numel() == T * (H / kMxBlock),
+              name, ": the scale of ", what, " has shape ", scale.sizes(), ", expected ", T,
+              " rows of ", H / kMxBlock);
+  contiguous_check(name, what, codes);
+  TORCH_CHECK(scale.is_contiguous(), name, ": the scale of ", what, " must be contiguous");
+}
+
+uint8_t* bytes_of(const Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
+
+void c_mxfp4_quant(Tensor& result, const Tensor& input, Tensor& scale) {
+  const char* name = "mxfp4_quant";
+  dispatch_check(input.scalar_type(), name);
+  const auto [T, H] = rows_of(input);
+  TORCH_CHECK(input.stride(-1) == 1, name, ": last dimension of input must be contiguous");
+  const int64_t stride = row_stride(name, input, T, H);
+  mx_check(name, "result", result, scale, T, H);
+  on_device(name, {&result, &input, &scale});
+  const DeviceGuard guard(input.device());
+  check_rc(mcop_mxfp4_quant(bytes_of(result), bytes_of(scale), input.data_ptr(), T, H, stride,
+                            code_of(input.scalar_type()), stream_of(input)));
+}
+
+void c_mxfp4_dequant(Tensor& result, const Tensor& input, const Tensor& scale) {
+  const char* name = "mxfp4_dequant";
+  dispatch_check(result.scalar_type(), name);
+  const auto [T, H] = rows_of(result);
+  contiguous_check(name, "result", result);
+  mx_check(name, "input", input, scale, T, H);
+  on_device(name, {&result, &input, &scale});
+  const DeviceGuard guard(input.device());
+  check_rc(mcop_mxfp4_dequant(result.data_ptr(), code_of(result.scalar_type()), bytes_of(input),
+                              bytes_of(scale), T, H, stream_of(input)));
+}
+
+void c_rms_norm_mxfp4_quant(Tensor& result, const Tensor& input, const Tensor& weight,
+                            Tensor& scale, double epsilon, const OptTensor& residual,
+                            const OptTensor& after_res) {
+  const char* name = "rms_norm_mxfp4_quant";
+  dispatch_check(input.scalar_type(), name);
+  const auto [T, H] = rows_of(input);
+  contiguous_check(name, "input", input);
+  contiguous_check(name, "weight", weight);
+  numel_check(name, "weight", weight, H);
+  TORCH_CHECK(weight.scalar_type() == input.scalar_type(), name,
+              ": weight must have the input dtype ", input.scalar_type());
+  TORCH_CHECK(residual.has_value() == after_res.has_value(), name,
+              ": residual and after_res go together");
+  if (residual.has_value()) {
+    for (const auto& [what, t] : {std::pair<const char*, const Tensor*>{"residual", &*residual},
+                                  {"after_res", &*after_res}}) {
+      TORCH_CHECK(t->scalar_type() == input.scalar_type(), name, ": ", what,
+                  " must have the input dtype ", input.scalar_type());
+      contiguous_check(name, what, *t);
+      numel_check(name, what, *t, T * H);
+    }
+  }
+  mx_check(name, "result", result, scale, T, H);
+  on_device(name, {&result, &input, &weight, &scale, opt(residual), opt(after_res)});
+  const DeviceGuard guard(input.device());
+  check_rc(mcop_rms_norm_mxfp4_quant(
+      bytes_of(result), bytes_of(scale), input.data_ptr(), weight.data_ptr(),
+      residual.has_value() ? residual->data_ptr() : nullptr,
+      after_res.has_value() ? after_res->data_ptr() : nullptr, T, H,
+      code_of(input.scalar_type()), (float)epsilon, stream_of(input)));
+}
+
+void c_mxfp4_scaled_mm(Tensor& result, const Tensor& a, const Tensor& a_scale, const Tensor& b,
+                       const Tensor& b_scale, const OptTensor& bias) {
+  const char* name = "mxfp4_scaled_mm";
+  dispatch_check(result.scalar_type(), name);
+  const auto [M, half] = rows_of(a);
+  const int64_t K = half * 2;
+  mx_check(name, "a", a, a_scale, M, K);
+  TORCH_CHECK(b.dim() == 2, name, ": b must be [N, K / 2], got ", b.sizes());
+  const int64_t N = b.size(0);
+  mx_check(name, "b", b, b_scale, N, K);
+  TORCH_CHECK(result.dim() > 0 && result.size(-1) == N && result.numel() == M * N, name,
+              ": result has shape ", result.sizes(), ", expected ", M, " rows of ", N);
+  contiguous_check(name, "result", result);
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->scalar_type() == result.scalar_type(), name,
+                ": bias must have the result dtype ", result.scalar_type());
+    numel_check(name, "bias", *bias, N);
+    contiguous_check(name, "bias", *bias);
+  }
+  on_device(name, {&result, &a, &a_scale, &b, &b_scale, opt(bias)});
+  const DeviceGuard guard(a.device());
+  check_rc(mcop_mxfp4_scaled_mm(result.data_ptr(), code_of(result.scalar_type()), bytes_of(a),
+                                bytes_of(a_scale), bytes_of(b), bytes_of(b_scale),
+                                bias.has_value() ? bias->data_ptr() : nullptr, M, N, K,
+                                stream_of(a)));
+}
+
+mcop_dtype cache_code(const char* name, at::ScalarType t) {
+  if (t == at::kChar) return MCOP_I8;
+  if (t == at::kFloat8_e4m3fn) return MCOP_FP8_E4M3FN;
+  TORCH_CHECK(is_codes4(t), name, ": the cache must be int8, float8_e4m3fn or (4-bit codes) uint8 "
+              "or float4_e2m1fn_x2, got ", t);
+  return MCOP_MXFP4;
+}
+
+// One side of the cache and the plain tensor [tokens, heads, head_size] beside it.
+mcop_kv_side kv_side(const char* name, const char* what, const Tensor& plain, const Tensor& cache,
+                     const Tensor& scale, mcop_dtype format, const Tensor& key_cache) {
+  TORCH_CHECK(plain.dim() == 3, name, ": ", what, " must be [tokens, heads, head_size], got ",
+              plain.sizes());
+  TORCH_CHECK(cache.dim() == 4, name, ": the cache of ", what,
+              " must be [pages, page_size, heads, head_size], got ", cache.sizes());
+  const int64_t D = plain.size(2);
+  const bool four = format == MCOP_MXFP4;
+  TORCH_CHECK(!four || D % kMxBlock == 0, name, ": head_size ", D, " of ", what,
+              " is not a multiple of the block of 32");
+  TORCH_CHECK(cache.size(3) == (four ? D / 2 : D) && cache.size(2) == plain.size(1), name,
+              ": the cache of ", what, " has shape ", cache.sizes(), " beside ", plain.sizes());
+  TORCH_CHECK(cache.size(0) == key_cache.size(0) && cache.size(1) == key_cache.size(1) &&
+                  cache.size(2) == key_cache.size(2),
+              name, ": the caches' shapes differ: ", key_cache.sizes(), " and ", cache.sizes());
+  TORCH_CHECK(scale.dim() == (four ? 4 : 3) && scale.size(0) == cache.size(0) &&
+                  scale.size(1) == cache.size(1) && scale.size(2) == cache.size(2) &&
+                  (!four || scale.size(3) == D / kMxBlock),
+              name, ": the scale of ", what, " has shape ", scale.sizes(), " beside a cache of ",
+              cache.sizes());
+  TORCH_CHECK(four ? is_scale8(scale.scalar_type()) : scale.scalar_type() == at::kFloat, name,
+              ": the scale of ", what, " must be ",
+              four ? "uint8 or float8_e8m0fnu" : "float32", ", got ", scale.scalar_type());
+  TORCH_CHECK((plain.stride(2) == 1 || D == 1) && (cache.stride(3) == 1 || cache.size(3) == 1) &&
+                  (!four || scale.stride(3) == 1 || scale.size(3) == 1),
+              name, ": last dimension of ", what, ", its cache and its scale must be contiguous");
+  return mcop_kv_side{plain.data_ptr(), plain.stride(0),  plain.stride(1),
+                      cache.data_ptr(), cache.stride(0),  cache.stride(1), cache.stride(2),
+                      scale.data_ptr(), scale.stride(0),  scale.stride(1), scale.stride(2),
+                      D};
+}
+
+void no_overlap(const char* name, std::initializer_list<const Tensor*> outputs) {
+  for (const Tensor* t : outputs) {
+    TORCH_CHECK(at::has_internal_overlap(*t) != at::MemOverlap::Yes, name,
+                ": a tensor that is written has elements that share memory");
+  }
+}
+
+void kv_check(const char* name, const Tensor& key, const Tensor& value, const Tensor& key_cache,
+              const Tensor& value_cache) {
+  dispatch_check(key.scalar_type(), name);
+  TORCH_CHECK(value.scalar_type() == key.scalar_type(), name, ": value must have key's dtype ",
+              key.scalar_type());
+  TORCH_CHECK(value_cache.scalar_type() == key_cache.scalar_type(), name,
+              ": the caches must share a dtype, got ", key_cache.scalar_type(), " and ",
+              value_cache.scalar_type());
+  TORCH_CHECK(key.dim() == 3 && value.dim() == 3 && key.size(0) == value.size(0) &&
+                  key.size(1) == value.size(1) && key.size(1) > 0 && key_cache.dim() == 4,
+              name, ": key ", key.sizes(), " and value ", value.sizes(),
+              " must be [tokens, heads, head_size] of the same tokens and heads");
+}
+
+template <class T>
+const T* index_ptr(const char* name, const char* what, const Tensor& t, at::ScalarType type) {
+  TORCH_CHECK(t.scalar_type() == type, name, ": ", what, " must be ", c10::toString(type),
+              ", got ", t.scalar_type());
+  return static_cast<const T*>(t.data_ptr());
+}
+
+void c_kv_cache_write_quant(const Tensor& key, const Tensor& value, Tensor& key_cache,
+                            Tensor& value_cache, Tensor& key_scale, Tensor& value_scale,
+                            const Tensor& slot_mapping) {
+  const char* name = "kv_cache_write_quant";
+  kv_check(name, key, value, key_cache, value_cache);
+  const mcop_dtype format = cache_code(name, key_cache.scalar_type());
+  const auto* slots = index_ptr<int64_t>(name, "slot_mapping", slot_mapping, at::kLong);
+  TORCH_CHECK(slot_mapping.dim() == 1 && slot_mapping.is_contiguous() &&
+                  slot_mapping.size(0) <= key.size(0),
+              name, ": slot_mapping must be contiguous with at most one slot a token, got ",
+              slot_mapping.sizes(), " for ", key.size(0), " tokens");
+  const mcop_kv_side k = kv_side(name, "key", key, key_cache, key_scale, format, key_cache);
+  const mcop_kv_side v = kv_side(name, "value", value, value_cache, value_scale, format,
+                                 key_cache);
+  no_overlap(name, {&key_cache, &value_cache, &key_scale, &value_scale});
+  on_device(name, {&key, &value, &key_cache, &value_cache, &key_scale, &value_scale,
+                   &slot_mapping});
+  const DeviceGuard guard(key.device());
+  check_rc(mcop_kv_cache_write_quant(&k, &v, format, key_cache.size(0), key_cache.size(1),
+                                     key.size(1), slots, slot_mapping.size(0),
+                                     code_of(key.scalar_type()), stream_of(key)));
+}
+
+void c_kv_cache_read_dequant(Tensor& key, Tensor& value, const Tensor& key_cache,
+                             const Tensor& value_cache, const Tensor& key_scale,
+                             const Tensor& value_scale, const Tensor& block_table,
+                             const Tensor& cu_seqlens, const OptTensor& seq_starts) {
+  const char* name = "kv_cache_read_dequant";
+  kv_check(name, key, value, key_cache, value_cache);
+  const mcop_dtype format = cache_code(name, key_cache.scalar_type());
+  const auto* table = index_ptr<int32_t>(name, "block_table", block_table, at::kInt);
+  const auto* cu = index_ptr<int32_t>(name, "cu_seqlens", cu_seqlens, at::kInt);
+  TORCH_CHECK(block_table.dim() == 2 && (block_table.size(1) <= 1 || block_table.stride(1) == 1),
+              name, ": block_table must be [sequences, pages] with contiguous rows");
+  const int64_t B = block_table.size(0);
+  TORCH_CHECK(cu_seqlens.dim() == 1 && cu_seqlens.is_contiguous() && cu_seqlens.size(0) == B + 1,
+              name, ": cu_seqlens must be contiguous with ", B + 1, " elements, got ",
+              cu_seqlens.sizes());
+  const int32_t* starts = nullptr;
+  if (seq_starts.has_value()) {
+    starts = index_ptr<int32_t>(name, "seq_starts", *seq_starts, at::kInt);
+    TORCH_CHECK(seq_starts->dim() == 1 && seq_starts->is_contiguous() && seq_starts->size(0) == B,
+                name, ": seq_starts must be contiguous with ", B, " elements, got ",
+                seq_starts->sizes());
+  }
+  const mcop_kv_side k = kv_side(name, "key", key, key_cache, key_scale, format, key_cache);
+  const mcop_kv_side v = kv_side(name, "value", value, value_cache, value_scale, format,
+                                 key_cache);
+  no_overlap(name, {&key, &value});
+  on_device(name, {&key, &value, &key_cache, &value_cache, &key_scale, &value_scale, &block_table,
+                   &cu_seqlens, opt(seq_starts)});
+  const DeviceGuard guard(key.device());
+  check_rc(mcop_kv_cache_read_dequant(&k, &v, format, key_cache.size(0), key_cache.size(1),
+                                      key.size(1), table, B > 1 ? block_table.stride(0) : 0,
+                                      block_table.size(1), cu, starts, B, key.size(0),
+                                      code_of(key.scalar_type()), stream_of(key)));
+}
+
+// The allocating forms (custom_ops).
+
+std::vector<int64_t> with_last(const Tensor& t, int64_t last) {
+  std::vector<int64_t> shape = t.sizes().vec();
+  shape.back() = last;
+  return shape;
+}
+
+// New codes and scales for rows like input's (which the operators check).
+std::pair<Tensor, Tensor> mx_new(const Tensor& input) {
+  const int64_t H = rows_of(input).second;
+  const auto opts = input.options().dtype(at::kByte);
+  const py::gil_scoped_release allocating;  // it may wait for the device
+  return {at::empty(with_last(input, H / 2), opts), at::empty(with_last(input, H / kMxBlock), opts)};
+}
+
+std::tuple<Tensor, Tensor> mxfp4_quant_new(const Tensor& input) {
+  auto [codes, scale] = mx_new(input);
+  c_mxfp4_quant(codes, input, scale);
+  return {codes, scale};
+}
+
+Tensor mxfp4_dequant_new(const Tensor& codes, const Tensor& scale, py::object out_dtype) {
+  const at::ScalarType dt = torch::python::detail::py_object_to_dtype(out_dtype);
+  const int64_t half = rows_of(codes).second;
+  Tensor out;
+  {
+    const py::gil_scoped_release allocating;
+    out = at::empty(with_last(codes, half * 2), codes.options().dtype(dt));
+  }
+  c_mxfp4_dequant(out, codes, scale);
+  return out;
+}
+
+std::tuple<Tensor, Tensor, OptTensor> rms_norm_mxfp4_quant_new(const Tensor& input,
+                                                               const Tensor& weight,
+                                                               double epsilon,
+                                                               const OptTensor& residual) {
+  auto [codes, scale] = mx_new(input);
+  OptTensor after;
+  if (residual.has_value()) {
+    const py::gil_scoped_release allocating;
+    after = at::empty(residual->sizes(), residual->options());
+  }
+  c_rms_norm_mxfp4_quant(codes, input, weight, scale, epsilon, residual, after);
+  return {codes, scale, after};
+}
+
+Tensor mxfp4_scaled_mm_new(const Tensor& a, const Tensor& a_scale, const Tensor& b,
+                           const Tensor& b_scale, py::object out_dtype, const OptTensor& bias) {
+  const at::ScalarType dt = torch::python::detail::py_object_to_dtype(out_dtype);
+  TORCH_CHECK(a.dim() > 0 && b.dim() == 2, "mxfp4_scaled_mm: b must be [N, K / 2], got ",
+              b.sizes());
+  Tensor out;
+  {
+    const py::gil_scoped_release allocating;
+    out = at::empty(with_last(a, b.size(0)), a.options().dtype(dt));
+  }
+  c_mxfp4_scaled_mm(out, a, a_scale, b, b_scale, bias);
+  return out;
+}
+
+std::tuple<Tensor, Tensor> kv_cache_read_new(const Tensor& key_cache, const Tensor& value_cache,
+                                             const Tensor& key_scale, const Tensor& value_scale,
+                                             const Tensor& block_table, const Tensor& cu_seqlens,
+                                             int64_t num_tokens, py::object out_dtype,
+                                             const OptTensor& seq_starts) {
+  const char* name = "kv_cache_read_dequant";
+  const at::ScalarType dt = torch::python::detail::py_object_to_dtype(out_dtype);
+  TORCH_CHECK(key_cache.dim() == 4 && value_cache.dim() == 4 && num_tokens >= 0, name,
+              ": caches must be [pages, page_size, heads, head_size], num_tokens not negative");
+  const int64_t wide = is_codes4(key_cache.scalar_type()) ? 2 : 1;
+  const auto opts = key_cache.options().dtype(dt);
+  Tensor key, value;
+  {
+    const py::gil_scoped_release allocating;
+    key = at::empty({num_tokens, key_cache.size(2), key_cache.size(3) * wide}, opts);
+    value = at::empty({num_tokens, value_cache.size(2), value_cache.size(3) * wide}, opts);
+  }
+  c_kv_cache_read_dequant(key, value, key_cache, value_cache, key_scale, value_scale, block_table,
+                          cu_seqlens, seq_starts);
+  return {key, value};
+}
+
 // Meta kernel of the mutating _C ops (no outputs to describe): drop the arguments.
 void meta_noop(const c10::OperatorHandle& op, torch::jit::Stack* stack) {
   torch::jit::drop(*stack, op.schema().arguments().size());
@@ -602,6 +930,21 @@ constexpr VllmOp kVllmOps[] = {
     {"dynamic_per_token_scaled_fp8_quant",
      "dynamic_per_token_scaled_fp8_quant(Tensor! result, Tensor input, Tensor! scale, "
      "Tensor? scale_ub) -> ()"},
+    {"mxfp4_quant", "mxfp4_quant(Tensor! result, Tensor input, Tensor! scale) -> ()"},
+    {"mxfp4_dequant", "mxfp4_dequant(Tensor! result, Tensor input, Tensor scale) -> ()"},
+    {"rms_norm_mxfp4_quant",
+     "rms_norm_mxfp4_quant(Tensor! result, Tensor input, Tensor weight, Tensor! scale, "
+     "float epsilon, Tensor? residual, Tensor!? after_res) -> ()"},
+    {"mxfp4_scaled_mm",
+     "mxfp4_scaled_mm(Tensor! result, Tensor a, Tensor a_scale, Tensor b, Tensor b_scale, "
+     "Tensor? bias) -> ()"},
+    {"kv_cache_write_quant",
+     "kv_cache_write_quant(Tensor key, Tensor value, Tensor! key_cache, Tensor! value_cache, "
+     "Tensor! key_scale, Tensor! value_scale, Tensor slot_mapping) -> ()"},
+    {"kv_cache_read_dequant",
+     "kv_cache_read_dequant(Tensor! key, Tensor! value, Tensor key_cache, Tensor value_cache, "
+     "Tensor key_scale, Tensor value_scale, Tensor block_table, Tensor cu_seqlens, "
+     "Tensor? seq_starts) -> ()"},
 };
 
 // Registers the _C schemas (each only if no other library, e.g. vLLM's own _C, defined it) with
@@ -629,6 +972,12 @@ void register_vllm_ops() {
   cuda->impl("rms_norm_per_block_quant", TORCH_FN(c_per_block_quant));
   cuda->impl("dynamic_scaled_int8_quant", TORCH_FN(c_int8_quant));
   cuda->impl("dynamic_per_token_scaled_fp8_quant", TORCH_FN(c_fp8_quant));
+  cuda->impl("mxfp4_quant", TORCH_FN(c_mxfp4_quant));
+  cuda->impl("mxfp4_dequant", TORCH_FN(c_mxfp4_dequant));
+  cuda->impl("rms_norm_mxfp4_quant", TORCH_FN(c_rms_norm_mxfp4_quant));
+  cuda->impl("mxfp4_scaled_mm", TORCH_FN(c_mxfp4_scaled_mm));
+  cuda->impl("kv_cache_write_quant", TORCH_FN(c_kv_cache_write_quant));
+  cuda->impl("kv_cache_read_dequant", TORCH_FN(c_kv_cache_read_dequant));
   done = true;
 }
 
@@ -717,4 +1066,50 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("scale"), py::arg("azp") = py::none());
   m.def("c_dynamic_per_token_scaled_fp8_quant", &c_fp8_quant, py::arg("result"),
         py::arg("input"), py::arg("scale"), py::arg("scale_ub") = py::none());
+  m.def("c_mxfp4_quant", &c_mxfp4_quant,
+        "Rows of input (bf16, fp16, fp32; last dimension contiguous, a multiple of 32) as 4-bit "
+        "codes: result [..., H / 2] (uint8 or float4_e2m1fn_x2, element 2i in the low half of byte "
+        "i), scale [..., H / 32] (uint8 or float8_e8m0fnu).",
+        py::arg("result"), py::arg("input"), py::arg("scale"));
+  m.def("c_mxfp4_dequant", &c_mxfp4_dequant,
+        "The values of codes and scales of mxfp4_quant, rounded once to result's dtype.",
+        py::arg("result"), py::arg("input"), py::arg("scale"));
+  m.def("c_rms_norm_mxfp4_quant", &c_rms_norm_mxfp4_quant,
+        "(Residual add +) RMSNorm + mxfp4_quant of the normalized rows; after_res <- input + "
+        "residual (it may be the residual or the input itself; the two are given together).",
+        py::arg("result"), py::arg("input"), py::arg("weight"), py::arg("scale"),
+        py::arg("epsilon"), py::arg("residual") = py::none(), py::arg("after_res") = py::none());
+  m.def("c_mxfp4_scaled_mm", &c_mxfp4_scaled_mm,
+        "result [..., N] (bf16, fp16, fp32) <- a [..., K / 2] times the transpose of b [N, K / 2], "
+        "both codes with scales [..., K / 32], plus bias [N]; summed in fp32, rounded once.",
+        py::arg("result"), py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"),
+        py::arg("bias") = py::none());
+  m.def("c_kv_cache_write_quant", &c_kv_cache_write_quant,
+        "Quantizes key and value [tokens, heads, head_size] into the slots of a paged cache "
+        "[pages, page_size, heads, head_size] (int8 or float8_e4m3fn with fp32 scales [pages, "
+        "page_size, heads]; or 4-bit codes, uint8 [..., head_size / 2], with scales [..., "
+        "head_size / 32]). slot_mapping (int64) may cover fewer tokens; a negative slot, or one "
+        "past the cache, is not written. Slots that are written must differ.",
+        py::arg("key"), py::arg("value"), py::arg("key_cache"), py::arg("value_cache"),
+        py::arg("key_scale"), py::arg("value_scale"), py::arg("slot_mapping"));
+  m.def("c_kv_cache_read_dequant", &c_kv_cache_read_dequant,
+        "Gathers sequences of such a cache into key and value [tokens, heads, head_size]: rows "
+        "cu_seqlens[s] to cu_seqlens[s + 1] are positions from seq_starts[s] (or 0) on of sequence "
+        "s, whose pages block_table[s] lists. Rows past the last sequence are left as they were; "
+        "positions without a page read as NaN.",
+        py::arg("key"), py::arg("value"), py::arg("key_cache"), py::arg("value_cache"),
+        py::arg("key_scale"), py::arg("value_scale"), py::arg("block_table"),
+        py::arg("cu_seqlens"), py::arg("seq_starts") = py::none());
+  // custom_ops: the same into new tensors
+  m.def("mxfp4_quant_new", &mxfp4_quant_new, py::arg("input"));
+  m.def("mxfp4_dequant_new", &mxfp4_dequant_new, py::arg("codes"), py::arg("scale"),
+        py::arg("out_dtype"));
+  m.def("rms_norm_mxfp4_quant_new", &rms_norm_mxfp4_quant_new, py::arg("input"),
+        py::arg("weight"), py::arg("epsilon"), py::arg("residual") = py::none());
+  m.def("mxfp4_scaled_mm_new", &mxfp4_scaled_mm_new, py::arg("a"), py::arg("a_scale"),
+        py::arg("b"), py::arg("b_scale"), py::arg("out_dtype"), py::arg("bias") = py::none());
+  m.def("kv_cache_read_new", &kv_cache_read_new, py::arg("key_cache"), py::arg("value_cache"),
+        py::arg("key_scale"), py::arg("value_scale"), py::arg("block_table"),
+        py::arg("cu_seqlens"), py::arg("num_tokens"), py::arg("out_dtype"),
+        py::arg("seq_starts") = py::none());
 }

@@ -1,0 +1,151 @@
+"""The operators as a serving step uses them together: residual add + norm to 4-bit codes, the fused
+QKV product, the key heads' norm, the write to the quantized cache and the read of the context; eager,
+on another stream, captured and replayed, and through torch.compile."""
+
+import pytest
+import torch
+
+import mcoplib_amd._C  # noqa: F401
+import mx_plain
+from gpu_util import DEV, randn, say, weight
+from mcoplib import custom_ops, op
+
+pytestmark = pytest.mark.gpu
+
+H, QH, KH, D, PAGE, EPS = 512, 4, 2, 64, 16, 1e-6
+N = (QH + 2 * KH) * D
+CODES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn, "mxfp4": torch.uint8}
+
+
+class Layer:
+    def __init__(self, kind, pages=8):
+        self.kind = kind
+        self.norm = weight(H, 1, torch.bfloat16).to(DEV)
+        self.qkv = randn((N, H), 2, torch.bfloat16, scale=0.05)
+        self.w = custom_ops.mxfp4_quant(self.qkv.to(DEV))
+        self.bias = randn((N,), 3, torch.bfloat16, scale=0.1).to(DEV)
+        self.heads = torch.stack([weight(D, 10 + h, torch.bfloat16) for h in range(KH)]).to(DEV)
+        width = D // 2 if kind == "mxfp4" else D
+        tail = (D // 32,) if kind == "mxfp4" else ()
+        sdt = torch.uint8 if kind == "mxfp4" else torch.float32
+        self.cache = [torch.zeros(pages, PAGE, KH, width, dtype=CODES[kind], device=DEV)
+                      for _ in range(2)]
+        self.scale = [torch.zeros(pages, PAGE, KH, *tail, dtype=sdt, device=DEV) for _ in range(2)]
+
+    def step(self, x, residual, slots, table, cu, tokens):
+        codes, scale, after = custom_ops.rms_norm_mxfp4_quant(x, self.norm, EPS, residual)
+        qkv = custom_ops.mxfp4_scaled_mm(codes, scale, *self.w, torch.bfloat16, self.bias)
+        k = qkv[:, QH * D:(QH + KH) * D].unflatten(1, (KH, D)).contiguous()
+        v = qkv[:, (QH + KH) * D:].unflatten(1, (KH, D))
+        kn = torch.empty_like(k)
+        op.head_rms_norm(kn, k, self.heads, EPS, 0, KH)
+        custom_ops.kv_cache_write_quant(kn, v, *self.cache, *self.scale, slots)
+        return (*custom_ops.kv_cache_read_dequant(*self.cache, *self.scale, table, cu, tokens,
+                                                  torch.bfloat16), after, kn, v.contiguous())
+
+
+def _inputs(T, seed):
+    return (randn((T, H), seed, torch.bfloat16).to(DEV),
+            randn((T, H), seed + 1, torch.bfloat16).to(DEV))
+
+
+def _tables(T):
+    """Two sequences that share out the T tokens: one page apart, in pages 5, 1, 3, ..."""
+    first = T // 3
+    table = torch.tensor([[5, 1, 3], [2, 7, 0]], dtype=torch.int32)
+    cu = torch.tensor([0, first, T], dtype=torch.int32)
+    slots = torch.tensor([int(table[0, p // PAGE]) * PAGE + p % PAGE for p in range(first)]
+                         + [int(table[1, p // PAGE]) * PAGE + p % PAGE for p in range(T - first)])
+    return slots.to(DEV), table.to(DEV), cu.to(DEV)
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8", "mxfp4"])
+@pytest.mark.parametrize("T", [1, 45])
+def test_one_step(kind, T):
+    """The whole step, and each stage against its plain statement on the stage's own input."""
+    say(f"quant path {kind} {T} tokens")
+    layer = Layer(kind)
+    x, r = _inputs(T, 20)
+    slots, table, cu = _tables(T)
+    key, value, after, kn, v = layer.step(x, r, slots, table, cu, T)
+    y, want_after = mx_plain.norm_rows(x, layer.norm, EPS, r)
+    assert mx_plain.same(after, want_after)
+    a = mx_plain.values(*mx_plain.quant(y))
+    b = mx_plain.values(*mx_plain.quant(layer.qkv))
+    qkv = a @ b.t() + layer.bias.cpu().double()
+    # bf16's rounding (2^-9 of the value, 2^-8 / 2) and H additions of at most a step of sum|ab| each
+    room = 2.0 ** -8 * qkv.abs() + H * 2.0 ** -22 * (a.abs() @ b.abs().t()) + 1e-6
+    off = (v.cpu().double().flatten(1) - qkv[:, (QH + KH) * D:]).abs()
+    assert bool((off <= room[:, (QH + KH) * D:]).all())
+    for got, plain in ((key, kn), (value, v)):
+        q, s = mx_plain.vector_codes(plain, kind)
+        assert mx_plain.same(got, mx_plain.vector_values(q, s, kind, torch.bfloat16))
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8", "mxfp4"])
+def test_captured_and_replayed(kind):
+    """Captured once, replayed with new inputs and eager work between, each replay equal to the eager
+    step on a layer of its own."""
+    say(f"quant path graph {kind}")
+    T = 33
+    layer, eager = Layer(kind), Layer(kind)
+    x, r = _inputs(T, 1)
+    slots, table, cu = _tables(T)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        layer.step(x, r, slots, table, cu, T)
+        with torch.cuda.graph(g, stream=side):
+            outs = layer.step(x, r, slots, table, cu, T)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for rep in range(4):
+        nx, nr = _inputs(T, 50 + rep)
+        x.copy_(nx), r.copy_(nr)
+        g.replay()
+        want = eager.step(nx, nr, slots, table, cu, T)
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert mx_plain.same(a, b), rep
+        assert (nx * 2).sum().item() == (nx * 2).sum().item()
+
+
+def test_on_another_stream():
+    """Calls go to the stream that is current, after the work that is queued on it."""
+    layer, T = Layer("int8"), 45
+    slots, table, cu = _tables(T)
+    x, r = _inputs(T, 7)
+    want = [t.clone() for t in layer.step(x, r, slots, table, cu, T)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        late = torch.zeros_like(x)
+        big = torch.randn(2048, 2048, device=DEV)
+        for _ in range(20):
+            big = big @ big * 1e-3
+        late.copy_(x)
+        got = layer.step(late, r, slots, table, cu, T)
+    s.synchronize()
+    for a, b in zip(got, want):
+        assert mx_plain.same(a, b)
+
+
+def test_torch_compile_aot_eager():
+    layer, T = Layer("fp8"), 12
+    slots, table, cu = _tables(T)
+    x, r = _inputs(T, 3)
+
+    def step(x, r):
+        codes = torch.empty(T, H // 2, dtype=torch.uint8, device=DEV)
+        scale = torch.empty(T, H // 32, dtype=torch.uint8, device=DEV)
+        after = torch.empty_like(x)
+        torch.ops._C.rms_norm_mxfp4_quant(codes, x, layer.norm, scale, EPS, r, after)
+        out = torch.empty(T, N, dtype=torch.bfloat16, device=DEV)
+        torch.ops._C.mxfp4_scaled_mm(out, codes, scale, *layer.w, layer.bias)
+        return out, after
+
+    want = step(x, r)
+    got = torch.compile(step, backend="aot_eager", fullgraph=True)(x, r)
+    for a, b in zip(got, want):
+        assert mx_plain.same(a, b)
