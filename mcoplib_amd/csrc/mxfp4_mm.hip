@@ -25,16 +25,19 @@ __device__ __forceinline__ i32x8 fp4_operand(i32x4 v) {
   return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
 }
 
-// Scale bytes b..b+3 of a row of `blocks`, zero past its end (where the codes are zero as well).
+// Scale bytes b..b+3 of a row of `blocks`, zero past its end (where the codes count as zero as well),
+// by loads that stay inside the row.  DWORDS: `blocks` is a multiple of four, rows aligned to four.
 template <bool DWORDS>
 __device__ __forceinline__ uint32_t scales4(const uint8_t* row, int b, int blocks) {
   if constexpr (DWORDS) {
-    return b < blocks ? *reinterpret_cast<const uint32_t*>(row + b) : 0u;
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(row + min(b, blocks - 4));
+    return b < blocks ? v : 0u;
   } else {
     uint32_t v = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (b + e < blocks) v |= (uint32_t)row[b + e] << (8 * e);
+      const uint32_t x = row[min(b + e, blocks - 1)];
+      v |= b + e < blocks ? x << (8 * e) : 0u;
     }
     return v;
   }
@@ -96,12 +99,291 @@ k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   }
 }
 
+// Many rows: a workgroup of four waves (2 x 2) makes a (64 FM) x (64 FN) tile, each wave FM x FN
+// products of 32 x 32.  Codes go from memory to LDS in tiles of 256 along K (128 bytes a row), two
+// tiles in turn, without passing through registers; from there to the matrix units a step of 64 along
+// K ahead of the products.  In 32x32x64 instructions the lane of group g = lane / 32 takes blocks 4g..4g+3
+// of a tile, one a step, so that the scales of its row for the tile are one dword.
+//
+// LDS: a tile's row is 8 chunks of 16 bytes, chunk c at place c ^ (row & 7): the eight lanes that a
+// 16-byte read serves at once then take eight different places.  A direct load writes 64 x 16 bytes in
+// lane order (eight rows), so each lane's address is that of the chunk that belongs at its place.
+// Scales go through registers (they need no alignment), a row a thread.
+//
+// One barrier a tile: before the last step's products, whose operands are in registers by then, the
+// wave waits for its part of the next tile, meets the others, reads the next tile's first operands and
+// starts the loads of the tile after it, into the tile that all have finished reading.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kTileK = 8;     // blocks
+constexpr int kRowBytes = 128;
+
+// 16 bytes a lane from base + off to LDS at `to` + 16 * lane.  The compiler does not see what this
+// writes nor that it is in flight: wait_loads() and the barrier order it.
+__device__ __forceinline__ void load_to_lds(uint32_t to, const uint8_t* base, uint32_t off) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2"
+      :
+      : "s"(to), "v"(off), "s"(base)
+      : "memory", "m0");
+}
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+__device__ __forceinline__ void wait_lds() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
+template <class E, bool DWORDS, int FM, int FN>
+__global__ void __launch_bounds__(256, 1)
+k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
+                const uint8_t* __restrict__ as, const uint8_t* __restrict__ b,
+                const uint8_t* __restrict__ bs, const typename E::S* __restrict__ bias, int M, int N,
+                int blocks, int tiles_m, int tiles_n) {
+  constexpr int BM = 64 * FM, BN = 64 * FN, ROWS = BM + BN;
+  constexpr int TILE = ROWS * kRowBytes, SCALES = ROWS * kTileK;
+  constexpr int LOADS = ROWS / 8 / 4;  // direct loads of a wave and tile
+  constexpr int SR = (ROWS + 255) / 256;  // rows whose scales a thread reads
+  __shared__ alignas(1024) uint8_t lds[2 * TILE + 2 * SCALES];
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tile_m = (int)blockIdx.x % tiles_m, tile_n = (int)blockIdx.x / tiles_m;
+  const int m0 = tile_m * BM, n0 = tile_n * BN;
+  const int64_t pitch = (int64_t)blocks * 16;
+  const int last = (blocks - 1) / kTileK;
+
+  // Rows 0..BM-1 of the LDS tile are a's, the rest b's; a wave's first 2 FM loads of eight rows are of
+  // a, the rest of b.  Rows past an operand's end repeat its last.
+  const int chunk = (lane & 7) ^ ((lane >> 3) & 7);
+  auto first_row = [&](int j) {
+    return j < 2 * FM ? (wave * 2 * FM + j) * 8 : BM + (wave * 2 * FN + j - 2 * FM) * 8;
+  };
+  uint32_t off[LOADS];
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int row = first_row(j) + lane / 8;
+    const int r = j < 2 * FM ? min(row, M - 1 - m0) : min(row - BM, N - 1 - n0);
+    off[j] = (uint32_t)(r * pitch) + chunk * 16;
+  }
+  const uint8_t* abase = a + m0 * pitch;
+  const uint8_t* bbase = b + n0 * pitch;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  // Load j of tile t into buffer `to`.  Chunks past the row's end read the tile's first, and count as
+  // zero.
+  auto load_rows = [&](int j, int t, int to) {
+    const uint32_t back = chunk < blocks - t * kTileK ? 0 : chunk * 16;
+    load_to_lds(lds0 + to * TILE + first_row(j) * kRowBytes,
+                (j < 2 * FM ? abase : bbase) + t * kRowBytes, off[j] - back);
+  };
+  auto load_tile = [&](int t, int to) {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) load_rows(j, t, to);
+  };
+  // What a load gives is put together and masked when it is stored, not when it is started: looking at
+  // it would wait for it, and for the direct loads around it.
+  constexpr int PIECES = DWORDS ? 2 : 8;
+  uint32_t sv[SR][PIECES];
+  auto load_scales = [&](int t) {
+#pragma unroll
+    for (int k = 0; k < SR; ++k) {
+      const int row = min(tid + 256 * k, ROWS - 1);
+      const uint8_t* p = row < BM ? as + (int64_t)min(m0 + row, M - 1) * blocks
+                                  : bs + (int64_t)min(n0 + row - BM, N - 1) * blocks;
+#pragma unroll
+      for (int e = 0; e < PIECES; ++e) {
+        if constexpr (DWORDS) {
+          sv[k][e] = *reinterpret_cast<const uint32_t*>(p + min(t * kTileK + 4 * e, blocks - 4));
+        } else {
+          sv[k][e] = p[min(t * kTileK + e, blocks - 1)];
+        }
+      }
+    }
+  };
+  auto store_scales = [&](int t, int to) {
+#pragma unroll
+    for (int k = 0; k < SR; ++k) {
+      const int row = tid + 256 * k;
+      if (ROWS % 256 != 0 && row >= ROWS) continue;
+      uint32_t w[2] = {0, 0};
+#pragma unroll
+      for (int e = 0; e < PIECES; ++e) {
+        const bool in = t * kTileK + e * (8 / PIECES) < blocks;
+        if constexpr (DWORDS) w[e] = in ? sv[k][e] : 0u;
+        else w[e / 4] |= in ? sv[k][e] << (8 * (e % 4)) : 0u;
+      }
+      *reinterpret_cast<u32x2*>(lds + 2 * TILE + to * SCALES + row * 8) = u32x2{w[0], w[1]};
+    }
+  };
+
+  const int r32 = lane & 31, g = lane >> 5;
+  const int am = (wave & 1) * 32 * FM + r32, bn = BM + (wave >> 1) * 32 * FN + r32;
+  i32x4 fa[2][FM], fb[2][FN];
+  int sa[2][FM], sb[2][FN];
+  // Operand q of step s: a's first, then b's; and its scales for the tile.
+  auto read_codes = [&](int q, int from, int s, int into) {
+    const int place = ((4 * g + s) ^ (r32 & 7)) * 16 + from * TILE;
+    if (q < FM) {
+      fa[into][q] = *reinterpret_cast<const i32x4*>(lds + place + (am + 32 * q) * kRowBytes);
+    } else {
+      fb[into][q - FM] =
+          *reinterpret_cast<const i32x4*>(lds + place + (bn + 32 * (q - FM)) * kRowBytes);
+    }
+  };
+  auto read_scales = [&](int q, int from, int into) {
+    const int place = 2 * TILE + from * SCALES + 4 * g;
+    if (q < FM) {
+      sa[into][q] = *reinterpret_cast<const int*>(lds + place + (am + 32 * q) * 8);
+    } else {
+      sb[into][q - FM] = *reinterpret_cast<const int*>(lds + place + (bn + 32 * (q - FM)) * 8);
+    }
+  };
+  f32x16 sum[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sum[i][j][e] = 0.0f;
+    }
+  }
+  // The products of step s, with `other(q)` issued behind the q-th: the order is kept as written, so
+  // that reads and loads go out between products, each in the time one takes.
+  auto step = [&](auto s, auto other) {
+    constexpr int S = decltype(s)::value;
+#pragma unroll
+    for (int q = 0; q < FM * FN; ++q) {
+      const int i = q / FN, j = q % FN;
+      sum[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+          fp4_operand(fb[S & 1][j]), fp4_operand(fa[S & 1][i]), sum[i][j], kFp4, kFp4, S, sb[0][j], S,
+          sa[0][i]);
+      other(q);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  using S0 = std::integral_constant<int, 0>;
+  using S1 = std::integral_constant<int, 1>;
+  using S2 = std::integral_constant<int, 2>;
+  using S3 = std::integral_constant<int, 3>;
+  constexpr int OPS = FM + FN, MMS = FM * FN;
+  auto reading = [&](int from, int s) {  // the operands of step s, from the first products on
+    return [&, from, s](int q) {
+#pragma unroll
+      for (int o = 0; o < OPS; ++o) {
+        if (o * MMS / 2 / OPS == q) read_codes(o, from, s, s & 1);
+      }
+    };
+  };
+
+  load_scales(0);
+  load_tile(0, 0);
+  wait_loads();
+  store_scales(0, 0);
+  load_scales(min(1, last));
+  load_tile(min(1, last), 1);
+  wait_lds();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int o = 0; o < OPS; ++o) {
+    read_codes(o, 0, 0, 0);
+    read_scales(o, 0, 0);
+  }
+  for (int t = 0; t < last; ++t) {
+    const int cur = t & 1, then = min(t + 2, last);
+    __builtin_amdgcn_sched_barrier(0);
+    step(S0(), reading(cur, 1));
+    step(S1(), reading(cur, 2));
+    step(S2(), reading(cur, 3));
+    wait_loads();
+    store_scales(t + 1, cur ^ 1);
+    wait_lds();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    load_scales(then);
+    __builtin_amdgcn_sched_barrier(0);
+    step(S3(), [&](int q) {
+#pragma unroll
+      for (int o = 0; o < OPS; ++o) {
+        if (o * MMS / 2 / OPS == q) {
+          read_codes(o, cur ^ 1, 0, 0);
+          read_scales(o, cur ^ 1, 1);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        if (j * MMS / LOADS == q) load_rows(j, then, cur);
+      }
+    });
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sa[0][i] = sa[1][i];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) sb[0][i] = sb[1][i];
+  }
+  {  // the last tile, whose blocks past the rows' end count as zero: a's codes here, the scales above
+    auto mask = [&](int s) {
+      const bool in = last * kTileK + 4 * g + s < blocks;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) fa[s & 1][i][e] = in ? fa[s & 1][i][e] : 0;
+      }
+    };
+    const int cur = last & 1;
+    mask(0);
+    step(S0(), reading(cur, 1));
+    mask(1);
+    step(S1(), reading(cur, 2));
+    mask(2);
+    step(S2(), reading(cur, 3));
+    mask(3);
+    step(S3(), [](int) {});
+  }
+  wait_loads();  // the loads past the last tile: none may arrive after the workgroup's LDS is given on
+
+  // a lane holds n = 8 (e / 4) + 4 g + e % 4 of m = lane % 32 of each product
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = m0 + am + 32 * i;
+    if (m >= M) continue;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = n0 + (wave >> 1) * 32 * FN + 32 * j + 8 * q + 4 * g;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (n + e < N) {
+            float v = sum[i][j][4 * q + e];
+            if (bias != nullptr) v += E::to_f(bias[n + e]);
+            out[(int64_t)m * N + n + e] = E::from_f(v);
+          }
+        }
+      }
+    }
+  }
+}
+
 template <class E>
 static int product(void* out, const uint8_t* a, const uint8_t* as, const uint8_t* b,
                    const uint8_t* bs, const void* bias, int M, int N, int blocks, hipStream_t st) {
   using S = typename E::S;
   auto* o = static_cast<S*>(out);
   const auto* bi = static_cast<const S*>(bias);
+  const int64_t pitch = (int64_t)blocks * 16;
+  const int tm = (M + 255) / 256, tn = (N + 255) / 256;
+  if (M > 64 && pitch * 256 < ((int64_t)1 << 32) && (int64_t)tm * tn <= INT32_MAX) {
+    const dim3 grid((unsigned)(tm * tn)), block(256);
+    if (blocks % 4 == 0 && aligned(4, as, bs)) {
+      hipLaunchKernelGGL((k_mxfp4_mm_tile<E, true, 4, 4>), grid, block, 0, st, o, a, as, b, bs, bi, M,
+                         N, blocks, tm, tn);
+    } else {
+      hipLaunchKernelGGL((k_mxfp4_mm_tile<E, false, 4, 4>), grid, block, 0, st, o, a, as, b, bs, bi,
+                         M, N, blocks, tm, tn);
+    }
+    return check_launch("mxfp4_scaled_mm");
+  }
   const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), block(256);
   if (blocks % 4 == 0 && aligned(4, as, bs)) {
     hipLaunchKernelGGL((k_mxfp4_mm_rows<E, true>), grid, block, 0, st, o, a, as, b, bs, bi, M, N,
