@@ -108,7 +108,8 @@ k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 // LDS: a tile's row is 8 chunks of 16 bytes, chunk c at place c ^ (row & 7): the eight lanes that a
 // 16-byte read serves at once then take eight different places.  A direct load writes 64 x 16 bytes in
 // lane order (eight rows), so each lane's address is that of the chunk that belongs at its place.
-// Scales go through registers (they need no alignment), a row a thread.
+// Scales go through registers (their rows have any alignment), for two tiles at a time, a row a thread:
+// 16 bytes a row are one request of a line, as four would be.
 //
 // One barrier a tile: before the last step's products, whose operands are in registers by then, the
 // wave waits for its part of the next tile, meets the others, reads the next tile's first operands and
@@ -136,17 +137,18 @@ __device__ __forceinline__ void wait_lds() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-template <class E, bool DWORDS, int FM, int FN>
+template <class E, int FM, int FN>
 __global__ void __launch_bounds__(256, 1)
 k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
                 const uint8_t* __restrict__ as, const uint8_t* __restrict__ b,
                 const uint8_t* __restrict__ bs, const typename E::S* __restrict__ bias, int M, int N,
                 int blocks, int tiles_m, int tiles_n) {
   constexpr int BM = 64 * FM, BN = 64 * FN, ROWS = BM + BN;
-  constexpr int TILE = ROWS * kRowBytes, SCALES = ROWS * kTileK;
+  constexpr int TILE = ROWS * kRowBytes, SCALES = ROWS * 16;
   constexpr int LOADS = ROWS / 8 / 4;  // direct loads of a wave and tile
   constexpr int SR = (ROWS + 255) / 256;  // rows whose scales a thread reads
   __shared__ alignas(1024) uint8_t lds[2 * TILE + 2 * SCALES];
+  __shared__ alignas(16) float add[BN];  // the bias
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int tile_m = (int)blockIdx.x % tiles_m, tile_n = (int)blockIdx.x / tiles_m;
@@ -181,39 +183,44 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) load_rows(j, t, to);
   };
-  // What a load gives is put together and masked when it is stored, not when it is started: looking at
-  // it would wait for it, and for the direct loads around it.
-  constexpr int PIECES = DWORDS ? 2 : 8;
-  uint32_t sv[SR][PIECES];
-  auto load_scales = [&](int t) {
+  // Scales of pair p of tiles: 16 bytes of a row from wherever they start, or the last 16 of all where
+  // those would pass the end, moved and masked when they are stored (looking at them sooner would wait
+  // for them, and for the direct loads around them).
+  i32x4 sv[SR];
+  auto scale_row = [&](int k, int64_t* past, int p) {
+    const int row = min(tid + 256 * k, ROWS - 1);
+    const bool is_a = row < BM;
+    const int64_t at = (int64_t)(is_a ? min(m0 + row, M - 1) : min(n0 + row - BM, N - 1)) * blocks +
+                       min(p * 16, blocks - 1);
+    const int64_t end = (int64_t)(is_a ? M : N) * blocks - 16;
+    *past = at > end ? at - end : 0;
+    return (is_a ? as : bs) + (at > end ? end : at);
+  };
+  auto load_scales = [&](int p) {
 #pragma unroll
     for (int k = 0; k < SR; ++k) {
-      const int row = min(tid + 256 * k, ROWS - 1);
-      const uint8_t* p = row < BM ? as + (int64_t)min(m0 + row, M - 1) * blocks
-                                  : bs + (int64_t)min(n0 + row - BM, N - 1) * blocks;
-#pragma unroll
-      for (int e = 0; e < PIECES; ++e) {
-        if constexpr (DWORDS) {
-          sv[k][e] = *reinterpret_cast<const uint32_t*>(p + min(t * kTileK + 4 * e, blocks - 4));
-        } else {
-          sv[k][e] = p[min(t * kTileK + e, blocks - 1)];
-        }
-      }
+      int64_t past;
+      __builtin_memcpy(&sv[k], scale_row(k, &past, p), 16);
     }
   };
-  auto store_scales = [&](int t, int to) {
+  auto store_scales = [&](int p) {
+    const int left = blocks - p * 16;  // bytes of the pair inside a row
 #pragma unroll
     for (int k = 0; k < SR; ++k) {
       const int row = tid + 256 * k;
       if (ROWS % 256 != 0 && row >= ROWS) continue;
-      uint32_t w[2] = {0, 0};
-#pragma unroll
-      for (int e = 0; e < PIECES; ++e) {
-        const bool in = t * kTileK + e * (8 / PIECES) < blocks;
-        if constexpr (DWORDS) w[e] = in ? sv[k][e] : 0u;
-        else w[e / 4] |= in ? sv[k][e] << (8 * (e % 4)) : 0u;
-      }
-      *reinterpret_cast<u32x2*>(lds + 2 * TILE + to * SCALES + row * 8) = u32x2{w[0], w[1]};
+      int64_t past;
+      scale_row(k, &past, p);
+      uint64_t lo = (uint64_t)(uint32_t)sv[k][1] << 32 | (uint32_t)sv[k][0];
+      uint64_t hi = (uint64_t)(uint32_t)sv[k][3] << 32 | (uint32_t)sv[k][2];
+      if (past >= 8) lo = hi, hi = 0;
+      const int bits = ((int)past & 7) * 8;
+      lo = lo >> bits | (hi << 1) << (63 - bits);
+      hi >>= bits;
+      if (left < 8) lo &= ((uint64_t)1 << (8 * left)) - 1;
+      if (left < 16) hi &= left <= 8 ? 0 : ((uint64_t)1 << (8 * (left - 8))) - 1;
+      typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+      *reinterpret_cast<u64x2*>(lds + 2 * TILE + (p & 1) * SCALES + row * 16) = u64x2{lo, hi};
     }
   };
 
@@ -231,12 +238,12 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
           *reinterpret_cast<const i32x4*>(lds + place + (bn + 32 * (q - FM)) * kRowBytes);
     }
   };
-  auto read_scales = [&](int q, int from, int into) {
-    const int place = 2 * TILE + from * SCALES + 4 * g;
+  auto read_scales = [&](int q, int t, int into) {
+    const int place = 2 * TILE + (t >> 1 & 1) * SCALES + (t & 1) * 8 + 4 * g;
     if (q < FM) {
-      sa[into][q] = *reinterpret_cast<const int*>(lds + place + (am + 32 * q) * 8);
+      sa[into][q] = *reinterpret_cast<const int*>(lds + place + (am + 32 * q) * 16);
     } else {
-      sb[into][q - FM] = *reinterpret_cast<const int*>(lds + place + (bn + 32 * (q - FM)) * 8);
+      sb[into][q - FM] = *reinterpret_cast<const int*>(lds + place + (bn + 32 * (q - FM)) * 16);
     }
   };
   f32x16 sum[FM][FN];
@@ -276,11 +283,13 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     };
   };
 
+  if (bias != nullptr) {
+    for (int c = tid; c < BN; c += 256) add[c] = E::to_f(bias[min(n0 + c, N - 1)]);
+  }
   load_scales(0);
   load_tile(0, 0);
   wait_loads();
-  store_scales(0, 0);
-  load_scales(min(1, last));
+  store_scales(0);
   load_tile(min(1, last), 1);
   wait_lds();
   __builtin_amdgcn_s_barrier();
@@ -297,18 +306,18 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     step(S1(), reading(cur, 2));
     step(S2(), reading(cur, 3));
     wait_loads();
-    store_scales(t + 1, cur ^ 1);
+    if (cur) store_scales((t + 1) / 2);
     wait_lds();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    load_scales(then);
+    if (!cur) load_scales(t / 2 + 1);
     __builtin_amdgcn_sched_barrier(0);
     step(S3(), [&](int q) {
 #pragma unroll
       for (int o = 0; o < OPS; ++o) {
         if (o * MMS / 2 / OPS == q) {
           read_codes(o, cur ^ 1, 0, 0);
-          read_scales(o, cur ^ 1, 1);
+          read_scales(o, t + 1, 1);
         }
       }
 #pragma unroll
@@ -342,24 +351,51 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   }
   wait_loads();  // the loads past the last tile: none may arrive after the workgroup's LDS is given on
 
-  // a lane holds n = 8 (e / 4) + 4 g + e % 4 of m = lane % 32 of each product
+  // A lane holds n = 8 (e / 4) + 4 g + e % 4 of m = lane % 32 of each product: 8 or 16 bytes in a row.
+  // Each wave turns 32 rows at a time in LDS of its own and stores them 16 bytes a lane, whole lines in
+  // a row: as they are held, two or four bytes a store, the stores took 130 of 420 us (8192 x 8192 x
+  // 8192 bf16).
+  using S = typename E::S;
+  constexpr int WN = 32 * FN, LINE = WN * (int)sizeof(S) + 16;  // 16: rows start in other banks
+  static_assert(4 * 32 * LINE <= 2 * TILE, "the waves' rows fit the tiles");
+  __builtin_amdgcn_s_barrier();  // every wave has read its last operands
+  asm volatile("" ::: "memory");
+  uint8_t* own = lds + wave * 32 * LINE;
+  const int wn0 = n0 + (wave >> 1) * WN;
+  constexpr int VEC = 16 / (int)sizeof(S);
+  const bool whole = N % VEC == 0 && ((uintptr_t)out & 15) == 0;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
-    const int m = m0 + am + 32 * i;
-    if (m >= M) continue;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int n = n0 + (wave >> 1) * 32 * FN + 32 * j + 8 * q + 4 * g;
+        const int c = 32 * j + 8 * q + 4 * g;
+        f32x4 f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (n + e < N) {
-            float v = sum[i][j][4 * q + e];
-            if (bias != nullptr) v += E::to_f(bias[n + e]);
-            out[(int64_t)m * N + n + e] = E::from_f(v);
-          }
-        }
+        for (int e = 0; e < 4; ++e) f[e] = sum[i][j][4 * q + e];
+        if (bias != nullptr) f += *reinterpret_cast<const f32x4*>(add + (wave >> 1) * WN + c);
+        Pack<S, 4> v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v.v[e] = E::from_f(f[e]);
+        *reinterpret_cast<Pack<S, 4>*>(own + r32 * LINE + c * sizeof(S)) = v;
+      }
+    }
+    const int wm0 = m0 + (wave & 1) * 32 * FM + 32 * i;
+    if (whole) {
+      constexpr int PER = WN / VEC, STEPS = 32 * PER / 64;  // lanes a row
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k) {
+        const int r = (k * 64 + lane) / PER, c = (k * 64 + lane) % PER * VEC;
+        const Pack<S, VEC> v = *reinterpret_cast<const Pack<S, VEC>*>(own + r * LINE + c * sizeof(S));
+        if (wm0 + r < M && wn0 + c < N) st<S, VEC>(out + (int64_t)(wm0 + r) * N + wn0 + c, v);
+      }
+    } else {
+#pragma unroll 4
+      for (int k = lane; k < 32 * WN; k += 64) {
+        const int r = k / WN, c = k % WN;
+        const S v = *reinterpret_cast<const S*>(own + r * LINE + c * sizeof(S));
+        if (wm0 + r < M && wn0 + c < N) out[(int64_t)(wm0 + r) * N + wn0 + c] = v;
       }
     }
   }
@@ -373,15 +409,10 @@ static int product(void* out, const uint8_t* a, const uint8_t* as, const uint8_t
   const auto* bi = static_cast<const S*>(bias);
   const int64_t pitch = (int64_t)blocks * 16;
   const int tm = (M + 255) / 256, tn = (N + 255) / 256;
-  if (M > 64 && pitch * 256 < ((int64_t)1 << 32) && (int64_t)tm * tn <= INT32_MAX) {
+  if (M > 64 && N * (int64_t)blocks >= 16 && pitch * 256 < ((int64_t)1 << 32) && (int64_t)tm * tn <= INT32_MAX) {
     const dim3 grid((unsigned)(tm * tn)), block(256);
-    if (blocks % 4 == 0 && aligned(4, as, bs)) {
-      hipLaunchKernelGGL((k_mxfp4_mm_tile<E, true, 4, 4>), grid, block, 0, st, o, a, as, b, bs, bi, M,
-                         N, blocks, tm, tn);
-    } else {
-      hipLaunchKernelGGL((k_mxfp4_mm_tile<E, false, 4, 4>), grid, block, 0, st, o, a, as, b, bs, bi,
-                         M, N, blocks, tm, tn);
-    }
+    hipLaunchKernelGGL((k_mxfp4_mm_tile<E, 4, 4>), grid, block, 0, st, o, a, as, b, bs, bi, M, N,
+                       blocks, tm, tn);
     return check_launch("mxfp4_scaled_mm");
   }
   const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), block(256);
