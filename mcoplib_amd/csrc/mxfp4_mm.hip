@@ -105,8 +105,9 @@ k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 // K ahead of the products.  In 32x32x64 instructions the lane of group g = lane / 32 takes blocks 4g..4g+3
 // of a tile, one a step, so that the scales of its row for the tile are one dword.
 //
-// LDS: a tile's row is 8 chunks of 16 bytes, chunk c at place c ^ (row & 7): the eight lanes that a
-// 16-byte read serves at once then take eight different places.  A direct load writes 64 x 16 bytes in
+// LDS: a tile's row is 8 chunks of 16 bytes, chunk c at place c ^ (row / 2 & 7): two rows span the 64
+// banks, and the sixteen lanes that a 16-byte read serves at once have eight rows of each parity, which
+// then take eight different places (by row & 7 there were conflicts for half of the reads' cycles).  A direct load writes 64 x 16 bytes in
 // lane order (eight rows), so each lane's address is that of the chunk that belongs at its place.
 // Scales go through registers (their rows have any alignment), for two tiles at a time, a row a thread:
 // 16 bytes a row are one request of a line, as four would be.
@@ -146,7 +147,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   constexpr int BM = 64 * FM, BN = 64 * FN, ROWS = BM + BN;
   constexpr int TILE = ROWS * kRowBytes, SCALES = ROWS * 16;
   constexpr int LOADS = ROWS / 8 / 4;  // direct loads of a wave and tile
-  constexpr int SR = (ROWS + 255) / 256;  // rows whose scales a thread reads
+  constexpr int SR = ROWS / 64;  // rows whose scales a thread reads
   __shared__ alignas(1024) uint8_t lds[2 * TILE + 2 * SCALES];
   __shared__ alignas(16) float add[BN];  // the bias
   const int tid = (int)threadIdx.x, lane = tid & 63;
@@ -158,7 +159,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 
   // Rows 0..BM-1 of the LDS tile are a's, the rest b's; a wave's first 2 FM loads of eight rows are of
   // a, the rest of b.  Rows past an operand's end repeat its last.
-  const int chunk = (lane & 7) ^ ((lane >> 3) & 7);
+  auto chunk_of = [&](int j) { return (lane & 7) ^ (lane >> 4) ^ (j & 1) * 4; };  // row / 2 & 7
   auto first_row = [&](int j) {
     return j < 2 * FM ? (wave * 2 * FM + j) * 8 : BM + (wave * 2 * FN + j - 2 * FM) * 8;
   };
@@ -167,7 +168,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   for (int j = 0; j < LOADS; ++j) {
     const int row = first_row(j) + lane / 8;
     const int r = j < 2 * FM ? min(row, M - 1 - m0) : min(row - BM, N - 1 - n0);
-    off[j] = (uint32_t)(r * pitch) + chunk * 16;
+    off[j] = (uint32_t)(r * pitch) + chunk_of(j) * 16;
   }
   const uint8_t* abase = a + m0 * pitch;
   const uint8_t* bbase = b + n0 * pitch;
@@ -175,7 +176,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   // Load j of tile t into buffer `to`.  Chunks past the row's end read the tile's first, and count as
   // zero.
   auto load_rows = [&](int j, int t, int to) {
-    const uint32_t back = chunk < blocks - t * kTileK ? 0 : chunk * 16;
+    const uint32_t back = chunk_of(j) < blocks - t * kTileK ? 0 : chunk_of(j) * 16;
     load_to_lds(lds0 + to * TILE + first_row(j) * kRowBytes,
                 (j < 2 * FM ? abase : bbase) + t * kRowBytes, off[j] - back);
   };
@@ -183,44 +184,47 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) load_rows(j, t, to);
   };
-  // Scales of pair p of tiles: 16 bytes of a row from wherever they start, or the last 16 of all where
-  // those would pass the end, moved and masked when they are stored (looking at them sooner would wait
-  // for them, and for the direct loads around them).
+  // Scales: four pairs of tiles (64 bytes of a row) at a time, four lanes a row, so that a load touches
+  // 16 lines (a row a lane touched 64, and the requests held up the direct loads behind them: 8192 x
+  // 8192 x 8192 bf16 LATER us); put into LDS a pair at a time.  Those of the last pair may pass the row's end,
+  // and the tensor's: they are read before that, moved and masked when they are stored (looking at them
+  // sooner would wait for them, and for the direct loads around them).
   i32x4 sv[SR];
-  auto scale_row = [&](int k, int64_t* past, int p) {
-    const int row = min(tid + 256 * k, ROWS - 1);
-    const bool is_a = row < BM;
-    const int64_t at = (int64_t)(is_a ? min(m0 + row, M - 1) : min(n0 + row - BM, N - 1)) * blocks +
-                       min(p * 16, blocks - 1);
-    const int64_t end = (int64_t)(is_a ? M : N) * blocks - 16;
-    *past = at > end ? at - end : 0;
-    return (is_a ? as : bs) + (at > end ? end : at);
-  };
-  auto load_scales = [&](int p) {
+  const uint8_t* srow[SR];
+  int to_end[SR];  // bytes from the row to the end of its tensor, where those are few
+  const int piece = lane & 3;
+#pragma unroll
+  for (int k = 0; k < SR; ++k) {
+    const int row = tid / 4 + 64 * k;
+    const int r = row < BM ? min(m0 + row, M - 1) : min(n0 + row - BM, N - 1);
+    srow[k] = (row < BM ? as : bs) + (int64_t)r * blocks;
+    to_end[k] = (int)min((int64_t)((row < BM ? M : N) - r) * blocks, (int64_t)1 << 30);
+  }
+  auto load_scales = [&](int p0) {
+    const int at = (p0 + piece) * 16;
 #pragma unroll
     for (int k = 0; k < SR; ++k) {
-      int64_t past;
-      __builtin_memcpy(&sv[k], scale_row(k, &past, p), 16);
+      __builtin_memcpy(&sv[k], srow[k] + min(at, to_end[k] - 16), 16);
     }
   };
   auto store_scales = [&](int p) {
+    if (piece != (p & 3)) return;
+    typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
     const int left = blocks - p * 16;  // bytes of the pair inside a row
 #pragma unroll
     for (int k = 0; k < SR; ++k) {
-      const int row = tid + 256 * k;
-      if (ROWS % 256 != 0 && row >= ROWS) continue;
-      int64_t past;
-      scale_row(k, &past, p);
-      uint64_t lo = (uint64_t)(uint32_t)sv[k][1] << 32 | (uint32_t)sv[k][0];
-      uint64_t hi = (uint64_t)(uint32_t)sv[k][3] << 32 | (uint32_t)sv[k][2];
-      if (past >= 8) lo = hi, hi = 0;
-      const int bits = ((int)past & 7) * 8;
-      lo = lo >> bits | (hi << 1) << (63 - bits);
-      hi >>= bits;
-      if (left < 8) lo &= ((uint64_t)1 << (8 * left)) - 1;
-      if (left < 16) hi &= left <= 8 ? 0 : ((uint64_t)1 << (8 * (left - 8))) - 1;
-      typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
-      *reinterpret_cast<u64x2*>(lds + 2 * TILE + (p & 1) * SCALES + row * 16) = u64x2{lo, hi};
+      u64x2 v = __builtin_bit_cast(u64x2, sv[k]);
+      if (left < 16) {
+        const int past = max(p * 16 - (to_end[k] - 16), 0);
+        uint64_t lo = past >= 8 ? v[1] : v[0], hi = past >= 8 ? 0 : v[1];
+        const int bits = (past & 7) * 8;
+        lo = lo >> bits | (hi << 1) << (63 - bits);
+        hi >>= bits;
+        if (left < 8) lo &= ((uint64_t)1 << (8 * left)) - 1;
+        hi &= left <= 8 ? 0 : ((uint64_t)1 << (8 * (left - 8))) - 1;
+        v = u64x2{lo, hi};
+      }
+      *reinterpret_cast<u64x2*>(lds + 2 * TILE + (p & 1) * SCALES + (tid / 4 + 64 * k) * 16) = v;
     }
   };
 
@@ -230,7 +234,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   int sa[2][FM], sb[2][FN];
   // Operand q of step s: a's first, then b's; and its scales for the tile.
   auto read_codes = [&](int q, int from, int s, int into) {
-    const int place = ((4 * g + s) ^ (r32 & 7)) * 16 + from * TILE;
+    const int place = ((4 * g + s) ^ (r32 >> 1 & 7)) * 16 + from * TILE;
     if (q < FM) {
       fa[into][q] = *reinterpret_cast<const i32x4*>(lds + place + (am + 32 * q) * kRowBytes);
     } else {
@@ -286,6 +290,15 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   if (bias != nullptr) {
     for (int c = tid; c < BN; c += 256) add[c] = E::to_f(bias[min(n0 + c, N - 1)]);
   }
+  // The products so far are made before this point: they touch no memory, and without it the compiler
+  // moves them behind the barrier and the branches below, to where their results are next used.
+  auto here = [&]() {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) asm volatile("" : "+a"(sum[i][j]));
+    }
+  };
   load_scales(0);
   load_tile(0, 0);
   wait_loads();
@@ -305,12 +318,13 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     step(S0(), reading(cur, 1));
     step(S1(), reading(cur, 2));
     step(S2(), reading(cur, 3));
+    here();
     wait_loads();
     if (cur) store_scales((t + 1) / 2);
     wait_lds();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (!cur) load_scales(t / 2 + 1);
+    if ((t & 7) == 6) load_scales(t / 2 + 1);
     __builtin_amdgcn_sched_barrier(0);
     step(S3(), [&](int q) {
 #pragma unroll
@@ -388,7 +402,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
       for (int k = 0; k < STEPS; ++k) {
         const int r = (k * 64 + lane) / PER, c = (k * 64 + lane) % PER * VEC;
         const Pack<S, VEC> v = *reinterpret_cast<const Pack<S, VEC>*>(own + r * LINE + c * sizeof(S));
-        if (wm0 + r < M && wn0 + c < N) st<S, VEC>(out + (int64_t)(wm0 + r) * N + wn0 + c, v);
+        if (wm0 + r < M && wn0 + c < N) st_nt<S, VEC>(out + (int64_t)(wm0 + r) * N + wn0 + c, v);
       }
     } else {
 #pragma unroll 4
