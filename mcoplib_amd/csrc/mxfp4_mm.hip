@@ -3,11 +3,8 @@
 //
 // A scaled matrix instruction takes one block of each operand a lane -- 16 bytes of codes and a byte of
 // a scale register -- and multiplies by both scales as it sums, so codes go from memory to the
-// matrix unit as they are.  Which K a lane's block has is free as long as both operands agree: in
-// 16x16x128 instructions the lane of group g = lane / 16 takes blocks 4g..4g+3 of every 16 (512
-// values), one in each of four instructions, so that its scales are one dword whose bytes the
-// instructions pick in turn.  The weights are the first operand: a lane then holds four consecutive n
-// of one m.
+// matrix unit as they are.  Which K a lane's block has is free as long as both operands agree.  The
+// weights are the first operand: a lane then holds four consecutive n of one m.
 #include <hip/hip_runtime.h>
 
 #include "../../include/mcop_norm.h"
@@ -25,84 +22,173 @@ __device__ __forceinline__ i32x8 fp4_operand(i32x4 v) {
   return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
 }
 
-// Scale bytes b..b+3 of a row of `blocks`, zero past its end (where the codes count as zero as well),
-// by loads that stay inside the row.  DWORDS: `blocks` is a multiple of four, rows aligned to four.
-template <bool DWORDS>
-__device__ __forceinline__ uint32_t scales4(const uint8_t* row, int b, int blocks) {
-  if constexpr (DWORDS) {
-    const uint32_t v = *reinterpret_cast<const uint32_t*>(row + min(b, blocks - 4));
-    return b < blocks ? v : 0u;
+// The 16 (4 KS) scale bytes of a row from block b on, as dwords.  WHOLE: all inside the row; otherwise
+// zero past its end (where the codes count as zero as well), by loads that stay inside it.
+template <int KS, bool WHOLE>
+__device__ __forceinline__ void scale_dwords(uint32_t (&v)[KS], const uint8_t* row, int b,
+                                             int blocks) {
+  if constexpr (WHOLE) {
+    __builtin_memcpy(v, row + b, 4 * KS);
   } else {
-    uint32_t v = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t x = row[min(b + e, blocks - 1)];
-      v |= b + e < blocks ? x << (8 * e) : 0u;
+    for (int s = 0; s < KS; ++s) {
+      v[s] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = row[min(b + 4 * s + e, blocks - 1)];
+        v[s] |= b + 4 * s + e < blocks ? x << (8 * e) : 0u;
+      }
     }
-    return v;
   }
 }
 
-// Few rows: a workgroup makes 16 x 16 of the output, its four waves every fourth chunk of 512 along
-// K, straight from memory; the partial sums meet in LDS in the waves' order.
-template <class E, bool DWORDS>
-__global__ void __launch_bounds__(256)
+// Few rows: a workgroup makes 16 MT rows x 16 NT columns of the output, its W waves every W-th chunk of
+// KS * 128 along K, straight from memory to registers, one chunk ahead; the partial sums meet in LDS
+// and are added in the waves' order.  What bounds it is the weights' way from HBM: each is read by one
+// wave, and the rows of a, which every workgroup reads, come from the caches.
+// In instruction s of a chunk the lane of group g = lane / 16 has block 4 s + g, so that a load takes 64
+// bytes in a row of 16 rows; its scale is byte g of the row's dword s.
+template <class E, int MT, int NT, int W, int KS>
+__global__ void __launch_bounds__(64 * W)
 k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
                 const uint8_t* __restrict__ as, const uint8_t* __restrict__ b,
                 const uint8_t* __restrict__ bs, const typename E::S* __restrict__ bias, int M, int N,
                 int blocks) {
-  __shared__ f32x4 part[3][64];
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  using S = typename E::S;
+  constexpr int T = MT + NT, CHUNK = 4 * KS;  // operands, blocks
+  __shared__ f32x4 part[W][MT * NT][64];
+  const int lane = (int)threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = (int)blockIdx.x * 16, m0 = (int)blockIdx.y * 16;
-  const int64_t n = min(n0 + r, N - 1), m = min(m0 + r, M - 1);
-  const uint8_t* bp = b + n * blocks * 16;
-  const uint8_t* ap = a + m * blocks * 16;
-  const uint8_t* bsp = bs + n * blocks;
-  const uint8_t* asp = as + m * blocks;
-  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int k = wave * 16; k < blocks; k += 64) {
-    const int at = k + 4 * g;
-    const uint32_t sb = scales4<DWORDS>(bsp, at, blocks), sa = scales4<DWORDS>(asp, at, blocks);
-    i32x4 vb[4], va[4];
+  const int n0 = (int)blockIdx.x * 16 * NT, m0 = (int)blockIdx.y * 16 * MT;
+  // rows past an operand's end repeat its last
+  const uint8_t* code_row[T];
+  const uint8_t* scale_row[T];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      vb[s] = i32x4{0, 0, 0, 0}, va[s] = i32x4{0, 0, 0, 0};
-      if (at + s < blocks) {
-        vb[s] = *reinterpret_cast<const i32x4*>(bp + (int64_t)(at + s) * 16);
-        va[s] = *reinterpret_cast<const i32x4*>(ap + (int64_t)(at + s) * 16);
+  for (int o = 0; o < T; ++o) {
+    const int64_t row = o < NT ? min(n0 + 16 * o + r, N - 1) : min(m0 + 16 * (o - NT) + r, M - 1);
+    code_row[o] = (o < NT ? b : a) + (row * blocks + g) * 16;
+    scale_row[o] = (o < NT ? bs : as) + row * blocks;
+  }
+  f32x4 sum[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sum[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  struct Chunk {
+    i32x4 code[T][KS];
+    uint32_t scale[T][KS];
+  };
+  auto load = [&](Chunk& c, int k, auto whole) {  // the chunk from block k on
+    constexpr bool WHOLE = decltype(whole)::value;
+#pragma unroll
+    for (int o = 0; o < T; ++o) {
+      scale_dwords<KS, WHOLE>(c.scale[o], scale_row[o], k, blocks);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int64_t at = (int64_t)(k + 4 * s) * 16;
+        if constexpr (WHOLE) {
+          if (o < NT) {
+            c.code[o][s] = __builtin_nontemporal_load(
+                reinterpret_cast<const i32x4*>(code_row[o] + at));
+          } else {
+            c.code[o][s] = *reinterpret_cast<const i32x4*>(code_row[o] + at);
+          }
+        } else {
+          c.code[o][s] = i32x4{0, 0, 0, 0};
+          if (k + 4 * s + g < blocks) {
+            c.code[o][s] = *reinterpret_cast<const i32x4*>(code_row[o] + at);
+          }
+        }
       }
     }
-#define MCOP_MM(S)                                                                              \
-  sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(vb[S]), fp4_operand(va[S]), \
-                                                         sum, kFp4, kFp4, S, (int)sb, S, (int)sa)
-    MCOP_MM(0);
-    MCOP_MM(1);
-    MCOP_MM(2);
-    MCOP_MM(3);
-#undef MCOP_MM
+  };
+  auto multiply = [&](const Chunk& c) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      int sc[T];
+#pragma unroll
+      for (int o = 0; o < T; ++o) sc[o] = (int)(c.scale[o][s] >> (8 * g));
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+          sum[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              fp4_operand(c.code[i][s]), fp4_operand(c.code[NT + j][s]), sum[i][j], kFp4, kFp4, 0,
+              sc[i], 0, sc[NT + j]);
+        }
+      }
+    }
+  };
+  const int whole = blocks / CHUNK;
+  Chunk even, odd;
+  int c = wave;
+  // The order is kept as written: a chunk's loads all go out before the products of the one before (the
+  // compiler would put each next to its use, and wait for it there).
+  auto apart = []() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+  };
+  if (c < whole) {
+    load(even, c * CHUNK, std::true_type());
+    while (true) {
+      load(odd, min(c + W, whole - 1) * CHUNK, std::true_type());
+      apart();
+      multiply(even);
+      apart();
+      if ((c += W) >= whole) break;
+      load(even, min(c + W, whole - 1) * CHUNK, std::true_type());
+      apart();
+      multiply(odd);
+      apart();
+      if ((c += W) >= whole) break;
+    }
   }
-  if (wave > 0) part[wave - 1][lane] = sum;
+  if (whole * CHUNK < blocks && wave == whole % W) {  // what is left of the rows
+    load(even, whole * CHUNK, std::false_type());
+    multiply(even);
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+#pragma unroll
+    for (int j = 0; j < MT; ++j) part[wave][i * MT + j][lane] = sum[i][j];
+  }
   __syncthreads();
-  if (wave > 0) return;
+  // four n of one m a thread
+  const bool quads = N % 4 == 0 && ((uintptr_t)out & (4 * sizeof(S) - 1)) == 0;
 #pragma unroll
-  for (int w = 0; w < 3; ++w) sum += part[w][lane];
-  if (m0 + r >= M) return;
+  for (int e0 = 0; e0 < MT * NT * 64; e0 += 64 * W) {
+    const int e = e0 + (int)threadIdx.x;
+    if (MT * NT % W != 0 && e >= MT * NT * 64) break;
+    const int tile = e >> 6, l = e & 63;
+    f32x4 v = part[0][tile][l];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = n0 + 4 * g + i;
-    if (c < N) {
-      float v = sum[i];
-      if (bias != nullptr) v += E::to_f(bias[c]);
-      out[(int64_t)(m0 + r) * N + c] = E::from_f(v);
+    for (int w = 1; w < W; ++w) v += part[w][tile][l];
+    const int m = m0 + tile % MT * 16 + (l & 15), n = n0 + tile / MT * 16 + (l >> 4) * 4;
+    if (m >= M || n >= N) continue;
+    Pack<S, 4> o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (bias != nullptr) v[i] += E::to_f(bias[min(n + i, N - 1)]);
+      o.v[i] = E::from_f(v[i]);
+    }
+    S* p = out + (int64_t)m * N + n;
+    if (quads) {
+      st<S, 4>(p, o);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (n + i < N) p[i] = o.v[i];
+      }
     }
   }
 }
 
 // Many rows: a workgroup of four waves (2 x 2) makes a (64 FM) x (64 FN) tile, each wave FM x FN
 // products of 32 x 32.  Codes go from memory to LDS in tiles of 256 along K (128 bytes a row), two
-// tiles in turn, without passing through registers; from there to the matrix units a step of 64 along
-// K ahead of the products.  In 32x32x64 instructions the lane of group g = lane / 32 takes blocks 4g..4g+3
+// or more tiles in turn, without passing through registers; from there to registers three steps of 64
+// along K ahead of the products.  In 32x32x64 instructions the lane of group g = lane / 32 takes blocks 4g..4g+3
 // of a tile, one a step, so that the scales of its row for the tile are one dword.
 //
 // LDS: a tile's row is 8 chunks of 16 bytes, chunk c at place c ^ (row / 2 & 7): two rows span the 64
@@ -112,9 +198,9 @@ k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 // Scales go through registers (their rows have any alignment), for two tiles at a time, a row a thread:
 // 16 bytes a row are one request of a line, as four would be.
 //
-// One barrier a tile: before the last step's products, whose operands are in registers by then, the
-// wave waits for its part of the next tile, meets the others, reads the next tile's first operands and
-// starts the loads of the tile after it, into the tile that all have finished reading.
+// One barrier a tile, after the first step's products: the tile's last operands are in registers by
+// then, the wave waits for its part of the next tile, meets the others, reads on from the next tile and
+// starts the loads of a later one, into the tile that all have finished reading.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTileK = 8;     // blocks
@@ -131,14 +217,15 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, const uint8_t* base, ui
       : "s"(to), "v"(off), "s"(base)
       : "memory", "m0");
 }
+template <int N>  // at most N of the wave's requests are outstanding: the newest
 __device__ __forceinline__ void wait_loads() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void wait_lds() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-template <class E, int FM, int FN>
+template <class E, int FM, int FN, int NBUF, int LPR>
 __global__ void __launch_bounds__(256, 1)
 k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
                 const uint8_t* __restrict__ as, const uint8_t* __restrict__ b,
@@ -147,8 +234,9 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   constexpr int BM = 64 * FM, BN = 64 * FN, ROWS = BM + BN;
   constexpr int TILE = ROWS * kRowBytes, SCALES = ROWS * 16;
   constexpr int LOADS = ROWS / 8 / 4;  // direct loads of a wave and tile
-  constexpr int SR = ROWS / 64;  // rows whose scales a thread reads
-  __shared__ alignas(1024) uint8_t lds[2 * TILE + 2 * SCALES];
+  constexpr int SR = ROWS * LPR / 256;  // scale pieces of a thread
+  constexpr int SCALES0 = NBUF * TILE;
+  __shared__ alignas(1024) uint8_t lds[NBUF * TILE + 2 * SCALES];
   __shared__ alignas(16) float add[BN];  // the bias
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -192,10 +280,10 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   i32x4 sv[SR];
   const uint8_t* srow[SR];
   int to_end[SR];  // bytes from the row to the end of its tensor, where those are few
-  const int piece = lane & 3;
+  const int piece = lane & (LPR - 1);
 #pragma unroll
   for (int k = 0; k < SR; ++k) {
-    const int row = tid / 4 + 64 * k;
+    const int row = (tid + 256 * k) / LPR;
     const int r = row < BM ? min(m0 + row, M - 1) : min(n0 + row - BM, N - 1);
     srow[k] = (row < BM ? as : bs) + (int64_t)r * blocks;
     to_end[k] = (int)min((int64_t)((row < BM ? M : N) - r) * blocks, (int64_t)1 << 30);
@@ -208,7 +296,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     }
   };
   auto store_scales = [&](int p) {
-    if (piece != (p & 3)) return;
+    if (piece != (p & (LPR - 1))) return;
     typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
     const int left = blocks - p * 16;  // bytes of the pair inside a row
 #pragma unroll
@@ -224,26 +312,26 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
         hi &= left <= 8 ? 0 : ((uint64_t)1 << (8 * (left - 8))) - 1;
         v = u64x2{lo, hi};
       }
-      *reinterpret_cast<u64x2*>(lds + 2 * TILE + (p & 1) * SCALES + (tid / 4 + 64 * k) * 16) = v;
+      *reinterpret_cast<u64x2*>(lds + SCALES0 + (p & 1) * SCALES + (tid + 256 * k) / LPR * 16) = v;
     }
   };
 
   const int r32 = lane & 31, g = lane >> 5;
   const int am = (wave & 1) * 32 * FM + r32, bn = BM + (wave >> 1) * 32 * FN + r32;
-  i32x4 fa[2][FM], fb[2][FN];
+  i32x4 fa[4][FM], fb[4][FN];
   int sa[2][FM], sb[2][FN];
   // Operand q of step s: a's first, then b's; and its scales for the tile.
-  auto read_codes = [&](int q, int from, int s, int into) {
+  auto read_codes = [&](int q, int from, int s) {
     const int place = ((4 * g + s) ^ (r32 >> 1 & 7)) * 16 + from * TILE;
     if (q < FM) {
-      fa[into][q] = *reinterpret_cast<const i32x4*>(lds + place + (am + 32 * q) * kRowBytes);
+      fa[s][q] = *reinterpret_cast<const i32x4*>(lds + place + (am + 32 * q) * kRowBytes);
     } else {
-      fb[into][q - FM] =
+      fb[s][q - FM] =
           *reinterpret_cast<const i32x4*>(lds + place + (bn + 32 * (q - FM)) * kRowBytes);
     }
   };
   auto read_scales = [&](int q, int t, int into) {
-    const int place = 2 * TILE + (t >> 1 & 1) * SCALES + (t & 1) * 8 + 4 * g;
+    const int place = SCALES0 + (t >> 1 & 1) * SCALES + (t & 1) * 8 + 4 * g;
     if (q < FM) {
       sa[into][q] = *reinterpret_cast<const int*>(lds + place + (am + 32 * q) * 16);
     } else {
@@ -267,7 +355,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     for (int q = 0; q < FM * FN; ++q) {
       const int i = q / FN, j = q % FN;
       sum[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-          fp4_operand(fb[S & 1][j]), fp4_operand(fa[S & 1][i]), sum[i][j], kFp4, kFp4, S, sb[0][j], S,
+          fp4_operand(fb[S][j]), fp4_operand(fa[S][i]), sum[i][j], kFp4, kFp4, S, sb[0][j], S,
           sa[0][i]);
       other(q);
       __builtin_amdgcn_sched_barrier(0);
@@ -278,18 +366,13 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   using S2 = std::integral_constant<int, 2>;
   using S3 = std::integral_constant<int, 3>;
   constexpr int OPS = FM + FN, MMS = FM * FN;
-  auto reading = [&](int from, int s) {  // the operands of step s, from the first products on
-    return [&, from, s](int q) {
+  auto reading = [&](int q, int from, int s) {  // the operands of step s, from the first products on
 #pragma unroll
-      for (int o = 0; o < OPS; ++o) {
-        if (o * MMS / 2 / OPS == q) read_codes(o, from, s, s & 1);
-      }
-    };
+    for (int o = 0; o < OPS; ++o) {
+      if (o * MMS / 2 / OPS == q) read_codes(o, from, s);
+    }
   };
 
-  if (bias != nullptr) {
-    for (int c = tid; c < BN; c += 256) add[c] = E::to_f(bias[min(n0 + c, N - 1)]);
-  }
   // The products so far are made before this point: they touch no memory, and without it the compiler
   // moves them behind the barrier and the branches below, to where their results are next used.
   auto here = [&]() {
@@ -299,50 +382,75 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
       for (int j = 0; j < FN; ++j) asm volatile("" : "+a"(sum[i][j]));
     }
   };
+  auto have_scales = [&]() {  // waits for them here and not later, when other loads are in flight
+#pragma unroll
+    for (int k = 0; k < SR; ++k) asm volatile("" : "+v"(sv[k]));
+  };
+  if (bias != nullptr) {
+    for (int c = tid; c < BN; c += 256) add[c] = E::to_f(bias[min(n0 + c, N - 1)]);
+  }
   load_scales(0);
-  load_tile(0, 0);
-  wait_loads();
+#pragma unroll
+  for (int u = 0; u < NBUF; ++u) load_tile(min(u, last), u);
+  have_scales();
   store_scales(0);
-  load_tile(min(1, last), 1);
+  wait_loads<(NBUF - 1) * LOADS>();
   wait_lds();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
   for (int o = 0; o < OPS; ++o) {
-    read_codes(o, 0, 0, 0);
+    read_codes(o, 0, 0);
     read_scales(o, 0, 0);
   }
+#pragma unroll
+  for (int u = 1; u < 3; ++u) {
+#pragma unroll
+    for (int o = 0; o < OPS; ++o) read_codes(o, 0, u);
+  }
+  int cur = 0;
   for (int t = 0; t < last; ++t) {
-    const int cur = t & 1, then = min(t + 2, last);
+    const int then = min(t + NBUF, last), next = cur + 1 == NBUF ? 0 : cur + 1;
     __builtin_amdgcn_sched_barrier(0);
-    step(S0(), reading(cur, 1));
-    step(S1(), reading(cur, 2));
-    step(S2(), reading(cur, 3));
+    step(S0(), [&](int q) { reading(q, cur, 3); });
     here();
-    wait_loads();
-    if (cur) store_scales((t + 1) / 2);
+    if (t & 1) store_scales((t + 1) / 2);
+    wait_loads<(NBUF - 2) * LOADS>();
+    if constexpr (NBUF == 2) have_scales();
     wait_lds();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if ((t & 7) == 6) load_scales(t / 2 + 1);
+    if ((t & 1) != 0 && ((t + 3) / 2) % LPR == 0) {
+      load_scales((t + 3) / 2);
+      if constexpr (NBUF > 2) have_scales();
+    }
     __builtin_amdgcn_sched_barrier(0);
-    step(S3(), [&](int q) {
-#pragma unroll
-      for (int o = 0; o < OPS; ++o) {
-        if (o * MMS / 2 / OPS == q) {
-          read_codes(o, cur ^ 1, 0, 0);
-          read_scales(o, t + 1, 1);
-        }
-      }
+    auto loading = [&](int q, int s) {  // the tile after those that are held, over steps 1 and 2
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
-        if (j * MMS / LOADS == q) load_rows(j, then, cur);
+        if (j * 2 * MMS / LOADS == q + s * MMS) load_rows(j, then, cur);
+      }
+    };
+    step(S1(), [&](int q) {
+      reading(q, next, 0);
+      loading(q, 0);
+    });
+    step(S2(), [&](int q) {
+      reading(q, next, 1);
+      loading(q, 1);
+    });
+    step(S3(), [&](int q) {
+      reading(q, next, 2);
+#pragma unroll
+      for (int o = 0; o < OPS; ++o) {
+        if (o * MMS / 2 / OPS == q) read_scales(o, t + 1, 1);
       }
     });
 #pragma unroll
     for (int i = 0; i < FM; ++i) sa[0][i] = sa[1][i];
 #pragma unroll
     for (int i = 0; i < FN; ++i) sb[0][i] = sb[1][i];
+    cur = next;
   }
   {  // the last tile, whose blocks past the rows' end count as zero: a's codes here, the scales above
     auto mask = [&](int s) {
@@ -350,20 +458,21 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) fa[s & 1][i][e] = in ? fa[s & 1][i][e] : 0;
+        for (int e = 0; e < 4; ++e) fa[s][i][e] = in ? fa[s][i][e] : 0;
       }
     };
-    const int cur = last & 1;
+#pragma unroll
+    for (int o = 0; o < OPS; ++o) read_codes(o, cur, 3);
     mask(0);
-    step(S0(), reading(cur, 1));
+    step(S0(), [](int) {});
     mask(1);
-    step(S1(), reading(cur, 2));
+    step(S1(), [](int) {});
     mask(2);
-    step(S2(), reading(cur, 3));
+    step(S2(), [](int) {});
     mask(3);
     step(S3(), [](int) {});
   }
-  wait_loads();  // the loads past the last tile: none may arrive after the workgroup's LDS is given on
+  wait_loads<0>();  // the loads past the last tile: none may arrive after the workgroup's LDS is given on
 
   // A lane holds n = 8 (e / 4) + 4 g + e % 4 of m = lane % 32 of each product: 8 or 16 bytes in a row.
   // Each wave turns 32 rows at a time in LDS of its own and stores them 16 bytes a lane, whole lines in
@@ -371,7 +480,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   // 8192 bf16).
   using S = typename E::S;
   constexpr int WN = 32 * FN, LINE = WN * (int)sizeof(S) + 16;  // 16: rows start in other banks
-  static_assert(4 * 32 * LINE <= 2 * TILE, "the waves' rows fit the tiles");
+  static_assert(4 * 32 * LINE <= NBUF * TILE, "the waves' rows fit the tiles");
   __builtin_amdgcn_s_barrier();  // every wave has read its last operands
   asm volatile("" ::: "memory");
   uint8_t* own = lds + wave * 32 * LINE;
@@ -415,28 +524,47 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   }
 }
 
+static int64_t tiles_of(int M, int N, int bm, int bn) {
+  return (int64_t)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+}
+
+// Whether the tile kernel's 32-bit offsets and its reads of 16 scale bytes fit the operands.
+static bool tiles_fit(int M, int N, int blocks) {
+  return (int64_t)blocks * 16 * 256 < ((int64_t)1 << 32) && (int64_t)M * blocks >= 16 &&
+         (int64_t)N * blocks >= 16 && tiles_of(M, N, 64, 64) <= INT32_MAX;
+}
+
+template <class E, int FM, int FN, int NBUF, int LPR>
+static int product_tiles(typename E::S* out, const uint8_t* a, const uint8_t* as, const uint8_t* b,
+                         const uint8_t* bs, const typename E::S* bias, int M, int N, int blocks,
+                         hipStream_t st) {
+  const int tm = (M + 64 * FM - 1) / (64 * FM), tn = (N + 64 * FN - 1) / (64 * FN);
+  hipLaunchKernelGGL((k_mxfp4_mm_tile<E, FM, FN, NBUF, LPR>), dim3((unsigned)(tm * tn)), dim3(256), 0, st, out,
+                     a, as, b, bs, bias, M, N, blocks, tm, tn);
+  return check_launch("mxfp4_scaled_mm");
+}
+
 template <class E>
 static int product(void* out, const uint8_t* a, const uint8_t* as, const uint8_t* b,
                    const uint8_t* bs, const void* bias, int M, int N, int blocks, hipStream_t st) {
   using S = typename E::S;
   auto* o = static_cast<S*>(out);
   const auto* bi = static_cast<const S*>(bias);
-  const int64_t pitch = (int64_t)blocks * 16;
-  const int tm = (M + 255) / 256, tn = (N + 255) / 256;
-  if (M > 64 && N * (int64_t)blocks >= 16 && pitch * 256 < ((int64_t)1 << 32) && (int64_t)tm * tn <= INT32_MAX) {
-    const dim3 grid((unsigned)(tm * tn)), block(256);
-    hipLaunchKernelGGL((k_mxfp4_mm_tile<E, 4, 4>), grid, block, 0, st, o, a, as, b, bs, bi, M, N,
-                       blocks, tm, tn);
-    return check_launch("mxfp4_scaled_mm");
+  if (tiles_fit(M, N, blocks)) {
+    if (M > 128 && tiles_of(M, N, 256, 256) >= 192) {
+      return product_tiles<E, 4, 4, 2, 4>(o, a, as, b, bs, bi, M, N, blocks, st);
+    }
+    if (M > 64) return product_tiles<E, 2, 2, 4, 16>(o, a, as, b, bs, bi, M, N, blocks, st);
   }
-  const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), block(256);
-  if (blocks % 4 == 0 && aligned(4, as, bs)) {
-    hipLaunchKernelGGL((k_mxfp4_mm_rows<E, true>), grid, block, 0, st, o, a, as, b, bs, bi, M, N,
-                       blocks);
-  } else {
-    hipLaunchKernelGGL((k_mxfp4_mm_rows<E, false>), grid, block, 0, st, o, a, as, b, bs, bi, M, N,
-                       blocks);
-  }
+#define MCOP_ROWS(MT, NT, W, KS)                                                               \
+  hipLaunchKernelGGL((k_mxfp4_mm_rows<E, MT, NT, W, KS>),                                      \
+                     dim3((unsigned)((N + 16 * NT - 1) / (16 * NT)),                           \
+                          (unsigned)((M + 16 * MT - 1) / (16 * MT))),                          \
+                     dim3(64 * W), 0, st, o, a, as, b, bs, bi, M, N, blocks)
+  if (M <= 16) MCOP_ROWS(1, 1, 4, 4);
+  else if (M <= 32) MCOP_ROWS(2, 2, 4, 2);
+  else MCOP_ROWS(4, 2, 4, 2);
+#undef MCOP_ROWS
   return check_launch("mxfp4_scaled_mm");
 }
 
