@@ -185,26 +185,31 @@ k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   }
 }
 
-// Many rows: a workgroup of four waves (2 x 2) makes a (64 FM) x (64 FN) tile, each wave FM x FN
-// products of 32 x 32.  Codes go from memory to LDS in tiles of 256 along K (128 bytes a row), two
-// or more tiles in turn, without passing through registers; from there to registers three steps of 64
-// along K ahead of the products.  In 32x32x64 instructions the lane of group g = lane / 32 takes blocks 4g..4g+3
-// of a tile, one a step, so that the scales of its row for the tile are one dword.
+// Many rows: a group of WD x WD waves makes a (32 WD FM) x (32 WD FN) tile of the output, each wave
+// FM x FN products of 32 x 32; KS such groups of a workgroup share out K and add up in LDS at the end.  Codes go from
+// memory to LDS in tiles of 256 along K (128 bytes a row: whole lines), two tiles in turn, without
+// passing through registers; from there to registers three steps of 64 along K ahead of the products.
+// In 32x32x64 instructions the lane of group g = lane / 32 takes blocks 4g..4g+3 of a tile, one a step, so
+// that the scales of its row for the tile are one dword, whose bytes the instructions pick in turn.
 //
 // LDS: a tile's row is 8 chunks of 16 bytes, chunk c at place c ^ (row / 2 & 7): two rows span the 64
 // banks, and the sixteen lanes that a 16-byte read serves at once have eight rows of each parity, which
-// then take eight different places (by row & 7 there were conflicts for half of the reads' cycles).  A direct load writes 64 x 16 bytes in
-// lane order (eight rows), so each lane's address is that of the chunk that belongs at its place.
-// Scales go through registers (their rows have any alignment), for two tiles at a time, a row a thread:
-// 16 bytes a row are one request of a line, as four would be.
+// then take eight different places (by row & 7 there were conflicts for half of the reads' cycles).  A
+// direct load writes 64 x 16 bytes in lane order (eight rows), so each lane's address is that of the
+// chunk that belongs at its place.
 //
-// One barrier a tile, after the first step's products: the tile's last operands are in registers by
+// One barrier a tile (none for a group of one wave), after the first step's products: the tile's last operands are in registers by
 // then, the wave waits for its part of the next tile, meets the others, reads on from the next tile and
-// starts the loads of a later one, into the tile that all have finished reading.
+// starts the loads of the one after it, into the tile that all have finished reading.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kTileK = 8;     // blocks
-constexpr int kRowBytes = 128;
+constexpr int kTileK = 8;  // blocks
+constexpr int kRowBytes = kTileK * 16;
+// Tiles whose scales (32 bytes of a row) are read and put into LDS together, two lanes a row: a lane a
+// row with 16 bytes touches a line for each lane, and those requests hold up the direct loads behind
+// them; more at a time do not leave the room for two tiles of 256 x 256.
+constexpr int kScaleTiles = 4, kScaleBytes = kScaleTiles * kTileK;
 
 // 16 bytes a lane from base + off to LDS at `to` + 16 * lane.  The compiler does not see what this
 // writes nor that it is in flight: wait_loads() and the barrier order it.
@@ -217,125 +222,141 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, const uint8_t* base, ui
       : "s"(to), "v"(off), "s"(base)
       : "memory", "m0");
 }
-template <int N>  // at most N of the wave's requests are outstanding: the newest
 __device__ __forceinline__ void wait_loads() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 __device__ __forceinline__ void wait_lds() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
+__device__ __forceinline__ void meet() {
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
-template <class E, int FM, int FN, int NBUF, int LPR>
-__global__ void __launch_bounds__(256, 1)
+template <class E, int FM, int FN, int WD, int KS>
+__global__ void __launch_bounds__(64 * WD * WD * KS, 1)
 k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
                 const uint8_t* __restrict__ as, const uint8_t* __restrict__ b,
                 const uint8_t* __restrict__ bs, const typename E::S* __restrict__ bias, int M, int N,
-                int blocks, int tiles_m, int tiles_n) {
-  constexpr int BM = 64 * FM, BN = 64 * FN, ROWS = BM + BN;
-  constexpr int TILE = ROWS * kRowBytes, SCALES = ROWS * 16;
-  constexpr int LOADS = ROWS / 8 / 4;  // direct loads of a wave and tile
-  constexpr int SR = ROWS * LPR / 256;  // scale pieces of a thread
-  constexpr int SCALES0 = NBUF * TILE;
-  __shared__ alignas(1024) uint8_t lds[NBUF * TILE + 2 * SCALES];
-  __shared__ alignas(16) float add[BN];  // the bias
-  const int tid = (int)threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int tile_m = (int)blockIdx.x % tiles_m, tile_n = (int)blockIdx.x / tiles_m;
-  const int m0 = tile_m * BM, n0 = tile_n * BN;
+                int blocks, int tiles_m, int tiles) {
+  using S = typename E::S;
+  constexpr int GW = WD * WD, THREADS = 64 * GW * KS;  // waves of a group
+  constexpr int BM = 32 * WD * FM, BN = 32 * WD * FN, ROWS = BM + BN;
+  constexpr int TILE = ROWS * kRowBytes, SCALES = ROWS * kScaleBytes;
+  constexpr int GROUP = 2 * (TILE + SCALES);  // LDS of a group
+  constexpr int ALOADS = BM / 8 / GW, LOADS = ROWS / 8 / GW;  // direct loads of a wave and tile
+  constexpr int SR = ROWS * 2 / (64 * GW);                    // 16-byte scale pieces of a thread
+  __shared__ alignas(1024) uint8_t lds_all[KS * GROUP];
+  const int lane = (int)threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) & (GW - 1);  // of its group
+  const int part = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) / GW;        // the group
+  const int tid = (int)threadIdx.x & (64 * GW - 1);
+  const int wm = wave % WD, wn = wave / WD;
+  uint8_t* lds = lds_all + part * GROUP;
+  const int m0 = (int)blockIdx.x % tiles_m * BM, n0 = (int)blockIdx.x / tiles_m * BN;
   const int64_t pitch = (int64_t)blocks * 16;
-  const int last = (blocks - 1) / kTileK;
 
-  // Rows 0..BM-1 of the LDS tile are a's, the rest b's; a wave's first 2 FM loads of eight rows are of
-  // a, the rest of b.  Rows past an operand's end repeat its last.
+  // The group's tiles: `tiles` from block `from` on, which may pass the rows' end.  What is past it
+  // counts as zero by its scales: 0 stands for 2^-127, and with that of both operands every product
+  // is below binary32's range.  Its codes are read from the group's last tile, or the rows' first.
+  const int start = part * tiles * kTileK;
+  const int from = start < blocks ? start : 0, have = start < blocks ? blocks - start : 0;
+  const int last_full = max(have - 1, 0) / kTileK;
+
+  // Rows 0..BM-1 of the LDS tile are a's, the rest b's; a wave's first loads of eight rows are of a, the
+  // rest of b.  Rows past an operand's end repeat its last.
   auto chunk_of = [&](int j) { return (lane & 7) ^ (lane >> 4) ^ (j & 1) * 4; };  // row / 2 & 7
   auto first_row = [&](int j) {
-    return j < 2 * FM ? (wave * 2 * FM + j) * 8 : BM + (wave * 2 * FN + j - 2 * FM) * 8;
+    return j < ALOADS ? (wave * ALOADS + j) * 8
+                      : BM + (wave * (LOADS - ALOADS) + j - ALOADS) * 8;
   };
   uint32_t off[LOADS];
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) {
     const int row = first_row(j) + lane / 8;
-    const int r = j < 2 * FM ? min(row, M - 1 - m0) : min(row - BM, N - 1 - n0);
+    const int r = j < ALOADS ? min(row, M - 1 - m0) : min(row - BM, N - 1 - n0);
     off[j] = (uint32_t)(r * pitch) + chunk_of(j) * 16;
   }
-  const uint8_t* abase = a + m0 * pitch;
-  const uint8_t* bbase = b + n0 * pitch;
+  const uint8_t* abase = a + m0 * pitch + (int64_t)from * 16;
+  const uint8_t* bbase = b + n0 * pitch + (int64_t)from * 16;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  // Load j of tile t into buffer `to`.  Chunks past the row's end read the tile's first, and count as
-  // zero.
+  // Load j of tile t into buffer `to`.  Chunks past the row's end read the tile's first.
   auto load_rows = [&](int j, int t, int to) {
-    const uint32_t back = chunk_of(j) < blocks - t * kTileK ? 0 : chunk_of(j) * 16;
+    const int u = min(t, last_full), c = chunk_of(j);
+    const uint32_t back = c < blocks - from - u * kTileK ? 0 : c * 16;
     load_to_lds(lds0 + to * TILE + first_row(j) * kRowBytes,
-                (j < 2 * FM ? abase : bbase) + t * kRowBytes, off[j] - back);
+                (j < ALOADS ? abase : bbase) + u * kRowBytes, off[j] - back);
   };
-  auto load_tile = [&](int t, int to) {
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) load_rows(j, t, to);
-  };
-  // Scales: four pairs of tiles (64 bytes of a row) at a time, four lanes a row, so that a load touches
-  // 16 lines (a row a lane touched 64, and the requests held up the direct loads behind them: 8192 x
-  // 8192 x 8192 bf16 LATER us); put into LDS a pair at a time.  Those of the last pair may pass the row's end,
-  // and the tensor's: they are read before that, moved and masked when they are stored (looking at them
-  // sooner would wait for them, and for the direct loads around them).
+
+  // Scales of tiles 4 s to 4 s + 3: two lanes a row, 16 bytes each.  Those of the row's end may pass it,
+  // and the tensor's: they are read before that, moved and masked when they are stored (looking at
+  // them sooner would wait for them, and for the direct loads around them).
   i32x4 sv[SR];
   const uint8_t* srow[SR];
-  int to_end[SR];  // bytes from the row to the end of its tensor, where those are few
-  const int piece = lane & (LPR - 1);
+  int to_end[SR];  // bytes from `from` in the row to the end of its tensor, where those are few
+  const int piece = (lane & 1) * 16;
 #pragma unroll
   for (int k = 0; k < SR; ++k) {
-    const int row = (tid + 256 * k) / LPR;
+    const int row = tid / 2 + 32 * GW * k;
     const int r = row < BM ? min(m0 + row, M - 1) : min(n0 + row - BM, N - 1);
-    srow[k] = (row < BM ? as : bs) + (int64_t)r * blocks;
-    to_end[k] = (int)min((int64_t)((row < BM ? M : N) - r) * blocks, (int64_t)1 << 30);
+    srow[k] = (row < BM ? as : bs) + (int64_t)r * blocks + from;
+    to_end[k] =
+        (int)min((int64_t)((row < BM ? M : N) - r) * blocks - from, (int64_t)1 << 30);
   }
-  auto load_scales = [&](int p0) {
-    const int at = (p0 + piece) * 16;
+  auto load_scales = [&](int s) {
+    const int at = s * kScaleBytes + piece;
 #pragma unroll
     for (int k = 0; k < SR; ++k) {
       __builtin_memcpy(&sv[k], srow[k] + min(at, to_end[k] - 16), 16);
     }
   };
-  auto store_scales = [&](int p) {
-    if (piece != (p & (LPR - 1))) return;
-    typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
-    const int left = blocks - p * 16;  // bytes of the pair inside a row
+  auto store_scales = [&](int s) {
+    if (have - s * kScaleBytes < kScaleBytes) {
+      const int at = s * kScaleBytes + piece, left = min(max(have - at, 0), 16);
 #pragma unroll
-    for (int k = 0; k < SR; ++k) {
-      u64x2 v = __builtin_bit_cast(u64x2, sv[k]);
-      if (left < 16) {
-        const int past = max(p * 16 - (to_end[k] - 16), 0);
+      for (int k = 0; k < SR; ++k) {
+        const int past = max(at - (to_end[k] - 16), 0);
+        const u64x2 v = __builtin_bit_cast(u64x2, sv[k]);
         uint64_t lo = past >= 8 ? v[1] : v[0], hi = past >= 8 ? 0 : v[1];
         const int bits = (past & 7) * 8;
         lo = lo >> bits | (hi << 1) << (63 - bits);
         hi >>= bits;
         if (left < 8) lo &= ((uint64_t)1 << (8 * left)) - 1;
-        hi &= left <= 8 ? 0 : ((uint64_t)1 << (8 * (left - 8))) - 1;
-        v = u64x2{lo, hi};
+        if (left < 16) hi &= left <= 8 ? 0 : ((uint64_t)1 << (8 * (left - 8))) - 1;
+        sv[k] = __builtin_bit_cast(i32x4, u64x2{lo, hi});
       }
-      *reinterpret_cast<u64x2*>(lds + SCALES0 + (p & 1) * SCALES + (tid + 256 * k) / LPR * 16) = v;
     }
+    uint8_t* to = lds + 2 * TILE + (s & 1) * SCALES + tid * 16;
+#pragma unroll
+    for (int k = 0; k < SR; ++k) *reinterpret_cast<i32x4*>(to + k * 1024 * GW) = sv[k];
+  };
+  auto have_scales = [&]() {  // waits for them here and not later, when other loads are in flight
+#pragma unroll
+    for (int k = 0; k < SR; ++k) asm volatile("" : "+v"(sv[k]));
   };
 
   const int r32 = lane & 31, g = lane >> 5;
-  const int am = (wave & 1) * 32 * FM + r32, bn = BM + (wave >> 1) * 32 * FN + r32;
+  const int am = wm * 32 * FM + r32, bn = BM + wn * 32 * FN + r32;
   i32x4 fa[4][FM], fb[4][FN];
   int sa[2][FM], sb[2][FN];
-  // Operand q of step s: a's first, then b's; and its scales for the tile.
-  auto read_codes = [&](int q, int from, int s) {
-    const int place = ((4 * g + s) ^ (r32 >> 1 & 7)) * 16 + from * TILE;
-    if (q < FM) {
-      fa[s][q] = *reinterpret_cast<const i32x4*>(lds + place + (am + 32 * q) * kRowBytes);
+  constexpr int OPS = FM + FN, MMS = FM * FN, LSTEPS = 3;
+  // Operand o of step s: a's first, then b's; and its scales for the tile.
+  auto read_codes = [&](int o, int buf, int s) {
+    const int place = ((4 * g + s) ^ (r32 >> 1 & 7)) * 16 + buf * TILE;
+    if (o < FM) {
+      fa[s][o] = *reinterpret_cast<const i32x4*>(lds + place + (am + 32 * o) * kRowBytes);
     } else {
-      fb[s][q - FM] =
-          *reinterpret_cast<const i32x4*>(lds + place + (bn + 32 * (q - FM)) * kRowBytes);
+      fb[s][o - FM] =
+          *reinterpret_cast<const i32x4*>(lds + place + (bn + 32 * (o - FM)) * kRowBytes);
     }
   };
-  auto read_scales = [&](int q, int t, int into) {
-    const int place = SCALES0 + (t >> 1 & 1) * SCALES + (t & 1) * 8 + 4 * g;
-    if (q < FM) {
-      sa[into][q] = *reinterpret_cast<const int*>(lds + place + (am + 32 * q) * 16);
+  auto read_scales = [&](int o, int t, int into) {
+    const int place = 2 * TILE + (t / kScaleTiles & 1) * SCALES + t % kScaleTiles * kTileK + 4 * g;
+    if (o < FM) {
+      sa[into][o] = *reinterpret_cast<const int*>(lds + place + (am + 32 * o) * kScaleBytes);
     } else {
-      sb[into][q - FM] = *reinterpret_cast<const int*>(lds + place + (bn + 32 * (q - FM)) * 16);
+      sb[into][o - FM] =
+          *reinterpret_cast<const int*>(lds + place + (bn + 32 * (o - FM)) * kScaleBytes);
     }
   };
   f32x16 sum[FM][FN];
@@ -350,12 +371,12 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   // The products of step s, with `other(q)` issued behind the q-th: the order is kept as written, so
   // that reads and loads go out between products, each in the time one takes.
   auto step = [&](auto s, auto other) {
-    constexpr int S = decltype(s)::value;
+    constexpr int ST = decltype(s)::value;
 #pragma unroll
-    for (int q = 0; q < FM * FN; ++q) {
+    for (int q = 0; q < MMS; ++q) {
       const int i = q / FN, j = q % FN;
       sum[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-          fp4_operand(fb[S][j]), fp4_operand(fa[S][i]), sum[i][j], kFp4, kFp4, S, sb[0][j], S,
+          fp4_operand(fb[ST][j]), fp4_operand(fa[ST][i]), sum[i][j], kFp4, kFp4, ST, sb[0][j], ST,
           sa[0][i]);
       other(q);
       __builtin_amdgcn_sched_barrier(0);
@@ -365,14 +386,12 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   using S1 = std::integral_constant<int, 1>;
   using S2 = std::integral_constant<int, 2>;
   using S3 = std::integral_constant<int, 3>;
-  constexpr int OPS = FM + FN, MMS = FM * FN;
-  auto reading = [&](int q, int from, int s) {  // the operands of step s, from the first products on
+  auto reading = [&](int q, int buf, int s) {  // the operands of step s, from the first products on
 #pragma unroll
     for (int o = 0; o < OPS; ++o) {
-      if (o * MMS / 2 / OPS == q) read_codes(o, from, s);
+      if (o * MMS / 2 / OPS == q) read_codes(o, buf, s);
     }
   };
-
   // The products so far are made before this point: they touch no memory, and without it the compiler
   // moves them behind the barrier and the branches below, to where their results are next used.
   auto here = [&]() {
@@ -382,22 +401,17 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
       for (int j = 0; j < FN; ++j) asm volatile("" : "+a"(sum[i][j]));
     }
   };
-  auto have_scales = [&]() {  // waits for them here and not later, when other loads are in flight
-#pragma unroll
-    for (int k = 0; k < SR; ++k) asm volatile("" : "+v"(sv[k]));
-  };
-  if (bias != nullptr) {
-    for (int c = tid; c < BN; c += 256) add[c] = E::to_f(bias[min(n0 + c, N - 1)]);
-  }
+
   load_scales(0);
 #pragma unroll
-  for (int u = 0; u < NBUF; ++u) load_tile(min(u, last), u);
+  for (int j = 0; j < LOADS; ++j) load_rows(j, 0, 0);
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) load_rows(j, 1, 1);
   have_scales();
   store_scales(0);
-  wait_loads<(NBUF - 1) * LOADS>();
+  wait_loads();
   wait_lds();
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
+  if constexpr (GW > 1) meet();
 #pragma unroll
   for (int o = 0; o < OPS; ++o) {
     read_codes(o, 0, 0);
@@ -408,117 +422,156 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 #pragma unroll
     for (int o = 0; o < OPS; ++o) read_codes(o, 0, u);
   }
-  int cur = 0;
-  for (int t = 0; t < last; ++t) {
-    const int then = min(t + NBUF, last), next = cur + 1 == NBUF ? 0 : cur + 1;
+  for (int t = 0; t + 1 < tiles; ++t) {
+    const int cur = t & 1;
     __builtin_amdgcn_sched_barrier(0);
     step(S0(), [&](int q) { reading(q, cur, 3); });
     here();
-    if (t & 1) store_scales((t + 1) / 2);
-    wait_loads<(NBUF - 2) * LOADS>();
-    if constexpr (NBUF == 2) have_scales();
+    if (t % kScaleTiles == kScaleTiles - 1) store_scales(t / kScaleTiles + 1);
+    wait_loads();
+    have_scales();
     wait_lds();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if ((t & 1) != 0 && ((t + 3) / 2) % LPR == 0) {
-      load_scales((t + 3) / 2);
-      if constexpr (NBUF > 2) have_scales();
-    }
+    if constexpr (GW > 1) meet();
+    if (t % kScaleTiles == 0) load_scales(t / kScaleTiles + 1);
     __builtin_amdgcn_sched_barrier(0);
-    auto loading = [&](int q, int s) {  // the tile after those that are held, over steps 1 and 2
+    auto loading = [&](int q, int s) {  // over the steps but the first
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
-        if (j * 2 * MMS / LOADS == q + s * MMS) load_rows(j, then, cur);
+        if (j * LSTEPS * MMS / LOADS == q + s * MMS) load_rows(j, t + 2, cur);
       }
     };
     step(S1(), [&](int q) {
-      reading(q, next, 0);
-      loading(q, 0);
-    });
-    step(S2(), [&](int q) {
-      reading(q, next, 1);
-      loading(q, 1);
-    });
-    step(S3(), [&](int q) {
-      reading(q, next, 2);
+      reading(q, cur ^ 1, 0);
 #pragma unroll
       for (int o = 0; o < OPS; ++o) {
         if (o * MMS / 2 / OPS == q) read_scales(o, t + 1, 1);
       }
+      loading(q, 0);
+    });
+    step(S2(), [&](int q) {
+      reading(q, cur ^ 1, 1);
+      loading(q, 1);
+    });
+    step(S3(), [&](int q) {
+      reading(q, cur ^ 1, 2);
+      loading(q, 2);
     });
 #pragma unroll
     for (int i = 0; i < FM; ++i) sa[0][i] = sa[1][i];
 #pragma unroll
     for (int i = 0; i < FN; ++i) sb[0][i] = sb[1][i];
-    cur = next;
   }
-  {  // the last tile, whose blocks past the rows' end count as zero: a's codes here, the scales above
-    auto mask = [&](int s) {
-      const bool in = last * kTileK + 4 * g + s < blocks;
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) fa[s][i][e] = in ? fa[s][i][e] : 0;
-      }
-    };
-#pragma unroll
-    for (int o = 0; o < OPS; ++o) read_codes(o, cur, 3);
-    mask(0);
-    step(S0(), [](int) {});
-    mask(1);
-    step(S1(), [](int) {});
-    mask(2);
-    step(S2(), [](int) {});
-    mask(3);
-    step(S3(), [](int) {});
-  }
-  wait_loads<0>();  // the loads past the last tile: none may arrive after the workgroup's LDS is given on
+  for (int o = 0; o < OPS; ++o) read_codes(o, (tiles - 1) & 1, 3);
+  step(S0(), [](int) {});
+  step(S1(), [](int) {});
+  step(S2(), [](int) {});
+  step(S3(), [](int) {});
+  wait_loads();  // the loads past the last tile, before other uses of their LDS
+  meet();        // every wave has read its last operands
 
   // A lane holds n = 8 (e / 4) + 4 g + e % 4 of m = lane % 32 of each product: 8 or 16 bytes in a row.
-  // Each wave turns 32 rows at a time in LDS of its own and stores them 16 bytes a lane, whole lines in
-  // a row: as they are held, two or four bytes a store, the stores took 130 of 420 us (8192 x 8192 x
-  // 8192 bf16).
-  using S = typename E::S;
-  constexpr int WN = 32 * FN, LINE = WN * (int)sizeof(S) + 16;  // 16: rows start in other banks
-  static_assert(4 * 32 * LINE <= NBUF * TILE, "the waves' rows fit the tiles");
-  __builtin_amdgcn_s_barrier();  // every wave has read its last operands
-  asm volatile("" ::: "memory");
-  uint8_t* own = lds + wave * 32 * LINE;
-  const int wn0 = n0 + (wave >> 1) * WN;
+  // The rows are turned in LDS and stored 16 bytes a lane, whole lines in a row: as they are held, two
+  // or four bytes a store, the stores took 130 of 420 us (8192 x 8192 x 8192 bf16).
   constexpr int VEC = 16 / (int)sizeof(S);
   const bool whole = N % VEC == 0 && ((uintptr_t)out & 15) == 0;
+  if constexpr (KS > 1) {
+    // every group's tile in fp32, added in the groups' order by all
+    constexpr int LINE = BN * 4 + 16;  // 16: rows start in other banks
+    static_assert(BM * LINE <= GROUP, "a group's sums fit its LDS");
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
+    for (int i = 0; i < FM; ++i) {
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
+      for (int j = 0; j < FN; ++j) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = 32 * j + 8 * q + 4 * g;
-        f32x4 f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = sum[i][j][4 * q + e];
-        if (bias != nullptr) f += *reinterpret_cast<const f32x4*>(add + (wave >> 1) * WN + c);
-        Pack<S, 4> v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v.v[e] = E::from_f(f[e]);
-        *reinterpret_cast<Pack<S, 4>*>(own + r32 * LINE + c * sizeof(S)) = v;
+        for (int q = 0; q < 4; ++q) {
+          const int c = wn * 32 * FN + 32 * j + 8 * q + 4 * g;
+          *reinterpret_cast<f32x4*>(lds + (am + 32 * i) * LINE + c * 4) =
+              f32x4{sum[i][j][4 * q], sum[i][j][4 * q + 1], sum[i][j][4 * q + 2],
+                    sum[i][j][4 * q + 3]};
+        }
       }
     }
-    const int wm0 = m0 + (wave & 1) * 32 * FM + 32 * i;
-    if (whole) {
-      constexpr int PER = WN / VEC, STEPS = 32 * PER / 64;  // lanes a row
+    __syncthreads();
+    constexpr int PER = BN / VEC;  // lanes a row
 #pragma unroll
-      for (int k = 0; k < STEPS; ++k) {
-        const int r = (k * 64 + lane) / PER, c = (k * 64 + lane) % PER * VEC;
-        const Pack<S, VEC> v = *reinterpret_cast<const Pack<S, VEC>*>(own + r * LINE + c * sizeof(S));
-        if (wm0 + r < M && wn0 + c < N) st_nt<S, VEC>(out + (int64_t)(wm0 + r) * N + wn0 + c, v);
+    for (int k = 0; k < BM * PER / THREADS; ++k) {
+      const int at = k * THREADS + (int)threadIdx.x, r = at / PER, c = at % PER * VEC;
+      const int m = m0 + r, n = n0 + c;
+      if (m >= M || n >= N) continue;
+      Pack<S, VEC> v;
+#pragma unroll
+      for (int h = 0; h < VEC / 4; ++h) {
+        f32x4 f = *reinterpret_cast<const f32x4*>(lds_all + r * LINE + (c + 4 * h) * 4);
+#pragma unroll
+        for (int p = 1; p < KS; ++p) {
+          f += *reinterpret_cast<const f32x4*>(lds_all + p * GROUP + r * LINE + (c + 4 * h) * 4);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (bias != nullptr) f[e] += E::to_f(bias[min(n + 4 * h + e, N - 1)]);
+          v.v[4 * h + e] = E::from_f(f[e]);
+        }
       }
-    } else {
+      S* to = out + (int64_t)m * N + n;
+      if (whole) {
+        st<S, VEC>(to, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          if (n + e < N) to[e] = v.v[e];
+        }
+      }
+    }
+  } else {
+    // 32 rows of each wave at a time
+    constexpr int WN = 32 * FN, LINE = WN * (int)sizeof(S) + 16;
+    constexpr int ADD = GW * 32 * LINE;  // the bias, behind the waves' rows
+    static_assert(ADD + BN * 4 <= 2 * TILE, "what reuses the tiles");
+    if (bias != nullptr) {
+      for (int c = tid; c < BN; c += 64 * GW) {
+        *reinterpret_cast<float*>(lds + ADD + c * 4) = E::to_f(bias[min(n0 + c, N - 1)]);
+      }
+      __syncthreads();
+    }
+    uint8_t* own = lds + wave * 32 * LINE;
+    const int wn0 = n0 + wn * WN;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c = 32 * j + 8 * q + 4 * g;
+          f32x4 f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[e] = sum[i][j][4 * q + e];
+          if (bias != nullptr) {
+            f += *reinterpret_cast<const f32x4*>(lds + ADD + (wn * WN + c) * 4);
+          }
+          Pack<S, 4> v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v.v[e] = E::from_f(f[e]);
+          *reinterpret_cast<Pack<S, 4>*>(own + r32 * LINE + c * sizeof(S)) = v;
+        }
+      }
+      const int wm0 = m0 + wm * 32 * FM + 32 * i;
+      if (whole) {
+        constexpr int PER = WN / VEC, STEPS = 32 * PER / 64;  // lanes a row
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+          const int r = (k * 64 + lane) / PER, c = (k * 64 + lane) % PER * VEC;
+          const Pack<S, VEC> v =
+              *reinterpret_cast<const Pack<S, VEC>*>(own + r * LINE + c * sizeof(S));
+          if (wm0 + r < M && wn0 + c < N) st_nt<S, VEC>(out + (int64_t)(wm0 + r) * N + wn0 + c, v);
+        }
+      } else {
 #pragma unroll 4
-      for (int k = lane; k < 32 * WN; k += 64) {
-        const int r = k / WN, c = k % WN;
-        const S v = *reinterpret_cast<const S*>(own + r * LINE + c * sizeof(S));
-        if (wm0 + r < M && wn0 + c < N) out[(int64_t)(wm0 + r) * N + wn0 + c] = v;
+        for (int k = lane; k < 32 * WN; k += 64) {
+          const int r = k / WN, c = k % WN;
+          const S v = *reinterpret_cast<const S*>(own + r * LINE + c * sizeof(S));
+          if (wm0 + r < M && wn0 + c < N) out[(int64_t)(wm0 + r) * N + wn0 + c] = v;
+        }
       }
     }
   }
@@ -534,13 +587,15 @@ static bool tiles_fit(int M, int N, int blocks) {
          (int64_t)N * blocks >= 16 && tiles_of(M, N, 64, 64) <= INT32_MAX;
 }
 
-template <class E, int FM, int FN, int NBUF, int LPR>
+template <class E, int FM, int FN, int WD, int KS>
 static int product_tiles(typename E::S* out, const uint8_t* a, const uint8_t* as, const uint8_t* b,
                          const uint8_t* bs, const typename E::S* bias, int M, int N, int blocks,
                          hipStream_t st) {
-  const int tm = (M + 64 * FM - 1) / (64 * FM), tn = (N + 64 * FN - 1) / (64 * FN);
-  hipLaunchKernelGGL((k_mxfp4_mm_tile<E, FM, FN, NBUF, LPR>), dim3((unsigned)(tm * tn)), dim3(256), 0, st, out,
-                     a, as, b, bs, bias, M, N, blocks, tm, tn);
+  constexpr int BM = 32 * WD * FM, BN = 32 * WD * FN;
+  const int tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN;
+  const int tiles = (blocks + kTileK * KS - 1) / (kTileK * KS);  // of a group
+  hipLaunchKernelGGL((k_mxfp4_mm_tile<E, FM, FN, WD, KS>), dim3((unsigned)(tm * tn)),
+                     dim3(64 * WD * WD * KS), 0, st, out, a, as, b, bs, bias, M, N, blocks, tm, tiles);
   return check_launch("mxfp4_scaled_mm");
 }
 
@@ -552,9 +607,9 @@ static int product(void* out, const uint8_t* a, const uint8_t* as, const uint8_t
   const auto* bi = static_cast<const S*>(bias);
   if (tiles_fit(M, N, blocks)) {
     if (M > 128 && tiles_of(M, N, 256, 256) >= 192) {
-      return product_tiles<E, 4, 4, 2, 4>(o, a, as, b, bs, bi, M, N, blocks, st);
+      return product_tiles<E, 4, 4, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
     }
-    if (M > 64) return product_tiles<E, 2, 2, 4, 16>(o, a, as, b, bs, bi, M, N, blocks, st);
+    if (M > 64) return product_tiles<E, 2, 2, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
   }
 #define MCOP_ROWS(MT, NT, W, KS)                                                               \
   hipLaunchKernelGGL((k_mxfp4_mm_rows<E, MT, NT, W, KS>),                                      \
