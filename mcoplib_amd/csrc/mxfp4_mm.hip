@@ -7,6 +7,9 @@
 // weights are the first operand: a lane then holds four consecutive n of one m.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "../../include/mcop_norm.h"
 #include "mxfp4.h"
 
@@ -17,6 +20,23 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kFp4 = 4;  // operand format of the matrix instructions
+
+// VEC values of a row from column n on, of those inside its N: one store at any alignment, but at the
+// row's end (one element a store took 24 us for 1237 x 4099 fp32, this 11).
+template <class S, int VEC, bool NT>
+__device__ __forceinline__ void store_row(S* to, const Pack<S, VEC>& v, int n, int N, bool whole) {
+  if (whole) {
+    if constexpr (NT) st_nt<S, VEC>(to, v);
+    else st<S, VEC>(to, v);
+  } else if (n + VEC <= N) {
+    __builtin_memcpy(to, &v, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if (n + e < N) to[e] = v.v[e];
+    }
+  }
+}
 
 __device__ __forceinline__ i32x8 fp4_operand(i32x4 v) {
   return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
@@ -173,15 +193,7 @@ k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
       if (bias != nullptr) v[i] += E::to_f(bias[min(n + i, N - 1)]);
       o.v[i] = E::from_f(v[i]);
     }
-    S* p = out + (int64_t)m * N + n;
-    if (quads) {
-      st<S, 4>(p, o);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (n + i < N) p[i] = o.v[i];
-      }
-    }
+    store_row<S, 4, false>(out + (int64_t)m * N + n, o, n, N, quads);
   }
 }
 
@@ -513,15 +525,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
           v.v[4 * h + e] = E::from_f(f[e]);
         }
       }
-      S* to = out + (int64_t)m * N + n;
-      if (whole) {
-        st<S, VEC>(to, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          if (n + e < N) to[e] = v.v[e];
-        }
-      }
+      store_row<S, VEC, false>(out + (int64_t)m * N + n, v, n, N, whole);
     }
   } else {
     // 32 rows of each wave at a time
@@ -556,22 +560,14 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
         }
       }
       const int wm0 = m0 + wm * 32 * FM + 32 * i;
-      if (whole) {
-        constexpr int PER = WN / VEC, STEPS = 32 * PER / 64;  // lanes a row
+      constexpr int PER = WN / VEC, STEPS = 32 * PER / 64;  // lanes a row
 #pragma unroll
-        for (int k = 0; k < STEPS; ++k) {
-          const int r = (k * 64 + lane) / PER, c = (k * 64 + lane) % PER * VEC;
-          const Pack<S, VEC> v =
-              *reinterpret_cast<const Pack<S, VEC>*>(own + r * LINE + c * sizeof(S));
-          if (wm0 + r < M && wn0 + c < N) st_nt<S, VEC>(out + (int64_t)(wm0 + r) * N + wn0 + c, v);
-        }
-      } else {
-#pragma unroll 4
-        for (int k = lane; k < 32 * WN; k += 64) {
-          const int r = k / WN, c = k % WN;
-          const S v = *reinterpret_cast<const S*>(own + r * LINE + c * sizeof(S));
-          if (wm0 + r < M && wn0 + c < N) out[(int64_t)(wm0 + r) * N + wn0 + c] = v;
-        }
+      for (int k = 0; k < STEPS; ++k) {
+        const int r = (k * 64 + lane) / PER, c = (k * 64 + lane) % PER * VEC;
+        const int m = wm0 + r, n = wn0 + c;
+        const Pack<S, VEC> v =
+            *reinterpret_cast<const Pack<S, VEC>*>(own + r * LINE + c * sizeof(S));
+        if (m < M && n < N) store_row<S, VEC, true>(out + (int64_t)m * N + n, v, n, N, whole);
       }
     }
   }
@@ -599,27 +595,63 @@ static int product_tiles(typename E::S* out, const uint8_t* a, const uint8_t* as
   return check_launch("mxfp4_scaled_mm");
 }
 
+// The form for a product: the one of the lowest estimated time.  The estimates (us) are fits to calls of
+// every form over M from 8 to 4096, N from 512 to 8192 and K of 512, 2048 and 8192 (bf16, operands from
+// HBM): a part for the launch, one for each round of workgroups on the 256 CUs, and one for the way
+// along K.  Measured where one gives way to the next (K = 8192 unless given):
+//   rows (16 x 16 straight from memory) and 32 x 64: 32 x 512 7.8 and 7.4, 64 x 4099 31.6 and 10.2;
+//     K = 512 128 x 2048 4.8 and 5.1
+//   32 x 64 and 64 x 64 without barriers: 64 x 4099 10.2 and 11.8, 128 x 4099 20.5 and 12.7
+//   those 64 x 64, one workgroup a CU, and 64 x 64 with barriers, four: 512 x 2048 15.9 and 20.3, 256 x
+//     8192 29.9 and 35.1; K = 512 14.8 and 5.9 (512 x 4099)
+//   64 x 64 and 128 x 128: 1024 x 2048 22.0 and 26.7, 512 x 8192 48.0 and 30.2
+//   128 x 128 and 256 x 256: 1024 x 8192 50.9 and 51.7, 2048 x 8192 86.0 and 73.8, 4096 x 4099 (272
+//     tiles of the larger) 100 and 114
+enum MmForm { MM_ROWS, MM_32X64, MM_64X64_APART, MM_64X64, MM_128X128, MM_256X256 };
+
+static MmForm form_of(int M, int N, int blocks) {
+  auto waves = [&](int bm, int bn) {  // workgroups of such tiles a CU
+    return (double)((M + bm - 1) / bm) * ((N + bn - 1) / bn) / 256.0;
+  };
+  const double k = blocks / 256.0;  // in units of K = 8192
+  double best = 3.3 + std::max(4.5 * k, waves(16, 16) * k * (3.5 + 2.5 * k));
+  MmForm form = MM_ROWS;
+  auto offer = [&](MmForm f, double us) {
+    if (us < best) best = us, form = f;
+  };
+  if (!tiles_fit(M, N, blocks)) return MM_ROWS;
+  double w = waves(32, 64);
+  offer(MM_32X64, w <= 1 ? 4.7 + k * (3.5 + 6 * w) : 3.3 + std::ceil(w) * (3 + 6 * k));
+  w = waves(64, 64);
+  offer(MM_64X64_APART, w <= 1 ? 5.5 + k * (4 + 6 * w) : 3.3 + std::ceil(w) * (4 + 8 * k));
+  offer(MM_64X64, std::max(3.7 + 15.5 * k, 3.5 + w * (0.1 + 10 * k)));
+  w = waves(128, 128);
+  offer(MM_128X128, w <= 1   ? 3.9 + 21 * k
+                    : w <= 2 ? 3.9 + k * (7 + 20 * w)
+                             : 3 + w * (2.6 + 20.5 * k));
+  w = waves(256, 256);
+  offer(MM_256X256, w <= 1 ? 8 + k * (36 + 30 * w * w) : std::ceil(w) * (6 + 64 * k));
+  return form;
+}
+
 template <class E>
 static int product(void* out, const uint8_t* a, const uint8_t* as, const uint8_t* b,
                    const uint8_t* bs, const void* bias, int M, int N, int blocks, hipStream_t st) {
   using S = typename E::S;
   auto* o = static_cast<S*>(out);
   const auto* bi = static_cast<const S*>(bias);
-  if (tiles_fit(M, N, blocks)) {
-    if (M > 128 && tiles_of(M, N, 256, 256) >= 192) {
-      return product_tiles<E, 4, 4, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
-    }
-    if (M > 64) return product_tiles<E, 2, 2, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
+  switch (form_of(M, N, blocks)) {
+    case MM_32X64: return product_tiles<E, 1, 2, 1, 4>(o, a, as, b, bs, bi, M, N, blocks, st);
+    case MM_64X64_APART:
+      return product_tiles<E, 2, 2, 1, 4>(o, a, as, b, bs, bi, M, N, blocks, st);
+    case MM_64X64: return product_tiles<E, 1, 1, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
+    case MM_128X128: return product_tiles<E, 2, 2, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
+    case MM_256X256: return product_tiles<E, 4, 4, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
+    default: break;
   }
-#define MCOP_ROWS(MT, NT, W, KS)                                                               \
-  hipLaunchKernelGGL((k_mxfp4_mm_rows<E, MT, NT, W, KS>),                                      \
-                     dim3((unsigned)((N + 16 * NT - 1) / (16 * NT)),                           \
-                          (unsigned)((M + 16 * MT - 1) / (16 * MT))),                          \
-                     dim3(64 * W), 0, st, o, a, as, b, bs, bi, M, N, blocks)
-  if (M <= 16) MCOP_ROWS(1, 1, 4, 4);
-  else if (M <= 32) MCOP_ROWS(2, 2, 4, 2);
-  else MCOP_ROWS(4, 2, 4, 2);
-#undef MCOP_ROWS
+  const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), block(256);
+  hipLaunchKernelGGL((k_mxfp4_mm_rows<E, 1, 1, 4, 4>), grid, block, 0, st, o, a, as, b, bs, bi, M, N,
+                     blocks);
   return check_launch("mxfp4_scaled_mm");
 }
 
