@@ -14,6 +14,8 @@
 // Workgroups of blockIdx.y = 0 do the keys, 1 the values.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/mcop_norm.h"
 #include "mxfp4.h"
 
@@ -34,6 +36,7 @@ struct KvSide {
   int64_t c_page, c_token, c_head;
   int64_t s_page, s_token, s_head;
   int dim, lanes;
+  Divisor by_passes;  // waves that a token's heads take
 };
 struct KvSides {
   KvSide side[2];
@@ -79,7 +82,103 @@ __device__ __forceinline__ uint32_t load_dword(const uint8_t* p) {
   return v;
 }
 
-// WHOLE: vectors are whole units, and every tensor's vectors are aligned to theirs.  NU: units a lane.
+// Quantizes one vector, whose `lanes` lanes hold NU units each (left[n]: elements of unit n inside the
+// vector; a unit past its end holds copies of the first, or zeros), and stores codes and scales.
+// WHOLE: vectors are whole units, and every tensor's vectors are aligned to theirs.
+template <class E, int FMT, bool WHOLE, int NU>
+__device__ __forceinline__ void write_vector(const Pack<typename E::S, 8> (&v)[NU],
+                                             const int (&left)[NU], int j, int lanes, bool store,
+                                             uint8_t* dst, void* scales, int64_t s_at) {
+  if constexpr (FMT == KV_MXFP4) {
+    uint8_t* sd = static_cast<uint8_t*>(scales) + s_at;
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      const int unit = j + n * lanes;
+      // vectors are whole blocks: a block's four lanes are all inside or all past the end
+      const uint32_t e = mx_scale(lanes_max(absmax8<E>(v[n]), 4));
+      if (!store || left[n] <= 0) continue;
+      store_dword<WHOLE>(dst + unit * 4, mx_codes8<E>(v[n], e));
+      if ((unit & 3) == 0) sd[unit >> 2] = (uint8_t)e;
+    }
+  } else {
+    float A;
+    bool ordinary;  // no NaN in the vector, and A where the short forms below hold
+    if constexpr (sizeof(typename E::S) == 2) {
+      // the largest magnitude by its bits, two values an instruction; NaN's are above infinity's
+      uint32_t m = 0;
+#pragma unroll
+      for (int n = 0; n < NU; ++n) {
+        const Pack<uint32_t, 4> w = __builtin_bit_cast(Pack<uint32_t, 4>, v[n]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = max_u16x2(m, w.v[e] & 0x7fff7fffu);
+      }
+      m = lanes_max(max(m & 0xffffu, m >> 16), lanes);
+      A = E::to_f((uint16_t)m);
+      ordinary = A <= 0x1p100f && (FMT == KV_FP8 || A >= 0x1p-100f);
+    } else {
+      ordinary = false;
+    }
+    float f[NU][8], s;
+    Codes<8> q[NU];
+#pragma unroll
+    for (int n = 0; n < NU; ++n) widen<E, 8>(f[n], v[n]);
+    if (sizeof(typename E::S) == 2 && __builtin_amdgcn_ballot_w64(!ordinary) == 0) {
+      if constexpr (FMT == KV_INT8) {
+        s = div_floored<127>(A);
+        const float r = rcp_in_domain(A), h = 127.0f * r;  // 127 / A, as row_ratio
+        const float inv = __builtin_fmaf(__builtin_fmaf(-h, A, 127.0f), r, h);
+#pragma unroll
+        for (int n = 0; n < NU; ++n) q[n] = i8_codes_in_range<8>(f[n], inv);
+      } else {
+        s = __builtin_fmaxf(div_floored<448>(A), 1.0f / 229376.0f);
+        const float inv = rcp_in_domain(s);
+        // fp8_quotient_codes' bounded form; without NaN its upper clamp gives the conversion's code
+#pragma unroll
+        for (int n = 0; n < NU; ++n) {
+          float c[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float q0 = f[n][e] * inv;
+            const float r = __builtin_fmaf(-q0, s, f[n][e]);
+            c[e] = __builtin_copysignf(__builtin_fmaf(r, inv, q0), f[n][e]);
+          }
+          q[n] = cvt_fp8<8>(c);
+        }
+      }
+    } else {
+      float m = 0.0f;  // NaN is ignored, as in a row's absmax
+#pragma unroll
+      for (int n = 0; n < NU; ++n) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = __builtin_fmaxf(m, __builtin_fabsf(f[n][e]));
+      }
+      A = __builtin_bit_cast(float, lanes_max(__builtin_bit_cast(uint32_t, m), lanes));
+      float inv;
+      if constexpr (FMT == KV_INT8) {
+        s = row_div<127>(A);
+        inv = row_ratio(127.0f, A);
+      } else {
+        s = __builtin_fmaxf(div_floored<448>(A), 1.0f / 229376.0f);
+        inv = row_rcp(s);
+      }
+#pragma unroll
+      for (int n = 0; n < NU; ++n) {
+        if constexpr (FMT == KV_INT8) q[n] = i8_codes<-127, 8>(f[n], inv);
+        else q[n] = fp8_quotient_codes<8>(f[n], s, inv, mcop_divisor_ok(s), s <= 0x1p100f);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      if (store && left[n] > 0) {
+        store_unit<uint8_t, WHOLE>(dst + (j + n * lanes) * 8,
+                                   __builtin_bit_cast(Pack<uint8_t, 8>, q[n]), left[n]);
+      }
+    }
+    if (store && j == 0) static_cast<float*>(scales)[s_at] = s;
+  }
+}
+
+// Vectors of few lanes: a vector a group of lanes, wherever its token is.  NU: units a lane.
 template <class E, int FMT, bool WHOLE, int NU>
 __global__ void __launch_bounds__(kKvLanes)
 k_kv_cache_write(KvSides a, const int64_t* __restrict__ slots, uint32_t vectors, int64_t num_slots,
@@ -111,49 +210,64 @@ k_kv_cache_write(KvSides a, const int64_t* __restrict__ slots, uint32_t vectors,
   const uint32_t off = (store ? (uint32_t)slot : 0u) - page * (uint32_t)page_size;
   uint8_t* dst = k.codes + page * k.c_page + off * k.c_token + head * k.c_head;
   const int64_t s_at = page * k.s_page + off * k.s_token + head * k.s_head;
-  if constexpr (FMT == KV_MXFP4) {
-    uint8_t* sd = static_cast<uint8_t*>(k.scales) + s_at;
+  write_vector<E, FMT, WHOLE, NU>(v, left, j, k.lanes, store, dst, k.scales, s_at);
+}
+
+// Tokens of a wave or more: a wave takes 64 / lanes heads of TW tokens, so that everything a token stands
+// for (its slot, its page, their addresses) is computed in scalar registers; with a vector a group of
+// lanes that arithmetic took longer than the memory.  The waves of a token are neighbours, so that what a
+// token writes is written together (apart, by blockIdx.y, 65536 tokens of 8 x 128 read in 105 us, 89
+// with the heads in a loop).
+__device__ __forceinline__ int uniform_int(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+template <class E, int FMT, bool WHOLE, int NU, int TW>
+__global__ void __launch_bounds__(kKvLanes)
+k_kv_cache_write_tokens(KvSides a, const int64_t* __restrict__ slots, int tokens, int64_t num_slots,
+                        int page_size) {
+  using S = typename E::S;
+  const KvSide& k = a.side[blockIdx.y];
+  const int sh = 31 - __builtin_clz((unsigned)k.lanes), lane = (int)threadIdx.x & 63;
+  const int j = lane & (k.lanes - 1);
+  const uint32_t item = (uint32_t)uniform_int(
+      (int)(blockIdx.x * (kKvLanes / 64) + (threadIdx.x >> 6)));
+  const int t0 = (int)k.by_passes.quotient(item) * TW;
+  const int pass = (int)(item - k.by_passes.quotient(item) * k.by_passes.d);
+  if (t0 >= tokens) return;
+  int left[NU], at[NU];
+#pragma unroll
+  for (int n = 0; n < NU; ++n) {
+    at[n] = (j + n * k.lanes) * 8;
+    left[n] = k.dim - at[n];
+    if (WHOLE && left[n] <= 0) at[n] = 0;
+  }
+  const int head = pass * (64 >> sh) + (lane >> sh);
+  const bool live = head < a.heads;
+  const int64_t h = live ? head : 0;
+  Pack<S, 8> v[TW][NU];
+#pragma unroll
+  for (int i = 0; i < TW; ++i) {
+    const S* src = static_cast<const S*>(k.plain) + min(t0 + i, tokens - 1) * k.p_token;
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
-      const int unit = j + n * k.lanes;
-      // vectors are whole blocks: a block's four lanes are all inside or all past the end
-      const uint32_t e = mx_scale(lanes_max(absmax8<E>(v[n]), 4));
-      if (!store || left[n] <= 0) continue;
-      store_dword<WHOLE>(dst + unit * 4, mx_codes8<E>(v[n], e));
-      if ((unit & 3) == 0) sd[unit >> 2] = (uint8_t)e;
+      v[i][n] = load_unit<E, WHOLE>(src + (h * k.p_head + at[n]), left[n]);
     }
-  } else {
-    float f[NU][8], m = 0.0f;
+  }
+  int64_t dst[TW], s_at[TW];
+  bool store[TW];
 #pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      widen<E, 8>(f[n], v[n]);
+  for (int i = 0; i < TW; ++i) {
+    const int64_t slot = slots[min(t0 + i, tokens - 1)];
+    store[i] = t0 + i < tokens && slot >= 0 && slot < num_slots;
+    const uint32_t in = store[i] ? (uint32_t)slot : 0u;
+    const uint32_t page = a.by_page.quotient(in), off = in - page * (uint32_t)page_size;
+    dst[i] = page * k.c_page + off * k.c_token;
+    s_at[i] = page * k.s_page + off * k.s_token;
+  }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float t = __builtin_fabsf(f[n][e]);
-        // a unit past the end holds copies of the first; NaN is ignored, as in a row's absmax
-        m = __builtin_fmaxf(m, t);
-      }
-    }
-    const float A = __builtin_bit_cast(float, lanes_max(__builtin_bit_cast(uint32_t, m), k.lanes));
-    float s, inv;
-    if constexpr (FMT == KV_INT8) {
-      s = row_div<127>(A);
-      inv = row_ratio(127.0f, A);
-    } else {
-      s = __builtin_fmaxf(div_floored<448>(A), 1.0f / 229376.0f);
-      inv = row_rcp(s);
-    }
-#pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      const int at = (j + n * k.lanes) * 8;
-      Codes<8> q;
-      if constexpr (FMT == KV_INT8) q = i8_codes<-127, 8>(f[n], inv);
-      else q = fp8_quotient_codes<8>(f[n], s, inv, mcop_divisor_ok(s), s <= 0x1p100f);
-      if (store && left[n] > 0) {
-        store_unit<uint8_t, WHOLE>(dst + at, __builtin_bit_cast(Pack<uint8_t, 8>, q), left[n]);
-      }
-    }
-    if (store && j == 0) static_cast<float*>(k.scales)[s_at] = s;
+  for (int i = 0; i < TW; ++i) {
+    if (!store[i]) continue;
+    write_vector<E, FMT, WHOLE, NU>(v[i], left, j, k.lanes, live, k.codes + dst[i] + h * k.c_head,
+                                    k.scales, s_at[i] + h * k.s_head);
   }
 }
 
@@ -165,6 +279,50 @@ __device__ __forceinline__ void widen_fp8(float* f, uint32_t w, float s) {
   f[0] = a[0] * s, f[1] = a[1] * s, f[2] = b[0] * s, f[3] = b[1] * s;
 }
 
+// One unit of a vector as it lies in the cache, and its values.
+template <int FMT>
+struct KvUnit {
+  Pack<uint8_t, 8> q;
+  uint32_t c, e;
+  float s;
+};
+template <int FMT, bool WHOLE>
+__device__ __forceinline__ KvUnit<FMT> load_codes(const uint8_t* src, const void* scales,
+                                                  int64_t s_at, int unit, int left) {
+  KvUnit<FMT> u;
+  if constexpr (FMT == KV_MXFP4) {
+    u.c = load_dword<WHOLE>(src + unit * 4);
+    u.e = static_cast<const uint8_t*>(scales)[s_at + (unit >> 2)];
+  } else {
+    if constexpr (WHOLE) {
+      u.q = ld_nt<uint8_t, 8>(src + unit * 8);
+    } else {
+#pragma unroll
+      for (int b = 0; b < 8; ++b) u.q.v[b] = b < left ? src[unit * 8 + b] : 0;
+    }
+    u.s = static_cast<const float*>(scales)[s_at];
+  }
+  return u;
+}
+template <class E, int FMT>
+__device__ __forceinline__ Pack<typename E::S, 8> values_of(const KvUnit<FMT>& u, bool none) {
+  float f[8];
+  if constexpr (FMT == KV_MXFP4) {
+    mx_widen8(f, u.c, u.e);
+  } else if constexpr (FMT == KV_INT8) {
+#pragma unroll
+    for (int b = 0; b < 8; ++b) f[b] = (float)(int8_t)u.q.v[b] * u.s;
+  } else {
+    const Pack<uint32_t, 2> w = __builtin_bit_cast(Pack<uint32_t, 2>, u.q);
+    widen_fp8(f, w.v[0], u.s);
+    widen_fp8(f + 4, w.v[1], u.s);
+  }
+  Pack<typename E::S, 8> o;
+#pragma unroll
+  for (int b = 0; b < 8; ++b) o.v[b] = E::from_f(none ? __builtin_nanf("") : f[b]);
+  return o;
+}
+
 // The sequence that holds token t: how many of cu[1..n] are <= t (the wave counts together).
 __device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int n, int64_t t) {
   int s = 0;
@@ -174,6 +332,27 @@ __device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int n
     s += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(below));
   }
   return s;
+}
+
+// Where a token of the gathered tensors lies: 1 in the cache (at page and off), 2 nowhere (no such page),
+// 0 past the last sequence.  `s` is at most the token's sequence, and becomes it.
+__device__ __forceinline__ int find_token(int64_t token, int& s, const int32_t* __restrict__ cu,
+                                          const int32_t* __restrict__ starts, int sequences,
+                                          const int32_t* __restrict__ table, int64_t table_stride,
+                                          int columns, int64_t pages, int page_size,
+                                          const Divisor& by_page, uint32_t* page, uint32_t* off) {
+  *page = *off = 0;
+  while (s < sequences && cu[s + 1] <= token) ++s;
+  if (s >= sequences) return 0;
+  const int64_t p = token - cu[s] + (starts != nullptr ? starts[s] : 0);
+  if (p < 0 || p > INT32_MAX) return 2;
+  const uint32_t column = by_page.quotient((uint32_t)p);
+  if (column >= (uint32_t)columns) return 2;
+  const int32_t g = table[s * table_stride + column];
+  if (g < 0 || g >= pages) return 2;
+  *page = (uint32_t)g;
+  *off = (uint32_t)p - column * (uint32_t)page_size;
+  return 1;
 }
 
 template <class E, int FMT, bool WHOLE, int NU, int R>
@@ -199,24 +378,12 @@ k_kv_cache_read(KvSides a, const int32_t* __restrict__ table, int64_t table_stri
     const uint32_t token = a.by_heads.quotient(i < vectors ? i : vectors - 1);
     const uint32_t head = (i < vectors ? i : vectors - 1) - token * (uint32_t)a.heads;
     int s = s0;
-    while (s < sequences && cu[s + 1] <= (int64_t)token) ++s;
+    uint32_t page, off;
     dst[r] = static_cast<S*>(k.plain) + token * k.p_token + head * k.p_head;
-    state[r] = i < vectors && s < sequences ? 2 : 0;
-    uint32_t page = 0, off = 0;
-    if (state[r] != 0) {
-      const int64_t p = (int64_t)token - cu[s] + (starts != nullptr ? starts[s] : 0);
-      if (p >= 0 && p <= INT32_MAX) {
-        const uint32_t column = a.by_page.quotient((uint32_t)p);
-        if (column < (uint32_t)columns) {
-          const int32_t g = table[s * table_stride + column];
-          if (g >= 0 && g < pages) {
-            page = (uint32_t)g;
-            off = (uint32_t)p - column * (uint32_t)page_size;
-            state[r] = 1;
-          }
-        }
-      }
-    }
+    state[r] = i >= vectors ? 0
+                            : find_token(token, s, cu, starts, sequences, table, table_stride, columns,
+                                         pages, page_size, a.by_page, &page, &off);
+    if (i >= vectors) page = off = 0;
     src[r] = k.codes + page * k.c_page + off * k.c_token + head * k.c_head;
     s_at[r] = page * k.s_page + off * k.s_token + head * k.s_head;
   }
@@ -224,46 +391,67 @@ k_kv_cache_read(KvSides a, const int32_t* __restrict__ table, int64_t table_stri
   for (int n = 0; n < NU; ++n) {
     const int unit = j + n * k.lanes, at = unit * 8, left = k.dim - at;
     if (left <= 0) continue;
-    Pack<uint8_t, 8> q[R];
-    uint32_t c[R];
-    float s[R];
-    uint32_t e[R];
+    KvUnit<FMT> u[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (state[r] != 1) continue;
-      if constexpr (FMT == KV_MXFP4) {
-        c[r] = load_dword<WHOLE>(src[r] + unit * 4);
-        e[r] = static_cast<const uint8_t*>(k.scales)[s_at[r] + (unit >> 2)];
-      } else {
-        if constexpr (WHOLE) {
-          q[r] = ld_nt<uint8_t, 8>(src[r] + at);
-        } else {
-#pragma unroll
-          for (int b = 0; b < 8; ++b) q[r].v[b] = b < left ? src[r][at + b] : 0;
-        }
-        s[r] = static_cast<const float*>(k.scales)[s_at[r]];
-      }
+      if (state[r] == 1) u[r] = load_codes<FMT, WHOLE>(src[r], k.scales, s_at[r], unit, left);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       if (state[r] == 0) continue;
-      float f[8];
-      if constexpr (FMT == KV_MXFP4) {
-        mx_widen8(f, c[r], e[r]);
-      } else if constexpr (FMT == KV_INT8) {
+      store_unit<S, WHOLE>(dst[r] + at, values_of<E, FMT>(u[r], state[r] == 2), left);
+    }
+  }
+}
+
+// Tokens of a wave or more, as for the write: a wave takes whole tokens, and finds them in scalar
+// registers (65536 tokens of 8 x 128 int8: 112 us with a vector a group of lanes, LATER so).
+template <class E, int FMT, bool WHOLE, int NU, int TW>
+__global__ void __launch_bounds__(kKvLanes)
+k_kv_cache_read_tokens(KvSides a, const int32_t* __restrict__ table, int64_t table_stride,
+                       int columns, const int32_t* __restrict__ cu,
+                       const int32_t* __restrict__ starts, int sequences, int tokens, int64_t pages,
+                       int page_size) {
+  using S = typename E::S;
+  const KvSide& k = a.side[blockIdx.y];
+  const int sh = 31 - __builtin_clz((unsigned)k.lanes), lane = (int)threadIdx.x & 63;
+  const int j = lane & (k.lanes - 1);
+  const uint32_t item = (uint32_t)uniform_int(
+      (int)(blockIdx.x * (kKvLanes / 64) + (threadIdx.x >> 6)));
+  const int t0 = (int)k.by_passes.quotient(item) * TW;
+  const int pass = (int)(item - k.by_passes.quotient(item) * k.by_passes.d);
+  if (t0 >= tokens) return;
+  int s = uniform_int(sequence_of(cu, sequences, t0));
+  int64_t src[TW], s_at[TW];
+  int state[TW];
 #pragma unroll
-        for (int b = 0; b < 8; ++b) f[b] = (float)(int8_t)q[r].v[b] * s[r];
-      } else {
-        const Pack<uint32_t, 2> w = __builtin_bit_cast(Pack<uint32_t, 2>, q[r]);
-        widen_fp8(f, w.v[0], s[r]);
-        widen_fp8(f + 4, w.v[1], s[r]);
-      }
-      Pack<S, 8> o;
+  for (int i = 0; i < TW; ++i) {
+    uint32_t page = 0, off = 0;
+    state[i] = t0 + i >= tokens ? 0
+                                : find_token(t0 + i, s, cu, starts, sequences, table, table_stride,
+                                             columns, pages, page_size, a.by_page, &page, &off);
+    src[i] = page * k.c_page + off * k.c_token;
+    s_at[i] = page * k.s_page + off * k.s_token;
+  }
+  const int64_t head = pass * (64 >> sh) + (lane >> sh);
+  if (head >= a.heads) return;
 #pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        o.v[b] = E::from_f(state[r] == 2 ? __builtin_nanf("") : f[b]);
+  for (int n = 0; n < NU; ++n) {
+    const int unit = j + n * k.lanes, at = unit * 8, left = k.dim - at;
+    if (left <= 0) continue;
+    KvUnit<FMT> u[TW];
+#pragma unroll
+    for (int i = 0; i < TW; ++i) {
+      if (state[i] == 1) {
+        u[i] = load_codes<FMT, WHOLE>(k.codes + src[i] + head * k.c_head, k.scales,
+                                      s_at[i] + head * k.s_head, unit, left);
       }
-      store_unit<S, WHOLE>(dst[r] + at, o, left);
+    }
+#pragma unroll
+    for (int i = 0; i < TW; ++i) {
+      if (state[i] == 0) continue;
+      S* dst = static_cast<S*>(k.plain) + (t0 + i) * k.p_token;
+      store_unit<S, WHOLE>(dst + (head * k.p_head + at), values_of<E, FMT>(u[i], state[i] == 2), left);
     }
   }
 }
@@ -302,7 +490,7 @@ int side_of(const char* name, const char* what, const mcop_kv_side& in, int fmt,
   *out = KvSide{in.plain, static_cast<uint8_t*>(in.codes), in.scales, in.token_stride,
                 in.head_stride, in.code_page_stride, in.code_token_stride, in.code_head_stride,
                 in.scale_page_stride, in.scale_token_stride, in.scale_head_stride,
-                (int)in.head_size, lanes};
+                (int)in.head_size, lanes, Divisor((uint32_t)((heads * lanes + 63) / 64))};
   return MCOP_OK;
 }
 
@@ -365,11 +553,42 @@ unsigned kv_blocks(const KvSides& a, int64_t vectors, int r) {
 
 bool two_units(const KvSides& a) { return a.side[0].dim > 512 || a.side[1].dim > 512; }
 
+// Whether a token's vectors fill a wave on both sides; the passes over its heads, of the side that has
+// more; and the workgroups for those.
+bool by_tokens(const KvSides& a) {
+  return a.heads * a.side[0].lanes >= 64 && a.heads * a.side[1].lanes >= 64;
+}
+int64_t head_passes(const KvSides& a) {
+  const int lanes = std::max(a.side[0].lanes, a.side[1].lanes);
+  return ((int64_t)a.heads * lanes + 63) / 64;
+}
+bool token_grid(const KvSides& a, int64_t tokens, int tw, dim3* grid) {
+  const int64_t items = (tokens + tw - 1) / tw * head_passes(a), waves = kKvLanes / 64;
+  *grid = dim3((unsigned)((items + waves - 1) / waves), 2);
+  return items + waves <= INT32_MAX;
+}
+// Tokens a wave: four where that leaves 4096 waves or more, else one.
+bool four_tokens(const KvSides& a, int64_t tokens) { return tokens * head_passes(a) >= 8192; }
+
 template <class E, int FMT, bool WHOLE>
 void write_of(const KvSides& a, const int64_t* slots, int64_t vectors, int64_t num_slots,
               int page_size, hipStream_t st) {
   const dim3 grid(kv_blocks(a, vectors, 1), 2), block(kKvLanes);
-  if (two_units(a)) {
+  const int tokens = (int)(vectors / a.heads);
+  dim3 by;
+  if (by_tokens(a) && token_grid(a, tokens, four_tokens(a, tokens) ? 4 : 1, &by)) {
+#define MCOP_WRITE(NU, TW)                                                                        \
+  hipLaunchKernelGGL((k_kv_cache_write_tokens<E, FMT, WHOLE, NU, TW>), by, block, 0, st, a, slots, \
+                     tokens, num_slots, page_size)
+    if (two_units(a)) {
+      if (four_tokens(a, tokens)) MCOP_WRITE(2, 4);
+      else MCOP_WRITE(2, 1);
+    } else {
+      if (four_tokens(a, tokens)) MCOP_WRITE(1, 4);
+      else MCOP_WRITE(1, 1);
+    }
+#undef MCOP_WRITE
+  } else if (two_units(a)) {
     hipLaunchKernelGGL((k_kv_cache_write<E, FMT, WHOLE, 2>), grid, block, 0, st, a, slots,
                        (uint32_t)vectors, num_slots, page_size);
   } else {
@@ -383,7 +602,21 @@ void read_of(const KvSides& a, const int32_t* table, int64_t table_stride, int c
              const int32_t* cu, const int32_t* starts, int sequences, int64_t vectors,
              int64_t pages, int page_size, hipStream_t st) {
   const dim3 block(kKvLanes);
-  if (two_units(a)) {
+  const int tokens = (int)(vectors / a.heads);
+  dim3 by;
+  if (by_tokens(a) && token_grid(a, tokens, four_tokens(a, tokens) ? 4 : 1, &by)) {
+#define MCOP_READ(NU, TW)                                                                         \
+  hipLaunchKernelGGL((k_kv_cache_read_tokens<E, FMT, WHOLE, NU, TW>), by, block, 0, st, a, table, \
+                     table_stride, columns, cu, starts, sequences, tokens, pages, page_size)
+    if (two_units(a)) {
+      if (four_tokens(a, tokens)) MCOP_READ(2, 4);
+      else MCOP_READ(2, 1);
+    } else {
+      if (four_tokens(a, tokens)) MCOP_READ(1, 4);
+      else MCOP_READ(1, 1);
+    }
+#undef MCOP_READ
+  } else if (two_units(a)) {
     hipLaunchKernelGGL((k_kv_cache_read<E, FMT, WHOLE, 2, 1>), dim3(kv_blocks(a, vectors, 1), 2),
                        block, 0, st, a, table, table_stride, columns, cu, starts, sequences,
                        (uint32_t)vectors, pages, page_size);

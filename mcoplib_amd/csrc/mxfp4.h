@@ -140,8 +140,10 @@ __device__ __forceinline__ void mx_widen8(float* f, uint32_t codes, uint32_t e) 
   f[4] = c[0] * s, f[5] = c[1] * s, f[6] = d[0] * s, f[7] = d[1] * s;
 }
 
-// Eight values as one or two 16-byte accesses, streamed or not, at any element alignment (LOOSE).
-template <class T, bool LOOSE, bool NT = true>
+// Eight values as one 16-byte access, streamed, or (fp32) two, each half of every 32 bytes and therefore
+// not: streamed, the halves went to memory apart (65536 tokens of 8 x 128 read to fp32 257 us, LATER
+// so).  LOOSE: at any element alignment.
+template <class T, bool LOOSE, bool NT = (sizeof(T) < 4)>
 __device__ __forceinline__ Pack<T, 8> load8(const T* p) {
   constexpr int N = 16 / (int)sizeof(T) < 8 ? 16 / (int)sizeof(T) : 8, K = 8 / N;
   constexpr int F = LOOSE ? FORM_RAGGED : FORM_ROWS;
@@ -162,7 +164,8 @@ __device__ __forceinline__ void store8(T* p, const Pack<T, 8>& v) {
     Pack<T, N> o;
 #pragma unroll
     for (int e = 0; e < N; ++e) o.v[e] = v.v[k * N + e];
-    stf_nt<(LOOSE ? FORM_RAGGED : FORM_ROWS), T, N>(p + k * N, o);
+    if constexpr (K == 1) stf_nt<(LOOSE ? FORM_RAGGED : FORM_ROWS), T, N>(p + k * N, o);
+    else __builtin_memcpy(p + k * N, &o, sizeof(o));
   }
 }
 
