@@ -44,12 +44,14 @@ struct KvSides {
   Divisor by_heads, by_page;
 };
 
-// The eight (or, past the vector's end, fewer) elements of unit j.
+// The eight (or, past the vector's end, fewer) elements of a unit: not WHOLE, at any alignment where there
+// are eight, else one by one (all of them so, 65536 tokens of 8 x 61 int8 read in 125 us, LATER so).
 template <class E, bool WHOLE>
 __device__ __forceinline__ Pack<typename E::S, 8> load_unit(const typename E::S* p, int n) {
   if constexpr (WHOLE) {
-    return load8<typename E::S, false>(p);
+    return load8<typename E::S, false, false>(p);
   } else {
+    if (n >= 8) return load8<typename E::S, true, false>(p);
     Pack<typename E::S, 8> v;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v.v[e] = e < n ? p[e] : typename E::S(0);
@@ -61,6 +63,8 @@ __device__ __forceinline__ void store_unit(T* p, const Pack<T, 8>& v, int n) {
   if constexpr (WHOLE) {
     if constexpr (sizeof(T) == 1) st_nt<T, 8>(p, v);
     else store8<T, false>(p, v);
+  } else if (n >= 8) {
+    __builtin_memcpy(p, &v, sizeof(v));
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -77,7 +81,7 @@ __device__ __forceinline__ void store_dword(uint8_t* p, uint32_t v) {
 template <bool WHOLE>
 __device__ __forceinline__ uint32_t load_dword(const uint8_t* p) {
   uint32_t v;
-  if constexpr (WHOLE) v = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+  if constexpr (WHOLE) v = *reinterpret_cast<const uint32_t*>(p);
   else __builtin_memcpy(&v, p, 4);
   return v;
 }
@@ -252,14 +256,18 @@ k_kv_cache_write_tokens(KvSides a, const int64_t* __restrict__ slots, int tokens
       v[i][n] = load_unit<E, WHOLE>(src + (h * k.p_head + at[n]), left[n]);
     }
   }
+  // lane i looks for token i: one wait for all of them
+  const int mine = min(t0 + (lane < TW ? lane : 0), tokens - 1);
+  const int64_t slot = slots[mine];
+  const bool in = slot >= 0 && slot < num_slots;
+  const uint32_t my_page = a.by_page.quotient(in ? (uint32_t)slot : 0u);
+  const uint32_t my_off = (in ? (uint32_t)slot : 0u) - my_page * (uint32_t)page_size;
   int64_t dst[TW], s_at[TW];
   bool store[TW];
 #pragma unroll
   for (int i = 0; i < TW; ++i) {
-    const int64_t slot = slots[min(t0 + i, tokens - 1)];
-    store[i] = t0 + i < tokens && slot >= 0 && slot < num_slots;
-    const uint32_t in = store[i] ? (uint32_t)slot : 0u;
-    const uint32_t page = a.by_page.quotient(in), off = in - page * (uint32_t)page_size;
+    store[i] = t0 + i < tokens && __builtin_amdgcn_readlane((int)in, i) != 0;
+    const uint32_t page = lane_value(my_page, i), off = lane_value(my_off, i);
     dst[i] = page * k.c_page + off * k.c_token;
     s_at[i] = page * k.s_page + off * k.s_token;
   }
@@ -295,7 +303,9 @@ __device__ __forceinline__ KvUnit<FMT> load_codes(const uint8_t* src, const void
     u.e = static_cast<const uint8_t*>(scales)[s_at + (unit >> 2)];
   } else {
     if constexpr (WHOLE) {
-      u.q = ld_nt<uint8_t, 8>(src + unit * 8);
+      u.q = ld<uint8_t, 8>(src + unit * 8);
+    } else if (left >= 8) {
+      __builtin_memcpy(&u.q, src + unit * 8, 8);
     } else {
 #pragma unroll
       for (int b = 0; b < 8; ++b) u.q.v[b] = b < left ? src[unit * 8 + b] : 0;
@@ -421,15 +431,19 @@ k_kv_cache_read_tokens(KvSides a, const int32_t* __restrict__ table, int64_t tab
   const int t0 = (int)k.by_passes.quotient(item) * TW;
   const int pass = (int)(item - k.by_passes.quotient(item) * k.by_passes.d);
   if (t0 >= tokens) return;
-  int s = uniform_int(sequence_of(cu, sequences, t0));
+  // lane i looks for token i: one way through the tables for all of them (token after token in scalar
+  // registers, 65536 tokens of 8 x 128 int8 took 78 us)
+  const int mine = min(t0 + (lane < TW ? lane : 0), tokens - 1);
+  int s = sequence_of(cu, sequences, t0);
+  uint32_t my_page, my_off;
+  const int my_state = find_token(mine, s, cu, starts, sequences, table, table_stride, columns, pages,
+                                  page_size, a.by_page, &my_page, &my_off);
   int64_t src[TW], s_at[TW];
   int state[TW];
 #pragma unroll
   for (int i = 0; i < TW; ++i) {
-    uint32_t page = 0, off = 0;
-    state[i] = t0 + i >= tokens ? 0
-                                : find_token(t0 + i, s, cu, starts, sequences, table, table_stride,
-                                             columns, pages, page_size, a.by_page, &page, &off);
+    state[i] = t0 + i < tokens ? __builtin_amdgcn_readlane(my_state, i) : 0;
+    const uint32_t page = lane_value(my_page, i), off = lane_value(my_off, i);
     src[i] = page * k.c_page + off * k.c_token;
     s_at[i] = page * k.s_page + off * k.s_token;
   }
