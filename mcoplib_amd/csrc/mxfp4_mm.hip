@@ -22,7 +22,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kFp4 = 4;  // operand format of the matrix instructions
 
 // VEC values of a row from column n on, of those inside its N: one store at any alignment, but at the
-// row's end (one element a store took 24 us for 1237 x 4099 fp32, this 11).
+// row's end (memory takes vectors at any address).
 template <class S, int VEC, bool NT>
 __device__ __forceinline__ void store_row(S* to, const Pack<S, VEC>& v, int n, int N, bool whole) {
   if (whole) {
@@ -62,54 +62,45 @@ __device__ __forceinline__ void scale_dwords(uint32_t (&v)[KS], const uint8_t* r
   }
 }
 
-// Few rows: a workgroup makes 16 MT rows x 16 NT columns of the output, its W waves every W-th chunk of
+// Few rows: a workgroup makes 16 rows x 16 columns of the output, its W waves every W-th chunk of
 // KS * 128 along K, straight from memory to registers, one chunk ahead; the partial sums meet in LDS
-// and are added in the waves' order.  What bounds it is the weights' way from HBM: each is read by one
-// wave, and the rows of a, which every workgroup reads, come from the caches.
+// and are added in the waves' order.  It has the shortest way to its first product, and takes operands
+// of any size; what bounds it then are its loads, 64 bytes of each of 16 rows, which a CU's cache answers
+// at 36 bytes a nanosecond (whole lines: 120).
 // In instruction s of a chunk the lane of group g = lane / 16 has block 4 s + g, so that a load takes 64
 // bytes in a row of 16 rows; its scale is byte g of the row's dword s.
-template <class E, int MT, int NT, int W, int KS>
+template <class E, int W, int KS>
 __global__ void __launch_bounds__(64 * W)
 k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
                 const uint8_t* __restrict__ as, const uint8_t* __restrict__ b,
                 const uint8_t* __restrict__ bs, const typename E::S* __restrict__ bias, int M, int N,
                 int blocks) {
   using S = typename E::S;
-  constexpr int T = MT + NT, CHUNK = 4 * KS;  // operands, blocks
-  __shared__ f32x4 part[W][MT * NT][64];
+  constexpr int CHUNK = 4 * KS;  // blocks
+  __shared__ f32x4 part[W][64];
   const int lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = (int)blockIdx.x * 16 * NT, m0 = (int)blockIdx.y * 16 * MT;
-  // rows past an operand's end repeat its last
-  const uint8_t* code_row[T];
-  const uint8_t* scale_row[T];
-#pragma unroll
-  for (int o = 0; o < T; ++o) {
-    const int64_t row = o < NT ? min(n0 + 16 * o + r, N - 1) : min(m0 + 16 * (o - NT) + r, M - 1);
-    code_row[o] = (o < NT ? b : a) + (row * blocks + g) * 16;
-    scale_row[o] = (o < NT ? bs : as) + row * blocks;
-  }
-  f32x4 sum[NT][MT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-#pragma unroll
-    for (int j = 0; j < MT; ++j) sum[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  const int n0 = (int)blockIdx.x * 16, m0 = (int)blockIdx.y * 16;
+  // b's row and a's; rows past an operand's end repeat its last
+  const int64_t row[2] = {min(n0 + r, N - 1), min(m0 + r, M - 1)};
+  const uint8_t* code_row[2] = {b + (row[0] * blocks + g) * 16, a + (row[1] * blocks + g) * 16};
+  const uint8_t* scale_row[2] = {bs + row[0] * blocks, as + row[1] * blocks};
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
   struct Chunk {
-    i32x4 code[T][KS];
-    uint32_t scale[T][KS];
+    i32x4 code[2][KS];
+    uint32_t scale[2][KS];
   };
   auto load = [&](Chunk& c, int k, auto whole) {  // the chunk from block k on
     constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-    for (int o = 0; o < T; ++o) {
+    for (int o = 0; o < 2; ++o) {
       scale_dwords<KS, WHOLE>(c.scale[o], scale_row[o], k, blocks);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int64_t at = (int64_t)(k + 4 * s) * 16;
         if constexpr (WHOLE) {
-          if (o < NT) {
+          if (o == 0) {
             c.code[o][s] = __builtin_nontemporal_load(
                 reinterpret_cast<const i32x4*>(code_row[o] + at));
           } else {
@@ -127,18 +118,9 @@ k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   auto multiply = [&](const Chunk& c) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      int sc[T];
-#pragma unroll
-      for (int o = 0; o < T; ++o) sc[o] = (int)(c.scale[o][s] >> (8 * g));
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          sum[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              fp4_operand(c.code[i][s]), fp4_operand(c.code[NT + j][s]), sum[i][j], kFp4, kFp4, 0,
-              sc[i], 0, sc[NT + j]);
-        }
-      }
+      sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+          fp4_operand(c.code[0][s]), fp4_operand(c.code[1][s]), sum, kFp4, kFp4, 0,
+          (int)(c.scale[0][s] >> (8 * g)), 0, (int)(c.scale[1][s] >> (8 * g)));
     }
   };
   const int whole = blocks / CHUNK;
@@ -169,37 +151,27 @@ k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     load(even, whole * CHUNK, std::false_type());
     multiply(even);
   }
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-#pragma unroll
-    for (int j = 0; j < MT; ++j) part[wave][i * MT + j][lane] = sum[i][j];
-  }
+  part[wave][lane] = sum;
   __syncthreads();
-  // four n of one m a thread
-  const bool quads = N % 4 == 0 && ((uintptr_t)out & (4 * sizeof(S) - 1)) == 0;
+  if (wave != 0) return;
+  f32x4 v = part[0][lane];
 #pragma unroll
-  for (int e0 = 0; e0 < MT * NT * 64; e0 += 64 * W) {
-    const int e = e0 + (int)threadIdx.x;
-    if (MT * NT % W != 0 && e >= MT * NT * 64) break;
-    const int tile = e >> 6, l = e & 63;
-    f32x4 v = part[0][tile][l];
+  for (int w = 1; w < W; ++w) v += part[w][lane];
+  const int m = m0 + r, n = n0 + 4 * g;  // four n of one m a lane
+  if (m >= M || n >= N) return;
+  Pack<S, 4> o;
 #pragma unroll
-    for (int w = 1; w < W; ++w) v += part[w][tile][l];
-    const int m = m0 + tile % MT * 16 + (l & 15), n = n0 + tile / MT * 16 + (l >> 4) * 4;
-    if (m >= M || n >= N) continue;
-    Pack<S, 4> o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (bias != nullptr) v[i] += E::to_f(bias[min(n + i, N - 1)]);
-      o.v[i] = E::from_f(v[i]);
-    }
-    store_row<S, 4, false>(out + (int64_t)m * N + n, o, n, N, quads);
+  for (int i = 0; i < 4; ++i) {
+    if (bias != nullptr) v[i] += E::to_f(bias[min(n + i, N - 1)]);
+    o.v[i] = E::from_f(v[i]);
   }
+  const bool quads = N % 4 == 0 && ((uintptr_t)out & (4 * sizeof(S) - 1)) == 0;
+  store_row<S, 4, false>(out + (int64_t)m * N + n, o, n, N, quads);
 }
 
-// Many rows: a group of WD x WD waves makes a (32 WD FM) x (32 WD FN) tile of the output, each wave
-// FM x FN products of 32 x 32; KS such groups of a workgroup share out K and add up in LDS at the end.  Codes go from
-// memory to LDS in tiles of 256 along K (128 bytes a row: whole lines), two tiles in turn, without
+// Tiles: a group of WD x WD waves makes a (32 WD FM) x (32 WD FN) tile of the output, each wave FM x FN
+// products of 32 x 32; KS such groups of a workgroup share out K and add up in LDS at the end.  Codes go
+// from memory to LDS in tiles of 256 along K (128 bytes a row: whole lines), D tiles in turn, without
 // passing through registers; from there to registers three steps of 64 along K ahead of the products.
 // In 32x32x64 instructions the lane of group g = lane / 32 takes blocks 4g..4g+3 of a tile, one a step, so
 // that the scales of its row for the tile are one dword, whose bytes the instructions pick in turn.
@@ -210,9 +182,10 @@ k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 // direct load writes 64 x 16 bytes in lane order (eight rows), so each lane's address is that of the
 // chunk that belongs at its place.
 //
-// One barrier a tile (none for a group of one wave), after the first step's products: the tile's last operands are in registers by
-// then, the wave waits for its part of the next tile, meets the others, reads on from the next tile and
-// starts the loads of the one after it, into the tile that all have finished reading.
+// One barrier a tile (none for a group of one wave), after the first step's products: the tile's last
+// operands are in registers by then, the wave waits for its part of the next tile, meets the others,
+// reads on from the next tile and starts the loads of the tile D on, into the one that all have read.
+// Of what it waits for the scales are the youngest: every fourth tile waits for all loads.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 
@@ -234,8 +207,9 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, const uint8_t* base, ui
       : "s"(to), "v"(off), "s"(base)
       : "memory", "m0");
 }
+template <int LEFT>
 __device__ __forceinline__ void wait_loads() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
 }
 __device__ __forceinline__ void wait_lds() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -245,7 +219,7 @@ __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
 }
 
-template <class E, int FM, int FN, int WD, int KS>
+template <class E, int FM, int FN, int WD, int KS, int D>
 __global__ void __launch_bounds__(64 * WD * WD * KS, 1)
 k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
                 const uint8_t* __restrict__ as, const uint8_t* __restrict__ b,
@@ -255,7 +229,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   constexpr int GW = WD * WD, THREADS = 64 * GW * KS;  // waves of a group
   constexpr int BM = 32 * WD * FM, BN = 32 * WD * FN, ROWS = BM + BN;
   constexpr int TILE = ROWS * kRowBytes, SCALES = ROWS * kScaleBytes;
-  constexpr int GROUP = 2 * (TILE + SCALES);  // LDS of a group
+  constexpr int GROUP = D * TILE + 2 * SCALES;  // LDS of a group
   constexpr int ALOADS = BM / 8 / GW, LOADS = ROWS / 8 / GW;  // direct loads of a wave and tile
   constexpr int SR = ROWS * 2 / (64 * GW);                    // 16-byte scale pieces of a thread
   __shared__ alignas(1024) uint8_t lds_all[KS * GROUP];
@@ -265,7 +239,15 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   const int tid = (int)threadIdx.x & (64 * GW - 1);
   const int wm = wave % WD, wn = wave / WD;
   uint8_t* lds = lds_all + part * GROUP;
-  const int m0 = (int)blockIdx.x % tiles_m * BM, n0 = (int)blockIdx.x / tiles_m * BN;
+  // Workgroups go to the eight dies in turn.  Each die takes consecutive tiles of an order in bands of 8
+  // along M, so that those it has at a time share rows of both operands in its L2: with tiles counted
+  // along M alone 1237 x 4099 x 5152 took 36.9 us, this 30.8.  The grid is a multiple of 8.
+  const int tile = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+  const int band_tiles = 8 * ((N + BN - 1) / BN), band = tile / band_tiles, in = tile % band_tiles;
+  const int high = min(8, tiles_m - band * 8);  // of the last band
+  if (high <= 0) return;
+  const int m0 = (band * 8 + in % high) * BM, n0 = in / high * BN;
+  if (n0 >= N) return;
   const int64_t pitch = (int64_t)blocks * 16;
 
   // The group's tiles: `tiles` from block `from` on, which may pass the rows' end.  What is past it
@@ -338,7 +320,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
         sv[k] = __builtin_bit_cast(i32x4, u64x2{lo, hi});
       }
     }
-    uint8_t* to = lds + 2 * TILE + (s & 1) * SCALES + tid * 16;
+    uint8_t* to = lds + D * TILE + (s & 1) * SCALES + tid * 16;
 #pragma unroll
     for (int k = 0; k < SR; ++k) *reinterpret_cast<i32x4*>(to + k * 1024 * GW) = sv[k];
   };
@@ -363,7 +345,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     }
   };
   auto read_scales = [&](int o, int t, int into) {
-    const int place = 2 * TILE + (t / kScaleTiles & 1) * SCALES + t % kScaleTiles * kTileK + 4 * g;
+    const int place = D * TILE + (t / kScaleTiles & 1) * SCALES + t % kScaleTiles * kTileK + 4 * g;
     if (o < FM) {
       sa[into][o] = *reinterpret_cast<const int*>(lds + place + (am + 32 * o) * kScaleBytes);
     } else {
@@ -421,7 +403,12 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   for (int j = 0; j < LOADS; ++j) load_rows(j, 1, 1);
   have_scales();
   store_scales(0);
-  wait_loads();
+  wait_loads<0>();
+#pragma unroll
+  for (int u = 2; u < D; ++u) {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) load_rows(j, u, u);
+  }
   wait_lds();
   if constexpr (GW > 1) meet();
 #pragma unroll
@@ -434,14 +421,23 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 #pragma unroll
     for (int o = 0; o < OPS; ++o) read_codes(o, 0, u);
   }
+  int cur = 0;
   for (int t = 0; t + 1 < tiles; ++t) {
-    const int cur = t & 1;
+    const int next = cur + 1 < D ? cur + 1 : 0;
     __builtin_amdgcn_sched_barrier(0);
     step(S0(), [&](int q) { reading(q, cur, 3); });
     here();
-    if (t % kScaleTiles == kScaleTiles - 1) store_scales(t / kScaleTiles + 1);
-    wait_loads();
-    have_scales();
+    if constexpr (D > 2) {
+      if (t % kScaleTiles == kScaleTiles - 1) {
+        have_scales();
+        store_scales(t / kScaleTiles + 1);
+      }
+      wait_loads<(D - 2) * LOADS>();
+    } else {
+      if (t % kScaleTiles == kScaleTiles - 1) store_scales(t / kScaleTiles + 1);
+      wait_loads<0>();
+      have_scales();
+    }
     wait_lds();
     if constexpr (GW > 1) meet();
     if (t % kScaleTiles == 0) load_scales(t / kScaleTiles + 1);
@@ -449,11 +445,11 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     auto loading = [&](int q, int s) {  // over the steps but the first
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
-        if (j * LSTEPS * MMS / LOADS == q + s * MMS) load_rows(j, t + 2, cur);
+        if (j * LSTEPS * MMS / LOADS == q + s * MMS) load_rows(j, t + D, cur);
       }
     };
     step(S1(), [&](int q) {
-      reading(q, cur ^ 1, 0);
+      reading(q, next, 0);
 #pragma unroll
       for (int o = 0; o < OPS; ++o) {
         if (o * MMS / 2 / OPS == q) read_scales(o, t + 1, 1);
@@ -461,25 +457,26 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
       loading(q, 0);
     });
     step(S2(), [&](int q) {
-      reading(q, cur ^ 1, 1);
+      reading(q, next, 1);
       loading(q, 1);
     });
     step(S3(), [&](int q) {
-      reading(q, cur ^ 1, 2);
+      reading(q, next, 2);
       loading(q, 2);
     });
 #pragma unroll
     for (int i = 0; i < FM; ++i) sa[0][i] = sa[1][i];
 #pragma unroll
     for (int i = 0; i < FN; ++i) sb[0][i] = sb[1][i];
+    cur = next;
   }
 #pragma unroll
-  for (int o = 0; o < OPS; ++o) read_codes(o, (tiles - 1) & 1, 3);
+  for (int o = 0; o < OPS; ++o) read_codes(o, cur, 3);
   step(S0(), [](int) {});
   step(S1(), [](int) {});
   step(S2(), [](int) {});
   step(S3(), [](int) {});
-  wait_loads();  // the loads past the last tile, before other uses of their LDS
+  wait_loads<0>();  // the loads past the last tile, before other uses of their LDS
   meet();        // every wave has read its last operands
 
   // A lane holds n = 8 (e / 4) + 4 g + e % 4 of m = lane % 32 of each product: 8 or 16 bytes in a row.
@@ -507,10 +504,10 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     __syncthreads();
     constexpr int PER = BN / VEC;  // lanes a row
 #pragma unroll
-    for (int k = 0; k < BM * PER / THREADS; ++k) {
+    for (int k = 0; k < (BM * PER + THREADS - 1) / THREADS; ++k) {
       const int at = k * THREADS + (int)threadIdx.x, r = at / PER, c = at % PER * VEC;
       const int m = m0 + r, n = n0 + c;
-      if (m >= M || n >= N) continue;
+      if (r >= BM || m >= M || n >= N) continue;
       Pack<S, VEC> v;
 #pragma unroll
       for (int h = 0; h < VEC / 4; ++h) {
@@ -531,7 +528,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     // 32 rows of each wave at a time
     constexpr int WN = 32 * FN, LINE = WN * (int)sizeof(S) + 16;
     constexpr int ADD = GW * 32 * LINE;  // the bias, behind the waves' rows
-    static_assert(ADD + BN * 4 <= 2 * TILE, "what reuses the tiles");
+    static_assert(ADD + BN * 4 <= D * TILE, "what reuses the tiles");
     if (bias != nullptr) {
       for (int c = tid; c < BN; c += 64 * GW) {
         *reinterpret_cast<float*>(lds + ADD + c * 4) = E::to_f(bias[min(n0 + c, N - 1)]);
@@ -580,55 +577,64 @@ static int64_t tiles_of(int M, int N, int bm, int bn) {
 // Whether the tile kernel's 32-bit offsets and its reads of 16 scale bytes fit the operands.
 static bool tiles_fit(int M, int N, int blocks) {
   return (int64_t)blocks * 16 * 256 < ((int64_t)1 << 32) && (int64_t)M * blocks >= 16 &&
-         (int64_t)N * blocks >= 16 && tiles_of(M, N, 64, 64) <= INT32_MAX;
+         (int64_t)N * blocks >= 16;
 }
 
-template <class E, int FM, int FN, int WD, int KS>
+template <class E, int FM, int FN, int WD, int KS, int D = 2>
 static int product_tiles(typename E::S* out, const uint8_t* a, const uint8_t* as, const uint8_t* b,
                          const uint8_t* bs, const typename E::S* bias, int M, int N, int blocks,
                          hipStream_t st) {
   constexpr int BM = 32 * WD * FM, BN = 32 * WD * FN;
   const int tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN;
   const int tiles = (blocks + kTileK * KS - 1) / (kTileK * KS);  // of a group
-  hipLaunchKernelGGL((k_mxfp4_mm_tile<E, FM, FN, WD, KS>), dim3((unsigned)(tm * tn)),
+  hipLaunchKernelGGL((k_mxfp4_mm_tile<E, FM, FN, WD, KS, D>), dim3((unsigned)((tm * tn + 7) / 8 * 8)),
                      dim3(64 * WD * WD * KS), 0, st, out, a, as, b, bs, bias, M, N, blocks, tm, tiles);
   return check_launch("mxfp4_scaled_mm");
 }
 
 // The form for a product: the one of the lowest estimated time.  The estimates (us) are fits to calls of
-// every form over M from 8 to 4096, N from 512 to 8192 and K of 512, 2048 and 8192 (bf16, operands from
-// HBM): a part for the launch, one for each round of workgroups on the 256 CUs, and one for the way
-// along K.  Measured where one gives way to the next (K = 8192 unless given):
-//   rows (16 x 16 straight from memory) and 32 x 64: 32 x 512 7.8 and 7.4, 64 x 4099 31.6 and 10.2;
-//     K = 512 128 x 2048 4.8 and 5.1
-//   32 x 64 and 64 x 64 without barriers: 64 x 4099 10.2 and 11.8, 128 x 4099 20.5 and 12.7
-//   those 64 x 64, one workgroup a CU, and 64 x 64 with barriers, four: 512 x 2048 15.9 and 20.3, 256 x
-//     8192 29.9 and 35.1; K = 512 14.8 and 5.9 (512 x 4099)
-//   64 x 64 and 128 x 128: 1024 x 2048 22.0 and 26.7, 512 x 8192 48.0 and 30.2
-//   128 x 128 and 256 x 256: 1024 x 8192 50.9 and 51.7, 2048 x 8192 86.0 and 73.8, 4096 x 4099 (272
-//     tiles of the larger) 100 and 114
-enum MmForm { MM_ROWS, MM_32X64, MM_64X64_APART, MM_64X64, MM_128X128, MM_256X256 };
+// every form over M from 1 to 4096, N from 512 to 16384 and K from 512 to 12288 (bf16, operands from
+// HBM); what they choose takes 1.6% more than the best form on average there.  Measured (us) where one
+// gives way to the next (M x N x K):
+//   rows (16 x 16, straight from memory) and 32 x 32 of four waves: 1 x 512 x 5120 4.5 and 5.2, 1 x 8192 x
+//     5120 8.2 and 7.0, 16 x 8192 x 12288 20.0 and 14.6
+//   32 x 32 of four waves and of eight, whose LDS is a whole CU's: 1 x 4099 x 12288 10.0 and 8.2, 48 x 4099
+//     x 5120 (two rounds) 8.0 and 11.1
+//   32 x 32 and 64 x 64 of four waves, without barriers: 48 x 8192 x 12288 19.0 and 21.6, 48 x 16384 x
+//     12288 36.7 and 26.8, 100 x 8192 x 5120 12.8 and 9.8
+//   the latter and 64 x 64 with barriers: 256 x 8192 x 5120 18.0 and 15.0, 256 x 8192 x 512 10.2 and 5.0,
+//     100 x 16384 x 12288 41.2 and 44.4
+//   64 x 64 and 128 x 128: 700 x 4099 x 5120 18.5 and 16.3, 256 x 4099 x 5120 14.4 and 16.0, 700 x 1500 x
+//     512 4.9 and 6.4
+//   128 x 128 and 256 x 256: 700 x 8192 x 5120 23.8 and 33.3, 2048 x 4099 x 5120 43.2 and 37.8, 4096 x 4099
+//     x 5120 (272 tiles of the larger) 69.6 and 78.2
+enum MmForm { MM_ROWS, MM_32X32_LONG, MM_32X32, MM_64X64_APART, MM_64X64, MM_128X128, MM_256X256 };
 
 static MmForm form_of(int M, int N, int blocks) {
   auto waves = [&](int bm, int bn) {  // workgroups of such tiles a CU
     return (double)((M + bm - 1) / bm) * ((N + bn - 1) / bn) / 256.0;
   };
+  auto part = [](double w) { return (w + std::ceil(w)) / 2; };  // rounds, where the last is not full
   const double k = blocks / 256.0;  // in units of K = 8192
-  double best = 3.3 + std::max(4.5 * k, waves(16, 16) * k * (3.5 + 2.5 * k));
+  double w = waves(16, 16);
+  double best = 3.2 + k * (w <= 1 ? (M == 1 ? 3.2 : 4.8) : w * (3.5 + 2.5 * k));
   MmForm form = MM_ROWS;
   auto offer = [&](MmForm f, double us) {
-    if (us < best) best = us, form = f;
+    if (us < best && w < 65000) best = us, form = f;  // a launch takes fewer than 2^32 threads
   };
   if (!tiles_fit(M, N, blocks)) return MM_ROWS;
-  double w = waves(32, 64);
-  offer(MM_32X64, w <= 1 ? 4.7 + k * (3.5 + 6 * w) : 3.3 + std::ceil(w) * (3 + 6 * k));
+  w = waves(32, 32);
+  if (w <= 1) offer(MM_32X32_LONG, 3.8 + k * (2.6 + 3.7 * w * w));
+  offer(MM_32X32, w <= 1   ? 3.5 + k * (4 + 2.8 * w * w)
+                  : w <= 2 ? 3.4 + k * (2 + 4.2 * w)
+                           : 2 + part(w) * (0.9 + 5.7 * k));
   w = waves(64, 64);
-  offer(MM_64X64_APART, w <= 1 ? 5.5 + k * (4 + 6 * w) : 3.3 + std::ceil(w) * (4 + 8 * k));
-  offer(MM_64X64, std::max(3.7 + 15.5 * k, 3.5 + w * (0.1 + 10 * k)));
+  offer(MM_64X64_APART, w <= 1 ? 4.6 + k * (5 + 8 * w) : 3.3 + std::ceil(w) * (4 + 8 * k));
+  offer(MM_64X64, std::max(3.7 + 15.5 * k, 3.5 + w * (0.25 + 7.7 * k)));
   w = waves(128, 128);
-  offer(MM_128X128, w <= 1   ? 3.9 + 21 * k
-                    : w <= 2 ? 3.9 + k * (7 + 20 * w)
-                             : 3 + w * (2.6 + 20.5 * k));
+  offer(MM_128X128, w <= 1   ? 5 + k * (14 + 6 * w)
+                    : w <= 2 ? 4 + k * (6 + 17 * w)
+                             : 3 + part(w) * (2.6 + 20.5 * k));
   w = waves(256, 256);
   offer(MM_256X256, w <= 1 ? 8 + k * (36 + 30 * w * w) : std::ceil(w) * (6 + 64 * k));
   return form;
@@ -641,16 +647,24 @@ static int product(void* out, const uint8_t* a, const uint8_t* as, const uint8_t
   auto* o = static_cast<S*>(out);
   const auto* bi = static_cast<const S*>(bias);
   switch (form_of(M, N, blocks)) {
-    case MM_32X64: return product_tiles<E, 1, 2, 1, 4>(o, a, as, b, bs, bi, M, N, blocks, st);
+    case MM_32X32_LONG:
+      return product_tiles<E, 1, 1, 1, 8>(o, a, as, b, bs, bi, M, N, blocks, st);
+    case MM_32X32: return product_tiles<E, 1, 1, 1, 4>(o, a, as, b, bs, bi, M, N, blocks, st);
     case MM_64X64_APART:
       return product_tiles<E, 2, 2, 1, 4>(o, a, as, b, bs, bi, M, N, blocks, st);
     case MM_64X64: return product_tiles<E, 1, 1, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
-    case MM_128X128: return product_tiles<E, 2, 2, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
+    case MM_128X128:
+      // one workgroup a CU has room for a third tile in flight: 1024 x 4096 x 5120 17.7 us, 20.3 with two;
+      // where two share a CU they overlap, 2048 x 4096 x 4096 23.5 us and 28.0
+      if (tiles_of(M, N, 128, 128) <= 256) {
+        return product_tiles<E, 2, 2, 2, 1, 3>(o, a, as, b, bs, bi, M, N, blocks, st);
+      }
+      return product_tiles<E, 2, 2, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
     case MM_256X256: return product_tiles<E, 4, 4, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
     default: break;
   }
   const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), block(256);
-  hipLaunchKernelGGL((k_mxfp4_mm_rows<E, 1, 1, 4, 4>), grid, block, 0, st, o, a, as, b, bs, bi, M, N,
+  hipLaunchKernelGGL((k_mxfp4_mm_rows<E, 4, 4>), grid, block, 0, st, o, a, as, b, bs, bi, M, N,
                      blocks);
   return check_launch("mxfp4_scaled_mm");
 }
@@ -672,10 +686,10 @@ extern "C" int mcop_mxfp4_scaled_mm(void* out, mcop_dtype out_dtype, const uint8
                      (long long)K);
   }
   if (M == 0 || N == 0) return MCOP_OK;
-  // the grid: at most 2^31 - 1 workgroups along N, 65535 along M
-  if (N > ((int64_t)1 << 30) || M > (int64_t)65535 * 16) {
+  // the grid: at most 65535 workgroups along M, and fewer than 2^32 threads along N
+  if (N > ((int64_t)1 << 27) || M > (int64_t)65535 * 16) {
     return set_error(MCOP_E_UNSUPPORTED, "%s: M %lld or N %lld is more than one launch takes "
-                     "(%d and 2^30)", name, (long long)M, (long long)N, 65535 * 16);
+                     "(%d and 2^27)", name, (long long)M, (long long)N, 65535 * 16);
   }
   if (!out || !a || !a_scales || !b || !b_scales) {
     return set_error(MCOP_E_INVALID, "%s: null pointer", name);
