@@ -133,3 +133,38 @@ def test_random_shapes():
         a, b = _operand(M, K, i), _operand(N, K, 100 + i)
         ref = (_values(a) @ _values(b).t()).float()
         assert mx_plain.same(_product(a, b, shift=i % 2), ref), (M, N, K)
+
+
+# Sizes of every way the product is made, each with rows and columns inside a tile and tails of K of one
+# block, or none.
+LARGE = [(16, 8192, 8224), (3, 2050, 9248), (33, 4099, 8224), (40, 16400, 4128), (100, 8192, 5152),
+         (100, 4099, 2080), (130, 2050, 4128), (700, 4099, 1056), (1030, 2050, 1568),
+         (700, 4099, 5152), (900, 4099, 4128), (2300, 1700, 512), (2300, 1700, 544),
+         (2100, 2050, 2080), (1300, 4099, 1056), (2500, 2500, 544), (2100, 4100, 3104),
+         (3000, 3001, 1056), (4000, 4001, 544), (4096, 4096, 512)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N,K", LARGE)
+def test_exact_sums_of_large_products(M, N, K, dtype):
+    """As test_exact_sums; the rounding to bf16 of an exact sum is one too.  The 64-bit product is
+    made on the device."""
+    say(f"mxfp4 mm large {M}x{N}x{K} {dtype}")
+    a, b = _operand(M, K, M + K), _operand(N, K, N + 3 * K)
+    ref = (_values(a).to(DEV) @ _values(b).to(DEV).t()).to(torch.float32).to(dtype)
+    got = _product(a, b, dtype, shift=3)
+    assert torch.equal(got, ref), int((got != ref).sum())
+    bias = torch.randint(-8, 9, (N,), generator=torch.Generator().manual_seed(5)).to(dtype)
+    ref = (_values(a).to(DEV) @ _values(b).to(DEV).t() + bias.to(DEV).double()).float().to(dtype)
+    assert torch.equal(_product(a, b, dtype, bias.to(DEV)), ref)
+
+
+@pytest.mark.parametrize("M,N,K", [(70, 4099, 2080), (900, 4099, 4128), (2100, 4100, 3104)])
+def test_nan_scales_in_large_products(M, N, K):
+    a, b = _operand(M, K, 1), _operand(N, K, 2)
+    rows, columns = [0, 31, M - 1], [5, 64, N - 1]
+    a[1][rows, K // 32 - 1], b[1][columns, 3] = 255, 255
+    a[0][rows], b[0][columns] = 0x22, 0x22
+    nan = torch.zeros(M, N, dtype=torch.bool)
+    nan[rows], nan[:, columns] = True, True
+    assert torch.equal(torch.isnan(_product(a, b)).cpu(), nan)
