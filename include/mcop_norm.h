@@ -283,8 +283,9 @@ int mcop_rms_norm_mxfp4_quant(uint8_t* out, uint8_t* scales, const void* input, 
 /* Product of two such operands: out[m, n] = round(sum_k a[m, k] * b[n, k] (+ bias[n])), summed in
  * fp32. a: codes [M, K / 2], scales [M, K / 32]; b: [N, K / 2], [N, K / 32]; all contiguous, codes
  * aligned to 16 bytes. out [M, N] and bias [N] (or NULL) are out_dtype (bf16, fp16, fp32). K is a
- * multiple of 32. Needs no workspace. A NaN scale makes its row (of a) or column (of b) NaN. The order
- * of the sum depends on M, N and K only. No counterpart in the reference. */
+ * multiple of 32, M at most 1048560, N at most 2^27. Needs no workspace. A NaN scale makes its row (of
+ * a) or column (of b) NaN. The order of the sum depends on M, N and K only. No counterpart in the
+ * reference. */
 int mcop_mxfp4_scaled_mm(void* out, mcop_dtype out_dtype, const uint8_t* a,
                          const uint8_t* a_scales, const uint8_t* b, const uint8_t* b_scales,
                          const void* bias, int64_t M, int64_t N, int64_t K, void* stream);

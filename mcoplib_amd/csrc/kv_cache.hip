@@ -558,11 +558,13 @@ int kv_sides(const char* name, const mcop_kv_side* key, const mcop_kv_side* valu
   return MCOP_OK;
 }
 
+// A launch takes fewer than 2^32 threads along x.
+constexpr int64_t kMostBlocks = ((int64_t)1 << 32) / kKvLanes - 1;
+
 // Workgroups for `vectors` vectors at `r` rounds a workgroup, of the side that needs more.
-unsigned kv_blocks(const KvSides& a, int64_t vectors, int r) {
-  const int lanes = a.side[0].lanes > a.side[1].lanes ? a.side[0].lanes : a.side[1].lanes;
-  const int64_t per = (int64_t)kKvLanes / lanes * r;
-  return (unsigned)((vectors + per - 1) / per);
+int64_t kv_blocks(const KvSides& a, int64_t vectors, int r) {
+  const int64_t per = (int64_t)kKvLanes / std::max(a.side[0].lanes, a.side[1].lanes) * r;
+  return (vectors + per - 1) / per;
 }
 
 bool two_units(const KvSides& a) { return a.side[0].dim > 512 || a.side[1].dim > 512; }
@@ -576,86 +578,105 @@ int64_t head_passes(const KvSides& a) {
   const int lanes = std::max(a.side[0].lanes, a.side[1].lanes);
   return ((int64_t)a.heads * lanes + 63) / 64;
 }
-bool token_grid(const KvSides& a, int64_t tokens, int tw, dim3* grid) {
+int64_t token_blocks(const KvSides& a, int64_t tokens, int tw) {
   const int64_t items = (tokens + tw - 1) / tw * head_passes(a), waves = kKvLanes / 64;
-  *grid = dim3((unsigned)((items + waves - 1) / waves), 2);
-  return items + waves <= INT32_MAX;
+  return (items + waves - 1) / waves;
+}
+// Whether a launch takes so many workgroups; sets the grid, or the error.
+bool kv_grid(const char* name, int64_t blocks, dim3* grid) {
+  *grid = dim3((unsigned)blocks, 2);
+  if (blocks <= kMostBlocks) return true;
+  set_error(MCOP_E_UNSUPPORTED, "%s: more vectors than one launch takes (%lld workgroups)", name,
+            (long long)blocks);
+  return false;
 }
 // Tokens a wave: four where that leaves 4096 waves or more, else one.
 bool four_tokens(const KvSides& a, int64_t tokens) { return tokens * head_passes(a) >= 8192; }
 
 template <class E, int FMT, bool WHOLE>
-void write_of(const KvSides& a, const int64_t* slots, int64_t vectors, int64_t num_slots,
-              int page_size, hipStream_t st) {
-  const dim3 grid(kv_blocks(a, vectors, 1), 2), block(kKvLanes);
+int write_of(const char* name, const KvSides& a, const int64_t* slots, int64_t vectors,
+             int64_t num_slots, int page_size, hipStream_t st) {
+  const dim3 block(kKvLanes);
+  dim3 grid;
   const int tokens = (int)(vectors / a.heads);
-  dim3 by;
-  if (by_tokens(a) && token_grid(a, tokens, four_tokens(a, tokens) ? 4 : 1, &by)) {
-#define MCOP_WRITE(NU, TW)                                                                        \
-  hipLaunchKernelGGL((k_kv_cache_write_tokens<E, FMT, WHOLE, NU, TW>), by, block, 0, st, a, slots, \
-                     tokens, num_slots, page_size)
+  if (by_tokens(a)) {
+    const bool four = four_tokens(a, tokens);
+    if (!kv_grid(name, token_blocks(a, tokens, four ? 4 : 1), &grid)) return MCOP_E_UNSUPPORTED;
+#define MCOP_WRITE(NU, TW)                                                                       \
+  hipLaunchKernelGGL((k_kv_cache_write_tokens<E, FMT, WHOLE, NU, TW>), grid, block, 0, st, a, \
+                     slots, tokens, num_slots, page_size)
     if (two_units(a)) {
-      if (four_tokens(a, tokens)) MCOP_WRITE(2, 4);
+      if (four) MCOP_WRITE(2, 4);
       else MCOP_WRITE(2, 1);
     } else {
-      if (four_tokens(a, tokens)) MCOP_WRITE(1, 4);
+      if (four) MCOP_WRITE(1, 4);
       else MCOP_WRITE(1, 1);
     }
 #undef MCOP_WRITE
-  } else if (two_units(a)) {
-    hipLaunchKernelGGL((k_kv_cache_write<E, FMT, WHOLE, 2>), grid, block, 0, st, a, slots,
-                       (uint32_t)vectors, num_slots, page_size);
   } else {
-    hipLaunchKernelGGL((k_kv_cache_write<E, FMT, WHOLE, 1>), grid, block, 0, st, a, slots,
-                       (uint32_t)vectors, num_slots, page_size);
+    if (!kv_grid(name, kv_blocks(a, vectors, 1), &grid)) return MCOP_E_UNSUPPORTED;
+    if (two_units(a)) {
+      hipLaunchKernelGGL((k_kv_cache_write<E, FMT, WHOLE, 2>), grid, block, 0, st, a, slots,
+                         (uint32_t)vectors, num_slots, page_size);
+    } else {
+      hipLaunchKernelGGL((k_kv_cache_write<E, FMT, WHOLE, 1>), grid, block, 0, st, a, slots,
+                         (uint32_t)vectors, num_slots, page_size);
+    }
   }
+  return check_launch(name);
 }
 
 template <class E, int FMT, bool WHOLE>
-void read_of(const KvSides& a, const int32_t* table, int64_t table_stride, int columns,
-             const int32_t* cu, const int32_t* starts, int sequences, int64_t vectors,
-             int64_t pages, int page_size, hipStream_t st) {
+int read_of(const char* name, const KvSides& a, const int32_t* table, int64_t table_stride,
+            int columns, const int32_t* cu, const int32_t* starts, int sequences, int64_t vectors,
+            int64_t pages, int page_size, hipStream_t st) {
   const dim3 block(kKvLanes);
+  dim3 grid;
   const int tokens = (int)(vectors / a.heads);
-  dim3 by;
-  if (by_tokens(a) && token_grid(a, tokens, four_tokens(a, tokens) ? 4 : 1, &by)) {
-#define MCOP_READ(NU, TW)                                                                         \
-  hipLaunchKernelGGL((k_kv_cache_read_tokens<E, FMT, WHOLE, NU, TW>), by, block, 0, st, a, table, \
-                     table_stride, columns, cu, starts, sequences, tokens, pages, page_size)
+  if (by_tokens(a)) {
+    const bool four = four_tokens(a, tokens);
+    if (!kv_grid(name, token_blocks(a, tokens, four ? 4 : 1), &grid)) return MCOP_E_UNSUPPORTED;
+#define MCOP_READ(NU, TW)                                                                        \
+  hipLaunchKernelGGL((k_kv_cache_read_tokens<E, FMT, WHOLE, NU, TW>), grid, block, 0, st, a,     \
+                     table, table_stride, columns, cu, starts, sequences, tokens, pages, page_size)
     if (two_units(a)) {
-      if (four_tokens(a, tokens)) MCOP_READ(2, 4);
+      if (four) MCOP_READ(2, 4);
       else MCOP_READ(2, 1);
     } else {
-      if (four_tokens(a, tokens)) MCOP_READ(1, 4);
+      if (four) MCOP_READ(1, 4);
       else MCOP_READ(1, 1);
     }
 #undef MCOP_READ
-  } else if (two_units(a)) {
-    hipLaunchKernelGGL((k_kv_cache_read<E, FMT, WHOLE, 2, 1>), dim3(kv_blocks(a, vectors, 1), 2),
-                       block, 0, st, a, table, table_stride, columns, cu, starts, sequences,
-                       (uint32_t)vectors, pages, page_size);
   } else {
-    hipLaunchKernelGGL((k_kv_cache_read<E, FMT, WHOLE, 1, 4>), dim3(kv_blocks(a, vectors, 4), 2),
-                       block, 0, st, a, table, table_stride, columns, cu, starts, sequences,
-                       (uint32_t)vectors, pages, page_size);
+    const int rounds = two_units(a) ? 1 : 4;
+    if (!kv_grid(name, kv_blocks(a, vectors, rounds), &grid)) return MCOP_E_UNSUPPORTED;
+    if (two_units(a)) {
+      hipLaunchKernelGGL((k_kv_cache_read<E, FMT, WHOLE, 2, 1>), grid, block, 0, st, a, table,
+                         table_stride, columns, cu, starts, sequences, (uint32_t)vectors, pages,
+                         page_size);
+    } else {
+      hipLaunchKernelGGL((k_kv_cache_read<E, FMT, WHOLE, 1, 4>), grid, block, 0, st, a, table,
+                         table_stride, columns, cu, starts, sequences, (uint32_t)vectors, pages,
+                         page_size);
+    }
   }
+  return check_launch(name);
 }
 
-// f.template operator()<E, FMT, WHOLE>() for the launch's types.
+// f(E, FMT, WHOLE) for the launch's types.
 template <class F>
-void for_types(mcop_dtype dtype, int fmt, bool whole, F f) {
+int for_types(mcop_dtype dtype, int fmt, bool whole, F f) {
   auto by_form = [&](auto e, auto m) {
-    if (whole) f(e, m, std::true_type());
-    else f(e, m, std::false_type());
+    return whole ? f(e, m, std::true_type()) : f(e, m, std::false_type());
   };
   auto by_format = [&](auto e) {
-    if (fmt == KV_INT8) by_form(e, std::integral_constant<int, KV_INT8>());
-    else if (fmt == KV_FP8) by_form(e, std::integral_constant<int, KV_FP8>());
-    else by_form(e, std::integral_constant<int, KV_MXFP4>());
+    if (fmt == KV_INT8) return by_form(e, std::integral_constant<int, KV_INT8>());
+    if (fmt == KV_FP8) return by_form(e, std::integral_constant<int, KV_FP8>());
+    return by_form(e, std::integral_constant<int, KV_MXFP4>());
   };
-  if (dtype == MCOP_BF16) by_format(BF16());
-  else if (dtype == MCOP_F16) by_format(F16());
-  else by_format(F32());
+  if (dtype == MCOP_BF16) return by_format(BF16());
+  if (dtype == MCOP_F16) return by_format(F16());
+  return by_format(F32());
 }
 
 }  // namespace
@@ -680,11 +701,10 @@ extern "C" int mcop_kv_cache_write_quant(const mcop_kv_side* key, const mcop_kv_
   if (!slot_mapping) return set_error(MCOP_E_INVALID, "%s: null pointer", name);
   if (num_pages == 0) return MCOP_OK;  // no slot to write to
   auto st = static_cast<hipStream_t>(stream);
-  for_types(in_dtype, fmt, whole, [&](auto e, auto m, auto w) {
-    write_of<decltype(e), decltype(m)::value, decltype(w)::value>(
-        a, slot_mapping, num_tokens * num_heads, num_pages * page_size, (int)page_size, st);
+  return for_types(in_dtype, fmt, whole, [&](auto e, auto m, auto w) {
+    return write_of<decltype(e), decltype(m)::value, decltype(w)::value>(
+        name, a, slot_mapping, num_tokens * num_heads, num_pages * page_size, (int)page_size, st);
   });
-  return check_launch(name);
 }
 
 extern "C" int mcop_kv_cache_read_dequant(const mcop_kv_side* key, const mcop_kv_side* value,
@@ -715,10 +735,9 @@ extern "C" int mcop_kv_cache_read_dequant(const mcop_kv_side* key, const mcop_kv
     return set_error(MCOP_E_INVALID, "%s: null pointer", name);
   }
   auto st = static_cast<hipStream_t>(stream);
-  for_types(out_dtype, fmt, whole, [&](auto e, auto m, auto w) {
-    read_of<decltype(e), decltype(m)::value, decltype(w)::value>(
-        a, block_table, table_row_stride, (int)table_columns, cu_seqlens, seq_starts,
+  return for_types(out_dtype, fmt, whole, [&](auto e, auto m, auto w) {
+    return read_of<decltype(e), decltype(m)::value, decltype(w)::value>(
+        name, a, block_table, table_row_stride, (int)table_columns, cu_seqlens, seq_starts,
         (int)num_sequences, num_tokens * num_heads, num_pages, (int)page_size, st);
   });
-  return check_launch(name);
 }

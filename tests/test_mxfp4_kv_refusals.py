@@ -217,6 +217,7 @@ def test_c_abi_refuses_bad_arguments_without_a_device():
     refused(lib.mcop_mxfp4_scaled_mm(p, 0, ctypes.c_void_p(24), p, p, p, None, 4, 8, 64, None),
             "aligned to 16")
     refused(lib.mcop_mxfp4_scaled_mm(p, 0, p, p, p, p, None, 1 << 40, 8, 64, None), "one launch", -2)
+    refused(lib.mcop_mxfp4_scaled_mm(p, 0, p, p, p, p, None, 4, 1 << 28, 64, None), "one launch", -2)
     assert lib.mcop_mxfp4_scaled_mm(None, 0, None, None, None, None, None, 0, 8, 64, None) == 0
 
     def write(k, v, fmt=3, pages=2, page=16, heads=2, tokens=4, dtype=0, slots=p):
@@ -231,6 +232,11 @@ def test_c_abi_refuses_bad_arguments_without_a_device():
     refused(write(good, good, pages=1 << 30, page=2), "2^31 - 1 slots")
     refused(write(good, good, tokens=1 << 31), "2^31 vectors", -2)
     refused(write(good, good, slots=None), "null pointer")
+    # 2^32 threads or more: 2^30 vectors of 8 lanes, and four times 2^26 vectors of 64 lanes by fours
+    refused(write(good, good, tokens=1 << 29), "one launch", -2)
+    refused(write(_side(head_size=512), good, tokens=1 << 28), "one launch", -2)
+    wide = _side(head_size=512)
+    refused(write(wide, wide, tokens=1 << 27), "one launch", -2)
     refused(write(_side(head_size=0), good), "key head_size 0")
     refused(write(good, _side(head_size=1025)), "value head_size 1025")
     refused(write(_side(head_size=48), good, fmt=5), "multiple of the block")
