@@ -228,10 +228,10 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   using S = typename E::S;
   constexpr int GW = WD * WD, THREADS = 64 * GW * KS;  // waves of a group
   constexpr int BM = 32 * WD * FM, BN = 32 * WD * FN, ROWS = BM + BN;
-  constexpr int TILE = ROWS * kRowBytes, SCALES = ROWS * kScaleBytes;
+  constexpr int SR = (ROWS * 2 + 64 * GW - 1) / (64 * GW);  // 16-byte scale pieces of a thread
+  constexpr int TILE = ROWS * kRowBytes, SCALES = SR * 32 * GW * kScaleBytes;
   constexpr int GROUP = D * TILE + 2 * SCALES;  // LDS of a group
   constexpr int ALOADS = BM / 8 / GW, LOADS = ROWS / 8 / GW;  // direct loads of a wave and tile
-  constexpr int SR = ROWS * 2 / (64 * GW);                    // 16-byte scale pieces of a thread
   __shared__ alignas(1024) uint8_t lds_all[KS * GROUP];
   const int lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) & (GW - 1);  // of its group
@@ -593,8 +593,8 @@ static int product_tiles(typename E::S* out, const uint8_t* a, const uint8_t* as
 }
 
 // The form for a product: the one of the lowest estimated time.  The estimates (us) are fits to calls of
-// every form over M from 1 to 4096, N from 512 to 16384 and K from 512 to 12288 (bf16, operands from
-// HBM); what they choose takes 1.6% more than the best form on average there.  Measured (us) where one
+// every form over M from 1 to 4096, N from 512 to 16384 and K from 512 to 14336 (bf16; weights of several
+// sets in turn); what they choose takes 1% more than the best form on average there.  Measured (us) where one
 // gives way to the next (M x N x K):
 //   rows (16 x 16, straight from memory) and 32 x 32 of four waves: 1 x 512 x 5120 4.5 and 5.2, 1 x 8192 x
 //     5120 8.2 and 7.0, 16 x 8192 x 12288 20.0 and 14.6
@@ -606,9 +606,13 @@ static int product_tiles(typename E::S* out, const uint8_t* a, const uint8_t* as
 //     100 x 16384 x 12288 41.2 and 44.4
 //   64 x 64 and 128 x 128: 700 x 4099 x 5120 18.5 and 16.3, 256 x 4099 x 5120 14.4 and 16.0, 700 x 1500 x
 //     512 4.9 and 6.4
+//   128 x 128 and 192 x 128, where the latter is one round: 1500 x 4096 x 4096 20.4 and 18.5, 700 x 8192 x
+//     5120 23.8 and 21.8, 2048 x 4096 x 4096 (1.4 rounds) 23.1 and 32.3
 //   128 x 128 and 256 x 256: 700 x 8192 x 5120 23.8 and 33.3, 2048 x 4099 x 5120 43.2 and 37.8, 4096 x 4099
 //     x 5120 (272 tiles of the larger) 69.6 and 78.2
-enum MmForm { MM_ROWS, MM_32X32_LONG, MM_32X32, MM_64X64_APART, MM_64X64, MM_128X128, MM_256X256 };
+enum MmForm {
+  MM_ROWS, MM_32X32_LONG, MM_32X32, MM_64X64_APART, MM_64X64, MM_128X128, MM_192X128, MM_256X256
+};
 
 static MmForm form_of(int M, int N, int blocks) {
   auto waves = [&](int bm, int bn) {  // workgroups of such tiles a CU
@@ -617,7 +621,7 @@ static MmForm form_of(int M, int N, int blocks) {
   auto part = [](double w) { return (w + std::ceil(w)) / 2; };  // rounds, where the last is not full
   const double k = blocks / 256.0;  // in units of K = 8192
   double w = waves(16, 16);
-  double best = 3.2 + k * (w <= 1 ? (M == 1 ? 3.2 : 4.8) : w * (3.5 + 2.5 * k));
+  double best = 2.9 + k * (w <= 1 ? (M == 1 ? 3.7 : 5.3) : w * (3 + 2.5 * k));
   MmForm form = MM_ROWS;
   auto offer = [&](MmForm f, double us) {
     if (us < best && w < 65000) best = us, form = f;  // a launch takes fewer than 2^32 threads
@@ -626,17 +630,19 @@ static MmForm form_of(int M, int N, int blocks) {
   w = waves(32, 32);
   if (w <= 1) offer(MM_32X32_LONG, 3.8 + k * (2.6 + 3.7 * w * w));
   offer(MM_32X32, w <= 1   ? 3.5 + k * (4 + 2.8 * w * w)
-                  : w <= 2 ? 3.4 + k * (2 + 4.2 * w)
+                  : w <= 2 ? 3.4 + k * (1.5 + 3.3 * w)
                            : 2 + part(w) * (0.9 + 5.7 * k));
   w = waves(64, 64);
   offer(MM_64X64_APART, w <= 1 ? 4.6 + k * (5 + 8 * w) : 3.3 + std::ceil(w) * (4 + 8 * k));
-  offer(MM_64X64, std::max(3.7 + 15.5 * k, 3.5 + w * (0.25 + 7.7 * k)));
+  offer(MM_64X64, std::max(3.7 + 15.5 * k, 3.5 + part(w) * ((w <= 4 ? 0.25 : 0.6) + 7.7 * k)));
   w = waves(128, 128);
-  offer(MM_128X128, w <= 1   ? 5 + k * (14 + 6 * w)
-                    : w <= 2 ? 4 + k * (6 + 17 * w)
-                             : 3 + part(w) * (2.6 + 20.5 * k));
+  offer(MM_128X128, w <= 1   ? 5.4 + k * (13.4 + 6 * w)
+                    : w <= 2 ? 4 + k * (25 + 7 * w)
+                             : 3 + part(w) * (2 + 20.5 * k));
+  w = waves(192, 128);
+  if (w <= 1) offer(MM_192X128, 5.5 + k * (21 + 5 * w));
   w = waves(256, 256);
-  offer(MM_256X256, w <= 1 ? 8 + k * (36 + 30 * w * w) : std::ceil(w) * (6 + 64 * k));
+  offer(MM_256X256, w <= 1 ? 8 + k * (36 + 30 * w * w) : std::ceil(w) * (8.5 + 61 * k));
   return form;
 }
 
@@ -660,6 +666,8 @@ static int product(void* out, const uint8_t* a, const uint8_t* as, const uint8_t
         return product_tiles<E, 2, 2, 2, 1, 3>(o, a, as, b, bs, bi, M, N, blocks, st);
       }
       return product_tiles<E, 2, 2, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
+    case MM_192X128:
+      return product_tiles<E, 3, 2, 2, 1, 3>(o, a, as, b, bs, bi, M, N, blocks, st);
     case MM_256X256: return product_tiles<E, 4, 4, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
     default: break;
   }

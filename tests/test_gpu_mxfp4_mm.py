@@ -141,7 +141,9 @@ LARGE = [(16, 8192, 8224), (3, 2050, 9248), (33, 4099, 8224), (40, 16400, 4128),
          (100, 4099, 2080), (130, 2050, 4128), (700, 4099, 1056), (1030, 2050, 1568),
          (700, 4099, 5152), (900, 4099, 4128), (2300, 1700, 512), (2300, 1700, 544),
          (2100, 2050, 2080), (1300, 4099, 1056), (2500, 2500, 544), (2100, 4100, 3104),
-         (3000, 3001, 1056), (4000, 4001, 544), (4096, 4096, 512)]
+         (3000, 3001, 1056), (4000, 4001, 544), (4096, 4096, 512), (500, 16300, 160),
+         (500, 16300, 288), (500, 16300, 544), (1237, 4099, 5152), (1500, 3001, 4128),
+         (250, 16300, 672), (250, 16300, 800)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
