@@ -14,6 +14,10 @@ Surfaces (same names, argument order and in-place conventions as the reference):
                              torch.ops._C.dynamic_scaled_int8_quant and
                              torch.ops._C.dynamic_per_token_scaled_fp8_quant
 
+Beyond the reference, in _C and custom_ops: mxfp4_quant, mxfp4_dequant, rms_norm_mxfp4_quant and
+mxfp4_scaled_mm (4-bit microscaled operands), kv_cache_write_quant and kv_cache_read_dequant (a
+paged key/value cache quantized as it is written).
+
 op and _C are C++ (csrc/torch_ops.cpp, built into _torch_ops.so) and custom_ops is Python, as
 in the reference; all of them call libmcop_norm.so (hand-written HIP kernels, C ABI in
 include/mcop_norm.h).  Importing the package fails if either library is not built: there is no

@@ -56,6 +56,8 @@ FOUR_WAVE_KERNELS = (
 # Exact-row forms, which the launch takes by the row's shape alone: none may spill.
 EXACT_KERNELS = (r"^void mcop::k_(rms_norm_quant|fused_add_rms_norm|rms_norm|rms_norm_smooth_quant|"
                  r"add_rms_norm_quant_padded|per_token_quant|rms_norm_group_quant)<.*, (true|1)>\(")
+# Kernels of the 4-bit operators and the quantized cache that a launch takes by shape alone.
+SHAPE_KERNELS = r"^void mcop::k_(mxfp4_(quant|dequant|mm_rows|mm_tile)|kv_cache_(write|read)(_tokens)?)<"
 RESOURCES = "resource_usage.json"
 
 
@@ -108,6 +110,7 @@ def check_resources(records: list[dict]) -> list[str]:
     """Problems with the compiled kernels' resources (empty = fine):
     - a multi-pass kernel (k_*_wide) that spills (they are launched without a resource check);
     - an exact-row form that spills (launched without a resource check too);
+    - a kernel of the 4-bit operators or the quantized cache that spills (launched by shape alone);
     - a split-row kernel that spills (the planner passes those over: nothing would launch it);
     - a kernel built with the four-waves request that spills or misses four waves per SIMD;
     - no kernel matching one of those requests (a renamed kernel would escape the check).
@@ -120,6 +123,8 @@ def check_resources(records: list[dict]) -> list[str]:
             bad.append(f"multi-pass kernel spills {r['scratch']} B/lane: {k}")
         if re.search(EXACT_KERNELS, k) and r.get("scratch", 0) != 0:
             bad.append(f"exact-row kernel spills {r['scratch']} B/lane: {k}")
+        if re.search(SHAPE_KERNELS, k) and r.get("scratch", 0) != 0:
+            bad.append(f"kernel spills {r['scratch']} B/lane: {k}")
         if "_split<" in k and r.get("scratch", 0) != 0:
             bad.append(f"split-row kernel spills {r['scratch']} B/lane: {k}")
     for pat in FOUR_WAVE_KERNELS:

@@ -251,3 +251,31 @@ def test_a_cache_past_32_bit_offsets(kind):
     key, _ = custom_ops.kv_cache_read_dequant(codes, codes, scales, scales, table, cu, T,
                                               torch.bfloat16)
     assert mx_plain.same(key, mx_plain.vector_values(q, s, kind, torch.bfloat16))
+
+
+# Tokens enough for waves of several, with a last wave that is not full; the sides differ in how many
+# waves a token takes.
+MANY = [(4101, 8, 128, 128), (2051, 16, 128, 32), (4099, 9, 61, 64), (8195, 1, 576, 512),
+        (8193, 3, 1024, 520)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T,heads,dk,dv", MANY)
+def test_write_many_tokens(T, heads, dk, dv, kind):
+    if kind == "mxfp4" and (dk % 32 or dv % 32):
+        pytest.skip("4-bit vectors are whole blocks of 32")
+    say(f"kv write {kind} {T} tokens of {heads} x {dk}/{dv}")
+    _check_write(kind, torch.bfloat16, T, heads, dk, dv, 16)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,heads,dk,dv", MANY)
+def test_read_many_tokens(T, heads, dk, dv, kind, dtype):
+    """Sequences of every length from 0 to 6 among long ones, so that a wave's tokens are of several."""
+    if kind == "mxfp4" and (dk % 32 or dv % 32):
+        pytest.skip("4-bit vectors are whole blocks of 32")
+    say(f"kv read {kind} {dtype} {T} tokens of {heads} x {dk}/{dv}")
+    lengths = [n % 7 for n in range(150)] + [700, 0, 0, 1]
+    lengths.append(T - sum(lengths))
+    _check_read(kind, dtype, lengths, [n % 5 for n in range(len(lengths))], heads, dk, dv, 16)

@@ -73,7 +73,7 @@ def test_one_step(kind, T):
     a = mx_plain.values(*mx_plain.quant(y))
     b = mx_plain.values(*mx_plain.quant(layer.qkv))
     qkv = a @ b.t() + layer.bias.cpu().double()
-    # bf16's rounding (2^-9 of the value, 2^-8 / 2) and H additions of at most a step of sum|ab| each
+    # bf16's rounding (half a step, 2^-8 of the value) and H additions of at most a step of sum|ab| each
     room = 2.0 ** -8 * qkv.abs() + H * 2.0 ** -22 * (a.abs() @ b.abs().t()) + 1e-6
     off = (v.cpu().double().flatten(1) - qkv[:, (QH + KH) * D:]).abs()
     assert bool((off <= room[:, (QH + KH) * D:]).all())
@@ -109,6 +109,34 @@ def test_captured_and_replayed(kind):
         for a, b in zip(outs, want):
             assert mx_plain.same(a, b), rep
         assert (nx * 2).sum().item() == (nx * 2).sum().item()
+
+
+def test_replayed_with_other_tables():
+    """Slots, block table and sequence lengths are read when a graph is replayed, not when it is made."""
+    T = 33
+    layer, eager = Layer("int8"), Layer("int8")
+    x, r = _inputs(T, 1)
+    slots, table, cu = _tables(T)
+    g = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer.step(x, r, slots, table, cu, T)
+        with torch.cuda.graph(g, stream=side):
+            outs = layer.step(x, r, slots, table, cu, T)
+    torch.cuda.current_stream().wait_stream(side)
+    for first in (0, 5, 32, 33):
+        pages = torch.randperm(8, generator=torch.Generator().manual_seed(first)).view(2, 4)
+        cpu_slots = [int(pages[0, p // PAGE]) * PAGE + p % PAGE for p in range(first)]
+        cpu_slots += [int(pages[1, p // PAGE]) * PAGE + p % PAGE for p in range(T - first)]
+        slots.copy_(torch.tensor(cpu_slots))
+        table.copy_(pages[:, :3])
+        cu.copy_(torch.tensor([0, first, T]))
+        g.replay()
+        want = eager.step(x, r, slots.clone(), table.clone(), cu.clone(), T)
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert mx_plain.same(a, b), first
 
 
 def test_on_another_stream():
