@@ -185,7 +185,7 @@ k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 // One barrier a tile (none for a group of one wave), after the first step's products: the tile's last
 // operands are in registers by then, the wave waits for its part of the next tile, meets the others,
 // reads on from the next tile and starts the loads of the tile D on, into the one that all have read.
-// Of what it waits for the scales are the youngest: every fourth tile waits for all loads.
+// Scales that pass through registers are waited for with all other loads, every fourth tile.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 
@@ -207,6 +207,16 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, const uint8_t* base, ui
       : "s"(to), "v"(off), "s"(base)
       : "memory", "m0");
 }
+// The same of four bytes a lane.
+__device__ __forceinline__ void load_to_lds4(uint32_t to, const uint8_t* base, uint32_t off) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %1, %2"
+      :
+      : "s"(to), "v"(off), "s"(base)
+      : "memory", "m0");
+}
 template <int LEFT>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
@@ -219,7 +229,10 @@ __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
 }
 
-template <class E, int FM, int FN, int WD, int KS, int D>
+// DS: rows of scales are whole dwords, and go to LDS by direct loads too, so that no tile waits for more
+// than its own (300 x 5000 x 4096: tiles of 128 x 64 three deep 11.7 us, 10.7 so; two deep every tile
+// waits for all loads anyway, and 4096 x 4096 x 8192 takes 69.1 us, 71.3 so).
+template <class E, int FM, int FN, int WD, int KS, int D, bool DS>
 __global__ void __launch_bounds__(64 * WD * WD * KS, 1)
 k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
                 const uint8_t* __restrict__ as, const uint8_t* __restrict__ b,
@@ -297,7 +310,19 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     to_end[k] =
         (int)min((int64_t)((row < BM ? M : N) - r) * blocks - from, (int64_t)1 << 30);
   }
+  const uint8_t* asbase = as + (int64_t)m0 * blocks + from;
+  const uint8_t* bsbase = bs + (int64_t)n0 * blocks + from;
+  auto direct_scales = [&](int s) {  // the rows of the codes' loads, a dword a lane; past the end the first
+    const int at = s * kScaleBytes + (lane & 7) * 4;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      load_to_lds4(lds0 + D * TILE + (s & 1) * SCALES + first_row(j) * kScaleBytes,
+                   j < ALOADS ? asbase : bsbase,
+                   (off[j] >> 4) - chunk_of(j) + (at < have ? at : 0));
+    }
+  };
   auto load_scales = [&](int s) {
+    if constexpr (DS) return direct_scales(s);
     const int at = s * kScaleBytes + piece;
 #pragma unroll
     for (int k = 0; k < SR; ++k) {
@@ -305,6 +330,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     }
   };
   auto store_scales = [&](int s) {
+    if constexpr (DS) return;
     if (have - s * kScaleBytes < kScaleBytes) {
       const int at = s * kScaleBytes + piece, left = min(max(have - at, 0), 16);
 #pragma unroll
@@ -325,6 +351,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     for (int k = 0; k < SR; ++k) *reinterpret_cast<i32x4*>(to + k * 1024 * GW) = sv[k];
   };
   auto have_scales = [&]() {  // waits for them here and not later, when other loads are in flight
+    if constexpr (DS) return;
 #pragma unroll
     for (int k = 0; k < SR; ++k) asm volatile("" : "+v"(sv[k]));
   };
@@ -345,12 +372,14 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
     }
   };
   auto read_scales = [&](int o, int t, int into) {
+    const bool in = !DS || t * kTileK + 4 * g < have;
     const int place = D * TILE + (t / kScaleTiles & 1) * SCALES + t % kScaleTiles * kTileK + 4 * g;
     if (o < FM) {
-      sa[into][o] = *reinterpret_cast<const int*>(lds + place + (am + 32 * o) * kScaleBytes);
+      const int v = *reinterpret_cast<const int*>(lds + place + (am + 32 * o) * kScaleBytes);
+      sa[into][o] = in ? v : 0;
     } else {
-      sb[into][o - FM] =
-          *reinterpret_cast<const int*>(lds + place + (bn + 32 * (o - FM)) * kScaleBytes);
+      const int v = *reinterpret_cast<const int*>(lds + place + (bn + 32 * (o - FM)) * kScaleBytes);
+      sb[into][o - FM] = in ? v : 0;
     }
   };
   f32x16 sum[FM][FN];
@@ -587,8 +616,16 @@ static int product_tiles(typename E::S* out, const uint8_t* a, const uint8_t* as
   constexpr int BM = 32 * WD * FM, BN = 32 * WD * FN;
   const int tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN;
   const int tiles = (blocks + kTileK * KS - 1) / (kTileK * KS);  // of a group
-  hipLaunchKernelGGL((k_mxfp4_mm_tile<E, FM, FN, WD, KS, D>), dim3((unsigned)((tm * tn + 7) / 8 * 8)),
-                     dim3(64 * WD * WD * KS), 0, st, out, a, as, b, bs, bias, M, N, blocks, tm, tiles);
+  const dim3 grid((unsigned)((tm * tn + 7) / 8 * 8)), block(64 * WD * WD * KS);
+  if constexpr (D > 2) {
+    if (blocks % 4 == 0 && aligned(4, as, bs)) {
+      hipLaunchKernelGGL((k_mxfp4_mm_tile<E, FM, FN, WD, KS, D, true>), grid, block, 0, st, out, a, as,
+                         b, bs, bias, M, N, blocks, tm, tiles);
+      return check_launch("mxfp4_scaled_mm");
+    }
+  }
+  hipLaunchKernelGGL((k_mxfp4_mm_tile<E, FM, FN, WD, KS, D, false>), grid, block, 0, st, out, a, as, b,
+                     bs, bias, M, N, blocks, tm, tiles);
   return check_launch("mxfp4_scaled_mm");
 }
 
@@ -600,18 +637,19 @@ static int product_tiles(typename E::S* out, const uint8_t* a, const uint8_t* as
 //     5120 8.2 and 7.0, 16 x 8192 x 12288 20.0 and 14.6
 //   32 x 32 of four waves and of eight, whose LDS is a whole CU's: 1 x 4099 x 12288 10.0 and 8.2, 48 x 4099
 //     x 5120 (two rounds) 8.0 and 11.1
-//   32 x 32 and 64 x 64 of four waves, without barriers: 48 x 8192 x 12288 19.0 and 21.6, 48 x 16384 x
-//     12288 36.7 and 26.8, 100 x 8192 x 5120 12.8 and 9.8
-//   the latter and 64 x 64 with barriers: 256 x 8192 x 5120 18.0 and 15.0, 256 x 8192 x 512 10.2 and 5.0,
-//     100 x 16384 x 12288 41.2 and 44.4
-//   64 x 64 and 128 x 128: 700 x 4099 x 5120 18.5 and 16.3, 256 x 4099 x 5120 14.4 and 16.0, 700 x 1500 x
-//     512 4.9 and 6.4
+//   32 x 32 and 64 x 64 of four waves, without barriers: 40 x 8192 x 14336 14.9 and 18.0, 100 x 6144 x 8192
+//     15.8 and 12.1
+//   the latter and 64 x 64 with barriers: 100 x 6144 x 8192 12.1 and 13.1, 64 x 16384 x 5120 12.9 and 10.3
+//   64 x 64 and 128 x 64, where the latter is one round: 256 x 8192 x 5120 13.4 and 12.5, 128 x 8192 x 8192
+//     16.2 and 19.1
+//   128 x 64 and 128 x 128: 1024 x 4096 x 5120 23.2 and 18.0, 256 x 8192 x 5120 12.5 and 15.3
 //   128 x 128 and 192 x 128, where the latter is one round: 1500 x 4096 x 4096 20.4 and 18.5, 700 x 8192 x
 //     5120 23.8 and 21.8, 2048 x 4096 x 4096 (1.4 rounds) 23.1 and 32.3
 //   128 x 128 and 256 x 256: 700 x 8192 x 5120 23.8 and 33.3, 2048 x 4099 x 5120 43.2 and 37.8, 4096 x 4099
 //     x 5120 (272 tiles of the larger) 69.6 and 78.2
 enum MmForm {
-  MM_ROWS, MM_32X32_LONG, MM_32X32, MM_64X64_APART, MM_64X64, MM_128X128, MM_192X128, MM_256X256
+  MM_ROWS, MM_32X32_LONG, MM_32X32, MM_64X64_APART, MM_64X64, MM_128X64, MM_128X128, MM_192X128,
+  MM_256X256
 };
 
 static MmForm form_of(int M, int N, int blocks) {
@@ -620,21 +658,27 @@ static MmForm form_of(int M, int N, int blocks) {
   };
   auto part = [](double w) { return (w + std::ceil(w)) / 2; };  // rounds, where the last is not full
   const double k = blocks / 256.0;  // in units of K = 8192
-  double w = waves(16, 16);
-  double best = 2.9 + k * (w <= 1 ? (M == 1 ? 3.7 : 5.3) : w * (3 + 2.5 * k));
+  double w = waves(16, 16), best = 1e30;
   MmForm form = MM_ROWS;
   auto offer = [&](MmForm f, double us) {
     if (us < best && w < 65000) best = us, form = f;  // a launch takes fewer than 2^32 threads
   };
+  offer(MM_ROWS, 2.9 + k * (w > 1 ? w * ((M > 16 ? 4.5 : 3) + 2.5 * k) : M == 1 ? 3.7 : 5.3));
   if (!tiles_fit(M, N, blocks)) return MM_ROWS;
   w = waves(32, 32);
   if (w <= 1) offer(MM_32X32_LONG, 3.8 + k * (2.6 + 3.7 * w * w));
   offer(MM_32X32, w <= 1   ? 3.5 + k * (4 + 2.8 * w * w)
-                  : w <= 2 ? 3.4 + k * (1.5 + 3.3 * w)
+                  : w <= 2 ? 3.2 + k * (1.5 + 2.8 * w)
                            : 2 + part(w) * (0.9 + 5.7 * k));
   w = waves(64, 64);
-  offer(MM_64X64_APART, w <= 1 ? 4.6 + k * (5 + 8 * w) : 3.3 + std::ceil(w) * (4 + 8 * k));
-  offer(MM_64X64, std::max(3.7 + 15.5 * k, 3.5 + part(w) * ((w <= 4 ? 0.25 : 0.6) + 7.7 * k)));
+  offer(MM_64X64_APART, w <= 1 ? std::max(5.2 + k * (6.2 + 1.5 * w),
+                                          4 + ((double)M + N) * blocks * 17 / 5e6)  // from memory
+                               : 3.3 + std::ceil(w) * (4 + 8 * k));
+  offer(MM_64X64, w <= 2   ? 3.2 + k * (9 + 2.5 * w)
+                  : w <= 4 ? 3.5 + part(w) * (0.25 + 7.7 * k)
+                           : 3.5 + part(w) * (0.6 + 7.7 * k));
+  w = waves(128, 64);
+  if (w <= 1) offer(MM_128X64, 3.7 + k * (10.5 + 2 * w));
   w = waves(128, 128);
   offer(MM_128X128, w <= 1   ? 5.4 + k * (13.4 + 6 * w)
                     : w <= 2 ? 4 + k * (25 + 7 * w)
@@ -658,7 +702,14 @@ static int product(void* out, const uint8_t* a, const uint8_t* as, const uint8_t
     case MM_32X32: return product_tiles<E, 1, 1, 1, 4>(o, a, as, b, bs, bi, M, N, blocks, st);
     case MM_64X64_APART:
       return product_tiles<E, 2, 2, 1, 4>(o, a, as, b, bs, bi, M, N, blocks, st);
-    case MM_64X64: return product_tiles<E, 1, 1, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
+    case MM_64X64:
+      // as below; two workgroups a CU: 128 x 8192 x 8192 16.2 us, 25.4 with two tiles; 1024 x 4096 x 5120
+      // (four a CU) 24.8 and 23.4
+      if (tiles_of(M, N, 64, 64) <= 512) {
+        return product_tiles<E, 1, 1, 2, 1, 3>(o, a, as, b, bs, bi, M, N, blocks, st);
+      }
+      return product_tiles<E, 1, 1, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
+    case MM_128X64: return product_tiles<E, 2, 1, 2, 1, 3>(o, a, as, b, bs, bi, M, N, blocks, st);
     case MM_128X128:
       // one workgroup a CU has room for a third tile in flight: 1024 x 4096 x 5120 17.7 us, 20.3 with two;
       // where two share a CU they overlap, 2048 x 4096 x 4096 23.5 us and 28.0

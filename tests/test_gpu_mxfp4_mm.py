@@ -143,7 +143,9 @@ LARGE = [(16, 8192, 8224), (3, 2050, 9248), (33, 4099, 8224), (40, 16400, 4128),
          (2100, 2050, 2080), (1300, 4099, 1056), (2500, 2500, 544), (2100, 4100, 3104),
          (3000, 3001, 1056), (4000, 4001, 544), (4096, 4096, 512), (500, 16300, 160),
          (500, 16300, 288), (500, 16300, 544), (1237, 4099, 5152), (1500, 3001, 4128),
-         (250, 16300, 672), (250, 16300, 800)]
+         (250, 16300, 672), (250, 16300, 800), (250, 16300, 768), (700, 4099, 5248),
+         (900, 4099, 4224), (250, 8100, 5152), (256, 8192, 5120), (400, 4099, 4224),
+         (64, 16300, 128), (64, 16300, 384), (500, 4000, 640), (500, 4000, 2176)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
