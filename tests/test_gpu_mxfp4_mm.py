@@ -172,3 +172,20 @@ def test_nan_scales_in_large_products(M, N, K):
     nan = torch.zeros(M, N, dtype=torch.bool)
     nan[rows], nan[:, columns] = True, True
     assert torch.equal(torch.isnan(_product(a, b)).cpu(), nan)
+
+
+def test_operands_past_32_bit_offsets():
+    """Weights of 8 GiB of codes: the columns at their end are those of the end alone (exact sums, so
+    that the forms of the two products do not matter)."""
+    N, K = (1 << 20) + 3, 16384
+    g = torch.Generator(device=DEV).manual_seed(4)
+    b = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8, device=DEV)
+    sb = torch.randint(127, 129, (N, K // 32), generator=g, dtype=torch.uint8, device=DEV)
+    for M in (1, 40):
+        say(f"mxfp4 mm {M}x{N}x{K}")
+        a, sa = (t.to(DEV) for t in _operand(M, K, M))
+        out = torch.empty(M, N, dtype=torch.float32, device=DEV)
+        torch.ops._C.mxfp4_scaled_mm(out, a, sa, b, sb, None)
+        for part in (slice(0, 70), slice(N - 131, N)):
+            ref = (_values((a, sa)) @ _values((b[part], sb[part])).t()).float()
+            assert mx_plain.same(out[:, part], ref)
