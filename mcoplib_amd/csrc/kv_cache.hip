@@ -572,7 +572,7 @@ bool two_units(const KvSides& a) { return a.side[0].dim > 512 || a.side[1].dim >
 // Whether a token's vectors fill a wave on both sides; the passes over its heads, of the side that has
 // more; and the workgroups for those.
 bool by_tokens(const KvSides& a) {
-  return a.heads * a.side[0].lanes >= 64 && a.heads * a.side[1].lanes >= 64;
+  return (int64_t)a.heads * std::min(a.side[0].lanes, a.side[1].lanes) >= 64;
 }
 int64_t head_passes(const KvSides& a) {
   const int lanes = std::max(a.side[0].lanes, a.side[1].lanes);

@@ -67,7 +67,8 @@ int main() {
     }
   }
   for (int64_t T : kRows) {
-    for (int64_t heads : {0, 1, 2, 8, 100000}) {
+    for (int64_t heads : {(int64_t)0, (int64_t)1, (int64_t)2, (int64_t)8, (int64_t)100000,
+                          (int64_t)1 << 26, (int64_t)1 << 30}) {
       for (int64_t D : {0, 8, 32, 61, 64, 128, 576, 1024, 1025}) {
         for (mcop_dtype c : {MCOP_I8, MCOP_FP8_E4M3FN, MCOP_MXFP4, MCOP_BF16}) {
           for (int mis : {0, 1}) {
