@@ -671,9 +671,10 @@ static MmForm form_of(int M, int N, int blocks) {
                   : w <= 2 ? 3.2 + k * (1.5 + 2.8 * w)
                            : 2 + part(w) * (0.9 + 5.7 * k));
   w = waves(64, 64);
-  offer(MM_64X64_APART, w <= 1 ? std::max(5.2 + k * (6.2 + 1.5 * w),
-                                          4 + ((double)M + N) * blocks * 17 / 5e6)  // from memory
-                               : 3.3 + std::ceil(w) * (4 + 8 * k));
+  if (w <= 1) {
+    const double memory = 4 + ((double)M + N) * blocks * 17 / 5e6;  // its operands' way, if that is longer
+    offer(MM_64X64_APART, std::max(5.2 + k * (6.2 + 1.5 * w), memory));
+  }
   offer(MM_64X64, w <= 2   ? 3.2 + k * (9 + 2.5 * w)
                   : w <= 4 ? 3.5 + part(w) * (0.25 + 7.7 * k)
                            : 3.5 + part(w) * (0.6 + 7.7 * k));
