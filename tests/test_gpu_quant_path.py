@@ -177,3 +177,44 @@ def test_torch_compile_aot_eager():
     got = torch.compile(step, backend="aot_eager", fullgraph=True)(x, r)
     for a, b in zip(got, want):
         assert mx_plain.same(a, b)
+
+
+@pytest.mark.parametrize("kind", ["fp8", "mxfp4"])
+def test_torch_compile_of_the_cache(kind):
+    """Writes to a cache are seen by the reads behind them, also where the graph is functionalized."""
+    layer, other, T = Layer(kind), Layer(kind), 45
+    slots, table, cu = _tables(T)
+    k = randn((T, KH, D), 5, torch.bfloat16).to(DEV)
+    v = randn((T, KH, D), 6, torch.bfloat16).to(DEV)
+
+    def step(k, v, kc, vc, ks, vs):
+        torch.ops._C.kv_cache_write_quant(k, v, kc, vc, ks, vs, slots)
+        key, value = torch.empty_like(k), torch.empty_like(v)
+        torch.ops._C.kv_cache_read_dequant(key, value, kc, vc, ks, vs, table, cu, None)
+        return key, value
+
+    want = step(k, v, *layer.cache, *layer.scale)
+    got = torch.compile(step, backend="aot_eager", fullgraph=True)(k, v, *other.cache, *other.scale)
+    for a, b in zip((*got, *other.cache, *other.scale), (*want, *layer.cache, *layer.scale)):
+        assert mx_plain.same(a, b)
+
+
+def test_two_streams_at_once():
+    """The same operators on two streams, on tensors of their own, give what each gives alone."""
+    layers = [Layer("int8"), Layer("mxfp4")]
+    T = 45
+    slots, table, cu = _tables(T)
+    x, r = _inputs(T, 9)
+    want = [[t.clone() for t in layer.step(x, r, slots, table, cu, T)] for layer in layers]
+    streams = [torch.cuda.Stream() for _ in layers]
+    got = []
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, layer in zip(streams, layers):
+            with torch.cuda.stream(s):
+                got.append(layer.step(x, r, slots, table, cu, T))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        for s, t in zip(a, b):
+            assert mx_plain.same(s, t)
