@@ -224,7 +224,10 @@ __device__ __forceinline__ void wait_loads() {
 __device__ __forceinline__ void wait_lds() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
+// The group's barrier, behind the wave's own LDS reads and writes: the barrier alone orders neither, and
+// what is read here may be written over by the next wave that has passed it.
 __device__ __forceinline__ void meet() {
+  wait_lds();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -415,6 +418,10 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
       if (o * MMS / 2 / OPS == q) read_codes(o, buf, s);
     }
   };
+  auto together = [&]() {  // the group's waves; one alone waits for itself
+    if constexpr (GW > 1) meet();
+    else wait_lds();
+  };
   // The products so far are made before this point: they touch no memory, and without it the compiler
   // moves them behind the barrier and the branches below, to where their results are next used.
   auto here = [&]() {
@@ -438,8 +445,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) load_rows(j, u, u);
   }
-  wait_lds();
-  if constexpr (GW > 1) meet();
+  together();
 #pragma unroll
   for (int o = 0; o < OPS; ++o) {
     read_codes(o, 0, 0);
@@ -467,8 +473,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
       wait_loads<0>();
       have_scales();
     }
-    wait_lds();
-    if constexpr (GW > 1) meet();
+    together();
     if (t % kScaleTiles == 0) load_scales(t / kScaleTiles + 1);
     __builtin_amdgcn_sched_barrier(0);
     auto loading = [&](int q, int s) {  // over the steps but the first
@@ -506,7 +511,7 @@ k_mxfp4_mm_tile(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
   step(S2(), [](int) {});
   step(S3(), [](int) {});
   wait_loads<0>();  // the loads past the last tile, before other uses of their LDS
-  meet();        // every wave has read its last operands
+  meet();           // every wave has read its last operands
 
   // A lane holds n = 8 (e / 4) + 4 g + e % 4 of m = lane % 32 of each product: 8 or 16 bytes in a row.
   // The rows are turned in LDS and stored 16 bytes a lane, whole lines in a row: as they are held, two
