@@ -196,26 +196,25 @@ constexpr int kRowBytes = kTileK * 16;
 // them; more at a time do not leave the room for two tiles of 256 x 256.
 constexpr int kScaleTiles = 4, kScaleBytes = kScaleTiles * kTileK;
 
-// 16 bytes a lane from base + off to LDS at `to` + 16 * lane.  The compiler does not see what this
-// writes nor that it is in flight: wait_loads() and the barrier order it.
+// 16 bytes a lane from base + off to LDS at `to` + 16 * lane, which the instruction takes from m0 (a state
+// after its write).  The compiler does not see what this writes nor that it is in flight: wait_loads()
+// and the barrier order it.
 __device__ __forceinline__ void load_to_lds(uint32_t to, const uint8_t* base, uint32_t off) {
   asm volatile(
-      "s_mov_b32 m0, %0\n\t"
       "s_nop 0\n\t"
       "global_load_lds_dwordx4 %1, %2"
       :
-      : "s"(to), "v"(off), "s"(base)
-      : "memory", "m0");
+      : "{m0}"(to), "v"(off), "s"(base)
+      : "memory");
 }
 // The same of four bytes a lane.
 __device__ __forceinline__ void load_to_lds4(uint32_t to, const uint8_t* base, uint32_t off) {
   asm volatile(
-      "s_mov_b32 m0, %0\n\t"
       "s_nop 0\n\t"
       "global_load_lds_dword %1, %2"
       :
-      : "s"(to), "v"(off), "s"(base)
-      : "memory", "m0");
+      : "{m0}"(to), "v"(off), "s"(base)
+      : "memory");
 }
 template <int LEFT>
 __device__ __forceinline__ void wait_loads() {
