@@ -71,6 +71,8 @@ def _load() -> ctypes.CDLL:
     lib.mcop_debug_set_launch_override.argtypes = [I, I]
     lib.mcop_debug_set_split_rows.argtypes = [I]
     lib.mcop_debug_fail_split_waits.argtypes = [I]
+    lib.mcop_debug_mxfp4_mm_form.argtypes = [I64, I64, I64, I]
+    lib.mcop_debug_mxfp4_mm_form.restype = ctypes.c_char_p
     for fn in ("mcop_fused_add_rms_norm", "mcop_rms_norm_dynamic_per_token_quant",
                "mcop_rms_norm_dynamic_per_token_quant_noalloc",
                "mcop_rms_norm_smooth_quant", "mcop_scale_dynamic_quant",
@@ -135,3 +137,9 @@ def fail_split_waits(on: bool = True) -> None:
     (their error word set before the kernel starts; a test hook for the failure path: such rows
     get NaN scales, or NaN outputs for the norms); False restores normal launches."""
     check(lib.mcop_debug_fail_split_waits(1 if on else 0))
+
+
+def mxfp4_mm_form(M: int, N: int, K: int, aligned_scales: bool = True) -> str:
+    """The kernel that mxfp4_scaled_mm runs for M x N x K, as its trace line names it (a debug hook for
+    tests; decided on the host); "" for sizes it refuses or has nothing to do for."""
+    return lib.mcop_debug_mxfp4_mm_form(M, N, K, 1 if aligned_scales else 0).decode()

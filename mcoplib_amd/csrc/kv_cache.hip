@@ -15,6 +15,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cstdio>
 
 #include "../../include/mcop_norm.h"
 #include "mxfp4.h"
@@ -590,6 +591,16 @@ bool kv_grid(const char* name, int64_t blocks, dim3* grid) {
             (long long)blocks);
   return false;
 }
+// The launch's trace line; a_wave: tokens a wave takes at a time, 0 where it takes vectors.
+void trace_kv(const char* name, const KvSides& a, int64_t tokens, bool whole, int a_wave,
+              const dim3& grid) {
+  if (!trace_enabled()) return;
+  char how[48] = "a vector a group of lanes";
+  if (a_wave > 0) snprintf(how, sizeof(how), "whole tokens a wave, %d at a time", a_wave);
+  trace_launch(name, "tokens=%lld heads=%d head sizes %d and %d: %s, %d units a lane, %s, wgs=%u x 2",
+               (long long)tokens, a.heads, a.side[0].dim, a.side[1].dim, how, two_units(a) ? 2 : 1,
+               whole ? "whole units" : "any alignment", grid.x);
+}
 // Tokens a wave: four where that leaves 4096 waves or more, else one.
 bool four_tokens(const KvSides& a, int64_t tokens) { return tokens * head_passes(a) >= 8192; }
 
@@ -602,6 +613,7 @@ int write_of(const char* name, const KvSides& a, const int64_t* slots, int64_t v
   if (by_tokens(a)) {
     const bool four = four_tokens(a, tokens);
     if (!kv_grid(name, token_blocks(a, tokens, four ? 4 : 1), &grid)) return MCOP_E_UNSUPPORTED;
+    trace_kv(name, a, tokens, WHOLE, four ? 4 : 1, grid);
 #define MCOP_WRITE(NU, TW)                                                                       \
   hipLaunchKernelGGL((k_kv_cache_write_tokens<E, FMT, WHOLE, NU, TW>), grid, block, 0, st, a, \
                      slots, tokens, num_slots, page_size)
@@ -615,6 +627,7 @@ int write_of(const char* name, const KvSides& a, const int64_t* slots, int64_t v
 #undef MCOP_WRITE
   } else {
     if (!kv_grid(name, kv_blocks(a, vectors, 1), &grid)) return MCOP_E_UNSUPPORTED;
+    trace_kv(name, a, tokens, WHOLE, 0, grid);
     if (two_units(a)) {
       hipLaunchKernelGGL((k_kv_cache_write<E, FMT, WHOLE, 2>), grid, block, 0, st, a, slots,
                          (uint32_t)vectors, num_slots, page_size);
@@ -636,6 +649,7 @@ int read_of(const char* name, const KvSides& a, const int32_t* table, int64_t ta
   if (by_tokens(a)) {
     const bool four = four_tokens(a, tokens);
     if (!kv_grid(name, token_blocks(a, tokens, four ? 4 : 1), &grid)) return MCOP_E_UNSUPPORTED;
+    trace_kv(name, a, tokens, WHOLE, four ? 4 : 1, grid);
 #define MCOP_READ(NU, TW)                                                                        \
   hipLaunchKernelGGL((k_kv_cache_read_tokens<E, FMT, WHOLE, NU, TW>), grid, block, 0, st, a,     \
                      table, table_stride, columns, cu, starts, sequences, tokens, pages, page_size)
@@ -650,6 +664,7 @@ int read_of(const char* name, const KvSides& a, const int32_t* table, int64_t ta
   } else {
     const int rounds = two_units(a) ? 1 : 4;
     if (!kv_grid(name, kv_blocks(a, vectors, rounds), &grid)) return MCOP_E_UNSUPPORTED;
+    trace_kv(name, a, tokens, WHOLE, 0, grid);
     if (two_units(a)) {
       hipLaunchKernelGGL((k_kv_cache_read<E, FMT, WHOLE, 2, 1>), grid, block, 0, st, a, table,
                          table_stride, columns, cu, starts, sequences, (uint32_t)vectors, pages,

@@ -57,6 +57,12 @@ int mcop_debug_set_split_rows(int enabled);
  * on = 0 restores normal launches. Calls that take no split-row kernel are unaffected. */
 int mcop_debug_fail_split_waits(int on);
 
+/* The kernel that mcop_mxfp4_scaled_mm runs for a product of M x N x K, in the words of its trace line;
+ * "" for sizes it refuses or has nothing to do for. aligned_scales: both scale tensors start at multiples
+ * of four bytes. Decided on the host alone, without a device. The text is the calling thread's until its
+ * next call. For the tests that name the form they check. */
+const char* mcop_debug_mxfp4_mm_form(int64_t M, int64_t N, int64_t K, int aligned_scales);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,8 +9,10 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdio>
 
 #include "../../include/mcop_norm.h"
+#include "mcop_testing.h"
 #include "mxfp4.h"
 
 namespace mcop {
@@ -616,13 +618,13 @@ static bool tiles_fit(int M, int N, int blocks) {
 template <class E, int FM, int FN, int WD, int KS, int D = 2>
 static int product_tiles(typename E::S* out, const uint8_t* a, const uint8_t* as, const uint8_t* b,
                          const uint8_t* bs, const typename E::S* bias, int M, int N, int blocks,
-                         hipStream_t st) {
+                         bool direct, hipStream_t st) {
   constexpr int BM = 32 * WD * FM, BN = 32 * WD * FN;
   const int tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN;
   const int tiles = (blocks + kTileK * KS - 1) / (kTileK * KS);  // of a group
   const dim3 grid((unsigned)((tm * tn + 7) / 8 * 8)), block(64 * WD * WD * KS);
   if constexpr (D > 2) {
-    if (blocks % 4 == 0 && aligned(4, as, bs)) {
+    if (direct) {
       hipLaunchKernelGGL((k_mxfp4_mm_tile<E, FM, FN, WD, KS, D, true>), grid, block, 0, st, out, a, as,
                          b, bs, bias, M, N, blocks, tm, tiles);
       return check_launch("mxfp4_scaled_mm");
@@ -695,38 +697,73 @@ static MmForm form_of(int M, int N, int blocks) {
   return form;
 }
 
+// A product's form, whether it has three tiles in flight, and whether scales go to LDS by direct loads.
+struct MmPlan {
+  MmForm form;
+  bool deep, direct;
+};
+static MmPlan plan_of(int M, int N, int blocks, bool aligned_scales) {
+  MmPlan p{form_of(M, N, blocks), false, false};
+  switch (p.form) {
+    case MM_64X64:
+      // as below; two workgroups a CU: 128 x 8192 x 8192 16.2 us, 25.4 with two tiles; 1024 x 4096 x 5120
+      // (four a CU) 24.8 and 23.4
+      p.deep = tiles_of(M, N, 64, 64) <= 512;
+      break;
+    case MM_128X128:
+      // one workgroup a CU has room for a third tile in flight: 1024 x 4096 x 5120 17.7 us, 20.3 with two;
+      // where two share a CU they overlap, 2048 x 4096 x 4096 23.5 us and 28.0
+      p.deep = tiles_of(M, N, 128, 128) <= 256;
+      break;
+    case MM_128X64:
+    case MM_192X128: p.deep = true; break;
+    default: break;
+  }
+  p.direct = p.deep && blocks % 4 == 0 && aligned_scales;
+  return p;
+}
+
+struct MmName {
+  char text[64];
+};
+static MmName name_of(const MmPlan& p) {
+  static const char* const forms[] = {"rows", "32x32 by eight waves", "32x32", "64x64 by waves apart",
+                                      "64x64", "128x64", "128x128", "192x128", "256x256"};
+  MmName n;
+  snprintf(n.text, sizeof(n.text), "%s%s%s", forms[p.form], p.deep ? ", three tiles" : "",
+           p.direct ? ", direct scales" : "");
+  return n;
+}
+
 template <class E>
 static int product(void* out, const uint8_t* a, const uint8_t* as, const uint8_t* b,
                    const uint8_t* bs, const void* bias, int M, int N, int blocks, hipStream_t st) {
   using S = typename E::S;
   auto* o = static_cast<S*>(out);
   const auto* bi = static_cast<const S*>(bias);
-  switch (form_of(M, N, blocks)) {
-    case MM_32X32_LONG:
-      return product_tiles<E, 1, 1, 1, 8>(o, a, as, b, bs, bi, M, N, blocks, st);
-    case MM_32X32: return product_tiles<E, 1, 1, 1, 4>(o, a, as, b, bs, bi, M, N, blocks, st);
-    case MM_64X64_APART:
-      return product_tiles<E, 2, 2, 1, 4>(o, a, as, b, bs, bi, M, N, blocks, st);
+  const MmPlan p = plan_of(M, N, blocks, aligned(4, as, bs));
+  if (trace_enabled()) {
+    trace_launch("mxfp4_scaled_mm", "M=%d N=%d K=%lld: %s", M, N, (long long)blocks * kMxBlock,
+                 name_of(p).text);
+  }
+#define MCOP_TILES(...) \
+  return product_tiles<E, __VA_ARGS__>(o, a, as, b, bs, bi, M, N, blocks, p.direct, st)
+  switch (p.form) {
+    case MM_32X32_LONG: MCOP_TILES(1, 1, 1, 8);
+    case MM_32X32: MCOP_TILES(1, 1, 1, 4);
+    case MM_64X64_APART: MCOP_TILES(2, 2, 1, 4);
     case MM_64X64:
-      // as below; two workgroups a CU: 128 x 8192 x 8192 16.2 us, 25.4 with two tiles; 1024 x 4096 x 5120
-      // (four a CU) 24.8 and 23.4
-      if (tiles_of(M, N, 64, 64) <= 512) {
-        return product_tiles<E, 1, 1, 2, 1, 3>(o, a, as, b, bs, bi, M, N, blocks, st);
-      }
-      return product_tiles<E, 1, 1, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
-    case MM_128X64: return product_tiles<E, 2, 1, 2, 1, 3>(o, a, as, b, bs, bi, M, N, blocks, st);
+      if (p.deep) MCOP_TILES(1, 1, 2, 1, 3);
+      MCOP_TILES(1, 1, 2, 1);
+    case MM_128X64: MCOP_TILES(2, 1, 2, 1, 3);
     case MM_128X128:
-      // one workgroup a CU has room for a third tile in flight: 1024 x 4096 x 5120 17.7 us, 20.3 with two;
-      // where two share a CU they overlap, 2048 x 4096 x 4096 23.5 us and 28.0
-      if (tiles_of(M, N, 128, 128) <= 256) {
-        return product_tiles<E, 2, 2, 2, 1, 3>(o, a, as, b, bs, bi, M, N, blocks, st);
-      }
-      return product_tiles<E, 2, 2, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
-    case MM_192X128:
-      return product_tiles<E, 3, 2, 2, 1, 3>(o, a, as, b, bs, bi, M, N, blocks, st);
-    case MM_256X256: return product_tiles<E, 4, 4, 2, 1>(o, a, as, b, bs, bi, M, N, blocks, st);
+      if (p.deep) MCOP_TILES(2, 2, 2, 1, 3);
+      MCOP_TILES(2, 2, 2, 1);
+    case MM_192X128: MCOP_TILES(3, 2, 2, 1, 3);
+    case MM_256X256: MCOP_TILES(4, 4, 2, 1);
     default: break;
   }
+#undef MCOP_TILES
   const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), block(256);
   hipLaunchKernelGGL((k_mxfp4_mm_rows<E, 4, 4>), grid, block, 0, st, o, a, as, b, bs, bi, M, N,
                      blocks);
@@ -771,4 +808,15 @@ extern "C" int mcop_mxfp4_scaled_mm(void* out, mcop_dtype out_dtype, const uint8
       return set_error(MCOP_E_INVALID, "%s: out dtype %d is not bf16/fp16/fp32", name,
                        (int)out_dtype);
   }
+}
+
+extern "C" const char* mcop_debug_mxfp4_mm_form(int64_t M, int64_t N, int64_t K, int aligned_scales) {
+  using namespace mcop;
+  static thread_local MmName name;
+  if (M <= 0 || N <= 0 || K <= 0 || K % kMxBlock != 0 || K > INT32_MAX ||
+      N > ((int64_t)1 << 27) || M > (int64_t)65535 * 16) {
+    return "";
+  }
+  name = name_of(plan_of((int)M, (int)N, (int)(K / kMxBlock), aligned_scales != 0));
+  return name.text;
 }

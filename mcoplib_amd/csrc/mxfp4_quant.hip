@@ -72,6 +72,12 @@ static unsigned quant_blocks(int64_t units) {
   return (unsigned)((units + kQuantLanes * kQuantUnits - 1) / (kQuantLanes * kQuantUnits));
 }
 
+static void trace_rows(const char* name, int64_t rows, int64_t hidden, bool whole, unsigned blocks) {
+  trace_launch(name, "rows=%lld hidden=%lld: %d units of 8 values a lane, %s, wgs=%u",
+               (long long)rows, (long long)hidden, kQuantUnits,
+               whole ? "aligned to 16 bytes" : "any alignment", blocks);
+}
+
 template <class E>
 static int quant(uint8_t* out, uint8_t* scales, const void* input, int64_t rows, int64_t hidden,
                  int64_t stride, hipStream_t st) {
@@ -85,6 +91,7 @@ static int quant(uint8_t* out, uint8_t* scales, const void* input, int64_t rows,
     const S* x = static_cast<const S*>(input) + r * stride;
     const Divisor row((uint32_t)(hidden / 8));
     const dim3 grid(quant_blocks(units)), block(kQuantLanes);
+    trace_rows("mxfp4_quant", n, hidden, whole, grid.x);
     if (whole) {
       hipLaunchKernelGGL((k_mxfp4_quant<E, false>), grid, block, 0, st, o, s, x, stride,
                          (uint32_t)units, row);
@@ -108,6 +115,7 @@ static int dequant(void* out, const uint8_t* codes, const uint8_t* scales, int64
     const auto* c = reinterpret_cast<const uint32_t*>(codes + r * (hidden / 2));
     const uint8_t* s = scales + r * (hidden / kMxBlock);
     const dim3 grid(quant_blocks(units)), block(kQuantLanes);
+    trace_rows("mxfp4_dequant", n, hidden, aligned(16, out), grid.x);
     if (aligned(16, out)) {
       hipLaunchKernelGGL((k_mxfp4_dequant<E, false>), grid, block, 0, st, o, c, s,
                          (uint32_t)units);
