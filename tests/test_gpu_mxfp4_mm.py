@@ -135,8 +135,8 @@ def test_random_shapes():
         assert mx_plain.same(_product(a, b, shift=i % 2), ref), (M, N, K)
 
 
-# Sizes of every way the product is made, each with rows and columns inside a tile and tails of K of one
-# block, or none.
+# Sizes of every tile shape, each with rows and columns inside a tile and tails of K of one block, or none;
+# with scales off dwords, which go through registers (test_gpu_mxfp4_mm_forms.py has every form by name).
 LARGE = [(16, 8192, 8224), (3, 2050, 9248), (33, 4099, 8224), (40, 16400, 4128), (100, 8192, 5152),
          (100, 4099, 2080), (130, 2050, 4128), (700, 4099, 1056), (1030, 2050, 1568),
          (700, 4099, 5152), (900, 4099, 4128), (2300, 1700, 512), (2300, 1700, 544),

@@ -43,3 +43,8 @@ def test_sizes_of_the_gpu_tests():
         last = -(-size[2] // 256) - 1
         assert form.split(",")[0] in ("128x128", "192x128", "256x256"), (size, form)
         assert last % (3 if "three" in form else 2) == 0, (size, form)
+    from test_gpu_mxfp4_mm_forms import FORMS
+
+    assert [_lib.mxfp4_mm_form(*size) for size, _ in FORMS] == [form for _, form in FORMS]
+    forms = {form for _, form in FORMS}
+    assert {form for _, form in CHOICES} <= forms
