@@ -218,3 +218,38 @@ def test_two_streams_at_once():
     for a, b in zip(got, want):
         for s, t in zip(a, b):
             assert mx_plain.same(s, t)
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8", "mxfp4"])
+def test_replays_among_other_allocations(kind):
+    """Between replays other work allocates tensors of the step's sizes, fills them with bytes that spoil
+    whatever reads them, and frees them: each replay still gives the eager step's results, and touches
+    none of those tensors."""
+    say(f"quant path graph among allocations {kind}")
+    T = 33
+    layer, eager = Layer(kind), Layer(kind)
+    x, r = _inputs(T, 1)
+    slots, table, cu = _tables(T)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        layer.step(x, r, slots, table, cu, T)
+        with torch.cuda.graph(g, stream=side):
+            outs = layer.step(x, r, slots, table, cu, T)
+    torch.cuda.current_stream().wait_stream(side)
+    sizes = [t.numel() * t.element_size() for t in outs]
+    sizes += [T * H // 2, T * H // 32, T * N * 2, T * KH * D * 2]  # what the step makes on its way
+    held = []
+    for rep in range(4):
+        nx, nr = _inputs(T, 50 + rep)
+        want = [t.clone() for t in eager.step(nx, nr, slots, table, cu, T)]
+        held = [torch.full((n,), 255, dtype=torch.uint8, device=DEV) for n in sizes for _ in range(3)]
+        x.copy_(nx), r.copy_(nr)
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert mx_plain.same(a, b), rep
+        assert all(bool((t == 255).all()) for t in held), rep
+        if rep % 2:
+            held = []  # the next round's go where these lay
