@@ -97,14 +97,18 @@ std::pair<int64_t, int64_t> rows_of(const Tensor& t) {
   return {t.numel() / h, h};
 }
 
-// Element stride between the rows of t, for tensors whose rows are uniformly strided.
+// Element stride between the rows of t, for tensors whose rows are uniformly strided.  Dimensions of
+// size one may have any stride and say nothing of the others'.
 int64_t row_stride(const char* name, const Tensor& t, int64_t T, int64_t H) {
-  if (t.dim() < 2 || T <= 1) return H;
-  for (int64_t d = 0; d + 2 < t.dim(); ++d) {
-    TORCH_CHECK(t.size(d) <= 1 || t.stride(d) == t.stride(d + 1) * t.size(d + 1), name,
-                ": rows must be uniformly strided");
+  if (T <= 1) return H;
+  int64_t stride = 0, rows = 0;  // of the dimensions so far, the last first
+  for (int64_t d = t.dim() - 2; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    TORCH_CHECK(rows == 0 || t.stride(d) == stride * rows, name, ": rows must be uniformly strided");
+    if (rows == 0) stride = t.stride(d);
+    rows = (rows == 0 ? 1 : rows) * t.size(d);
   }
-  return t.stride(-2);
+  return stride;
 }
 
 const float* ub_ptr(const char* name, const OptTensor& scale_ub) {
@@ -447,17 +451,11 @@ void c_fused_add_rms_norm(Tensor& input, Tensor& residual, const Tensor& weight,
   const auto [T, H] = rows_of(input);
   numel_check(name, "residual", residual, T * H);
   numel_check(name, "weight", weight, H);
-  // rows of `input` are addressed as row * stride(-2) (the reference's input_stride)
-  int64_t stride = H;
-  if (input.dim() >= 2 && T > 1) {
-    TORCH_CHECK(input.stride(-1) == 1, name, ": input must be contiguous in its last dimension");
-    for (int64_t d = 0; d + 2 < input.dim(); ++d) {
-      TORCH_CHECK(input.size(d) <= 1 ||
-                      input.stride(d) == input.stride(d + 1) * input.size(d + 1),
-                  name, ": input rows must be uniformly strided");
-    }
-    stride = input.stride(-2);
-  }
+  // rows of `input` are addressed as row * stride, its stride(-2) (the reference's input_stride) unless
+  // that dimension has one row
+  TORCH_CHECK(T <= 1 || input.stride(-1) == 1, name,
+              ": input must be contiguous in its last dimension");
+  const int64_t stride = row_stride(name, input, T, H);
   const DeviceGuard guard(input.device());
   check_rc(mcop_fused_add_rms_norm(input.data_ptr(), stride, residual.data_ptr(),
                                    weight.data_ptr(), T, H, code_of(input.scalar_type()),
