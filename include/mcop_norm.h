@@ -312,7 +312,8 @@ typedef struct {
  *   MCOP_MXFP4       blocks of 32 as above (head sizes multiples of 32)
  * (the arithmetic of mcop_dynamic_scaled_int8_quant and mcop_dynamic_per_token_scaled_fp8_quant).
  * Slots that are given must differ from each other: two tokens of one slot leave it with parts of
- * either. num_pages * page_size is below 2^31. No counterpart in the reference's path. */
+ * either. The two sides' codes and scales must not overlap each other. num_pages * page_size is below
+ * 2^31. No counterpart in the reference's path. */
 int mcop_kv_cache_write_quant(const mcop_kv_side* key, const mcop_kv_side* value,
                               mcop_dtype cache_dtype, int64_t num_pages, int64_t page_size,
                               int64_t num_heads, const int64_t* slot_mapping, int64_t num_tokens,

@@ -182,7 +182,9 @@ k_mxfp4_mm_rows(typename E::S* __restrict__ out, const uint8_t* __restrict__ a,
 // banks, and the sixteen lanes that a 16-byte read serves at once have eight rows of each parity, which
 // then take eight different places (by row & 7 there were conflicts for half of the reads' cycles).  A
 // direct load writes 64 x 16 bytes in lane order (eight rows), so each lane's address is that of the
-// chunk that belongs at its place.
+// chunk that belongs at its place.  Scales are not placed so: their rows are 32 bytes, and a dword of each of
+// 32 rows falls on eight banks, some 15 cycles of conflict a read (8192 x 8192 x 8192: 16.3 M, 13% of the
+// CUs' cycles).
 //
 // One barrier a tile (none for a group of one wave), after the first step's products: the tile's last
 // operands are in registers by then, the wave waits for its part of the next tile, meets the others,
@@ -637,8 +639,9 @@ static int product_tiles(typename E::S* out, const uint8_t* a, const uint8_t* as
 
 // The form for a product: the one of the lowest estimated time.  The estimates (us) are fits to calls of
 // every form over M from 1 to 4096, N from 512 to 16384 and K from 512 to 14336 (bf16; weights of several
-// sets in turn); what they choose takes 1% more than the best form on average there.  Measured (us) where one
-// gives way to the next (M x N x K):
+// sets in turn).  They know sizes only: fp32 outputs, K that is not a multiple of 256 and sizes past those
+// take longer than estimated (1237 x 4099 x 5152 fp32 21.5 us estimated, 29-31 measured) and may have a
+// faster form than the one chosen.  Measured (us) where one gives way to the next (M x N x K):
 //   rows (16 x 16, straight from memory) and 32 x 32 of four waves: 1 x 512 x 5120 4.5 and 5.2, 1 x 8192 x
 //     5120 8.2 and 7.0, 16 x 8192 x 12288 20.0 and 14.6
 //   32 x 32 of four waves and of eight, whose LDS is a whole CU's: 1 x 4099 x 12288 10.0 and 8.2, 48 x 4099

@@ -1087,7 +1087,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "[pages, page_size, heads, head_size] (int8 or float8_e4m3fn with fp32 scales [pages, "
         "page_size, heads]; or 4-bit codes, uint8 [..., head_size / 2], with scales [..., "
         "head_size / 32]). slot_mapping (int64) may cover fewer tokens; a negative slot, or one "
-        "past the cache, is not written. Slots that are written must differ.",
+        "past the cache, is not written. Slots that are written must differ, and the caches and "
+        "scales must not overlap.",
         py::arg("key"), py::arg("value"), py::arg("key_cache"), py::arg("value_cache"),
         py::arg("key_scale"), py::arg("value_scale"), py::arg("slot_mapping"));
   m.def("c_kv_cache_read_dequant", &c_kv_cache_read_dequant,

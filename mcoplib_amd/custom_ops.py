@@ -72,7 +72,7 @@ def kv_cache_write_quant(key: torch.Tensor, value: torch.Tensor, key_cache: torc
     float8_e4m3fn with fp32 scales [pages, page_size, heads], one a token and head, or 4-bit codes,
     uint8 [..., head_size / 2] with uint8 scales [..., head_size / 32].  slot_mapping may cover fewer
     tokens than key has; negative slots (padding) and slots past the cache are not written.  Slots that
-    are written must differ from each other."""
+    are written must differ from each other, and the caches and scales must not overlap."""
     _torch_ops.c_kv_cache_write_quant(key, value, key_cache, value_cache, key_scale, value_scale,
                                       slot_mapping)
 
