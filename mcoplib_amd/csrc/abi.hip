@@ -57,6 +57,7 @@ bool aligned(int bytes, const void* p0, const void* p1, const void* p2, const vo
   return true;
 }
 
+namespace {
 // MCOP_DEBUG_TRACE=1|ON prints every launch decision to stdout (the reference's env switch of
 // the same name prints every operator's arguments).
 bool trace_enabled() {
@@ -67,18 +68,6 @@ bool trace_enabled() {
   return on;
 }
 
-void trace_launch(const char* op, const char* fmt, ...) {
-  if (!trace_enabled()) return;
-  char line[256];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(line, sizeof(line), fmt, ap);
-  va_end(ap);
-  fprintf(stdout, "[mcop] %s %s\n", op, line);
-  fflush(stdout);
-}
-
-namespace {
 // Attributes of one kernel (hipFuncGetAttributes, cached; the answer depends only on the code
 // object).  `spills`: the kernel keeps registers in private (scratch) memory, whose per-lane
 // traffic would compete with the streamed rows.

@@ -18,6 +18,7 @@
 #include <cstdio>
 
 #include "../../include/mcop_norm.h"
+#include "launch_trace.h"
 #include "mxfp4.h"
 
 namespace mcop {
@@ -594,7 +595,7 @@ bool kv_grid(const char* name, int64_t blocks, dim3* grid) {
 // The launch's trace line; a_wave: tokens a wave takes at a time, 0 where it takes vectors.
 void trace_kv(const char* name, const KvSides& a, int64_t tokens, bool whole, int a_wave,
               const dim3& grid) {
-  if (!trace_enabled()) return;
+  if (!launches_traced()) return;
   char how[48] = "a vector a group of lanes";
   if (a_wave > 0) snprintf(how, sizeof(how), "whole tokens a wave, %d at a time", a_wave);
   trace_launch(name, "tokens=%lld heads=%d head sizes %d and %d: %s, %d units a lane, %s, wgs=%u x 2",

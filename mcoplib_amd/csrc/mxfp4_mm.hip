@@ -12,6 +12,7 @@
 #include <cstdio>
 
 #include "../../include/mcop_norm.h"
+#include "launch_trace.h"
 #include "mcop_testing.h"
 #include "mxfp4.h"
 
@@ -745,7 +746,7 @@ static int product(void* out, const uint8_t* a, const uint8_t* as, const uint8_t
   auto* o = static_cast<S*>(out);
   const auto* bi = static_cast<const S*>(bias);
   const MmPlan p = plan_of(M, N, blocks, aligned(4, as, bs));
-  if (trace_enabled()) {
+  if (launches_traced()) {
     trace_launch("mxfp4_scaled_mm", "M=%d N=%d K=%lld: %s", M, N, (long long)blocks * kMxBlock,
                  name_of(p).text);
   }

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include "../../include/mcop_norm.h"
+#include "launch_trace.h"
 #include "mxfp4.h"
 
 namespace mcop {

@@ -867,8 +867,5 @@ bool aligned(int bytes, const void* p0, const void* p1 = nullptr, const void* p2
 
 int set_error(int code, const char* fmt, ...);
 int check_launch(const char* what);
-// Whether launch decisions are traced, and the line of one that is not choose_geometry's.
-bool trace_enabled();
-void trace_launch(const char* op, const char* fmt, ...);
 
 }  // namespace mcop
