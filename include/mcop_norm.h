@@ -333,6 +333,31 @@ int mcop_kv_cache_read_dequant(const mcop_kv_side* key, const mcop_kv_side* valu
                                int64_t num_sequences, int64_t num_tokens, mcop_dtype out_dtype,
                                void* stream);
 
+/* Attention of one new token a sequence over such a cache. The key side's plain tensor holds the queries
+ * [num_sequences, query_heads, head_size] (read), the value side's the outputs (written), both of `dtype`
+ * with the strides that the sides give; query head h reads key head h / (query_heads / num_heads). Over the
+ * positions j of sequence b from max(0, n - window) (window 0: from 0) to n - 1, n = seq_lens[b], with page
+ * i of the sequence in block_table[b * table_row_stride + i]:
+ *   s_j = scale * <q, k_j>,  out = sum_j e^(s_j) v_j / sum_j e^(s_j),  lse = log sum_j e^(s_j)
+ * in fp32 (queries and weights enter the matrix units without loss beyond 2^-16 of a weight, 2^-24 for fp32),
+ * rounded once. lse is [num_sequences, query_heads] or NULL. A sequence of no positions gives 0 and -inf; one
+ * with a position that has no page of the cache (past the columns, or a page outside the cache) NaN.
+ * Slots behind a sequence's last position are not read. The order of the sums depends on the shapes and the
+ * lengths only. workspace: mcop_kv_cache_attention_workspace() bytes at a multiple of 16, used by this call
+ * alone until it ends on the stream. At most 2^24 sequences. No counterpart in the reference's path. */
+int mcop_kv_cache_attention(const mcop_kv_side* key, const mcop_kv_side* value, mcop_dtype cache_dtype,
+                            int64_t num_pages, int64_t page_size, int64_t num_heads,
+                            int64_t query_heads, const int32_t* block_table,
+                            int64_t table_row_stride, int64_t table_columns,
+                            const int32_t* seq_lens, int64_t num_sequences, float scale,
+                            int64_t window, mcop_dtype dtype, float* lse, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/* Bytes of the workspace that mcop_kv_cache_attention needs for such heads, whatever the lengths; or a
+ * negative MCOP_E_* code. No counterpart in the reference. */
+int64_t mcop_kv_cache_attention_workspace(int64_t num_heads, int64_t query_heads,
+                                          int64_t value_head_size);
+
 /* Message of the last failed call on this host thread ("" if none). Stands in for the
  * reference's TORCH_CHECK messages (c10::Error text), which its entry points raise directly. */
 const char* mcop_last_error(void);

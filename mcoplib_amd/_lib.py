@@ -67,6 +67,10 @@ def _load() -> ctypes.CDLL:
     lib.mcop_kv_cache_write_quant.argtypes = [side, side, I, I64, I64, I64, P, I64, I, P]
     lib.mcop_kv_cache_read_dequant.argtypes = [side, side, I, I64, I64, I64, P, I64, I64, P, P, I64,
                                                I64, I, P]
+    lib.mcop_kv_cache_attention.argtypes = [side, side, I, I64, I64, I64, I64, P, I64, I64, P, I64, F,
+                                            I64, I, P, P, I64, P]
+    lib.mcop_kv_cache_attention_workspace.argtypes = [I64, I64, I64]
+    lib.mcop_kv_cache_attention_workspace.restype = I64
     lib.mcop_check_row_scalars.argtypes = [P, ctypes.c_uint32, I64, I, F, P]
     lib.mcop_debug_set_launch_override.argtypes = [I, I]
     lib.mcop_debug_set_split_rows.argtypes = [I]
@@ -85,7 +89,7 @@ def _load() -> ctypes.CDLL:
                "mcop_vllm_rms_norm", "mcop_rms_norm_dynamic_per_token_quant_custom",
                "mcop_mxfp4_quant", "mcop_mxfp4_dequant", "mcop_rms_norm_mxfp4_quant",
                "mcop_mxfp4_scaled_mm", "mcop_kv_cache_write_quant",
-               "mcop_kv_cache_read_dequant"):
+               "mcop_kv_cache_read_dequant", "mcop_kv_cache_attention"):
         getattr(lib, fn).restype = I
     lib.mcop_last_error.restype = ctypes.c_char_p
     lib.mcop_last_error.argtypes = []

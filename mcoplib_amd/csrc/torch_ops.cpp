@@ -23,6 +23,8 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <cmath>
 #include <memory>
 #include <optional>
 #include <string>
@@ -700,9 +702,11 @@ mcop_dtype cache_code(const char* name, at::ScalarType t) {
   return MCOP_MXFP4;
 }
 
-// One side of the cache and the plain tensor [tokens, heads, head_size] beside it.
+// One side of the cache and the plain tensor [tokens, heads, head_size] beside it, whose heads are `group`
+// times the cache's.
 mcop_kv_side kv_side(const char* name, const char* what, const Tensor& plain, const Tensor& cache,
-                     const Tensor& scale, mcop_dtype format, const Tensor& key_cache) {
+                     const Tensor& scale, mcop_dtype format, const Tensor& key_cache,
+                     int64_t group = 1) {
   TORCH_CHECK(plain.dim() == 3, name, ": ", what, " must be [tokens, heads, head_size], got ",
               plain.sizes());
   TORCH_CHECK(cache.dim() == 4, name, ": the cache of ", what,
@@ -711,7 +715,7 @@ mcop_kv_side kv_side(const char* name, const char* what, const Tensor& plain, co
   const bool four = format == MCOP_MXFP4;
   TORCH_CHECK(!four || D % kMxBlock == 0, name, ": head_size ", D, " of ", what,
               " is not a multiple of the block of 32");
-  TORCH_CHECK(cache.size(3) == (four ? D / 2 : D) && cache.size(2) == plain.size(1), name,
+  TORCH_CHECK(cache.size(3) == (four ? D / 2 : D) && cache.size(2) * group == plain.size(1), name,
               ": the cache of ", what, " has shape ", cache.sizes(), " beside ", plain.sizes());
   TORCH_CHECK(cache.size(0) == key_cache.size(0) && cache.size(1) == key_cache.size(1) &&
                   cache.size(2) == key_cache.size(2),
@@ -761,6 +765,22 @@ const T* index_ptr(const char* name, const char* what, const Tensor& t, at::Scal
   return static_cast<const T*>(t.data_ptr());
 }
 
+const int32_t* table_ptr(const char* name, const Tensor& block_table) {
+  const auto* table = index_ptr<int32_t>(name, "block_table", block_table, at::kInt);
+  TORCH_CHECK(block_table.dim() == 2 && (block_table.size(1) <= 1 || block_table.stride(1) == 1),
+              name, ": block_table must be [sequences, pages] with contiguous rows");
+  return table;
+}
+
+// A contiguous vector of int32, of n elements (n < 0: any number).
+int32_t* ints_ptr(const char* name, const char* what, const Tensor& t, int64_t n) {
+  auto* p = const_cast<int32_t*>(index_ptr<int32_t>(name, what, t, at::kInt));
+  TORCH_CHECK(t.dim() == 1 && t.is_contiguous() && (n < 0 || t.size(0) == n), name, ": ", what,
+              " must be contiguous with ", n < 0 ? std::string("one dimension") :
+              std::to_string(n) + " elements", ", got ", t.sizes());
+  return p;
+}
+
 void c_kv_cache_write_quant(const Tensor& key, const Tensor& value, Tensor& key_cache,
                             Tensor& value_cache, Tensor& key_scale, Tensor& value_scale,
                             const Tensor& slot_mapping) {
@@ -791,10 +811,8 @@ void c_kv_cache_read_dequant(Tensor& key, Tensor& value, const Tensor& key_cache
   const char* name = "kv_cache_read_dequant";
   kv_check(name, key, value, key_cache, value_cache);
   const mcop_dtype format = cache_code(name, key_cache.scalar_type());
-  const auto* table = index_ptr<int32_t>(name, "block_table", block_table, at::kInt);
+  const auto* table = table_ptr(name, block_table);
   const auto* cu = index_ptr<int32_t>(name, "cu_seqlens", cu_seqlens, at::kInt);
-  TORCH_CHECK(block_table.dim() == 2 && (block_table.size(1) <= 1 || block_table.stride(1) == 1),
-              name, ": block_table must be [sequences, pages] with contiguous rows");
   const int64_t B = block_table.size(0);
   TORCH_CHECK(cu_seqlens.dim() == 1 && cu_seqlens.is_contiguous() && cu_seqlens.size(0) == B + 1,
               name, ": cu_seqlens must be contiguous with ", B + 1, " elements, got ",
@@ -817,6 +835,58 @@ void c_kv_cache_read_dequant(Tensor& key, Tensor& value, const Tensor& key_cache
                                       key.size(1), table, B > 1 ? block_table.stride(0) : 0,
                                       block_table.size(1), cu, starts, B, key.size(0),
                                       code_of(key.scalar_type()), stream_of(key)));
+}
+
+void c_kv_cache_attention(Tensor& result, const Tensor& query, const Tensor& key_cache,
+                          const Tensor& value_cache, const Tensor& key_scale,
+                          const Tensor& value_scale, const Tensor& block_table,
+                          const Tensor& seq_lens, double scale, int64_t window,
+                          const OptTensor& lse) {
+  const char* name = "kv_cache_attention";
+  dispatch_check(query.scalar_type(), name);
+  TORCH_CHECK(result.scalar_type() == query.scalar_type(), name, ": result must have query's dtype ",
+              query.scalar_type());
+  TORCH_CHECK(value_cache.scalar_type() == key_cache.scalar_type(), name,
+              ": the caches must share a dtype, got ", key_cache.scalar_type(), " and ",
+              value_cache.scalar_type());
+  TORCH_CHECK(query.dim() == 3 && result.dim() == 3 && query.size(0) == result.size(0) &&
+                  query.size(1) == result.size(1) && key_cache.dim() == 4,
+              name, ": query ", query.sizes(), " and result ", result.sizes(),
+              " must be [sequences, heads, head_size] of the same sequences and heads");
+  const int64_t B = query.size(0), heads = key_cache.size(2), queries = query.size(1);
+  TORCH_CHECK(heads > 0 && queries > 0 && queries % heads == 0, name, ": ", queries,
+              " query heads are not a multiple of ", heads, " key heads");
+  const mcop_dtype format = cache_code(name, key_cache.scalar_type());
+  const auto* table = table_ptr(name, block_table);
+  TORCH_CHECK(block_table.size(0) == B, name, ": block_table has ", block_table.size(0),
+              " rows for ", B, " sequences");
+  const auto* lens = ints_ptr(name, "seq_lens", seq_lens, B);
+  TORCH_CHECK(window >= 0, name, ": window must not be negative, got ", window);
+  if (lse.has_value()) {
+    TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->dim() == 2 && lse->size(0) == B &&
+                    lse->size(1) == queries && lse->is_contiguous(),
+                name, ": lse must be contiguous float32 [", B, ", ", queries, "], got ",
+                lse->scalar_type(), " ", lse->sizes());
+  }
+  const mcop_kv_side k = kv_side(name, "key", query, key_cache, key_scale, format, key_cache,
+                                 queries / heads);
+  const mcop_kv_side v = kv_side(name, "value", result, value_cache, value_scale, format, key_cache,
+                                 queries / heads);
+  no_overlap(name, {&result});
+  on_device(name, {&result, &query, &key_cache, &value_cache, &key_scale, &value_scale, &block_table,
+                   &seq_lens, opt(lse)});
+  if (B == 0) return;
+  const DeviceGuard guard(query.device());
+  const int64_t bytes = mcop_kv_cache_attention_workspace(heads, queries, v.head_size);
+  if (bytes < 0) check_rc((int)bytes);
+  // from torch's allocator: the memory stays this stream's (and a captured graph's own) until reused
+  const Tensor workspace = at::empty({bytes}, query.options().dtype(at::kByte));
+  check_rc(mcop_kv_cache_attention(&k, &v, format, key_cache.size(0), key_cache.size(1), heads,
+                                   queries, table, B > 1 ? block_table.stride(0) : 0,
+                                   block_table.size(1), lens, B, (float)scale, window,
+                                   code_of(query.scalar_type()),
+                                   lse.has_value() ? lse->data_ptr<float>() : nullptr,
+                                   workspace.data_ptr(), bytes, stream_of(query)));
 }
 
 // The allocating forms (custom_ops).
@@ -903,6 +973,31 @@ std::tuple<Tensor, Tensor> kv_cache_read_new(const Tensor& key_cache, const Tens
   return {key, value};
 }
 
+std::tuple<Tensor, OptTensor> kv_cache_attention_new(
+    const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale,
+    const Tensor& value_scale, const Tensor& block_table, const Tensor& seq_lens,
+    std::optional<double> scale, int64_t window, bool return_lse) {
+  const char* name = "kv_cache_attention";
+  TORCH_CHECK(query.dim() == 3 && value_cache.dim() == 4, name,
+              ": query must be [sequences, heads, head_size], got ", query.sizes(),
+              ", caches [pages, page_size, heads, head_size]");
+  const int64_t wide = is_codes4(value_cache.scalar_type()) ? 2 : 1;
+  Tensor out;
+  OptTensor lse;
+  {
+    const py::gil_scoped_release allocating;
+    out = at::empty({query.size(0), query.size(1), value_cache.size(3) * wide}, query.options());
+    if (return_lse) {
+      lse = at::empty({query.size(0), query.size(1)}, query.options().dtype(at::kFloat));
+    }
+    c_kv_cache_attention(out, query, key_cache, value_cache, key_scale, value_scale, block_table,
+                         seq_lens,
+                         scale.value_or(1.0 / std::sqrt((double)std::max<int64_t>(1, query.size(2)))),
+                         window, lse);
+  }
+  return {out, lse};
+}
+
 // Meta kernel of the mutating _C ops (no outputs to describe): drop the arguments.
 void meta_noop(const c10::OperatorHandle& op, torch::jit::Stack* stack) {
   torch::jit::drop(*stack, op.schema().arguments().size());
@@ -943,6 +1038,10 @@ constexpr VllmOp kVllmOps[] = {
      "kv_cache_read_dequant(Tensor! key, Tensor! value, Tensor key_cache, Tensor value_cache, "
      "Tensor key_scale, Tensor value_scale, Tensor block_table, Tensor cu_seqlens, "
      "Tensor? seq_starts) -> ()"},
+    {"kv_cache_attention",
+     "kv_cache_attention(Tensor! result, Tensor query, Tensor key_cache, Tensor value_cache, "
+     "Tensor key_scale, Tensor value_scale, Tensor block_table, Tensor seq_lens, float scale, "
+     "int window, Tensor!? lse) -> ()"},
 };
 
 // Registers the _C schemas (each only if no other library, e.g. vLLM's own _C, defined it) with
@@ -976,6 +1075,7 @@ void register_vllm_ops() {
   cuda->impl("mxfp4_scaled_mm", TORCH_FN(c_mxfp4_scaled_mm));
   cuda->impl("kv_cache_write_quant", TORCH_FN(c_kv_cache_write_quant));
   cuda->impl("kv_cache_read_dequant", TORCH_FN(c_kv_cache_read_dequant));
+  cuda->impl("kv_cache_attention", TORCH_FN(c_kv_cache_attention));
   done = true;
 }
 
@@ -1099,6 +1199,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("key"), py::arg("value"), py::arg("key_cache"), py::arg("value_cache"),
         py::arg("key_scale"), py::arg("value_scale"), py::arg("block_table"),
         py::arg("cu_seqlens"), py::arg("seq_starts") = py::none());
+  m.def("c_kv_cache_attention", &c_kv_cache_attention,
+        "Attention of one new token a sequence over such a cache: result [sequences, query heads, "
+        "value head_size] <- softmax(scale * query k) v over positions max(0, n - window) (window 0: "
+        "from 0) to n - 1 of each, n = seq_lens, whose pages block_table lists. query heads are a "
+        "multiple of the cache's. lse [sequences, query heads] (fp32) <- the log of each row's sum. A "
+        "sequence of no positions gives 0 and -inf, one with a position without a page NaN.",
+        py::arg("result"), py::arg("query"), py::arg("key_cache"), py::arg("value_cache"),
+        py::arg("key_scale"), py::arg("value_scale"), py::arg("block_table"), py::arg("seq_lens"),
+        py::arg("scale"), py::arg("window") = 0, py::arg("lse") = py::none(),
+        py::call_guard<py::gil_scoped_release>());  // it allocates its workspace
   // custom_ops: the same into new tensors
   m.def("mxfp4_quant_new", &mxfp4_quant_new, py::arg("input"));
   m.def("mxfp4_dequant_new", &mxfp4_dequant_new, py::arg("codes"), py::arg("scale"),
@@ -1111,4 +1221,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("key_scale"), py::arg("value_scale"), py::arg("block_table"),
         py::arg("cu_seqlens"), py::arg("num_tokens"), py::arg("out_dtype"),
         py::arg("seq_starts") = py::none());
+  m.def("kv_cache_attention_new", &kv_cache_attention_new, py::arg("query"), py::arg("key_cache"),
+        py::arg("value_cache"), py::arg("key_scale"), py::arg("value_scale"), py::arg("block_table"),
+        py::arg("seq_lens"), py::arg("scale") = py::none(), py::arg("window") = 0,
+        py::arg("return_lse") = false);
 }

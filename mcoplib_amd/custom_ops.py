@@ -5,7 +5,7 @@ key/value cache, which the reference does not have, are here in the same manner.
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -88,3 +88,22 @@ def kv_cache_read_dequant(key_cache: torch.Tensor, value_cache: torch.Tensor,
     rows past that are not written.  A position without a page of the cache reads as NaN."""
     return _torch_ops.kv_cache_read_new(key_cache, value_cache, key_scale, value_scale, block_table,
                                         cu_seqlens, num_tokens, out_dtype, seq_starts)
+
+
+def kv_cache_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                       key_scale: torch.Tensor, value_scale: torch.Tensor,
+                       block_table: torch.Tensor, seq_lens: torch.Tensor,
+                       scale: Optional[float] = None, window: int = 0, return_lse: bool = False
+                       ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Attention of one new token a sequence over the cache that kv_cache_write_quant fills: query
+    [sequences, query heads, head_size] (any strides but the last; query heads a multiple of the cache's
+    heads, query head h reads head h // (query heads // heads)) over positions max(0, n - window)
+    (window 0: from 0) to n - 1 of each sequence, n = seq_lens[s] (int32, the new token included), whose
+    pages block_table[s] lists.  scale is head_size ** -0.5 where it is None.  Returns the outputs
+    [sequences, query heads, value head_size] in query's dtype, with return_lse also the log of each
+    row's sum of e^(scale q k) in fp32 [sequences, query heads], for a join with other positions.  A
+    sequence of no positions gives 0 and -inf; one with a position without a page of the cache gives
+    NaN.  Lengths are read on the device: a captured graph replays with new ones."""
+    out, lse = _torch_ops.kv_cache_attention_new(query, key_cache, value_cache, key_scale, value_scale,
+                                                 block_table, seq_lens, scale, window, return_lse)
+    return (out, lse) if return_lse else out
