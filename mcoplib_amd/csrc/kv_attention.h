@@ -180,25 +180,26 @@ __device__ __forceinline__ float att_lse(float m, float l) {
   return l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// Joins the waves' parts of `rows` query heads from LDS (m, l [kAttWaves][stride_r], e [kAttWaves], o
+// Joins the waves' parts of `rows` query heads from LDS (m, l [kAttWaves][stride_m], e [kAttWaves], o
 // [kAttWaves][stride_r][stride_o]) and writes the outputs of query heads head0.. (or, of a split sequence,
 // its part) at elements d0.. of the value.
 template <class E>
 __device__ __forceinline__ void att_write(const AttArgs& a, const AttChunk& c, int head0, int rows,
                                           int d0, int width, const float* m, const float* l,
-                                          const int* e, const float* o, int stride_r, int stride_o) {
+                                          const int* e, const float* o, int stride_m,
+                                          int stride_r, int stride_o) {
   int unit = e[0];
 #pragma unroll
   for (int w = 1; w < kAttWaves; ++w) unit = max(unit, e[w]);
   for (int r = 0; r < rows; ++r) {
     float top = -__builtin_inff();
 #pragma unroll
-    for (int w = 0; w < kAttWaves; ++w) top = __builtin_fmaxf(top, m[w * stride_r + r]);
+    for (int w = 0; w < kAttWaves; ++w) top = __builtin_fmaxf(top, m[w * stride_m + r]);
     float f[kAttWaves], sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < kAttWaves; ++w) {
-      f[w] = att_weight(m[w * stride_r + r], top);
-      sum += l[w * stride_r + r] * f[w];
+      f[w] = att_weight(m[w * stride_m + r], top);
+      sum += l[w * stride_m + r] * f[w];
       f[w] *= att_power(e[w] - unit);
     }
     if (c.missing) sum = __builtin_nanf("");

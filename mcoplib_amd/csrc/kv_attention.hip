@@ -6,7 +6,7 @@
 #include <algorithm>
 
 #include "../../include/mcop_norm.h"
-#include "kv_attention.h"
+#include "kv_attention_tiles.h"
 #include "launch_trace.h"
 
 namespace mcop {
@@ -134,7 +134,7 @@ k_kv_attention_rows(AttArgs a) {
     }
   }
   __syncthreads();
-  att_write<E>(a, c, head0, rows, 0, a.value.dim, ms, ls, es, os, kAttRows, a.value.dim);
+  att_write<E>(a, c, head0, rows, 0, a.value.dim, ms, ls, es, os, kAttRows, kAttRows, a.value.dim);
 }
 
 // Joins the parts of split sequence blockIdx.y of the plan, a query head a workgroup: a group of 32 lanes
@@ -231,21 +231,43 @@ bool heads_ok(int64_t heads, int64_t query_heads) {
   return heads > 0 && query_heads > 0 && query_heads <= 65535 && query_heads % heads == 0;
 }
 
+// The matrix kernel for the head sizes, an index of kTileShapes; -1: none (wider than they hold, or less
+// than one of their units; nor do they take a cache without a page, which they read for any wrong one).
+int tile_shape(const AttArgs& a) {
+  if (a.pages == 0 || a.key.dim < 16) return -1;
+  for (int i = 0; i < (int)(sizeof(kTileShapes) / sizeof(kTileShapes[0])); ++i) {
+    const TileShape& s = kTileShapes[i];
+    if (a.key.dim <= 64 * s.kp && a.value.dim <= 16 * s.vd) return a.value.dim >= s.vd ? i : -1;
+  }
+  return -1;
+}
+
 template <class E, int FMT>
-int launch_of(const char* name, AttArgs a, int64_t chunks, bool joins, hipStream_t st) {
-  a.row_blocks = (a.group + kAttRows - 1) / kAttRows;
+int launch_of(const char* name, AttArgs a, mcop_dtype dtype, int64_t chunks, bool joins,
+              hipStream_t st) {
+  const int shape = tile_shape(a), rows = shape >= 0 ? kTileRows : kAttRows;
+  a.row_blocks = (a.group + rows - 1) / rows;
   const int64_t inner = (int64_t)a.heads * a.row_blocks, blocks = (chunks + 7) / 8 * 8 * inner;
   if (blocks >= ((int64_t)1 << 31) / 256) {
     return set_error(MCOP_E_UNSUPPORTED, "%s: more rows than one launch takes (%lld workgroups)", name,
                      (long long)blocks);
   }
   a.by_inner = Divisor((uint32_t)inner);
-  const size_t lds = (size_t)kAttWaves * kAttRows * (2 + a.value.dim) * sizeof(float) + kAttWaves * sizeof(int);
-  trace_launch(name, "sequences=%d heads=%d of %d head sizes %d and %d: vector kernel, wgs=%lld, %d "
+  const size_t lds =
+      sizeof(float) * kAttWaves *
+      (shape >= 0 ? 2 * kTileRows + 1 + (size_t)std::min(kTileRows, a.group) * (a.value.dim + 1)
+                  : 2 * kAttRows + 1 + (size_t)kAttRows * a.value.dim);
+  trace_launch(name, "sequences=%d heads=%d of %d head sizes %d and %d: %s kernel, wgs=%lld, %d "
                "chunks aimed at%s", a.sequences, a.heads, a.query_heads, a.key.dim, a.value.dim,
-               (long long)blocks, a.target, joins ? "" : ", none split");
+               shape >= 0 ? "matrix" : "vector", (long long)blocks, a.target, joins ? "" : ", none split");
   const dim3 grid((unsigned)blocks), block(kAttWaves * 64);
-  if (std::max(a.key.dim, a.value.dim) <= 256) {
+  if (shape >= 0) {
+    int rc;
+    if constexpr (FMT == KV_INT8) rc = attention_tiles_int8(shape, dtype, a, grid, lds, st);
+    else if constexpr (FMT == KV_FP8) rc = attention_tiles_fp8(shape, dtype, a, grid, lds, st);
+    else rc = attention_tiles_mxfp4(shape, dtype, a, grid, lds, st);
+    if (rc) return rc;
+  } else if (std::max(a.key.dim, a.value.dim) <= 256) {
     hipLaunchKernelGGL((k_kv_attention_rows<E, FMT, 4>), grid, block, lds, st, a);
   } else {
     hipLaunchKernelGGL((k_kv_attention_rows<E, FMT, 16>), grid, block, lds, st, a);
@@ -351,9 +373,9 @@ extern "C" int mcop_kv_cache_attention(const mcop_kv_side* key, const mcop_kv_si
   auto by_format = [&](auto e) {
     using E = decltype(e);
     const int64_t chunks = target + num_sequences;
-    if (fmt == KV_INT8) return launch_of<E, KV_INT8>(name, a, chunks, joins, st);
-    if (fmt == KV_FP8) return launch_of<E, KV_FP8>(name, a, chunks, joins, st);
-    return launch_of<E, KV_MXFP4>(name, a, chunks, joins, st);
+    if (fmt == KV_INT8) return launch_of<E, KV_INT8>(name, a, dtype, chunks, joins, st);
+    if (fmt == KV_FP8) return launch_of<E, KV_FP8>(name, a, dtype, chunks, joins, st);
+    return launch_of<E, KV_MXFP4>(name, a, dtype, chunks, joins, st);
   };
   if (dtype == MCOP_BF16) return by_format(BF16());
   if (dtype == MCOP_F16) return by_format(F16());
