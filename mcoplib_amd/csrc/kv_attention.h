@@ -30,7 +30,7 @@ namespace mcop {
 
 constexpr int kAttTile = 32;      // positions of a tile
 constexpr int kAttWaves = 4;      // of a workgroup, which share out a chunk's tiles
-constexpr int kAttLeastTiles = 4; // of a chunk
+constexpr int kAttLeastTiles = 1; // of a chunk
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttArgs {
@@ -100,6 +100,8 @@ __device__ __forceinline__ bool find_chunk(const AttArgs& a, uint32_t flat, bool
     if (i + lane < a.sequences) total += att_tiles(a, a.lens[i + lane]);
   }
   total = wave_sum(total);
+  total = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(total >> 32)) << 32 |
+          (uint32_t)__builtin_amdgcn_readfirstlane((int)total);
   uint64_t per = kAttLeastTiles;
   if (total > (uint64_t)a.target * kAttLeastTiles) {
     per = total >> 32 ? (total + a.target - 1) / a.target
@@ -119,13 +121,14 @@ __device__ __forceinline__ bool find_chunk(const AttArgs& a, uint32_t flat, bool
     if (!found && hit != 0) {
       found = true;
       const int at = __builtin_ctzll(hit);
-      const uint64_t from = __shfl((unsigned long long)(upto - mine), at, 64);
+      const uint32_t from = (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), at);
+      const uint32_t from_parts = (uint32_t)__builtin_amdgcn_readlane((int)((upto - mine) >> 32), at);
       const uint32_t tiles = (uint32_t)__builtin_amdgcn_readlane((int)t, at);
       c->sequence = i + at;
       c->end = __builtin_amdgcn_readlane(n, at);
       c->count = __builtin_amdgcn_readlane((int)k, at);
-      c->index = (int)(flat - (uint32_t)from);
-      c->part = (int)(from >> 32) + c->index;
+      c->index = (int)(flat - from);
+      c->part = (int)from_parts + c->index;
       c->missing = c->end > att_capacity(a);
       c->first = att_first(a, c->end);
       const uint32_t each = tiles / (uint32_t)c->count, more = tiles % (uint32_t)c->count;
@@ -142,10 +145,22 @@ __device__ __forceinline__ bool find_chunk(const AttArgs& a, uint32_t flat, bool
       if (!plans || flat != 0) return true;
     }
     splits += (int)__builtin_popcountll(split);
-    before = __shfl((unsigned long long)upto, 63, 64);
+    before = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(upto >> 32), 63) << 32 |
+             (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
   }
   if (plans && flat == 0 && lane == 0) a.plan[0] = splits;
   return found;
+}
+
+// A wave's place where every wave takes a chunk of one key head and block: heads and blocks of a chunk are
+// neighbours, so that what lies together in the cache is read together, and chunks go round the dies.
+__device__ __forceinline__ void att_wave_place(const AttArgs& a, uint32_t wave, uint32_t* flat, int* head, int* block) {
+  // inner padded to whole workgroups
+  const uint32_t die = blockIdx.x & 7, i = (blockIdx.x >> 3) * kAttWaves + wave;
+  const uint32_t row = a.by_inner.quotient(i), inner = i - row * a.by_inner.d;
+  *flat = row * 8 + die;
+  *head = (int)(inner / (uint32_t)a.row_blocks);
+  *block = (int)(inner - (uint32_t)*head * (uint32_t)a.row_blocks);
 }
 
 // Workgroup -> (chunk, key head, block of its query heads).  Workgroups go round the eight dies in turn,

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "../../include/mcop_norm.h"
 #include "kv_attention_tiles.h"
@@ -214,7 +215,7 @@ k_kv_attention_join(AttArgs a) {
 namespace {
 
 // Chunks aimed at: two workgroups a CU over all of a chunk's key heads and blocks of sixteen query heads.
-constexpr int kAttWorkgroups = 512;
+int kAttWorkgroups = getenv("MCOP_T") ? atoi(getenv("MCOP_T")) : 2048;
 int64_t target_of(int64_t heads, int64_t group) {
   return std::max<int64_t>(1, kAttWorkgroups / (heads * ((group + 15) / 16)));
 }
@@ -242,12 +243,26 @@ int tile_shape(const AttArgs& a) {
   return -1;
 }
 
+// Whether tiles can go through LDS: pages of whole halves of a tile, vectors of whole chunks of 16 bytes at
+// multiples of 16, a half's positions apart by less than 2^31 bytes.
+bool whole_lines(const AttArgs& a, int fmt) {
+  for (const KvSide* k : {&a.key, &a.value}) {
+    const int64_t bytes = fmt == KV_MXFP4 ? k->dim / 2 : k->dim;
+    if (bytes % 16 != 0 || !aligned(16, k->codes) || k->c_page % 16 != 0 || k->c_token % 16 != 0 ||
+        k->c_head % 16 != 0 || k->c_token >= ((int64_t)1 << 31) / 16 - 1024) {
+      return false;
+    }
+  }
+  return a.page_size % 16 == 0;
+}
+
 template <class E, int FMT>
 int launch_of(const char* name, AttArgs a, mcop_dtype dtype, int64_t chunks, bool joins,
               hipStream_t st) {
   const int shape = tile_shape(a), rows = shape >= 0 ? kTileRows : kAttRows;
   a.row_blocks = (a.group + rows - 1) / rows;
-  const int64_t inner = (int64_t)a.heads * a.row_blocks, blocks = (chunks + 7) / 8 * 8 * inner;
+  const int64_t inner = (int64_t)a.heads * a.row_blocks;
+  const int64_t blocks = shape >= 0 ? ((chunks + 7) / 8 * inner + kAttWaves - 1) / kAttWaves * 8 : (chunks + 7) / 8 * 8 * inner;
   if (blocks >= ((int64_t)1 << 31) / 256) {
     return set_error(MCOP_E_UNSUPPORTED, "%s: more rows than one launch takes (%lld workgroups)", name,
                      (long long)blocks);
@@ -255,17 +270,18 @@ int launch_of(const char* name, AttArgs a, mcop_dtype dtype, int64_t chunks, boo
   a.by_inner = Divisor((uint32_t)inner);
   const size_t lds =
       sizeof(float) * kAttWaves *
-      (shape >= 0 ? 2 * kTileRows + 1 + (size_t)std::min(kTileRows, a.group) * (a.value.dim + 1)
+      (shape >= 0 ? 0
                   : 2 * kAttRows + 1 + (size_t)kAttRows * a.value.dim);
   trace_launch(name, "sequences=%d heads=%d of %d head sizes %d and %d: %s kernel, wgs=%lld, %d "
                "chunks aimed at%s", a.sequences, a.heads, a.query_heads, a.key.dim, a.value.dim,
                shape >= 0 ? "matrix" : "vector", (long long)blocks, a.target, joins ? "" : ", none split");
   const dim3 grid((unsigned)blocks), block(kAttWaves * 64);
   if (shape >= 0) {
+    const bool lines = whole_lines(a, FMT);
     int rc;
-    if constexpr (FMT == KV_INT8) rc = attention_tiles_int8(shape, dtype, a, grid, lds, st);
-    else if constexpr (FMT == KV_FP8) rc = attention_tiles_fp8(shape, dtype, a, grid, lds, st);
-    else rc = attention_tiles_mxfp4(shape, dtype, a, grid, lds, st);
+    if constexpr (FMT == KV_INT8) rc = attention_tiles_int8(shape, lines, dtype, a, grid, st);
+    else if constexpr (FMT == KV_FP8) rc = attention_tiles_fp8(shape, lines, dtype, a, grid, st);
+    else rc = attention_tiles_mxfp4(shape, lines, dtype, a, grid, st);
     if (rc) return rc;
   } else if (std::max(a.key.dim, a.value.dim) <= 256) {
     hipLaunchKernelGGL((k_kv_attention_rows<E, FMT, 4>), grid, block, lds, st, a);

@@ -3,9 +3,9 @@
 
 namespace mcop {
 
-int attention_tiles_int8(int shape, mcop_dtype dtype, const AttArgs& a, dim3 grid, size_t lds,
+int attention_tiles_int8(int shape, bool lines, mcop_dtype dtype, const AttArgs& a, dim3 grid,
                          hipStream_t st) {
-  return attention_tiles_for<KV_INT8>(shape, dtype, a, grid, lds, st);
+  return attention_tiles_for<KV_INT8>(shape, lines, dtype, a, grid, st);
 }
 
 }  // namespace mcop

@@ -3,9 +3,9 @@
 
 namespace mcop {
 
-int attention_tiles_mxfp4(int shape, mcop_dtype dtype, const AttArgs& a, dim3 grid, size_t lds,
-                         hipStream_t st) {
-  return attention_tiles_for<KV_MXFP4>(shape, dtype, a, grid, lds, st);
+int attention_tiles_mxfp4(int shape, bool lines, mcop_dtype dtype, const AttArgs& a, dim3 grid,
+                          hipStream_t st) {
+  return attention_tiles_for<KV_MXFP4>(shape, lines, dtype, a, grid, st);
 }
 
 }  // namespace mcop

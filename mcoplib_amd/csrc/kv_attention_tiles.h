@@ -129,65 +129,77 @@ __device__ __forceinline__ float column_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-// What a lane knows of a tile's position lane % 32: its page (or where a wrong one was found), and its place
-// on it.  Positions before the first or behind the last stand for those.
-struct TilePlace {
-  int page;
-  uint32_t off;
-};
+// 16, 4 bytes a lane from its address to LDS at `to` + 16, 4 * lane, which the instruction takes from m0 (a
+// state after its write).  The compiler sees neither what this writes nor that it is in flight:
+// wait_tile() orders it.
+__device__ __forceinline__ void tile_to_lds16(uint32_t to, const uint8_t* base, uint32_t off) {
+  asm volatile(
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2"
+      :
+      : "{m0}"(to), "v"(off), "s"(base)
+      : "memory");
+}
+__device__ __forceinline__ void tile_to_lds4(uint32_t to, const uint8_t* from) {
+  asm volatile(
+      "s_nop 0\n\t"
+      "global_load_lds_dword %1, off"
+      :
+      : "{m0}"(to), "v"(from)
+      : "memory");
+}
+// All of the wave's loads have landed, and its LDS reads of what they may be followed by are done.
+__device__ __forceinline__ void wait_tile() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+}
 
-// A tile as it lies in the cache.
-template <int FMT, int KP, int VD>
-struct TileCodes {
-  static constexpr int KW = FMT == KV_MXFP4 ? 2 : 4;                          // dwords of 16 codes
-  static constexpr int VB = FMT == KV_MXFP4 ? VD / 2 : VD, VW = (VB + 3) / 4;  // bytes, dwords of VD codes
-  uint32_t k[2][KP][KW];
-  uint32_t v[8][VW];
-  float ks, vs;                 // scales of position lane % 32
-  uint32_t kb[2], vb[2];        // the same of 4-bit blocks
-};
-
+// A wave's query heads, its sums, and the two products of a tile, whose codes `src` gives:
+//   key(h, kp, w)      sixteen codes of position 16 h + c, and key_scale(h, kp) of 4-bit ones
+//   value(e, w)        VD codes of position(e), and value_scale(e) of 4-bit ones
+//   ks(e), vs(e)       fp32 scales of position(e)
+//   most_vs()          the lane's part of the tile's value scales
 template <class E, int FMT, int KP, int VD>
-struct TileKernel {
+struct AttWave {
   static constexpr int TQ = AttTerms<E>::Q, TP = AttTerms<E>::P;
-  using Codes = TileCodes<FMT, KP, VD>;
   static constexpr bool MX = FMT == KV_MXFP4;
+  static constexpr int KW = MX ? 2 : 4;                                 // dwords of 16 codes
+  static constexpr int VB = MX ? VD / 2 : VD, VW = (VB + 3) / 4;        // bytes, dwords of VD codes
 
   const AttArgs& a;
   const int lane, c, g;
-  const int32_t* row;                // of the table
-  const uint8_t *k_base, *v_base;    // of the key head
-  const void *ks_base, *vs_base;
   int first, end;
-  int k_at[KP], v_at;                // bytes
-  uint32_t k_sel[KP], v_sel;
   bf16x8 q[KP][2][TQ];
   f32x4 o[VD];
   float m, l;
   int unit;
-  bool missing;
 
-  __device__ __forceinline__ TileKernel(const AttArgs& args, const AttChunk& chunk, int head,
-                                        int head0, int rows)
-      : a(args), lane((int)threadIdx.x & 63), c(lane & 15), g(lane >> 4) {
-    row = a.table + chunk.sequence * a.table_stride;
-    k_base = a.key.codes + head * a.key.c_head;
-    v_base = a.value.codes + head * a.value.c_head;
-    const int es = MX ? 1 : 4;
-    ks_base = static_cast<const uint8_t*>(a.key.scales) + head * a.key.s_head * es;
-    vs_base = static_cast<const uint8_t*>(a.value.scales) + head * a.value.s_head * es;
-    first = chunk.first, end = chunk.end;
-    const int from = value_at(c);
-    v_at = MX ? from / 2 : from;
-    v_sel = MX ? scale_selector(from / kMxBlock, a.value.dim / kMxBlock) : 0;
+  __device__ __forceinline__ AttWave(const AttArgs& args, const AttChunk& chunk, int head0, int rows)
+      : a(args), lane((int)threadIdx.x & 63), c(lane & 15), g(lane >> 4), first(chunk.first),
+        end(chunk.end) {
     const typename E::S* src = static_cast<const typename E::S*>(a.key.plain) +
                                chunk.sequence * a.key.p_token +
                                (head0 + min(c, rows - 1)) * a.key.p_head;
+    Pack<typename E::S, 8> x[KP][2];
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
-      const int nominal = kp * 64 + g * 16, at = min(nominal, a.key.dim - 16);
-      k_at[kp] = MX ? at / 2 : at;
-      k_sel[kp] = MX ? scale_selector(at / kMxBlock, a.key.dim / kMxBlock) : 0;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) x[kp][j] = load8<typename E::S, true, false>(src + key_at(kp) + j * 8);
+    }
+    // the loads as they are, before what the elements' conditions would make of them
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        constexpr int W = sizeof(x[0][0]) / 4;
+        Pack<uint32_t, W> w = __builtin_bit_cast(Pack<uint32_t, W>, x[kp][j]);
+#pragma unroll
+        for (int i = 0; i < W; ++i) asm volatile("" : "+v"(w.v[i]));
+        x[kp][j] = __builtin_bit_cast(Pack<typename E::S, 8>, w);
+      }
+    }
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+      const int nominal = kp * 64 + g * 16, at = key_at(kp);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         uint32_t w[TQ][4];
@@ -196,8 +208,8 @@ struct TileKernel {
           float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int d = at + j * 8 + i * 2 + e;
-            f[e] = d >= nominal && c < rows ? E::to_f(src[d]) : 0.0f;
+            f[e] = E::to_f(x[kp][j].v[i * 2 + e]);
+            if (at + j * 8 + i * 2 + e < nominal || c >= rows) f[e] = 0.0f;
           }
 #pragma unroll
           for (int t = 0; t < TQ; ++t) w[t][i] = take_bf16(f[0], f[1]);
@@ -212,70 +224,55 @@ struct TileKernel {
     for (int n = 0; n < VD; ++n) o[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     m = -__builtin_inff(), l = 0.0f;
     unit = MX ? 0 : kAttNoUnit;
-    missing = false;
   }
 
-  // The first element of lane column r's unit of a value vector.
+  // The first of the lane's sixteen elements of pair kp of a key; of column r's unit of a value.
+  __device__ __forceinline__ int key_at(int kp) const { return min(kp * 64 + g * 16, a.key.dim - 16); }
   __device__ __forceinline__ int value_at(int r) const { return min(r * VD, a.value.dim - VD); }
-
-  __device__ __forceinline__ TilePlace place(int tile) const {
-    const int p = min(max(tile * kAttTile + (lane & 31), first), end - 1);
-    const uint32_t column = a.by_page.quotient((uint32_t)p);
-    return TilePlace{row[column], (uint32_t)p - column * (uint32_t)a.page_size};
-  }
-
-  __device__ __forceinline__ void load(Codes& t, const TilePlace& at) {
-    const bool none = at.page < 0 || at.page >= a.pages;
-    missing |= none;
-    const int64_t page = none ? 0 : at.page, off = at.off;
-    const int64_t ko = page * a.key.c_page + off * a.key.c_token;
-    const int64_t vo = page * a.value.c_page + off * a.value.c_token;
-    const int64_t kso = page * a.key.s_page + off * a.key.s_token;
-    const int64_t vso = page * a.value.s_page + off * a.value.s_token;
-    if constexpr (MX) {
-      load_scales8(t.kb, static_cast<const uint8_t*>(ks_base) + kso, a.key.dim / kMxBlock);
-      load_scales8(t.vb, static_cast<const uint8_t*>(vs_base) + vso, a.value.dim / kMxBlock);
-    } else {
-      t.ks = static_cast<const float*>(ks_base)[kso];
-      t.vs = static_cast<const float*>(vs_base)[vso];
-    }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const uint8_t* p = k_base + from_lane64(ko, s * 16 + c);
-#pragma unroll
-      for (int kp = 0; kp < KP; ++kp) load_bytes<Codes::KW * 4>(t.k[s][kp], p + k_at[kp]);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      load_bytes<Codes::VB>(t.v[e], v_base + from_lane64(vo, position(e)) + v_at);
-    }
-  }
-
   // The tile's position of element e of S, P and V.
   __device__ __forceinline__ int position(int e) const { return (e >> 2) * 16 + g * 4 + (e & 3); }
 
-  __device__ __forceinline__ void compute(Codes& t, int tile) {
-    f32x4 s[2];
+  template <class Src>
+  __device__ __forceinline__ void tile(Src& src, int t) {
+    // a tile that holds positions outside [first, end): no weight, and nothing that could spoil a sum
+    if (t * kAttTile < first || (uint32_t)t * kAttTile + kAttTile > (uint32_t)end) tile_of<true>(src, t);
+    else tile_of<false>(src, t);
+  }
+  template <bool EDGE, class Src>
+  __device__ __forceinline__ void tile_of(Src& src, int t) {
+    bool live[8];
+    if constexpr (EDGE) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t b[2] = {0, 0};
-      if constexpr (MX) {
-        b[0] = from_lane(t.kb[0], h * 16 + c);
-        if (KP > 2) b[1] = from_lane(t.kb[1], h * 16 + c);
+      for (int e = 0; e < 8; ++e) {
+        const int p = t * kAttTile + position(e);
+        live[e] = p >= first && p < end;
       }
-      s[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-      for (int kp = 0; kp < KP; ++kp) {
-        const float scale = MX ? scale_operand(b, k_sel[kp]) : 1.0f;
+    for (int kp = 0; kp < KP; ++kp) {
+      uint32_t w[2][KW];
+      float scale[2] = {1.0f, 1.0f};
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t* w = t.k[h][kp] + j * (Codes::KW / 2);
-          const bf16x8 k = __builtin_bit_cast(
-              bf16x8, (u32x4{code_pair<FMT>(w, 0, scale), code_pair<FMT>(w, 1, scale),
-                             code_pair<FMT>(w, 2, scale), code_pair<FMT>(w, 3, scale)}));
+      for (int h = 0; h < 2; ++h) {
+        src.key(h, kp, w[h]);
+        if constexpr (MX) scale[h] = src.key_scale(h, kp);
+      }
 #pragma unroll
-          for (int x = TQ - 1; x >= 0; --x) {  // the smallest terms first
-            s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[kp][j][x], s[h], 0, 0, 0);
+      for (int j = 0; j < 2; ++j) {
+        bf16x8 k[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t* x = w[h] + j * (KW / 2);
+          k[h] = __builtin_bit_cast(
+              bf16x8, (u32x4{code_pair<FMT>(x, 0, scale[h]), code_pair<FMT>(x, 1, scale[h]),
+                             code_pair<FMT>(x, 2, scale[h]), code_pair<FMT>(x, 3, scale[h])}));
+        }
+#pragma unroll
+        for (int x = TQ - 1; x >= 0; --x) {  // the smallest terms first
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[h], q[kp][j][x], s[h], 0, 0, 0);
           }
         }
       }
@@ -283,20 +280,8 @@ struct TileKernel {
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      f[e] = s[e >> 2][e & 3] * (MX ? a.scale : from_lane_f(t.ks * a.scale, position(e)));
-    }
-    // a tile that holds positions outside [first, end): no weight, and nothing that could spoil a sum
-    const bool edge = tile * kAttTile < first || tile * kAttTile + kAttTile > end;
-    if (edge) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int p = tile * kAttTile + position(e);
-        if (p < first || p >= end) {
-          f[e] = -__builtin_inff();
-#pragma unroll
-          for (int x = 0; x < Codes::VW; ++x) t.v[e][x] = 0;
-        }
-      }
+      f[e] = s[e >> 2][e & 3] * (MX ? a.scale : src.ks(e) * a.scale);
+      if (EDGE) f[e] = live[e] ? f[e] : -__builtin_inff();
     }
     float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(f[0], f[1]), __builtin_fmaxf(f[2], f[3])),
                                 __builtin_fmaxf(__builtin_fmaxf(f[4], f[5]), __builtin_fmaxf(f[6], f[7])));
@@ -304,12 +289,14 @@ struct TileKernel {
     int e_max = unit;
     bool wider = false;
     if constexpr (!MX) {
-      const int e = att_unit(t.vs);
+      const int p = t * kAttTile + (lane & 31);
+      const int e = EDGE && (p < first || p >= end) ? kAttNoUnit : att_unit(src.most_vs());
       wider = __builtin_amdgcn_ballot_w64(e > unit) != 0;
       if (wider) {
         e_max = max(e, unit);
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) e_max = max(e_max, __shfl_xor(e_max, d, 64));
+        e_max = __builtin_amdgcn_readfirstlane(e_max);
       }
     }
     if (wider || __builtin_amdgcn_ballot_w64(top > m) != 0) {
@@ -322,20 +309,13 @@ struct TileKernel {
       unit = e_max;
     }
     const float at = m == -__builtin_inff() ? 0.0f : m;
-    const float vs = MX ? 1.0f : __builtin_ldexpf(t.vs, -unit);
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float p = __builtin_amdgcn_exp2f(f[e] - at);
       l += p;
-      w[e] = MX ? p : p * from_lane_f(vs, position(e));
-    }
-    if (!MX && edge) {  // no 0 times a scale that is no number
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int p = tile * kAttTile + position(e);
-        if (p < first || p >= end) w[e] = 0.0f;
-      }
+      w[e] = MX ? p : p * __builtin_ldexpf(src.vs(e), -unit);
+      if (!MX && EDGE) w[e] = live[e] ? w[e] : 0.0f;  // no 0 times a scale that is no number
     }
     bf16x8 p[TP];
     {
@@ -350,18 +330,17 @@ struct TileKernel {
         p[x] = __builtin_bit_cast(bf16x8, (u32x4{d[x][0], d[x][1], d[x][2], d[x][3]}));
       }
     }
+    uint32_t v[8][VW];
     float scale[8];
-    if constexpr (MX) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        uint32_t b[2];
-        b[0] = from_lane(t.vb[0], position(e));
-        b[1] = VD > 8 ? from_lane(t.vb[1], position(e)) : 0;
-        scale[e] = scale_operand(b, v_sel);
-        if (edge) {
-          const int at_p = tile * kAttTile + position(e);
-          if (at_p < first || at_p >= end) scale[e] = 1.0f;
-        }
+    for (int e = 0; e < 8; ++e) {
+      src.value(e, v[e]);
+      scale[e] = 1.0f;
+      if constexpr (MX) scale[e] = src.value_scale(e);
+      if constexpr (EDGE) {
+        scale[e] = live[e] ? scale[e] : 1.0f;
+#pragma unroll
+        for (int x = 0; x < VW; ++x) v[e][x] = live[e] ? v[e][x] : 0;
       }
     }
 #pragma unroll
@@ -369,13 +348,13 @@ struct TileKernel {
       uint32_t even[4], odd[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t *x = t.v[i * 2], *y = t.v[i * 2 + 1];
+        const uint32_t *x = v[i * 2], *y = v[i * 2 + 1];
         if constexpr (FMT == KV_INT8) {
           even[i] = high_halves(i8_bits(x[n >> 2], n & 3), i8_bits(y[n >> 2], n & 3));
           odd[i] = high_halves(i8_bits(x[n >> 2], (n & 3) + 1), i8_bits(y[n >> 2], (n & 3) + 1));
         } else {
-          const uint32_t xs = code_pair<FMT>(x, n >> 1, MX ? scale[i * 2] : 1.0f);
-          const uint32_t ys = code_pair<FMT>(y, n >> 1, MX ? scale[i * 2 + 1] : 1.0f);
+          const uint32_t xs = code_pair<FMT>(x, n >> 1, scale[i * 2]);
+          const uint32_t ys = code_pair<FMT>(y, n >> 1, scale[i * 2 + 1]);
           even[i] = low_halves(xs, ys), odd[i] = high_halves(xs, ys);
         }
       }
@@ -388,64 +367,373 @@ struct TileKernel {
       }
     }
   }
+
+  // Writes the wave's query heads: the outputs, or of a split sequence its part.
+  __device__ __forceinline__ void write(const AttChunk& ch, int head0, int rows, bool missing) {
+    float sum = column_sum(l);
+    if (missing || ch.missing) sum = __builtin_nanf("");
+    if (c >= rows) return;
+    const int query = head0 + c;
+    if (g == 0) {
+      if (ch.count > 1) {
+        float* dst = a.sums + ((int64_t)ch.part * a.query_heads + query) * 4;
+        dst[0] = m, dst[1] = sum, dst[2] = (float)unit;
+      } else if (a.lse != nullptr) {
+        a.lse[(int64_t)ch.sequence * a.query_heads + query] = att_lse(m, sum);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = value_at(g * 4 + i);
+      if (ch.count > 1) {
+        float* dst = a.parts + ((int64_t)ch.part * a.query_heads + query) * a.value.dim + d;
+#pragma unroll
+        for (int n = 0; n < VD; ++n) dst[n] = o[n][i];
+      } else {
+        typename E::S* dst = static_cast<typename E::S*>(a.value.plain) +
+                             ch.sequence * a.value.p_token + query * a.value.p_head + d;
+#pragma unroll
+        for (int n = 0; n < VD; ++n) dst[n] = E::from_f(att_value(o[n][i], sum, unit));
+      }
+    }
+  }
+};
+
+// ---- Codes through LDS: pages of whole sixteens, vectors of whole 16-byte chunks at multiples of 16.
+//
+// A wave's loads are then whole cache lines (a lane a chunk, the chunks of a position next to each other),
+// where loads in the order of the products take one request a lane: 2 x 131072 positions of 8 x 128 fp8
+// took 131 us so, with the L1 busy for four fifths of it.  A half of a tile, 16 positions of one page, is
+// CR chunks a position; chunk x of position r goes to place (x + r / (16 / gcd(CR, 16))) mod CR of its row, so
+// that the reads of one chunk of sixteen positions fall on different banks.
+struct HalfLayout {
+  int row, turn;  // chunks a row; log2 of 16 / gcd(row, 16)
+  __device__ __forceinline__ explicit HalfLayout(int bytes) : row(bytes / 16) {
+    turn = 4 - min(4, (int)__builtin_ctz((unsigned)row));
+  }
+  __device__ __forceinline__ int place(int r, int x) const {
+    const int y = x + (r >> turn);
+    return r * row + (y >= row ? y - row * (int)((unsigned)y / (unsigned)row) : y);
+  }
+  // The chunk that belongs at place i.
+  __device__ __forceinline__ int chunk(int r, int i) const {
+    const int y = i - (r >> turn) % row;
+    return y < 0 ? y + row : y;
+  }
+};
+
+template <int FMT, int KP, int VD>
+struct LdsTile {  // bytes
+  static constexpr int KN = FMT == KV_MXFP4 ? (KP + 1) / 2 : KP;          // loads of a half's keys
+  static constexpr int VN = FMT == KV_MXFP4 ? (VD + 7) / 8 : (VD + 3) / 4;  // of its values
+  static constexpr int kHalf = 1024 * (KN + VN), kScales = 2 * kHalf;
+  static constexpr int kBytes = 2 * kHalf + (FMT == KV_MXFP4 ? 0 : 256);
+};
+
+template <class E, int FMT, int KP, int VD>
+struct LdsSource {
+  using W = AttWave<E, FMT, KP, VD>;
+  using T = LdsTile<FMT, KP, VD>;
+  static constexpr bool MX = W::MX;
+  const AttArgs& a;
+  const W& wave;
+  const int32_t* row;  // of the table
+  const uint8_t *k_base, *v_base, *ks_base, *vs_base;  // of the key head
+  uint32_t k_from[T::KN], v_from[T::VN];  // where the lane's chunks lie in a half of the cache
+  int64_t scale_from;                     // and its scale (lanes 0..31 a key's, then a value's)
+  int k_at[KP], v_at[4];                  // what the lane reads of a half in LDS
+  uint32_t k_sel[KP], v_sel;
+  // halves [base, base + 64) of the sequence: lane i knows half base + i
+  int base;
+  int64_t ko, vo, kso, vso;
+  bool missing;
+  uint32_t to;                // LDS of the wave
+  const uint8_t* at;          // the tile in turn, as the lanes read it
+  uint32_t kb[2], vb[2], kb_next[2], vb_next[2];  // scales of 4-bit blocks of position lane % 32
+
+  __device__ __forceinline__ LdsSource(const AttArgs& args, const W& w, const AttChunk& ch, int head,
+                                       uint8_t* lds, uint32_t lds_at)
+      : a(args), wave(w), to(lds_at), at(lds) {
+    row = a.table + ch.sequence * a.table_stride;
+    const int es = MX ? 1 : 4;
+    k_base = a.key.codes + head * a.key.c_head;
+    v_base = a.value.codes + head * a.value.c_head;
+    ks_base = static_cast<const uint8_t*>(a.key.scales) + head * a.key.s_head * es;
+    vs_base = static_cast<const uint8_t*>(a.value.scales) + head * a.value.s_head * es;
+    const int lane = w.lane, c = w.c, g = w.g;
+    const HalfLayout k(MX ? a.key.dim / 2 : a.key.dim), v(MX ? a.value.dim / 2 : a.value.dim);
+#pragma unroll
+    for (int i = 0; i < T::KN; ++i) {
+      const int x = min(i * 64 + lane, 16 * k.row - 1), r = (int)((unsigned)x / (unsigned)k.row);
+      k_from[i] = (uint32_t)(r * (int)a.key.c_token + k.chunk(r, x - r * k.row) * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < T::VN; ++i) {
+      const int x = min(i * 64 + lane, 16 * v.row - 1), r = (int)((unsigned)x / (unsigned)v.row);
+      v_from[i] = (uint32_t)(r * (int)a.value.c_token + v.chunk(r, x - r * v.row) * 16);
+    }
+    scale_from = (lane & 15) * (lane < 32 || MX ? a.key.s_token : a.value.s_token) * es;
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+      const int d = w.key_at(kp), b = MX ? d / 2 : d;
+      k_at[kp] = k.place(c, b / 16) * 16 + b % 16;
+      k_sel[kp] = MX ? scale_selector(d / kMxBlock, a.key.dim / kMxBlock) : 0;
+    }
+    const int d = w.value_at(c), b = MX ? d / 2 : d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v_at[i] = 1024 * T::KN + v.place(g * 4 + i, b / 16) * 16 + b % 16;
+    v_sel = MX ? scale_selector(d / kMxBlock, a.value.dim / kMxBlock) : 0;
+    missing = false;
+  }
+
+  // Looks up the pages of the halves from tile t on; those without a live position stand for their
+  // neighbours.
+  __device__ __forceinline__ void look_up(int t) {
+    base = t * 2;
+    const int p = min(max(base + wave.lane, wave.first / 16), (wave.end - 1) / 16) * 16;
+    const uint32_t column = a.by_page.quotient((uint32_t)p);
+    const int found = row[column];
+    const bool none = found < 0 || found >= a.pages;
+    const int64_t page = none ? 0 : found, off = (uint32_t)p - column * (uint32_t)a.page_size;
+    ko = page * a.key.c_page + off * a.key.c_token;
+    vo = page * a.value.c_page + off * a.value.c_token;
+    kso = (page * a.key.s_page + off * a.key.s_token) * (MX ? 1 : 4);
+    vso = (page * a.value.s_page + off * a.value.s_token) * (MX ? 1 : 4);
+    none_at = __builtin_amdgcn_ballot_w64(none);
+  }
+  uint64_t none_at;  // halves of base.. without a page
+
+  static __device__ __forceinline__ int64_t of_lane(int64_t v, int i) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)v, i));
+  }
+
+  // Starts the loads of tile t into buffer `turn`.
+  __device__ __forceinline__ void load(int t, int turn) {
+    if (t * 2 >= base + 64) look_up(t);
+    const int i = t * 2 - base;
+    missing |= (none_at >> i & 3) != 0;
+    const uint32_t dst = to + turn * T::kBytes;
+    int64_t ks[2], vs[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* k = k_base + of_lane(ko, i + h);
+      const uint8_t* v = v_base + of_lane(vo, i + h);
+      ks[h] = of_lane(kso, i + h), vs[h] = of_lane(vso, i + h);
+#pragma unroll
+      for (int x = 0; x < T::KN; ++x) tile_to_lds16(dst + h * T::kHalf + x * 1024, k, k_from[x]);
+#pragma unroll
+      for (int x = 0; x < T::VN; ++x) {
+        tile_to_lds16(dst + h * T::kHalf + (T::KN + x) * 1024, v, v_from[x]);
+      }
+    }
+    const bool high = (wave.lane & 16) != 0;
+    if constexpr (MX) {
+      const int64_t vs_from = (wave.lane & 15) * a.value.s_token;
+      load_scales8(kb_next, ks_base + (high ? ks[1] : ks[0]) + scale_from, a.key.dim / kMxBlock);
+      load_scales8(vb_next, vs_base + (high ? vs[1] : vs[0]) + vs_from, a.value.dim / kMxBlock);
+    } else {
+      const uint8_t* k = ks_base + (high ? ks[1] : ks[0]);
+      const uint8_t* v = vs_base + (high ? vs[1] : vs[0]);
+      tile_to_lds4(dst + T::kScales, (wave.lane < 32 ? k : v) + scale_from);
+    }
+  }
+  // What was loaded into `turn` is what the functions below give.
+  __device__ __forceinline__ void take(const uint8_t* lds, int turn) {
+    at = lds + turn * T::kBytes;
+    if constexpr (MX) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) kb[i] = kb_next[i], vb[i] = vb_next[i];
+    }
+  }
+
+  __device__ __forceinline__ void key(int h, int kp, uint32_t* w) const {
+    if constexpr (MX) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(at + h * T::kHalf + k_at[kp]);
+      w[0] = x[0], w[1] = x[1];
+    } else {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(at + h * T::kHalf + k_at[kp]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = x[i];
+    }
+  }
+  __device__ __forceinline__ float key_scale(int h, int kp) const {
+    uint32_t b[2];
+    b[0] = from_lane(kb[0], h * 16 + wave.c);
+    b[1] = KP > 2 ? from_lane(kb[1], h * 16 + wave.c) : 0;
+    return scale_operand(b, k_sel[kp]);
+  }
+  __device__ __forceinline__ void value(int e, uint32_t* w) const {
+    const uint8_t* p = at + (e >> 2) * T::kHalf + v_at[e & 3];
+    if constexpr (W::VB == 2) {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    } else {
+      const auto x = *reinterpret_cast<const Pack<uint32_t, W::VW>*>(p);
+#pragma unroll
+      for (int i = 0; i < W::VW; ++i) w[i] = x.v[i];
+    }
+  }
+  __device__ __forceinline__ float value_scale(int e) const {
+    uint32_t b[2];
+    b[0] = from_lane(vb[0], wave.position(e));
+    b[1] = VD > 8 ? from_lane(vb[1], wave.position(e)) : 0;
+    return scale_operand(b, v_sel);
+  }
+  __device__ __forceinline__ float ks(int e) const {
+    return reinterpret_cast<const float*>(at + T::kScales)[wave.position(e)];
+  }
+  __device__ __forceinline__ float vs(int e) const {
+    return reinterpret_cast<const float*>(at + T::kScales + 128)[wave.position(e)];
+  }
+  __device__ __forceinline__ float most_vs() const {
+    return reinterpret_cast<const float*>(at + T::kScales + 128)[wave.lane & 31];
+  }
+};
+
+template <class E, int FMT, int KP, int VD>
+__global__ void __launch_bounds__(kAttWaves * 64)
+k_kv_attention_lines(AttArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds_bytes[];  // [waves][2] tiles
+  using T = LdsTile<FMT, KP, VD>;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  uint32_t flat;
+  int head, block;
+  att_wave_place(a, (uint32_t)wave, &flat, &head, &block);
+  AttChunk c;
+  if (!find_chunk(a, flat, head == 0 && block == 0, &c)) return;
+  const int head0 = head * a.group + block * kTileRows;
+  const int rows = min(kTileRows, a.group - block * kTileRows);
+  AttWave<E, FMT, KP, VD> w(a, c, head0, rows);
+  uint8_t* mine = lds_bytes + wave * (2 * T::kBytes);
+  LdsSource<E, FMT, KP, VD> src(
+      a, w, c, head, mine,
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds_bytes + wave * (2 * T::kBytes));
+  if (c.tiles > 0) {
+    const int last = c.tile + c.tiles - 1;
+    src.look_up(c.tile);
+    src.load(c.tile, 0);
+    for (int t = c.tile, turn = 0; t <= last; ++t, turn ^= 1) {
+      wait_tile();
+      src.take(mine, turn);
+      if (t < last) src.load(t + 1, turn ^ 1);
+      w.tile(src, t);
+    }
+  }
+  w.write(c, head0, rows, src.missing);
+}
+
+// ---- Codes straight to registers, at any alignment and in pages of any size.
+template <class E, int FMT, int KP, int VD>
+struct RegisterSource {
+  using W = AttWave<E, FMT, KP, VD>;
+  static constexpr bool MX = W::MX;
+  const AttArgs& a;
+  const W& wave;
+  const int32_t* row;
+  const uint8_t *k_base, *v_base;
+  const void *ks_base, *vs_base;
+  int v_at;
+  uint32_t k_sel[KP], v_sel;
+  bool missing;
+  uint32_t k[2][KP][W::KW], v[8][W::VW], kb[2], vb[2];
+  float k_scale, v_scale;  // of position lane % 32
+
+  __device__ __forceinline__ RegisterSource(const AttArgs& args, const W& w, const AttChunk& ch,
+                                            int head)
+      : a(args), wave(w) {
+    row = a.table + ch.sequence * a.table_stride;
+    k_base = a.key.codes + head * a.key.c_head;
+    v_base = a.value.codes + head * a.value.c_head;
+    const int es = MX ? 1 : 4;
+    ks_base = static_cast<const uint8_t*>(a.key.scales) + head * a.key.s_head * es;
+    vs_base = static_cast<const uint8_t*>(a.value.scales) + head * a.value.s_head * es;
+    const int d = w.value_at(w.c);
+    v_at = MX ? d / 2 : d;
+    v_sel = MX ? scale_selector(d / kMxBlock, a.value.dim / kMxBlock) : 0;
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+      k_sel[kp] = MX ? scale_selector(w.key_at(kp) / kMxBlock, a.key.dim / kMxBlock) : 0;
+    }
+    missing = false;
+  }
+
+  // Loads tile t; positions before the first or behind the last stand for those.
+  __device__ __forceinline__ void load(int t) {
+    const int p = min(max(t * kAttTile + (wave.lane & 31), wave.first), wave.end - 1);
+    const uint32_t column = a.by_page.quotient((uint32_t)p);
+    const int found = row[column];
+    const bool none = found < 0 || found >= a.pages;
+    missing |= __builtin_amdgcn_ballot_w64(none) != 0;
+    const int64_t page = none ? 0 : found, off = (uint32_t)p - column * (uint32_t)a.page_size;
+    const int64_t ko = page * a.key.c_page + off * a.key.c_token;
+    const int64_t vo = page * a.value.c_page + off * a.value.c_token;
+    const int64_t kso = page * a.key.s_page + off * a.key.s_token;
+    const int64_t vso = page * a.value.s_page + off * a.value.s_token;
+    if constexpr (MX) {
+      load_scales8(kb, static_cast<const uint8_t*>(ks_base) + kso, a.key.dim / kMxBlock);
+      load_scales8(vb, static_cast<const uint8_t*>(vs_base) + vso, a.value.dim / kMxBlock);
+    } else {
+      k_scale = static_cast<const float*>(ks_base)[kso];
+      v_scale = static_cast<const float*>(vs_base)[vso];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* p = k_base + from_lane64(ko, h * 16 + wave.c);
+#pragma unroll
+      for (int kp = 0; kp < KP; ++kp) {
+        const int d = wave.key_at(kp);
+        load_bytes<W::KW * 4>(k[h][kp], p + (MX ? d / 2 : d));
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      load_bytes<W::VB>(v[e], v_base + from_lane64(vo, wave.position(e)) + v_at);
+    }
+  }
+
+  __device__ __forceinline__ void key(int h, int kp, uint32_t* w) const {
+#pragma unroll
+    for (int i = 0; i < W::KW; ++i) w[i] = k[h][kp][i];
+  }
+  __device__ __forceinline__ float key_scale(int h, int kp) const {
+    uint32_t b[2];
+    b[0] = from_lane(kb[0], h * 16 + wave.c);
+    b[1] = KP > 2 ? from_lane(kb[1], h * 16 + wave.c) : 0;
+    return scale_operand(b, k_sel[kp]);
+  }
+  __device__ __forceinline__ void value(int e, uint32_t* w) const {
+#pragma unroll
+    for (int i = 0; i < W::VW; ++i) w[i] = v[e][i];
+  }
+  __device__ __forceinline__ float value_scale(int e) const {
+    uint32_t b[2];
+    b[0] = from_lane(vb[0], wave.position(e));
+    b[1] = VD > 8 ? from_lane(vb[1], wave.position(e)) : 0;
+    return scale_operand(b, v_sel);
+  }
+  __device__ __forceinline__ float ks(int e) const { return from_lane_f(k_scale, wave.position(e)); }
+  __device__ __forceinline__ float vs(int e) const { return from_lane_f(v_scale, wave.position(e)); }
+  __device__ __forceinline__ float most_vs() const { return v_scale; }
 };
 
 template <class E, int FMT, int KP, int VD>
 __global__ void __launch_bounds__(kAttWaves * 64)
 k_kv_attention_tiles(AttArgs a) {
-  // m, l [waves][16], e [waves], o [waves][rows][value.dim + 1]
-  extern __shared__ float lds[];
-  using K = TileKernel<E, FMT, KP, VD>;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   uint32_t flat;
   int head, block;
-  att_place(a, &flat, &head, &block);
+  att_wave_place(a, (uint32_t)wave, &flat, &head, &block);
   AttChunk c;
-  if (!find_chunk(a, flat, head == 0 && block == 0 && wave == 0, &c)) return;
+  if (!find_chunk(a, flat, head == 0 && block == 0, &c)) return;
   const int head0 = head * a.group + block * kTileRows;
   const int rows = min(kTileRows, a.group - block * kTileRows);
-  K k(a, c, head, head0, rows);
-  const int last = c.tile + c.tiles - 1;
-  int tile = c.tile + wave;
-  if (tile <= last) {
-    // two tiles' codes in turn; a position's page is looked up two tiles ahead, its codes are loaded one
-    typename K::Codes t[2];
-    TilePlace next = k.place(min(tile + kAttWaves, last));
-    k.load(t[0], k.place(tile));
-    for (;;) {
-      TilePlace after = k.place(min(tile + 2 * kAttWaves, last));
-      if (tile + kAttWaves <= last) k.load(t[1], next);
-      k.compute(t[0], tile);
-      tile += kAttWaves;
-      if (tile > last) break;
-      next = k.place(min(tile + 2 * kAttWaves, last));
-      if (tile + kAttWaves <= last) k.load(t[0], after);
-      k.compute(t[1], tile);
-      tile += kAttWaves;
-      if (tile > last) break;
-    }
+  AttWave<E, FMT, KP, VD> w(a, c, head0, rows);
+  RegisterSource<E, FMT, KP, VD> src(a, w, c, head);
+  for (int t = c.tile; t < c.tile + c.tiles; ++t) {
+    src.load(t);
+    w.tile(src, t);
   }
-  const bool missing = __builtin_amdgcn_ballot_w64(k.missing) != 0;
-  const float l = column_sum(k.l);
-  float *ms = lds, *ls = ms + kAttWaves * kTileRows;
-  int* es = reinterpret_cast<int*>(ls + kAttWaves * kTileRows);
-  float* os = reinterpret_cast<float*>(es + kAttWaves);
-  const int most = min(kTileRows, a.group), stride = a.value.dim + 1;
-  if (k.g == 0) {
-    ms[wave * kTileRows + k.c] = k.m;
-    ls[wave * kTileRows + k.c] = missing ? __builtin_nanf("") : l;
-  }
-  if (k.lane == 0) es[wave] = k.unit;
-  if (k.c < rows) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float* dst = os + (wave * most + k.c) * stride + k.value_at(k.g * 4 + i);
-#pragma unroll
-      for (int n = 0; n < VD; ++n) dst[n] = k.o[n][i];
-    }
-  }
-  __syncthreads();
-  att_write<E>(a, c, head0, rows, 0, a.value.dim, ms, ls, es, os, kTileRows, most, stride);
+  w.write(c, head0, rows, src.missing);
 }
 
 // The kernels' head sizes: keys of up to 64 KP and values of up to 16 VD elements, at least a unit of each.
@@ -455,29 +743,38 @@ struct TileShape {
 constexpr TileShape kTileShapes[] = {{1, 4}, {2, 8}, {3, 8}, {4, 16}};
 
 // Launches the kernel of shape `shape` (an index above) on the sequences' chunks.
-int attention_tiles_int8(int shape, mcop_dtype dtype, const AttArgs& a, dim3 grid, size_t lds,
+int attention_tiles_int8(int shape, bool lines, mcop_dtype dtype, const AttArgs& a, dim3 grid,
                          hipStream_t st);
-int attention_tiles_fp8(int shape, mcop_dtype dtype, const AttArgs& a, dim3 grid, size_t lds,
+int attention_tiles_fp8(int shape, bool lines, mcop_dtype dtype, const AttArgs& a, dim3 grid,
                         hipStream_t st);
-int attention_tiles_mxfp4(int shape, mcop_dtype dtype, const AttArgs& a, dim3 grid, size_t lds,
+int attention_tiles_mxfp4(int shape, bool lines, mcop_dtype dtype, const AttArgs& a, dim3 grid,
                           hipStream_t st);
 
-template <int FMT, class E>
-void attention_tiles_of(int shape, const AttArgs& a, dim3 grid, size_t lds, hipStream_t st) {
+template <int FMT, class E, int KP, int VD>
+void attention_tiles_of(bool lines, const AttArgs& a, dim3 grid, hipStream_t st) {
   const dim3 block(kAttWaves * 64);
-  switch (shape) {
-    case 0: hipLaunchKernelGGL((k_kv_attention_tiles<E, FMT, 1, 4>), grid, block, lds, st, a); break;
-    case 1: hipLaunchKernelGGL((k_kv_attention_tiles<E, FMT, 2, 8>), grid, block, lds, st, a); break;
-    case 2: hipLaunchKernelGGL((k_kv_attention_tiles<E, FMT, 3, 8>), grid, block, lds, st, a); break;
-    default: hipLaunchKernelGGL((k_kv_attention_tiles<E, FMT, 4, 16>), grid, block, lds, st, a);
+  if (lines) {
+    constexpr size_t kLds = (size_t)kAttWaves * 2 * LdsTile<FMT, KP, VD>::kBytes;
+    hipLaunchKernelGGL((k_kv_attention_lines<E, FMT, KP, VD>), grid, block, kLds, st, a);
+  } else {
+    hipLaunchKernelGGL((k_kv_attention_tiles<E, FMT, KP, VD>), grid, block, 0, st, a);
   }
 }
 template <int FMT>
-int attention_tiles_for(int shape, mcop_dtype dtype, const AttArgs& a, dim3 grid, size_t lds,
+int attention_tiles_for(int shape, bool lines, mcop_dtype dtype, const AttArgs& a, dim3 grid,
                         hipStream_t st) {
-  if (dtype == MCOP_BF16) attention_tiles_of<FMT, BF16>(shape, a, grid, lds, st);
-  else if (dtype == MCOP_F16) attention_tiles_of<FMT, F16>(shape, a, grid, lds, st);
-  else attention_tiles_of<FMT, F32>(shape, a, grid, lds, st);
+  auto by_shape = [&](auto e) {
+    using E = decltype(e);
+    switch (shape) {
+      case 0: attention_tiles_of<FMT, E, 1, 4>(lines, a, grid, st); break;
+      case 1: attention_tiles_of<FMT, E, 2, 8>(lines, a, grid, st); break;
+      case 2: attention_tiles_of<FMT, E, 3, 8>(lines, a, grid, st); break;
+      default: attention_tiles_of<FMT, E, 4, 16>(lines, a, grid, st);
+    }
+  };
+  if (dtype == MCOP_BF16) by_shape(BF16());
+  else if (dtype == MCOP_F16) by_shape(F16());
+  else by_shape(F32());
   return check_launch("kv_cache_attention");
 }
 
