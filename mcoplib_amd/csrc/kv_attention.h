@@ -45,8 +45,9 @@ struct AttArgs {
   int page_size;
   Divisor by_page;
   int heads, group, query_heads;  // key heads, query heads of each, query heads
-  int row_blocks;                 // workgroups that a key head's query heads take
-  Divisor by_inner;               // heads * row_blocks
+  int row_blocks;                 // waves (or workgroups) that a key head's query heads take
+  Divisor by_inner, by_blocks;    // heads * row_blocks, row_blocks
+  Divisor k_chunks, v_chunks;     // chunks of 16 bytes of a key, of a value
   int window;
   int target;
   float scale;    // times log2 e
@@ -77,58 +78,58 @@ __device__ __forceinline__ uint32_t att_tiles(const AttArgs& a, int n) {
   return ((uint32_t)n + kAttTile - 1) / kAttTile - (uint32_t)att_first(a, n) / kAttTile;
 }
 
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor((unsigned long long)v, d, 64);
+// Inclusive sums over the wave's lanes, by register moves: within rows of 16, then across them.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return v;
 }
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint64_t o = __shfl_up((unsigned long long)v, d, 64);
-    if (lane >= d) v += o;
-  }
-  return v;
+__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(v), 63);
+}
+// The same of values below 2^44, 22 bits at a time.
+__device__ __forceinline__ uint64_t wave_total64(uint64_t v) {
+  return ((uint64_t)wave_total((uint32_t)(v >> 22)) << 22) + wave_total((uint32_t)v & 0x3fffff);
 }
 
 // The chunk of number `flat`; false past the last one.  A wave works together, 64 sequences at a time.
 // `plans`: this wave writes the plan of the sequence whose first chunk it finds.
 __device__ __forceinline__ bool find_chunk(const AttArgs& a, uint32_t flat, bool plans, AttChunk* c) {
   const int lane = (int)threadIdx.x & 63;
-  uint64_t total = 0;
-  for (int i = 0; i < a.sequences; i += 64) {
+  const int n0 = lane < a.sequences ? a.lens[lane] : 0;
+  uint64_t total = att_tiles(a, n0);
+  for (int i = 64; i < a.sequences; i += 64) {
     if (i + lane < a.sequences) total += att_tiles(a, a.lens[i + lane]);
   }
-  total = wave_sum(total);
-  total = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(total >> 32)) << 32 |
-          (uint32_t)__builtin_amdgcn_readfirstlane((int)total);
-  uint64_t per = kAttLeastTiles;
+  total = wave_total64(total);
+  uint32_t per = kAttLeastTiles;
   if (total > (uint64_t)a.target * kAttLeastTiles) {
-    per = total >> 32 ? (total + a.target - 1) / a.target
+    per = total >> 31 ? (uint32_t)min((total + a.target - 1) / a.target, (uint64_t)1 << 26)
                       : ((uint32_t)total - 1) / (uint32_t)a.target + 1;
   }
-  uint64_t before = 0;  // chunks of earlier sequences, and in the high half their parts
+  uint32_t before = 0, parts_before = 0;  // chunks of earlier sequences, and their parts
   int splits = 0;
   bool found = false;
   for (int i = 0; i < a.sequences; i += 64) {
-    const int n = i + lane < a.sequences ? a.lens[i + lane] : 0;
-    const uint32_t t = i + lane < a.sequences ? att_tiles(a, n) : 0;
-    const uint32_t k = i + lane >= a.sequences ? 0 : t <= per ? 1 : (t - 1) / (uint32_t)per + 1;
-    const uint64_t mine = k | (k > 1 ? (uint64_t)k << 32 : 0);
-    const uint64_t upto = wave_scan(mine, lane) + before;
+    const int n = i == 0 ? n0 : (i + lane < a.sequences ? a.lens[i + lane] : 0);
+    const uint32_t t = att_tiles(a, n);
+    const uint32_t k = i + lane >= a.sequences ? 0 : t <= per ? 1 : (t - 1) / per + 1;
+    const uint32_t upto = wave_scan(k) + before, parts = wave_scan(k > 1 ? k : 0) + parts_before;
     const uint64_t split = __builtin_amdgcn_ballot_w64(k > 1);
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(k > 0 && (uint32_t)upto > flat);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(k > 0 && upto > flat);
     if (!found && hit != 0) {
       found = true;
       const int at = __builtin_ctzll(hit);
-      const uint32_t from = (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), at);
-      const uint32_t from_parts = (uint32_t)__builtin_amdgcn_readlane((int)((upto - mine) >> 32), at);
       const uint32_t tiles = (uint32_t)__builtin_amdgcn_readlane((int)t, at);
       c->sequence = i + at;
       c->end = __builtin_amdgcn_readlane(n, at);
       c->count = __builtin_amdgcn_readlane((int)k, at);
-      c->index = (int)(flat - from);
-      c->part = (int)from_parts + c->index;
+      c->index = (int)flat - __builtin_amdgcn_readlane((int)(upto - k), at);
+      c->part = __builtin_amdgcn_readlane((int)(parts - k), at) + c->index;
       c->missing = c->end > att_capacity(a);
       c->first = att_first(a, c->end);
       const uint32_t each = tiles / (uint32_t)c->count, more = tiles % (uint32_t)c->count;
@@ -145,8 +146,8 @@ __device__ __forceinline__ bool find_chunk(const AttArgs& a, uint32_t flat, bool
       if (!plans || flat != 0) return true;
     }
     splits += (int)__builtin_popcountll(split);
-    before = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(upto >> 32), 63) << 32 |
-             (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    before = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    parts_before = (uint32_t)__builtin_amdgcn_readlane((int)parts, 63);
   }
   if (plans && flat == 0 && lane == 0) a.plan[0] = splits;
   return found;
@@ -159,7 +160,7 @@ __device__ __forceinline__ void att_wave_place(const AttArgs& a, uint32_t wave, 
   const uint32_t die = blockIdx.x & 7, i = (blockIdx.x >> 3) * kAttWaves + wave;
   const uint32_t row = a.by_inner.quotient(i), inner = i - row * a.by_inner.d;
   *flat = row * 8 + die;
-  *head = (int)(inner / (uint32_t)a.row_blocks);
+  *head = (int)a.by_blocks.quotient(inner);
   *block = (int)(inner - (uint32_t)*head * (uint32_t)a.row_blocks);
 }
 
@@ -169,7 +170,7 @@ __device__ __forceinline__ void att_place(const AttArgs& a, uint32_t* flat, int*
   const uint32_t die = blockIdx.x & 7, i = blockIdx.x >> 3;
   const uint32_t row = a.by_inner.quotient(i), inner = i - row * a.by_inner.d;
   *flat = row * 8 + die;
-  *head = (int)(inner / (uint32_t)a.row_blocks);
+  *head = (int)a.by_blocks.quotient(inner);
   *block = (int)(inner - (uint32_t)*head * (uint32_t)a.row_blocks);
 }
 

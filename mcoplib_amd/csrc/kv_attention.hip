@@ -268,6 +268,10 @@ int launch_of(const char* name, AttArgs a, mcop_dtype dtype, int64_t chunks, boo
                      (long long)blocks);
   }
   a.by_inner = Divisor((uint32_t)inner);
+  a.by_blocks = Divisor((uint32_t)a.row_blocks);
+  const int packed = FMT == KV_MXFP4 ? 32 : 16;
+  a.k_chunks = Divisor((uint32_t)std::max(1, a.key.dim / packed));
+  a.v_chunks = Divisor((uint32_t)std::max(1, a.value.dim / packed));
   const size_t lds =
       sizeof(float) * kAttWaves *
       (shape >= 0 ? 0

@@ -27,7 +27,8 @@ namespace mcop {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTileRows = 16;  // query heads of a workgroup
+constexpr int kTileRows = 16;    // query heads of a wave
+constexpr float kAttSlack = 8.0f;  // weights are at most 2^8
 
 template <class E>
 struct AttTerms {  // bf16 terms of a query, of a weight
@@ -299,7 +300,9 @@ struct AttWave {
         e_max = __builtin_amdgcn_readfirstlane(e_max);
       }
     }
-    if (wider || __builtin_amdgcn_ballot_w64(top > m) != 0) {
+    // the reference of the weights moves when a logit is 2^kAttSlack past it, not with every new maximum:
+    // of sixteen query heads one has a new one in nearly every tile
+    if (wider || __builtin_amdgcn_ballot_w64(top > m + kAttSlack) != 0) {
       const float keep = att_weight(m, top);
       const float keep_o = keep * att_power(unit - e_max);
       l *= keep;
@@ -407,18 +410,21 @@ struct AttWave {
 // CR chunks a position; chunk x of position r goes to place (x + r / (16 / gcd(CR, 16))) mod CR of its row, so
 // that the reads of one chunk of sixteen positions fall on different banks.
 struct HalfLayout {
+  const Divisor& by_row;
   int row, turn;  // chunks a row; log2 of 16 / gcd(row, 16)
-  __device__ __forceinline__ explicit HalfLayout(int bytes) : row(bytes / 16) {
+  __device__ __forceinline__ explicit HalfLayout(const Divisor& chunks)
+      : by_row(chunks), row((int)chunks.d) {
     turn = 4 - min(4, (int)__builtin_ctz((unsigned)row));
   }
-  __device__ __forceinline__ int place(int r, int x) const {
-    const int y = x + (r >> turn);
-    return r * row + (y >= row ? y - row * (int)((unsigned)y / (unsigned)row) : y);
+  __device__ __forceinline__ int mod(int y) const {
+    return y - row * (int)by_row.quotient((uint32_t)y);
   }
-  // The chunk that belongs at place i.
-  __device__ __forceinline__ int chunk(int r, int i) const {
-    const int y = i - (r >> turn) % row;
-    return y < 0 ? y + row : y;
+  __device__ __forceinline__ int place(int r, int x) const { return r * row + mod(x + (r >> turn)); }
+  // Where in the cache, from the half's start, the chunk of LDS place i (of 16 rows) lies.
+  __device__ __forceinline__ uint32_t from(int i, int token) const {
+    const int r = (int)by_row.quotient((uint32_t)i), turned = mod(r >> turn);
+    const int y = i - r * row - turned;
+    return (uint32_t)(r * token + (y < 0 ? y + row : y) * 16);
   }
 };
 
@@ -461,16 +467,14 @@ struct LdsSource {
     ks_base = static_cast<const uint8_t*>(a.key.scales) + head * a.key.s_head * es;
     vs_base = static_cast<const uint8_t*>(a.value.scales) + head * a.value.s_head * es;
     const int lane = w.lane, c = w.c, g = w.g;
-    const HalfLayout k(MX ? a.key.dim / 2 : a.key.dim), v(MX ? a.value.dim / 2 : a.value.dim);
+    const HalfLayout k(a.k_chunks), v(a.v_chunks);
 #pragma unroll
     for (int i = 0; i < T::KN; ++i) {
-      const int x = min(i * 64 + lane, 16 * k.row - 1), r = (int)((unsigned)x / (unsigned)k.row);
-      k_from[i] = (uint32_t)(r * (int)a.key.c_token + k.chunk(r, x - r * k.row) * 16);
+      k_from[i] = k.from(min(i * 64 + lane, 16 * k.row - 1), (int)a.key.c_token);
     }
 #pragma unroll
     for (int i = 0; i < T::VN; ++i) {
-      const int x = min(i * 64 + lane, 16 * v.row - 1), r = (int)((unsigned)x / (unsigned)v.row);
-      v_from[i] = (uint32_t)(r * (int)a.value.c_token + v.chunk(r, x - r * v.row) * 16);
+      v_from[i] = v.from(min(i * 64 + lane, 16 * v.row - 1), (int)a.value.c_token);
     }
     scale_from = (lane & 15) * (lane < 32 || MX ? a.key.s_token : a.value.s_token) * es;
 #pragma unroll
