@@ -249,7 +249,8 @@ bool whole_lines(const AttArgs& a, int fmt) {
   for (const KvSide* k : {&a.key, &a.value}) {
     const int64_t bytes = fmt == KV_MXFP4 ? k->dim / 2 : k->dim;
     if (bytes % 16 != 0 || !aligned(16, k->codes) || k->c_page % 16 != 0 || k->c_token % 16 != 0 ||
-        k->c_head % 16 != 0 || k->c_token >= ((int64_t)1 << 31) / 16 - 1024) {
+        k->c_head % 16 != 0 || k->c_token >= ((int64_t)1 << 31) / 16 - 1024 ||
+        k->s_token >= ((int64_t)1 << 31) / 64 - 16) {
       return false;
     }
   }
@@ -382,7 +383,7 @@ extern "C" int mcop_kv_cache_attention(const mcop_kv_side* key, const mcop_kv_si
   a.query_heads = (int)query_heads;
   a.group = (int)(query_heads / num_heads);
   a.window = (int)std::min<int64_t>(window, INT32_MAX);
-  a.target = (int)target;
+  a.target = (int)std::max<int64_t>(target - num_sequences, (target + 1) / 2);
   a.scale = scale * kLog2e;
   a.parts = static_cast<float*>(workspace);
   a.sums = a.parts + ws.parts / 4;

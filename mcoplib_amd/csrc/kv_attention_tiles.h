@@ -130,13 +130,21 @@ __device__ __forceinline__ float column_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-// 16, 4 bytes a lane from its address to LDS at `to` + 16, 4 * lane, which the instruction takes from m0 (a
-// state after its write).  The compiler sees neither what this writes nor that it is in flight:
-// wait_tile() orders it.
+// 16, 4 bytes, or one as a dword, a lane from its address to LDS at `to` + 16, 4 * lane, which the instruction
+// takes from m0 (a state after its write).  The compiler sees neither what this writes nor that it is in
+// flight: wait_loads() orders it.
 __device__ __forceinline__ void tile_to_lds16(uint32_t to, const uint8_t* base, uint32_t off) {
   asm volatile(
       "s_nop 0\n\t"
       "global_load_lds_dwordx4 %1, %2"
+      :
+      : "{m0}"(to), "v"(off), "s"(base)
+      : "memory");
+}
+__device__ __forceinline__ void tile_to_lds1(uint32_t to, const uint8_t* base, uint32_t off) {
+  asm volatile(
+      "s_nop 0\n\t"
+      "global_load_lds_ubyte %1, %2"
       :
       : "{m0}"(to), "v"(off), "s"(base)
       : "memory");
@@ -149,10 +157,12 @@ __device__ __forceinline__ void tile_to_lds4(uint32_t to, const uint8_t* from) {
       : "{m0}"(to), "v"(from)
       : "memory");
 }
-// All of the wave's loads have landed, and its LDS reads of what they may be followed by are done.
-__device__ __forceinline__ void wait_tile() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+// All but the wave's last LEFT loads have landed; its LDS reads are done.
+template <int LEFT>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
 }
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // A wave's query heads, its sums, and the two products of a tile, whose codes `src` gives:
 //   key(h, kp, w)      sixteen codes of position 16 h + c, and key_scale(h, kp) of 4-bit ones
@@ -429,11 +439,13 @@ struct HalfLayout {
 };
 
 template <int FMT, int KP, int VD>
-struct LdsTile {  // bytes
-  static constexpr int KN = FMT == KV_MXFP4 ? (KP + 1) / 2 : KP;          // loads of a half's keys
-  static constexpr int VN = FMT == KV_MXFP4 ? (VD + 7) / 8 : (VD + 3) / 4;  // of its values
-  static constexpr int kHalf = 1024 * (KN + VN), kScales = 2 * kHalf;
-  static constexpr int kBytes = 2 * kHalf + (FMT == KV_MXFP4 ? 0 : 256);
+struct LdsTile {  // loads of a half's keys, values and 4-bit blocks' scales; bytes
+  static constexpr bool MX = FMT == KV_MXFP4;
+  static constexpr int KN = MX ? (KP + 1) / 2 : KP, VN = MX ? (VD + 7) / 8 : (VD + 3) / 4;
+  static constexpr int KS = MX ? (KP + 1) / 2 : 0, VS = MX ? (VD + 7) / 8 : 0;
+  static constexpr int kScales = 1024 * (KN + VN), kHalf = kScales + 256 * (KS + VS);
+  static constexpr int kBytes = 2 * kHalf + (MX ? 0 : 256);
+  static constexpr int kLoads = 2 * (KN + VN + KS + VS) + (MX ? 0 : 1);
 };
 
 template <class E, int FMT, int KP, int VD>
@@ -446,20 +458,23 @@ struct LdsSource {
   const int32_t* row;  // of the table
   const uint8_t *k_base, *v_base, *ks_base, *vs_base;  // of the key head
   uint32_t k_from[T::KN], v_from[T::VN];  // where the lane's chunks lie in a half of the cache
-  int64_t scale_from;                     // and its scale (lanes 0..31 a key's, then a value's)
+  uint32_t ks_from[MX ? T::KS : 1], vs_from[MX ? T::VS : 1];  // and its scales
   int k_at[KP], v_at[4];                  // what the lane reads of a half in LDS
-  uint32_t k_sel[KP], v_sel;
+  int ks_at[KP], vs_at;
   // halves [base, base + 64) of the sequence: lane i knows half base + i
   int base;
   int64_t ko, vo, kso, vso;
+  uint64_t none_at;  // those without a page
   bool missing;
-  uint32_t to;                // LDS of the wave
-  const uint8_t* at;          // the tile in turn, as the lanes read it
-  uint32_t kb[2], vb[2], kb_next[2], vb_next[2];  // scales of 4-bit blocks of position lane % 32
+  const uint8_t* lds;  // of the wave
+  uint32_t to;
+  // the tile in turn
+  uint32_t k[2][KP][W::KW], v[8][W::VW];
+  float kscale[2][MX ? KP : 4], vscale[8], most;
 
   __device__ __forceinline__ LdsSource(const AttArgs& args, const W& w, const AttChunk& ch, int head,
-                                       uint8_t* lds, uint32_t lds_at)
-      : a(args), wave(w), to(lds_at), at(lds) {
+                                       const uint8_t* mine, uint32_t mine_at)
+      : a(args), wave(w), lds(mine), to(mine_at) {
     row = a.table + ch.sequence * a.table_stride;
     const int es = MX ? 1 : 4;
     k_base = a.key.codes + head * a.key.c_head;
@@ -467,26 +482,40 @@ struct LdsSource {
     ks_base = static_cast<const uint8_t*>(a.key.scales) + head * a.key.s_head * es;
     vs_base = static_cast<const uint8_t*>(a.value.scales) + head * a.value.s_head * es;
     const int lane = w.lane, c = w.c, g = w.g;
-    const HalfLayout k(a.k_chunks), v(a.v_chunks);
+    const HalfLayout kl(a.k_chunks), vl(a.v_chunks);
 #pragma unroll
     for (int i = 0; i < T::KN; ++i) {
-      k_from[i] = k.from(min(i * 64 + lane, 16 * k.row - 1), (int)a.key.c_token);
+      k_from[i] = kl.from(min(i * 64 + lane, 16 * kl.row - 1), (int)a.key.c_token);
     }
 #pragma unroll
     for (int i = 0; i < T::VN; ++i) {
-      v_from[i] = v.from(min(i * 64 + lane, 16 * v.row - 1), (int)a.value.c_token);
-    }
-    scale_from = (lane & 15) * (lane < 32 || MX ? a.key.s_token : a.value.s_token) * es;
-#pragma unroll
-    for (int kp = 0; kp < KP; ++kp) {
-      const int d = w.key_at(kp), b = MX ? d / 2 : d;
-      k_at[kp] = k.place(c, b / 16) * 16 + b % 16;
-      k_sel[kp] = MX ? scale_selector(d / kMxBlock, a.key.dim / kMxBlock) : 0;
+      v_from[i] = vl.from(min(i * 64 + lane, 16 * vl.row - 1), (int)a.value.c_token);
     }
     const int d = w.value_at(c), b = MX ? d / 2 : d;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v_at[i] = 1024 * T::KN + v.place(g * 4 + i, b / 16) * 16 + b % 16;
-    v_sel = MX ? scale_selector(d / kMxBlock, a.value.dim / kMxBlock) : 0;
+    for (int i = 0; i < 4; ++i) v_at[i] = 1024 * T::KN + vl.place(g * 4 + i, b / 16) * 16 + b % 16;
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+      const int dk = w.key_at(kp), bk = MX ? dk / 2 : dk;
+      k_at[kp] = kl.place(c, bk / 16) * 16 + bk % 16;
+      // a row of codes has as many chunks as blocks
+      if constexpr (MX) ks_at[kp] = T::kScales + (c * kl.row + dk / kMxBlock) * 4;
+    }
+    if constexpr (MX) {
+#pragma unroll
+      for (int i = 0; i < T::KS; ++i) {
+        const int x = min(i * 64 + lane, 16 * kl.row - 1), r = (int)kl.by_row.quotient((uint32_t)x);
+        ks_from[i] = (uint32_t)(r * (int)a.key.s_token + x - r * kl.row);
+      }
+#pragma unroll
+      for (int i = 0; i < T::VS; ++i) {
+        const int x = min(i * 64 + lane, 16 * vl.row - 1), r = (int)vl.by_row.quotient((uint32_t)x);
+        vs_from[i] = (uint32_t)(r * (int)a.value.s_token + x - r * vl.row);
+      }
+      vs_at = T::kScales + 256 * T::KS + (g * 4 * vl.row + d / kMxBlock) * 4;
+    } else {
+      ks_from[0] = (uint32_t)((lane & 15) * (int)(lane < 32 ? a.key.s_token : a.value.s_token) * 4);
+    }
     missing = false;
   }
 
@@ -505,97 +534,99 @@ struct LdsSource {
     vso = (page * a.value.s_page + off * a.value.s_token) * (MX ? 1 : 4);
     none_at = __builtin_amdgcn_ballot_w64(none);
   }
-  uint64_t none_at;  // halves of base.. without a page
 
   static __device__ __forceinline__ int64_t of_lane(int64_t v, int i) {
     return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32 |
                      (uint32_t)__builtin_amdgcn_readlane((int)v, i));
   }
 
-  // Starts the loads of tile t into buffer `turn`.
+  // Starts the T::kLoads loads of tile t into buffer `turn`.
   __device__ __forceinline__ void load(int t, int turn) {
     if (t * 2 >= base + 64) look_up(t);
     const int i = t * 2 - base;
     missing |= (none_at >> i & 3) != 0;
     const uint32_t dst = to + turn * T::kBytes;
-    int64_t ks[2], vs[2];
+    const uint8_t *ks[2], *vs[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint8_t* k = k_base + of_lane(ko, i + h);
-      const uint8_t* v = v_base + of_lane(vo, i + h);
-      ks[h] = of_lane(kso, i + h), vs[h] = of_lane(vso, i + h);
+      const uint32_t half = dst + h * T::kHalf;
+      const uint8_t* kp = k_base + of_lane(ko, i + h);
+      const uint8_t* vp = v_base + of_lane(vo, i + h);
+      ks[h] = ks_base + of_lane(kso, i + h), vs[h] = vs_base + of_lane(vso, i + h);
 #pragma unroll
-      for (int x = 0; x < T::KN; ++x) tile_to_lds16(dst + h * T::kHalf + x * 1024, k, k_from[x]);
+      for (int x = 0; x < T::KN; ++x) tile_to_lds16(half + x * 1024, kp, k_from[x]);
 #pragma unroll
-      for (int x = 0; x < T::VN; ++x) {
-        tile_to_lds16(dst + h * T::kHalf + (T::KN + x) * 1024, v, v_from[x]);
+      for (int x = 0; x < T::VN; ++x) tile_to_lds16(half + (T::KN + x) * 1024, vp, v_from[x]);
+#pragma unroll
+      for (int x = 0; x < T::KS; ++x) tile_to_lds1(half + T::kScales + x * 256, ks[h], ks_from[x]);
+#pragma unroll
+      for (int x = 0; x < T::VS; ++x) {
+        tile_to_lds1(half + T::kScales + (T::KS + x) * 256, vs[h], vs_from[x]);
       }
     }
-    const bool high = (wave.lane & 16) != 0;
-    if constexpr (MX) {
-      const int64_t vs_from = (wave.lane & 15) * a.value.s_token;
-      load_scales8(kb_next, ks_base + (high ? ks[1] : ks[0]) + scale_from, a.key.dim / kMxBlock);
-      load_scales8(vb_next, vs_base + (high ? vs[1] : vs[0]) + vs_from, a.value.dim / kMxBlock);
-    } else {
-      const uint8_t* k = ks_base + (high ? ks[1] : ks[0]);
-      const uint8_t* v = vs_base + (high ? vs[1] : vs[0]);
-      tile_to_lds4(dst + T::kScales, (wave.lane < 32 ? k : v) + scale_from);
+    if constexpr (!MX) {
+      const bool high = (wave.lane & 16) != 0;
+      const uint8_t *kp = high ? ks[1] : ks[0], *vp = high ? vs[1] : vs[0];
+      tile_to_lds4(dst + 2 * T::kHalf, (wave.lane < 32 ? kp : vp) + ks_from[0]);
     }
   }
-  // What was loaded into `turn` is what the functions below give.
-  __device__ __forceinline__ void take(const uint8_t* lds, int turn) {
-    at = lds + turn * T::kBytes;
-    if constexpr (MX) {
+
+  // Reads what has landed in buffer `turn`.
+  __device__ __forceinline__ void fetch(int turn) {
+    const uint8_t* at = lds + turn * T::kBytes;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) kb[i] = kb_next[i], vb[i] = vb_next[i];
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* half = at + h * T::kHalf;
+#pragma unroll
+      for (int kp = 0; kp < KP; ++kp) {
+        const auto x = *reinterpret_cast<const Pack<uint32_t, W::KW>*>(half + k_at[kp]);
+#pragma unroll
+        for (int i = 0; i < W::KW; ++i) k[h][kp][i] = x.v[i];
+        if constexpr (MX) kscale[h][kp] = mx_operand(*reinterpret_cast<const uint32_t*>(half + ks_at[kp]));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t* w = v[h * 4 + i];
+        if constexpr (W::VB == 2) {
+          w[0] = *reinterpret_cast<const uint16_t*>(half + v_at[i]);
+        } else {
+          const auto x = *reinterpret_cast<const Pack<uint32_t, W::VW>*>(half + v_at[i]);
+#pragma unroll
+          for (int n = 0; n < W::VW; ++n) w[n] = x.v[n];
+        }
+        if constexpr (MX) {
+          vscale[h * 4 + i] = mx_operand(
+              *reinterpret_cast<const uint32_t*>(half + vs_at + i * (int)a.v_chunks.d * 4));
+        }
+      }
+      if constexpr (!MX) {
+        const float* f = reinterpret_cast<const float*>(at + 2 * T::kHalf);
+        const auto x = *reinterpret_cast<const Pack<float, 4>*>(f + h * 16 + wave.g * 4);
+        const auto y = *reinterpret_cast<const Pack<float, 4>*>(f + 32 + h * 16 + wave.g * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kscale[h][i] = x.v[i], vscale[h * 4 + i] = y.v[i];
+      }
     }
+    if constexpr (!MX) most = reinterpret_cast<const float*>(at + 2 * T::kHalf)[32 + (wave.lane & 31)];
   }
 
   __device__ __forceinline__ void key(int h, int kp, uint32_t* w) const {
-    if constexpr (MX) {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(at + h * T::kHalf + k_at[kp]);
-      w[0] = x[0], w[1] = x[1];
-    } else {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(at + h * T::kHalf + k_at[kp]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = x[i];
-    }
+    for (int i = 0; i < W::KW; ++i) w[i] = k[h][kp][i];
   }
-  __device__ __forceinline__ float key_scale(int h, int kp) const {
-    uint32_t b[2];
-    b[0] = from_lane(kb[0], h * 16 + wave.c);
-    b[1] = KP > 2 ? from_lane(kb[1], h * 16 + wave.c) : 0;
-    return scale_operand(b, k_sel[kp]);
-  }
+  __device__ __forceinline__ float key_scale(int h, int kp) const { return kscale[h][kp]; }
   __device__ __forceinline__ void value(int e, uint32_t* w) const {
-    const uint8_t* p = at + (e >> 2) * T::kHalf + v_at[e & 3];
-    if constexpr (W::VB == 2) {
-      w[0] = *reinterpret_cast<const uint16_t*>(p);
-    } else {
-      const auto x = *reinterpret_cast<const Pack<uint32_t, W::VW>*>(p);
 #pragma unroll
-      for (int i = 0; i < W::VW; ++i) w[i] = x.v[i];
-    }
+    for (int i = 0; i < W::VW; ++i) w[i] = v[e][i];
   }
-  __device__ __forceinline__ float value_scale(int e) const {
-    uint32_t b[2];
-    b[0] = from_lane(vb[0], wave.position(e));
-    b[1] = VD > 8 ? from_lane(vb[1], wave.position(e)) : 0;
-    return scale_operand(b, v_sel);
-  }
-  __device__ __forceinline__ float ks(int e) const {
-    return reinterpret_cast<const float*>(at + T::kScales)[wave.position(e)];
-  }
-  __device__ __forceinline__ float vs(int e) const {
-    return reinterpret_cast<const float*>(at + T::kScales + 128)[wave.position(e)];
-  }
-  __device__ __forceinline__ float most_vs() const {
-    return reinterpret_cast<const float*>(at + T::kScales + 128)[wave.lane & 31];
-  }
+  __device__ __forceinline__ float value_scale(int e) const { return vscale[e]; }
+  __device__ __forceinline__ float ks(int e) const { return kscale[e >> 2][e & 3]; }
+  __device__ __forceinline__ float vs(int e) const { return vscale[e]; }
+  __device__ __forceinline__ float most_vs() const { return most; }
 };
 
 template <class E, int FMT, int KP, int VD>
-__global__ void __launch_bounds__(kAttWaves * 64)
+__global__ void __launch_bounds__(kAttWaves * 64, VD == 16 ? 1 : 2)
 k_kv_attention_lines(AttArgs a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds_bytes[];  // [waves][2] tiles
   using T = LdsTile<FMT, KP, VD>;
@@ -608,18 +639,21 @@ k_kv_attention_lines(AttArgs a) {
   const int head0 = head * a.group + block * kTileRows;
   const int rows = min(kTileRows, a.group - block * kTileRows);
   AttWave<E, FMT, KP, VD> w(a, c, head0, rows);
-  uint8_t* mine = lds_bytes + wave * (2 * T::kBytes);
   LdsSource<E, FMT, KP, VD> src(
-      a, w, c, head, mine,
+      a, w, c, head, lds_bytes + wave * (2 * T::kBytes),
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds_bytes + wave * (2 * T::kBytes));
   if (c.tiles > 0) {
     const int last = c.tile + c.tiles - 1;
     src.look_up(c.tile);
     src.load(c.tile, 0);
+    if (c.tiles > 1) src.load(c.tile + 1, 1);
     for (int t = c.tile, turn = 0; t <= last; ++t, turn ^= 1) {
-      wait_tile();
-      src.take(mine, turn);
-      if (t < last) src.load(t + 1, turn ^ 1);
+      // a tile is taken to registers whole, so that the loads of the one after the next follow at once
+      if (t < last) wait_loads<T::kLoads>();
+      else wait_loads<0>();
+      src.fetch(turn);
+      wait_lds();
+      if (t + 2 <= last) src.load(t + 2, turn);
       w.tile(src, t);
     }
   }
@@ -721,7 +755,7 @@ struct RegisterSource {
 };
 
 template <class E, int FMT, int KP, int VD>
-__global__ void __launch_bounds__(kAttWaves * 64)
+__global__ void __launch_bounds__(kAttWaves * 64, VD == 16 ? 1 : 2)
 k_kv_attention_tiles(AttArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   uint32_t flat;
