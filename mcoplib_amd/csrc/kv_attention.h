@@ -11,13 +11,11 @@
 // the values themselves do not.  An empty P gives o = 0 and lse = -inf; a position of P without a page of the
 // cache makes the sequence's rows NaN.
 //
-// Work is split by tiles of 32 positions.  The lengths are on the device, so every workgroup finds its
-// own share: all tiles of all sequences over the number of chunks aimed at (`target`) is a chunk's
-// length, a sequence takes as many chunks as that asks for, and the grid has room for all (at most
-// target + sequences).  So one long sequence among short ones fills the card as equal ones do, and no
-// call needs lengths on the host.  Sequences of one chunk are written at once; the others write parts
-// (at most 2 * target chunks, since a split sequence has more tiles than a chunk) that a second kernel
-// joins, in chunk order: results do not depend on timing.
+// Work is split by tiles of 32 positions.  The lengths are on the device, so every wave finds its own
+// share: the tiles of all sequences one after the other, cut into `target` equal shares, whatever the
+// sequences' lengths (one tile at least for each, also an empty one).  A share may end one sequence, hold
+// some whole and begin another: whole ones are written at once, the others as parts, of which a share has
+// two at most.  A second kernel joins each sequence's parts in order: results do not depend on timing.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -30,7 +28,7 @@ namespace mcop {
 
 constexpr int kAttTile = 32;      // positions of a tile
 constexpr int kAttWaves = 4;      // of a workgroup, which share out a chunk's tiles
-constexpr int kAttLeastTiles = 1; // of a chunk
+constexpr int kAttLeastTiles = 1; // of a share
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttArgs {
@@ -53,15 +51,15 @@ struct AttArgs {
   float scale;    // times log2 e
   float* parts;   // [2 * target][query heads][value.dim]
   float* sums;    // [2 * target][query heads][4]: m, l, e
-  int32_t* plan;  // the number of split sequences; then of each: sequence, first part, parts
+  int32_t* plan;  // split sequences, tiles a share; then of each: sequence, its first tile of all, its end
 };
 
+// The tiles of one sequence that a share holds.
 struct AttChunk {
   int sequence;
   int first, end;     // the sequence's positions
-  int tile, tiles;    // first tile and tiles of this chunk
-  int index, count;   // of the sequence's chunks
-  int part;           // where its part goes (count > 1)
+  int tile, tiles;
+  int part;           // where its part goes; -1: it is the whole sequence
   bool missing;       // longer than its row of the table
 };
 
@@ -91,85 +89,85 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 __device__ __forceinline__ uint32_t wave_total(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(v), 63);
 }
-// The same of values below 2^44, 22 bits at a time.
-__device__ __forceinline__ uint64_t wave_total64(uint64_t v) {
-  return ((uint64_t)wave_total((uint32_t)(v >> 22)) << 22) + wave_total((uint32_t)v & 0x3fffff);
-}
+// Walks the sequences of share `share`; a wave works together, 64 sequences at a time.
+struct AttWalk {
+  const AttArgs& a;
+  const int lane;
+  const bool plans;  // this wave writes the plan of the sequences that begin in its share
+  const uint32_t share;
+  uint32_t per, at, to, total;  // tiles a share; those of this share
+  int block, splits;            // the 64 sequences in the lanes; split ones before them
+  int n;
+  uint32_t tiles, from;         // of the lane's sequence
+  uint64_t split;
 
-// The chunk of number `flat`; false past the last one.  A wave works together, 64 sequences at a time.
-// `plans`: this wave writes the plan of the sequence whose first chunk it finds.
-__device__ __forceinline__ bool find_chunk(const AttArgs& a, uint32_t flat, bool plans, AttChunk* c) {
-  const int lane = (int)threadIdx.x & 63;
-  const int n0 = lane < a.sequences ? a.lens[lane] : 0;
-  uint64_t total = att_tiles(a, n0);
-  for (int i = 64; i < a.sequences; i += 64) {
-    if (i + lane < a.sequences) total += att_tiles(a, a.lens[i + lane]);
-  }
-  total = wave_total64(total);
-  uint32_t per = kAttLeastTiles;
-  if (total > (uint64_t)a.target * kAttLeastTiles) {
-    per = total >> 31 ? (uint32_t)min((total + a.target - 1) / a.target, (uint64_t)1 << 26)
-                      : ((uint32_t)total - 1) / (uint32_t)a.target + 1;
-  }
-  uint32_t before = 0, parts_before = 0;  // chunks of earlier sequences, and their parts
-  int splits = 0;
-  bool found = false;
-  for (int i = 0; i < a.sequences; i += 64) {
-    const int n = i == 0 ? n0 : (i + lane < a.sequences ? a.lens[i + lane] : 0);
-    const uint32_t t = att_tiles(a, n);
-    const uint32_t k = i + lane >= a.sequences ? 0 : t <= per ? 1 : (t - 1) / per + 1;
-    const uint32_t upto = wave_scan(k) + before, parts = wave_scan(k > 1 ? k : 0) + parts_before;
-    const uint64_t split = __builtin_amdgcn_ballot_w64(k > 1);
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(k > 0 && upto > flat);
-    if (!found && hit != 0) {
-      found = true;
-      const int at = __builtin_ctzll(hit);
-      const uint32_t tiles = (uint32_t)__builtin_amdgcn_readlane((int)t, at);
-      c->sequence = i + at;
-      c->end = __builtin_amdgcn_readlane(n, at);
-      c->count = __builtin_amdgcn_readlane((int)k, at);
-      c->index = (int)flat - __builtin_amdgcn_readlane((int)(upto - k), at);
-      c->part = __builtin_amdgcn_readlane((int)(parts - k), at) + c->index;
-      c->missing = c->end > att_capacity(a);
-      c->first = att_first(a, c->end);
-      const uint32_t each = tiles / (uint32_t)c->count, more = tiles % (uint32_t)c->count;
-      const uint32_t x = (uint32_t)c->index;
-      c->tile = (int)((uint32_t)c->first / kAttTile + x * each + min(x, more));
-      c->tiles = (int)(each + (x < more ? 1 : 0));
-      if (plans && c->count > 1 && c->index == 0 && lane == 0) {
-        const int rank = splits + (int)__builtin_popcountll(split & (((uint64_t)1 << at) - 1));
-        a.plan[1 + 3 * rank] = c->sequence;
-        a.plan[2 + 3 * rank] = c->part;
-        a.plan[3 + 3 * rank] = c->count;
-      }
-      // the first chunk's wave goes on to count the split sequences
-      if (!plans || flat != 0) return true;
+  __device__ __forceinline__ AttWalk(const AttArgs& args, uint32_t number, bool plan)
+      : a(args), lane((int)threadIdx.x & 63), plans(plan), share(number) {
+    n = lane < a.sequences ? a.lens[lane] : 0;
+    uint32_t t = lane < a.sequences ? max(att_tiles(a, n), 1u) : 0;
+    for (int i = 64; i < a.sequences; i += 64) {
+      if (i + lane < a.sequences) t += max(att_tiles(a, a.lens[i + lane]), 1u);
     }
-    splits += (int)__builtin_popcountll(split);
-    before = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-    parts_before = (uint32_t)__builtin_amdgcn_readlane((int)parts, 63);
+    total = wave_total(t);
+    per = max((total - 1) / (uint32_t)a.target + 1, (uint32_t)kAttLeastTiles);
+    at = share < (uint32_t)a.target ? share * per : total;
+    to = min(at + per, total);
+    block = 0, splits = 0;
+    enter(0);
   }
-  if (plans && flat == 0 && lane == 0) a.plan[0] = splits;
-  return found;
-}
+  // The sequences from `block` on to the lanes; `before`: tiles of those before.
+  __device__ __forceinline__ void enter(uint32_t before) {
+    tiles = block + lane < a.sequences ? max(att_tiles(a, n), 1u) : 0;
+    from = wave_scan(tiles) - tiles + before;
+    split = __builtin_amdgcn_ballot_w64(tiles > 0 && from / per != (from + tiles - 1) / per);
+  }
+  __device__ __forceinline__ uint32_t end_of_block() const {
+    return (uint32_t)__builtin_amdgcn_readlane((int)(from + tiles), 63);
+  }
+  // The share's next sequence; false behind the last.
+  __device__ __forceinline__ bool next(AttChunk* c) {
+    if (at >= to) return false;
+    while (at >= end_of_block()) {
+      const uint32_t before = end_of_block();
+      splits += (int)__builtin_popcountll(split);
+      block += 64;
+      n = block + lane < a.sequences ? a.lens[block + lane] : 0;
+      enter(before);
+    }
+    const int i = __builtin_ctzll(__builtin_amdgcn_ballot_w64(tiles > 0 && from + tiles > at));
+    const uint32_t begin = (uint32_t)__builtin_amdgcn_readlane((int)from, i);
+    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)tiles, i);
+    const uint32_t stop = min(to, begin + all);
+    c->sequence = block + i;
+    c->end = __builtin_amdgcn_readlane(n, i);
+    c->missing = c->end > att_capacity(a);
+    c->first = att_first(a, c->end);
+    c->tile = (int)((uint32_t)c->first / kAttTile + at - begin);
+    c->tiles = c->missing || c->end <= 0 ? 0 : (int)(stop - at);
+    const bool whole = stop - at == all;
+    c->part = whole ? -1 : (int)(2 * share + (at > share * per ? 1 : 0));
+    if (plans && lane == 0) {
+      if (!whole && at == begin) {
+        int32_t* p = a.plan + 2 + 3 * (splits + (int)__builtin_popcountll(split & (((uint64_t)1 << i) - 1)));
+        p[0] = c->sequence, p[1] = (int)begin, p[2] = (int)(begin + all);
+      }
+      if (stop == total) {  // all sequences are behind
+        a.plan[0] = splits + (int)__builtin_popcountll(split);
+        a.plan[1] = (int)per;
+      }
+    }
+    at = stop;
+    return true;
+  }
+};
 
-// A wave's place where every wave takes a chunk of one key head and block: heads and blocks of a chunk are
-// neighbours, so that what lies together in the cache is read together, and chunks go round the dies.
-__device__ __forceinline__ void att_wave_place(const AttArgs& a, uint32_t wave, uint32_t* flat, int* head, int* block) {
-  // inner padded to whole workgroups
-  const uint32_t die = blockIdx.x & 7, i = (blockIdx.x >> 3) * kAttWaves + wave;
+// The share, key head and block of its query heads of worker `i` of the die (a wave or a workgroup; workgroups
+// go round the eight dies in turn): the heads and blocks of a share are neighbours on one die, so that
+// what lies together in the cache is read together.
+__device__ __forceinline__ void att_place(const AttArgs& a, uint32_t i, uint32_t* share, int* head,
+                                          int* block) {
   const uint32_t row = a.by_inner.quotient(i), inner = i - row * a.by_inner.d;
-  *flat = row * 8 + die;
-  *head = (int)a.by_blocks.quotient(inner);
-  *block = (int)(inner - (uint32_t)*head * (uint32_t)a.row_blocks);
-}
-
-// Workgroup -> (chunk, key head, block of its query heads).  Workgroups go round the eight dies in turn,
-// so those of one chunk, which share its scales' cache lines, are put on the same die.
-__device__ __forceinline__ void att_place(const AttArgs& a, uint32_t* flat, int* head, int* block) {
-  const uint32_t die = blockIdx.x & 7, i = blockIdx.x >> 3;
-  const uint32_t row = a.by_inner.quotient(i), inner = i - row * a.by_inner.d;
-  *flat = row * 8 + die;
+  *share = row * 8 + (blockIdx.x & 7);
   *head = (int)a.by_blocks.quotient(inner);
   *block = (int)(inner - (uint32_t)*head * (uint32_t)a.row_blocks);
 }
@@ -196,44 +194,43 @@ __device__ __forceinline__ float att_lse(float m, float l) {
   return l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// Joins the waves' parts of `rows` query heads from LDS (m, l [kAttWaves][stride_m], e [kAttWaves], o
-// [kAttWaves][stride_r][stride_o]) and writes the outputs of query heads head0.. (or, of a split sequence,
-// its part) at elements d0.. of the value.
+// Joins the waves' parts of `rows` query heads from LDS (m, l [kAttWaves][most], e [kAttWaves], o
+// [kAttWaves][most][value.dim]) and writes the outputs of query heads head0.. (or, of a split sequence,
+// its part).
 template <class E>
 __device__ __forceinline__ void att_write(const AttArgs& a, const AttChunk& c, int head0, int rows,
-                                          int d0, int width, const float* m, const float* l,
-                                          const int* e, const float* o, int stride_m,
-                                          int stride_r, int stride_o) {
+                                          int most, const float* m, const float* l, const int* e,
+                                          const float* o) {
   int unit = e[0];
 #pragma unroll
   for (int w = 1; w < kAttWaves; ++w) unit = max(unit, e[w]);
   for (int r = 0; r < rows; ++r) {
     float top = -__builtin_inff();
 #pragma unroll
-    for (int w = 0; w < kAttWaves; ++w) top = __builtin_fmaxf(top, m[w * stride_m + r]);
+    for (int w = 0; w < kAttWaves; ++w) top = __builtin_fmaxf(top, m[w * most + r]);
     float f[kAttWaves], sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < kAttWaves; ++w) {
-      f[w] = att_weight(m[w * stride_m + r], top);
-      sum += l[w * stride_m + r] * f[w];
+      f[w] = att_weight(m[w * most + r], top);
+      sum += l[w * most + r] * f[w];
       f[w] *= att_power(e[w] - unit);
     }
     if (c.missing) sum = __builtin_nanf("");
     const int head = head0 + r;
-    for (int d = (int)threadIdx.x; d < width; d += kAttWaves * 64) {
+    for (int d = (int)threadIdx.x; d < a.value.dim; d += kAttWaves * 64) {
       float v = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kAttWaves; ++w) v += o[(w * stride_r + r) * stride_o + d] * f[w];
-      if (c.count > 1) {
-        a.parts[((int64_t)c.part * a.query_heads + head) * a.value.dim + d0 + d] = v;
+      for (int w = 0; w < kAttWaves; ++w) v += o[(w * most + r) * a.value.dim + d] * f[w];
+      if (c.part >= 0) {
+        a.parts[((int64_t)c.part * a.query_heads + head) * a.value.dim + d] = v;
       } else {
         static_cast<typename E::S*>(a.value.plain)[c.sequence * a.value.p_token +
-                                                   head * a.value.p_head + d0 + d] =
+                                                   head * a.value.p_head + d] =
             E::from_f(att_value(v, sum, unit));
       }
     }
-    if (threadIdx.x == 0 && d0 == 0) {
-      if (c.count > 1) {
+    if (threadIdx.x == 0) {
+      if (c.part >= 0) {
         float* s = a.sums + ((int64_t)c.part * a.query_heads + head) * 4;
         s[0] = top, s[1] = sum, s[2] = (float)unit;
       } else if (a.lse != nullptr) {

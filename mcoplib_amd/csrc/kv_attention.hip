@@ -33,109 +33,112 @@ __global__ void __launch_bounds__(kAttWaves * 64)
 k_kv_attention_rows(AttArgs a) {
   extern __shared__ float lds[];  // m, l [waves][rows], e [waves], o [waves][rows][value.dim]
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  uint32_t flat;
+  uint32_t share;
   int head, block;
-  att_place(a, &flat, &head, &block);
-  AttChunk c;
-  if (!find_chunk(a, flat, head == 0 && block == 0 && wave == 0, &c)) return;
+  att_place(a, blockIdx.x >> 3, &share, &head, &block);
   const int head0 = head * a.group + block * kAttRows;
   const int rows = min(kAttRows, a.group - block * kAttRows);
-  float q[kAttRows][N], o[kAttRows][N], m[kAttRows], l[kAttRows];
-#pragma unroll
-  for (int r = 0; r < kAttRows; ++r) {
-    const typename E::S* src = static_cast<const typename E::S*>(a.key.plain) +
-                               c.sequence * a.key.p_token + (head0 + min(r, rows - 1)) * a.key.p_head;
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int d = lane + n * 64;
-      q[r][n] = d < a.key.dim ? E::to_f(src[d]) : 0.0f;
-      o[r][n] = 0.0f;
-    }
-    m[r] = -__builtin_inff(), l[r] = 0.0f;
-  }
-  const int from = max(c.first, c.tile * kAttTile), to = min(c.end, (c.tile + c.tiles) * kAttTile);
-  bool missing = false;
-  int unit = FMT == KV_MXFP4 ? 0 : kAttNoUnit;
-  for (int p = from + wave; p < to; p += kAttWaves) {
-    uint32_t off;
-    const int page = att_page(a, c.sequence, (uint32_t)p, &off);
-    if (page < 0) {
-      missing = true;
-      continue;
-    }
-    const uint8_t* k = a.key.codes + page * a.key.c_page + off * a.key.c_token + head * a.key.c_head;
-    const uint8_t* v =
-        a.value.codes + page * a.value.c_page + off * a.value.c_token + head * a.value.c_head;
-    const int64_t ks = page * a.key.s_page + off * a.key.s_token + head * a.key.s_head;
-    const int64_t vs = page * a.value.s_page + off * a.value.s_token + head * a.value.s_head;
-    float kf[N], vf[N];
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int d = lane + n * 64;
-      kf[n] = vf[n] = 0.0f;
-      if (d < a.key.dim) {
-        kf[n] = code_value<FMT>(k, d);
-        if constexpr (FMT == KV_MXFP4) {
-          kf[n] *= mx_value(static_cast<const uint8_t*>(a.key.scales)[ks + (d >> 5)]);
-        }
-      }
-      if (d < a.value.dim) {
-        vf[n] = code_value<FMT>(v, d);
-        if constexpr (FMT == KV_MXFP4) {
-          vf[n] *= mx_value(static_cast<const uint8_t*>(a.value.scales)[vs + (d >> 5)]);
-        }
-      }
-    }
-    float k_scale = a.scale, v_scale = 1.0f;
-    if constexpr (FMT != KV_MXFP4) {
-      k_scale *= static_cast<const float*>(a.key.scales)[ks];
-      v_scale = static_cast<const float*>(a.value.scales)[vs];
-      const int e = att_unit(v_scale);
-      if (e > unit) {
-        const float down = att_power(unit - e);
-#pragma unroll
-        for (int r = 0; r < kAttRows; ++r) {
-#pragma unroll
-          for (int n = 0; n < N; ++n) o[r][n] *= down;
-        }
-        unit = e;
-      }
-      v_scale = __builtin_ldexpf(v_scale, -unit);
-    }
+  AttWalk walk(a, share, head == 0 && block == 0 && wave == 0);
+  AttChunk c;
+  while (walk.next(&c)) {
+    float q[kAttRows][N], o[kAttRows][N], m[kAttRows], l[kAttRows];
 #pragma unroll
     for (int r = 0; r < kAttRows; ++r) {
-      float s = 0.0f;
+      const typename E::S* src = static_cast<const typename E::S*>(a.key.plain) +
+                                 c.sequence * a.key.p_token + (head0 + min(r, rows - 1)) * a.key.p_head;
 #pragma unroll
-      for (int n = 0; n < N; ++n) s = __builtin_fmaf(q[r][n], kf[n], s);
-#pragma unroll
-      for (int x = 1; x < 64; x *= 2) s += __shfl_xor(s, x, 64);
-      s *= k_scale;
-      const float top = __builtin_fmaxf(m[r], s);
-      const float keep = att_weight(m[r], top), w = att_weight(s, top);
-      m[r] = top;
-      l[r] = l[r] * keep + w;
-#pragma unroll
-      for (int n = 0; n < N; ++n) o[r][n] = o[r][n] * keep + (w * v_scale) * vf[n];
+      for (int n = 0; n < N; ++n) {
+        const int d = lane + n * 64;
+        q[r][n] = d < a.key.dim ? E::to_f(src[d]) : 0.0f;
+        o[r][n] = 0.0f;
+      }
+      m[r] = -__builtin_inff(), l[r] = 0.0f;
     }
+    const int from = max(c.first, c.tile * kAttTile), to = min(c.end, (c.tile + c.tiles) * kAttTile);
+    bool missing = false;
+    int unit = FMT == KV_MXFP4 ? 0 : kAttNoUnit;
+    for (int p = from + wave; p < to; p += kAttWaves) {
+      uint32_t off;
+      const int page = att_page(a, c.sequence, (uint32_t)p, &off);
+      if (page < 0) {
+        missing = true;
+        continue;
+      }
+      const uint8_t* k = a.key.codes + page * a.key.c_page + off * a.key.c_token + head * a.key.c_head;
+      const uint8_t* v =
+          a.value.codes + page * a.value.c_page + off * a.value.c_token + head * a.value.c_head;
+      const int64_t ks = page * a.key.s_page + off * a.key.s_token + head * a.key.s_head;
+      const int64_t vs = page * a.value.s_page + off * a.value.s_token + head * a.value.s_head;
+      float kf[N], vf[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int d = lane + n * 64;
+        kf[n] = vf[n] = 0.0f;
+        if (d < a.key.dim) {
+          kf[n] = code_value<FMT>(k, d);
+          if constexpr (FMT == KV_MXFP4) {
+            kf[n] *= mx_value(static_cast<const uint8_t*>(a.key.scales)[ks + (d >> 5)]);
+          }
+        }
+        if (d < a.value.dim) {
+          vf[n] = code_value<FMT>(v, d);
+          if constexpr (FMT == KV_MXFP4) {
+            vf[n] *= mx_value(static_cast<const uint8_t*>(a.value.scales)[vs + (d >> 5)]);
+          }
+        }
+      }
+      float k_scale = a.scale, v_scale = 1.0f;
+      if constexpr (FMT != KV_MXFP4) {
+        k_scale *= static_cast<const float*>(a.key.scales)[ks];
+        v_scale = static_cast<const float*>(a.value.scales)[vs];
+        const int e = att_unit(v_scale);
+        if (e > unit) {
+          const float down = att_power(unit - e);
+#pragma unroll
+          for (int r = 0; r < kAttRows; ++r) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) o[r][n] *= down;
+          }
+          unit = e;
+        }
+        v_scale = __builtin_ldexpf(v_scale, -unit);
+      }
+#pragma unroll
+      for (int r = 0; r < kAttRows; ++r) {
+        float s = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; ++n) s = __builtin_fmaf(q[r][n], kf[n], s);
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) s += __shfl_xor(s, x, 64);
+        s *= k_scale;
+        const float top = __builtin_fmaxf(m[r], s);
+        const float keep = att_weight(m[r], top), w = att_weight(s, top);
+        m[r] = top;
+        l[r] = l[r] * keep + w;
+#pragma unroll
+        for (int n = 0; n < N; ++n) o[r][n] = o[r][n] * keep + (w * v_scale) * vf[n];
+      }
+    }
+    float *ms = lds, *ls = ms + kAttWaves * kAttRows;
+    int* es = reinterpret_cast<int*>(ls + kAttWaves * kAttRows);
+    float* os = reinterpret_cast<float*>(es + kAttWaves);
+    if (lane == 0) es[wave] = unit;
+#pragma unroll
+    for (int r = 0; r < kAttRows; ++r) {
+      if (lane == 0) {
+        ms[wave * kAttRows + r] = m[r];
+        ls[wave * kAttRows + r] = missing ? __builtin_nanf("") : l[r];
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int d = lane + n * 64;
+        if (d < a.value.dim) os[(wave * kAttRows + r) * a.value.dim + d] = o[r][n];
+      }
+    }
+    __syncthreads();
+    att_write<E>(a, c, head0, rows, kAttRows, ms, ls, es, os);
+    __syncthreads();  // LDS is free again
   }
-  float *ms = lds, *ls = ms + kAttWaves * kAttRows;
-  int* es = reinterpret_cast<int*>(ls + kAttWaves * kAttRows);
-  float* os = reinterpret_cast<float*>(es + kAttWaves);
-  if (lane == 0) es[wave] = unit;
-#pragma unroll
-  for (int r = 0; r < kAttRows; ++r) {
-    if (lane == 0) {
-      ms[wave * kAttRows + r] = m[r];
-      ls[wave * kAttRows + r] = missing ? __builtin_nanf("") : l[r];
-    }
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int d = lane + n * 64;
-      if (d < a.value.dim) os[(wave * kAttRows + r) * a.value.dim + d] = o[r][n];
-    }
-  }
-  __syncthreads();
-  att_write<E>(a, c, head0, rows, 0, a.value.dim, ms, ls, es, os, kAttRows, kAttRows, a.value.dim);
 }
 
 // Joins the parts of split sequence blockIdx.y of the plan, a query head a workgroup: a group of 32 lanes
@@ -149,8 +152,10 @@ k_kv_attention_join(AttArgs a) {
   __shared__ float ms[kJoinGroups], ls[kJoinGroups], os[kJoinGroups][kJoinLanes * 4];
   __shared__ int es[kJoinGroups];
   if ((int)blockIdx.y >= a.plan[0]) return;
-  const int sequence = a.plan[1 + 3 * blockIdx.y], part = a.plan[2 + 3 * blockIdx.y],
-            count = a.plan[3 + 3 * blockIdx.y];
+  const int32_t* plan = a.plan + 2 + 3 * blockIdx.y;
+  const int sequence = plan[0];
+  const uint32_t per = (uint32_t)a.plan[1], begin = (uint32_t)plan[1], end = (uint32_t)plan[2];
+  const int share = (int)(begin / per), count = (int)((end - 1) / per) - share + 1;
   const int head = (int)blockIdx.x, lane = (int)threadIdx.x & (kJoinLanes - 1),
             g = (int)threadIdx.x / kJoinLanes, dim = a.value.dim;
   typename E::S* out = static_cast<typename E::S*>(a.value.plain) + sequence * a.value.p_token +
@@ -161,7 +166,9 @@ k_kv_attention_join(AttArgs a) {
     int unit = -252;  // below any part's
 #pragma unroll 4
     for (int i = g; i < count; i += kJoinGroups) {
-      const int64_t row = (int64_t)(part + i) * a.query_heads + head;
+      // the first share's part is its second one where the share begins with another sequence
+      const int part = 2 * (share + i) + (i == 0 && begin > (uint32_t)share * per ? 1 : 0);
+      const int64_t row = (int64_t)part * a.query_heads + head;
       const float mi = a.sums[row * 4], li = a.sums[row * 4 + 1];
       const int ei = (int)a.sums[row * 4 + 2];
       float v[4];
@@ -214,10 +221,10 @@ k_kv_attention_join(AttArgs a) {
 
 namespace {
 
-// Chunks aimed at: two workgroups a CU over all of a chunk's key heads and blocks of sixteen query heads.
-int kAttWorkgroups = getenv("MCOP_T") ? atoi(getenv("MCOP_T")) : 2048;
+// Shares: waves for the card over all of a share's key heads and blocks of sixteen query heads.
+int kAttShares = getenv("MCOP_T") ? atoi(getenv("MCOP_T")) : 2048;
 int64_t target_of(int64_t heads, int64_t group) {
-  return std::max<int64_t>(1, kAttWorkgroups / (heads * ((group + 15) / 16)));
+  return std::max<int64_t>(1, kAttShares / (heads * ((group + 15) / 16)));
 }
 
 struct Workspace {
@@ -225,7 +232,7 @@ struct Workspace {
   int64_t bytes() const { return parts + sums + plan; }
 };
 Workspace workspace_of(int64_t target, int64_t query_heads, int64_t dim) {
-  return {2 * target * query_heads * dim * 4, 2 * target * query_heads * 16, (1 + 3 * target) * 4};
+  return {2 * target * query_heads * dim * 4, 2 * target * query_heads * 16, (2 + 3 * target) * 4};
 }
 
 bool heads_ok(int64_t heads, int64_t query_heads) {
@@ -258,12 +265,12 @@ bool whole_lines(const AttArgs& a, int fmt) {
 }
 
 template <class E, int FMT>
-int launch_of(const char* name, AttArgs a, mcop_dtype dtype, int64_t chunks, bool joins,
-              hipStream_t st) {
+int launch_of(const char* name, AttArgs a, mcop_dtype dtype, bool joins, hipStream_t st) {
   const int shape = tile_shape(a), rows = shape >= 0 ? kTileRows : kAttRows;
   a.row_blocks = (a.group + rows - 1) / rows;
-  const int64_t inner = (int64_t)a.heads * a.row_blocks;
-  const int64_t blocks = shape >= 0 ? ((chunks + 7) / 8 * inner + kAttWaves - 1) / kAttWaves * 8 : (chunks + 7) / 8 * 8 * inner;
+  // shares of a die times their heads and blocks, a wave each of the matrix kernels, else a workgroup
+  const int64_t inner = (int64_t)a.heads * a.row_blocks, workers = (int64_t)(a.target + 7) / 8 * inner;
+  const int64_t blocks = 8 * (shape >= 0 ? (workers + kAttWaves - 1) / kAttWaves : workers);
   if (blocks >= ((int64_t)1 << 31) / 256) {
     return set_error(MCOP_E_UNSUPPORTED, "%s: more rows than one launch takes (%lld workgroups)", name,
                      (long long)blocks);
@@ -278,7 +285,7 @@ int launch_of(const char* name, AttArgs a, mcop_dtype dtype, int64_t chunks, boo
       (shape >= 0 ? 0
                   : 2 * kAttRows + 1 + (size_t)kAttRows * a.value.dim);
   trace_launch(name, "sequences=%d heads=%d of %d head sizes %d and %d: %s kernel, wgs=%lld, %d "
-               "chunks aimed at%s", a.sequences, a.heads, a.query_heads, a.key.dim, a.value.dim,
+               "shares%s", a.sequences, a.heads, a.query_heads, a.key.dim, a.value.dim,
                shape >= 0 ? "matrix" : "vector", (long long)blocks, a.target, joins ? "" : ", none split");
   const dim3 grid((unsigned)blocks), block(kAttWaves * 64);
   if (shape >= 0) {
@@ -295,7 +302,8 @@ int launch_of(const char* name, AttArgs a, mcop_dtype dtype, int64_t chunks, boo
   }
   if (int rc = check_launch(name)) return rc;
   if (!joins) return MCOP_OK;
-  const dim3 pairs((unsigned)a.query_heads, (unsigned)std::min(a.sequences, a.target));
+  // each cut between two shares splits one sequence
+  const dim3 pairs((unsigned)a.query_heads, (unsigned)std::min(a.sequences, a.target - 1));
   hipLaunchKernelGGL((k_kv_attention_join<E>), pairs, dim3(kJoinLanes * kJoinGroups), 0, st, a);
   return check_launch(name);
 }
@@ -351,6 +359,12 @@ extern "C" int mcop_kv_cache_attention(const mcop_kv_side* key, const mcop_kv_si
     return set_error(MCOP_E_INVALID, "%s: bad block table: %lld sequences (at most 2^24) of %lld pages",
                      name, (long long)num_sequences, (long long)table_columns);
   }
+  // the kernels count tiles in 32 bits; a sequence has as many as its row of the table holds
+  const int64_t capacity = std::min<int64_t>(table_columns * page_size, INT32_MAX);
+  if ((capacity / kAttTile + 2) * num_sequences > INT32_MAX) {
+    return set_error(MCOP_E_UNSUPPORTED, "%s: %lld sequences of up to %lld positions are 2^31 tiles of 32 "
+                     "or more", name, (long long)num_sequences, (long long)capacity);
+  }
   if (window < 0) return set_error(MCOP_E_INVALID, "%s: negative window", name);
   AttArgs a;
   if (int rc = side_of(name, "key", *key, fmt, num_pages, page_size, query_heads, num_sequences,
@@ -383,20 +397,18 @@ extern "C" int mcop_kv_cache_attention(const mcop_kv_side* key, const mcop_kv_si
   a.query_heads = (int)query_heads;
   a.group = (int)(query_heads / num_heads);
   a.window = (int)std::min<int64_t>(window, INT32_MAX);
-  a.target = (int)std::max<int64_t>(target - num_sequences, (target + 1) / 2);
+  a.target = (int)target;
   a.scale = scale * kLog2e;
   a.parts = static_cast<float*>(workspace);
   a.sums = a.parts + ws.parts / 4;
   a.plan = reinterpret_cast<int32_t*>(a.sums + ws.sums / 4);
-  // a row of the table of at most a least chunk's positions is not split
-  const bool joins = table_columns * page_size > kAttLeastTiles * kAttTile;
+  const bool joins = target > 1;  // one share splits nothing
   auto st = static_cast<hipStream_t>(stream);
   auto by_format = [&](auto e) {
     using E = decltype(e);
-    const int64_t chunks = target + num_sequences;
-    if (fmt == KV_INT8) return launch_of<E, KV_INT8>(name, a, dtype, chunks, joins, st);
-    if (fmt == KV_FP8) return launch_of<E, KV_FP8>(name, a, dtype, chunks, joins, st);
-    return launch_of<E, KV_MXFP4>(name, a, dtype, chunks, joins, st);
+    if (fmt == KV_INT8) return launch_of<E, KV_INT8>(name, a, dtype, joins, st);
+    if (fmt == KV_FP8) return launch_of<E, KV_FP8>(name, a, dtype, joins, st);
+    return launch_of<E, KV_MXFP4>(name, a, dtype, joins, st);
   };
   if (dtype == MCOP_BF16) return by_format(BF16());
   if (dtype == MCOP_F16) return by_format(F16());

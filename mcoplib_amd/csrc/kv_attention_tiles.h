@@ -27,6 +27,13 @@ namespace mcop {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// Workgroups a CU that the kernel's registers are held to: two where that spills none of them.
+template <class E, int FMT, int KP, int VD>
+constexpr int kResident =
+    VD == 4 || (VD == 8 && !std::is_same_v<E, F32> &&
+                (KP == 2 ? FMT != KV_INT8 || std::is_same_v<E, BF16>
+                         : FMT == KV_MXFP4 || (FMT == KV_FP8 && std::is_same_v<E, BF16>))) ? 2 : 1;
+
 constexpr int kTileRows = 16;    // query heads of a wave
 constexpr float kAttSlack = 8.0f;  // weights are at most 2^8
 
@@ -388,7 +395,7 @@ struct AttWave {
     if (c >= rows) return;
     const int query = head0 + c;
     if (g == 0) {
-      if (ch.count > 1) {
+      if (ch.part >= 0) {
         float* dst = a.sums + ((int64_t)ch.part * a.query_heads + query) * 4;
         dst[0] = m, dst[1] = sum, dst[2] = (float)unit;
       } else if (a.lse != nullptr) {
@@ -398,7 +405,7 @@ struct AttWave {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int d = value_at(g * 4 + i);
-      if (ch.count > 1) {
+      if (ch.part >= 0) {
         float* dst = a.parts + ((int64_t)ch.part * a.query_heads + query) * a.value.dim + d;
 #pragma unroll
         for (int n = 0; n < VD; ++n) dst[n] = o[n][i];
@@ -626,38 +633,41 @@ struct LdsSource {
 };
 
 template <class E, int FMT, int KP, int VD>
-__global__ void __launch_bounds__(kAttWaves * 64, VD == 16 ? 1 : 2)
+__global__ void __launch_bounds__(kAttWaves * 64, (kResident<E, FMT, KP, VD>))
 k_kv_attention_lines(AttArgs a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds_bytes[];  // [waves][2] tiles
   using T = LdsTile<FMT, KP, VD>;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  uint32_t flat;
+  uint32_t share;
   int head, block;
-  att_wave_place(a, (uint32_t)wave, &flat, &head, &block);
-  AttChunk c;
-  if (!find_chunk(a, flat, head == 0 && block == 0, &c)) return;
+  att_place(a, (blockIdx.x >> 3) * kAttWaves + wave, &share, &head, &block);
   const int head0 = head * a.group + block * kTileRows;
   const int rows = min(kTileRows, a.group - block * kTileRows);
-  AttWave<E, FMT, KP, VD> w(a, c, head0, rows);
-  LdsSource<E, FMT, KP, VD> src(
-      a, w, c, head, lds_bytes + wave * (2 * T::kBytes),
-      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds_bytes + wave * (2 * T::kBytes));
-  if (c.tiles > 0) {
-    const int last = c.tile + c.tiles - 1;
-    src.look_up(c.tile);
-    src.load(c.tile, 0);
-    if (c.tiles > 1) src.load(c.tile + 1, 1);
-    for (int t = c.tile, turn = 0; t <= last; ++t, turn ^= 1) {
-      // a tile is taken to registers whole, so that the loads of the one after the next follow at once
-      if (t < last) wait_loads<T::kLoads>();
-      else wait_loads<0>();
-      src.fetch(turn);
-      wait_lds();
-      if (t + 2 <= last) src.load(t + 2, turn);
-      w.tile(src, t);
+  AttWalk walk(a, share, head == 0 && block == 0);
+  AttChunk c;
+  while (walk.next(&c)) {
+    AttWave<E, FMT, KP, VD> w(a, c, head0, rows);
+    LdsSource<E, FMT, KP, VD> src(
+        a, w, c, head, lds_bytes + wave * (2 * T::kBytes),
+        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds_bytes +
+            wave * (2 * T::kBytes));
+    if (c.tiles > 0) {
+      const int last = c.tile + c.tiles - 1;
+      src.look_up(c.tile);
+      src.load(c.tile, 0);
+      if (c.tiles > 1) src.load(c.tile + 1, 1);
+      for (int t = c.tile, turn = 0; t <= last; ++t, turn ^= 1) {
+        // a tile is taken to registers whole, so that the loads of the one after the next follow at once
+        if (t < last) wait_loads<T::kLoads>();
+        else wait_loads<0>();
+        src.fetch(turn);
+        wait_lds();
+        if (t + 2 <= last) src.load(t + 2, turn);
+        w.tile(src, t);
+      }
     }
+    w.write(c, head0, rows, src.missing);
   }
-  w.write(c, head0, rows, src.missing);
 }
 
 // ---- Codes straight to registers, at any alignment and in pages of any size.
@@ -755,23 +765,25 @@ struct RegisterSource {
 };
 
 template <class E, int FMT, int KP, int VD>
-__global__ void __launch_bounds__(kAttWaves * 64, VD == 16 ? 1 : 2)
+__global__ void __launch_bounds__(kAttWaves * 64, (kResident<E, FMT, KP, VD>))
 k_kv_attention_tiles(AttArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  uint32_t flat;
+  uint32_t share;
   int head, block;
-  att_wave_place(a, (uint32_t)wave, &flat, &head, &block);
-  AttChunk c;
-  if (!find_chunk(a, flat, head == 0 && block == 0, &c)) return;
+  att_place(a, (blockIdx.x >> 3) * kAttWaves + wave, &share, &head, &block);
   const int head0 = head * a.group + block * kTileRows;
   const int rows = min(kTileRows, a.group - block * kTileRows);
-  AttWave<E, FMT, KP, VD> w(a, c, head0, rows);
-  RegisterSource<E, FMT, KP, VD> src(a, w, c, head);
-  for (int t = c.tile; t < c.tile + c.tiles; ++t) {
-    src.load(t);
-    w.tile(src, t);
+  AttWalk walk(a, share, head == 0 && block == 0);
+  AttChunk c;
+  while (walk.next(&c)) {
+    AttWave<E, FMT, KP, VD> w(a, c, head0, rows);
+    RegisterSource<E, FMT, KP, VD> src(a, w, c, head);
+    for (int t = c.tile; t < c.tile + c.tiles; ++t) {
+      src.load(t);
+      w.tile(src, t);
+    }
+    w.write(c, head0, rows, src.missing);
   }
-  w.write(c, head0, rows, src.missing);
 }
 
 // The kernels' head sizes: keys of up to 64 KP and values of up to 16 VD elements, at least a unit of each.
