@@ -141,48 +141,94 @@ k_kv_attention_rows(AttArgs a) {
   }
 }
 
-// Joins the parts of split sequence blockIdx.y of the plan, a query head a workgroup: a group of 32 lanes
-// takes every eighth part, four elements a lane, with maximum and sum of its own, and the groups are
-// joined in LDS.
-constexpr int kJoinLanes = 32, kJoinGroups = 8;
+// Joins the parts of split sequence blockIdx.y of the plan: a group of 32 lanes takes parts of one query
+// head, four elements a lane, eight parts' loads at a time.  Few parts: a group takes all of a query head's,
+// and a workgroup eight query heads; many: the eight groups share out one query head's parts, and are joined
+// in LDS.
+constexpr int kJoinLanes = 32, kJoinGroups = 8, kJoinBatch = 8;
 
 template <class E>
 __global__ void __launch_bounds__(kJoinLanes * kJoinGroups)
 k_kv_attention_join(AttArgs a) {
   __shared__ float ms[kJoinGroups], ls[kJoinGroups], os[kJoinGroups][kJoinLanes * 4];
   __shared__ int es[kJoinGroups];
-  if ((int)blockIdx.y >= a.plan[0]) return;
+  // all of the plan at once, also where it says that there is no such entry
   const int32_t* plan = a.plan + 2 + 3 * blockIdx.y;
-  const int sequence = plan[0];
+  const int splits = a.plan[0], sequence = plan[0];
   const uint32_t per = (uint32_t)a.plan[1], begin = (uint32_t)plan[1], end = (uint32_t)plan[2];
+  if ((int)blockIdx.y >= splits) return;
   const int share = (int)(begin / per), count = (int)((end - 1) / per) - share + 1;
-  const int head = (int)blockIdx.x, lane = (int)threadIdx.x & (kJoinLanes - 1),
-            g = (int)threadIdx.x / kJoinLanes, dim = a.value.dim;
+  // the first share's part is its second one where the share begins with another sequence
+  const int first_part = 2 * share + (begin > (uint32_t)share * per ? 1 : 0);
+  const int lane = (int)threadIdx.x & (kJoinLanes - 1), g = (int)threadIdx.x / kJoinLanes;
+  const bool many = count > kJoinBatch;
+  if (!many && blockIdx.x % kJoinGroups != 0) return;
+  const int head = (int)blockIdx.x + (many ? 0 : g), dim = a.value.dim;
+  const int from = many ? g : 0, step = many ? kJoinGroups : 1;
+  if (head >= a.query_heads) return;  // only with few parts: no barrier then
   typename E::S* out = static_cast<typename E::S*>(a.value.plain) + sequence * a.value.p_token +
                        head * a.value.p_head;
   for (int d0 = 0; d0 < dim; d0 += kJoinLanes * 4) {
     const int d = d0 + lane * 4;
     float m = -__builtin_inff(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     int unit = -252;  // below any part's
-#pragma unroll 4
-    for (int i = g; i < count; i += kJoinGroups) {
-      // the first share's part is its second one where the share begins with another sequence
-      const int part = 2 * (share + i) + (i == 0 && begin > (uint32_t)share * per ? 1 : 0);
-      const int64_t row = (int64_t)part * a.query_heads + head;
-      const float mi = a.sums[row * 4], li = a.sums[row * 4 + 1];
-      const int ei = (int)a.sums[row * 4 + 2];
-      float v[4];
+    for (int i = from; i < count; i += step * kJoinBatch) {
+      float mi[kJoinBatch], li[kJoinBatch], v[kJoinBatch][4];
+      int ei[kJoinBatch];
+      // no load hangs on a condition: what is not there is another one's copy, without weight
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = d + e < dim ? a.parts[row * dim + d + e] : 0.0f;
-      const float top = __builtin_fmaxf(m, mi);
-      const float keep = att_weight(m, top), w = att_weight(mi, top);
-      m = top;
-      l = l * keep + li * w;
-      const int high = max(unit, ei);
-      const float keep_o = keep * att_power(unit - high), w_o = w * att_power(ei - high);
-      unit = high;
+      for (int j = 0; j < kJoinBatch; ++j) {
+        const int x = i + j * step;
+        const int64_t row =
+            (int64_t)(x == 0 || x >= count ? first_part : 2 * (share + x)) * a.query_heads + head;
+        const Pack<float, 4> s = ld<float, 4>(a.sums + row * 4);
+        mi[j] = s.v[0], li[j] = s.v[1], ei[j] = (int)s.v[2];
+        const float* src = a.parts + row * dim;
+        if (dim % 4 == 0) {
+          const Pack<float, 4> p = ld<float, 4>(src + min(d, dim - 4));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = o[e] * keep_o + v[e] * w_o;
+          for (int e = 0; e < 4; ++e) v[j][e] = p.v[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[j][e] = src[min(d + e, dim - 1)];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kJoinBatch; ++j) {
+        if (i + j * step < count) continue;
+        mi[j] = -__builtin_inff(), li[j] = 0.0f, ei[j] = -252;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[j][e] = 0.0f;
+      }
+      float top = m;
+      int high = unit;
+#pragma unroll
+      for (int j = 0; j < kJoinBatch; ++j) {
+        top = __builtin_fmaxf(top, mi[j]);
+        high = max(high, ei[j]);
+      }
+      const float keep = att_weight(m, top), keep_o = keep * att_power(unit - high);
+      m = top, unit = high;
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= keep_o;
+#pragma unroll
+      for (int j = 0; j < kJoinBatch; ++j) {
+        const float w = att_weight(mi[j], top), w_o = w * att_power(ei[j] - high);
+        l += li[j] * w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += v[j][e] * w_o;
+      }
+    }
+    if (!many) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (d + e < dim) out[d + e] = E::from_f(att_value(o[e], l, unit));
+      }
+      if (a.lse != nullptr && d == 0) {
+        a.lse[(int64_t)sequence * a.query_heads + head] = att_lse(m, l);
+      }
+      continue;
     }
     if (lane == 0) ms[g] = m, ls[g] = l, es[g] = unit;
 #pragma unroll

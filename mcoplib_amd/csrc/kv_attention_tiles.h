@@ -36,6 +36,9 @@ constexpr int kResident =
 
 constexpr int kTileRows = 16;    // query heads of a wave
 constexpr float kAttSlack = 8.0f;  // weights are at most 2^8
+// Outputs are in units of 2^0 while a tile's largest value scale has an exponent of -60..60, and until one has
+// an exponent more than this above the unit's.
+constexpr int kAttUnitSlack = 60;
 
 template <class E>
 struct AttTerms {  // bf16 terms of a query, of a weight
@@ -226,7 +229,7 @@ struct AttWave {
           float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            f[e] = E::to_f(x[kp][j].v[i * 2 + e]);
+            f[e] = E::to_f(x[kp][j].v[i * 2 + e]) * (a.scale < 0.0f ? -1.0f : 1.0f);
             if (at + j * 8 + i * 2 + e < nominal || c >= rows) f[e] = 0.0f;
           }
 #pragma unroll
@@ -295,26 +298,29 @@ struct AttWave {
         }
       }
     }
+    const float by = __builtin_fabsf(a.scale);  // its sign is the queries'
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      f[e] = s[e >> 2][e & 3] * (MX ? a.scale : src.ks(e) * a.scale);
+      f[e] = MX ? s[e >> 2][e & 3] : s[e >> 2][e & 3] * src.ks(e);
       if (EDGE) f[e] = live[e] ? f[e] : -__builtin_inff();
     }
     float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(f[0], f[1]), __builtin_fmaxf(f[2], f[3])),
                                 __builtin_fmaxf(__builtin_fmaxf(f[4], f[5]), __builtin_fmaxf(f[6], f[7])));
-    top = __builtin_fmaxf(m, column_max(top));
+    top = column_max(top);
+    top = top == -__builtin_inff() ? m : __builtin_fmaxf(m, top * by);
     int e_max = unit;
     bool wider = false;
     if constexpr (!MX) {
       const int p = t * kAttTile + (lane & 31);
       const int e = EDGE && (p < first || p >= end) ? kAttNoUnit : att_unit(src.most_vs());
-      wider = __builtin_amdgcn_ballot_w64(e > unit) != 0;
+      wider = __builtin_amdgcn_ballot_w64(e > unit + kAttUnitSlack) != 0;
       if (wider) {
-        e_max = max(e, unit);
+        e_max = e;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) e_max = max(e_max, __shfl_xor(e_max, d, 64));
         e_max = __builtin_amdgcn_readfirstlane(e_max);
+        if (e_max >= -kAttUnitSlack && e_max <= kAttUnitSlack) e_max = 0;
       }
     }
     // the reference of the weights moves when a logit is 2^kAttSlack past it, not with every new maximum:
@@ -332,10 +338,19 @@ struct AttWave {
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float p = __builtin_amdgcn_exp2f(f[e] - at);
+      float p = __builtin_amdgcn_exp2f(__builtin_fmaf(f[e], by, -at));
+      if (EDGE) p = live[e] ? p : 0.0f;
       l += p;
-      w[e] = MX ? p : p * __builtin_ldexpf(src.vs(e), -unit);
+      w[e] = MX ? p : p * src.vs(e);
       if (!MX && EDGE) w[e] = live[e] ? w[e] : 0.0f;  // no 0 times a scale that is no number
+    }
+    if (!MX && unit != 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        w[e] = EDGE && !live[e] ? 0.0f
+                                : __builtin_amdgcn_exp2f(__builtin_fmaf(f[e], by, -at)) *
+                                      __builtin_ldexpf(src.vs(e), -unit);
+      }
     }
     bf16x8 p[TP];
     {
