@@ -4,7 +4,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "../../include/mcop_norm.h"
 #include "kv_attention_tiles.h"
@@ -141,11 +140,10 @@ k_kv_attention_rows(AttArgs a) {
   }
 }
 
-// Joins the parts of split sequence blockIdx.y of the plan: a group of 32 lanes takes parts of one query
-// head, four elements a lane, eight parts' loads at a time.  Few parts: a group takes all of a query head's,
-// and a workgroup eight query heads; many: the eight groups share out one query head's parts, and are joined
-// in LDS.
-constexpr int kJoinLanes = 32, kJoinGroups = 8, kJoinBatch = 8;
+// Joins the parts of split sequence blockIdx.y of the plan, a query head a workgroup: a group of 32 lanes
+// takes every eighth part, four elements a lane, with maximum and sum of its own, and the groups are
+// joined in LDS.
+constexpr int kJoinLanes = 32, kJoinGroups = 8;
 
 template <class E>
 __global__ void __launch_bounds__(kJoinLanes * kJoinGroups)
@@ -158,77 +156,40 @@ k_kv_attention_join(AttArgs a) {
   const uint32_t per = (uint32_t)a.plan[1], begin = (uint32_t)plan[1], end = (uint32_t)plan[2];
   if ((int)blockIdx.y >= splits) return;
   const int share = (int)(begin / per), count = (int)((end - 1) / per) - share + 1;
-  // the first share's part is its second one where the share begins with another sequence
-  const int first_part = 2 * share + (begin > (uint32_t)share * per ? 1 : 0);
-  const int lane = (int)threadIdx.x & (kJoinLanes - 1), g = (int)threadIdx.x / kJoinLanes;
-  const bool many = count > kJoinBatch;
-  if (!many && blockIdx.x % kJoinGroups != 0) return;
-  const int head = (int)blockIdx.x + (many ? 0 : g), dim = a.value.dim;
-  const int from = many ? g : 0, step = many ? kJoinGroups : 1;
-  if (head >= a.query_heads) return;  // only with few parts: no barrier then
+  const int head = (int)blockIdx.x, lane = (int)threadIdx.x & (kJoinLanes - 1),
+            g = (int)threadIdx.x / kJoinLanes, dim = a.value.dim;
   typename E::S* out = static_cast<typename E::S*>(a.value.plain) + sequence * a.value.p_token +
                        head * a.value.p_head;
   for (int d0 = 0; d0 < dim; d0 += kJoinLanes * 4) {
-    const int d = d0 + lane * 4;
+    // the last four overlap those before them where there are not four more
+    const int d = min(d0 + lane * 4, max(dim - 4, 0));
     float m = -__builtin_inff(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     int unit = -252;  // below any part's
-    for (int i = from; i < count; i += step * kJoinBatch) {
-      float mi[kJoinBatch], li[kJoinBatch], v[kJoinBatch][4];
-      int ei[kJoinBatch];
-      // no load hangs on a condition: what is not there is another one's copy, without weight
+#pragma unroll 4
+    for (int i = g; i < count; i += kJoinGroups) {
+      // the first share's part is its second one where the share begins with another sequence
+      const int part = 2 * (share + i) + (i == 0 && begin > (uint32_t)share * per ? 1 : 0);
+      const int64_t row = (int64_t)part * a.query_heads + head;
+      const Pack<float, 4> s = ld<float, 4>(a.sums + row * 4);
+      const float mi = s.v[0], li = s.v[1];
+      const int ei = (int)s.v[2];
+      const float* src = a.parts + row * dim;
+      float v[4];
+      if (dim >= 4) {
+        __builtin_memcpy(v, src + d, sizeof(v));
+      } else {
 #pragma unroll
-      for (int j = 0; j < kJoinBatch; ++j) {
-        const int x = i + j * step;
-        const int64_t row =
-            (int64_t)(x == 0 || x >= count ? first_part : 2 * (share + x)) * a.query_heads + head;
-        const Pack<float, 4> s = ld<float, 4>(a.sums + row * 4);
-        mi[j] = s.v[0], li[j] = s.v[1], ei[j] = (int)s.v[2];
-        const float* src = a.parts + row * dim;
-        if (dim % 4 == 0) {
-          const Pack<float, 4> p = ld<float, 4>(src + min(d, dim - 4));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] = p.v[e];
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] = src[min(d + e, dim - 1)];
-        }
+        for (int e = 0; e < 4; ++e) v[e] = src[min(e, dim - 1)];
       }
+      const float top = __builtin_fmaxf(m, mi);
+      const float keep = att_weight(m, top), w = att_weight(mi, top);
+      m = top;
+      l = l * keep + li * w;
+      const int high = max(unit, ei);
+      const float keep_o = keep * att_power(unit - high), w_o = w * att_power(ei - high);
+      unit = high;
 #pragma unroll
-      for (int j = 0; j < kJoinBatch; ++j) {
-        if (i + j * step < count) continue;
-        mi[j] = -__builtin_inff(), li[j] = 0.0f, ei[j] = -252;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[j][e] = 0.0f;
-      }
-      float top = m;
-      int high = unit;
-#pragma unroll
-      for (int j = 0; j < kJoinBatch; ++j) {
-        top = __builtin_fmaxf(top, mi[j]);
-        high = max(high, ei[j]);
-      }
-      const float keep = att_weight(m, top), keep_o = keep * att_power(unit - high);
-      m = top, unit = high;
-      l *= keep;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] *= keep_o;
-#pragma unroll
-      for (int j = 0; j < kJoinBatch; ++j) {
-        const float w = att_weight(mi[j], top), w_o = w * att_power(ei[j] - high);
-        l += li[j] * w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += v[j][e] * w_o;
-      }
-    }
-    if (!many) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (d + e < dim) out[d + e] = E::from_f(att_value(o[e], l, unit));
-      }
-      if (a.lse != nullptr && d == 0) {
-        a.lse[(int64_t)sequence * a.query_heads + head] = att_lse(m, l);
-      }
-      continue;
+      for (int e = 0; e < 4; ++e) o[e] = o[e] * keep_o + v[e] * w_o;
     }
     if (lane == 0) ms[g] = m, ls[g] = l, es[g] = unit;
 #pragma unroll
@@ -248,12 +209,12 @@ k_kv_attention_join(AttArgs a) {
       sum += ls[i] * f[i];
       f[i] *= att_power(es[i] - high);
     }
-    const int e = (int)threadIdx.x;
-    if (e < kJoinLanes * 4 && d0 + e < dim) {
+    const int x = (int)threadIdx.x, at = min(d0 + (x & ~3), max(dim - 4, 0)) + (x & 3);
+    if (x < kJoinLanes * 4 && d0 + (x & ~3) < dim && at < dim) {
       float v = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kJoinGroups; ++i) v += os[i][e] * f[i];
-      out[d0 + e] = E::from_f(att_value(v, sum, high));
+      for (int i = 0; i < kJoinGroups; ++i) v += os[i][x] * f[i];
+      out[at] = E::from_f(att_value(v, sum, high));
     }
     if (a.lse != nullptr && d0 == 0 && threadIdx.x == 0) {
       a.lse[(int64_t)sequence * a.query_heads + head] = att_lse(top, sum);
@@ -267,10 +228,13 @@ k_kv_attention_join(AttArgs a) {
 
 namespace {
 
-// Shares: waves for the card over all of a share's key heads and blocks of sixteen query heads.
-int kAttShares = getenv("MCOP_T") ? atoi(getenv("MCOP_T")) : 2048;
-int64_t target_of(int64_t heads, int64_t group) {
-  return std::max<int64_t>(1, kAttShares / (heads * ((group + 15) / 16)));
+// Shares: waves for the card over all of a share's key heads and blocks of sixteen query heads.  Codes
+// through LDS: four waves a CU, which have two tiles each in flight (2 x 131072 positions of 8 x 128 fp8: 111
+// us, 116 with eight waves and twice the parts; 48 windows of 1024 of 4 x 256: 42 and 61); else eight (37
+// ragged sequences of 5 x 80 and 96 int8 to fp32: 36 us with four, 30 so).
+constexpr int kLineShares = 1024, kAttShares = 2048;
+int64_t target_of(int64_t shares, int64_t heads, int64_t group) {
+  return std::max<int64_t>(1, shares / (heads * ((group + 15) / 16)));
 }
 
 struct Workspace {
@@ -311,8 +275,11 @@ bool whole_lines(const AttArgs& a, int fmt) {
 }
 
 template <class E, int FMT>
-int launch_of(const char* name, AttArgs a, mcop_dtype dtype, bool joins, hipStream_t st) {
+int launch_of(const char* name, AttArgs a, mcop_dtype dtype, hipStream_t st) {
   const int shape = tile_shape(a), rows = shape >= 0 ? kTileRows : kAttRows;
+  const bool lines = shape >= 0 && whole_lines(a, FMT);
+  a.target = (int)target_of(lines ? kLineShares : kAttShares, a.heads, a.group);
+  const bool joins = a.target > 1;  // one share splits nothing
   a.row_blocks = (a.group + rows - 1) / rows;
   // shares of a die times their heads and blocks, a wave each of the matrix kernels, else a workgroup
   const int64_t inner = (int64_t)a.heads * a.row_blocks, workers = (int64_t)(a.target + 7) / 8 * inner;
@@ -332,10 +299,9 @@ int launch_of(const char* name, AttArgs a, mcop_dtype dtype, bool joins, hipStre
                   : 2 * kAttRows + 1 + (size_t)kAttRows * a.value.dim);
   trace_launch(name, "sequences=%d heads=%d of %d head sizes %d and %d: %s kernel, wgs=%lld, %d "
                "shares%s", a.sequences, a.heads, a.query_heads, a.key.dim, a.value.dim,
-               shape >= 0 ? "matrix" : "vector", (long long)blocks, a.target, joins ? "" : ", none split");
+               lines ? "matrix, through LDS," : shape >= 0 ? "matrix" : "vector", (long long)blocks, a.target, joins ? "" : ", none split");
   const dim3 grid((unsigned)blocks), block(kAttWaves * 64);
   if (shape >= 0) {
-    const bool lines = whole_lines(a, FMT);
     int rc;
     if constexpr (FMT == KV_INT8) rc = attention_tiles_int8(shape, lines, dtype, a, grid, st);
     else if constexpr (FMT == KV_FP8) rc = attention_tiles_fp8(shape, lines, dtype, a, grid, st);
@@ -366,8 +332,8 @@ extern "C" int64_t mcop_kv_cache_attention_workspace(int64_t num_heads, int64_t 
                      "head_size=%lld", (long long)num_heads, (long long)query_heads,
                      (long long)value_head_size);
   }
-  return workspace_of(target_of(num_heads, query_heads / num_heads), query_heads, value_head_size)
-      .bytes();
+  return workspace_of(target_of(kAttShares, num_heads, query_heads / num_heads), query_heads,
+                      value_head_size).bytes();
 }
 
 extern "C" int mcop_kv_cache_attention(const mcop_kv_side* key, const mcop_kv_side* value,
@@ -424,7 +390,7 @@ extern "C" int mcop_kv_cache_attention(const mcop_kv_side* key, const mcop_kv_si
   if (!seq_lens || (!block_table && table_columns > 0)) {
     return set_error(MCOP_E_INVALID, "%s: null pointer", name);
   }
-  const int64_t target = target_of(num_heads, query_heads / num_heads);
+  const int64_t target = target_of(kAttShares, num_heads, query_heads / num_heads);
   const Workspace ws = workspace_of(target, query_heads, a.value.dim);
   if (!workspace || !aligned(16, workspace) || workspace_bytes < ws.bytes()) {
     return set_error(MCOP_E_INVALID, "%s: the workspace must be %lld bytes at a multiple of 16", name,
@@ -443,18 +409,16 @@ extern "C" int mcop_kv_cache_attention(const mcop_kv_side* key, const mcop_kv_si
   a.query_heads = (int)query_heads;
   a.group = (int)(query_heads / num_heads);
   a.window = (int)std::min<int64_t>(window, INT32_MAX);
-  a.target = (int)target;
   a.scale = scale * kLog2e;
   a.parts = static_cast<float*>(workspace);
   a.sums = a.parts + ws.parts / 4;
   a.plan = reinterpret_cast<int32_t*>(a.sums + ws.sums / 4);
-  const bool joins = target > 1;  // one share splits nothing
   auto st = static_cast<hipStream_t>(stream);
   auto by_format = [&](auto e) {
     using E = decltype(e);
-    if (fmt == KV_INT8) return launch_of<E, KV_INT8>(name, a, dtype, joins, st);
-    if (fmt == KV_FP8) return launch_of<E, KV_FP8>(name, a, dtype, joins, st);
-    return launch_of<E, KV_MXFP4>(name, a, dtype, joins, st);
+    if (fmt == KV_INT8) return launch_of<E, KV_INT8>(name, a, dtype, st);
+    if (fmt == KV_FP8) return launch_of<E, KV_FP8>(name, a, dtype, st);
+    return launch_of<E, KV_MXFP4>(name, a, dtype, st);
   };
   if (dtype == MCOP_BF16) return by_format(BF16());
   if (dtype == MCOP_F16) return by_format(F16());

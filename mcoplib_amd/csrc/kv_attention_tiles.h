@@ -27,12 +27,15 @@ namespace mcop {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// Workgroups a CU that the kernel's registers are held to: two where that spills none of them.
-template <class E, int FMT, int KP, int VD>
+// Workgroups a CU that a kernel's registers are held to: two where that spills none of them.
+template <class E, int FMT, int KP, int VD, bool LINES>
 constexpr int kResident =
-    VD == 4 || (VD == 8 && !std::is_same_v<E, F32> &&
-                (KP == 2 ? FMT != KV_INT8 || std::is_same_v<E, BF16>
-                         : FMT == KV_MXFP4 || (FMT == KV_FP8 && std::is_same_v<E, BF16>))) ? 2 : 1;
+    VD == 4 ? 2
+    : VD == 16 ? 1
+    : LINES ? (std::is_same_v<E, F32> ? 1
+               : KP == 2              ? (FMT != KV_INT8 || std::is_same_v<E, BF16> ? 2 : 1)
+                                      : (FMT == KV_MXFP4 || (FMT == KV_FP8 && std::is_same_v<E, BF16>) ? 2 : 1))
+            : (KP == 2 || FMT == KV_MXFP4 || (FMT == KV_FP8 && !std::is_same_v<E, F32>) ? 2 : 1);
 
 constexpr int kTileRows = 16;    // query heads of a wave
 constexpr float kAttSlack = 8.0f;  // weights are at most 2^8
@@ -185,6 +188,8 @@ struct AttWave {
   static constexpr bool MX = FMT == KV_MXFP4;
   static constexpr int KW = MX ? 2 : 4;                                 // dwords of 16 codes
   static constexpr int VB = MX ? VD / 2 : VD, VW = (VB + 3) / 4;        // bytes, dwords of VD codes
+  // Wide fp32 kernels have no registers for a tile's values beside its keys: values are read when needed.
+  static constexpr bool LATE = VD == 16 && TQ == 3;
 
   const AttArgs& a;
   const int lane, c, g;
@@ -272,6 +277,7 @@ struct AttWave {
     f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
+      if constexpr (VD == 16) __builtin_amdgcn_sched_barrier(0);
       uint32_t w[2][KW];
       float scale[2] = {1.0f, 1.0f};
 #pragma unroll
@@ -281,6 +287,7 @@ struct AttWave {
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
+        if constexpr (VD == 16) __builtin_amdgcn_sched_barrier(0);
         bf16x8 k[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -299,6 +306,7 @@ struct AttWave {
       }
     }
     const float by = __builtin_fabsf(a.scale);  // its sign is the queries'
+    if constexpr (VD == 16) __builtin_amdgcn_sched_barrier(0);
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -352,6 +360,7 @@ struct AttWave {
                                       __builtin_ldexpf(src.vs(e), -unit);
       }
     }
+    if constexpr (VD == 16) __builtin_amdgcn_sched_barrier(0);
     bf16x8 p[TP];
     {
       uint32_t d[TP][4];
@@ -380,6 +389,8 @@ struct AttWave {
     }
 #pragma unroll
     for (int n = 0; n < VD; n += 2) {
+      // kernels at the end of their registers: no conversion ahead of its product
+      if constexpr (VD == 16) __builtin_amdgcn_sched_barrier(0);
       uint32_t even[4], odd[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -491,7 +502,8 @@ struct LdsSource {
   const uint8_t* lds;  // of the wave
   uint32_t to;
   // the tile in turn
-  uint32_t k[2][KP][W::KW], v[8][W::VW];
+  const uint8_t* at;
+  uint32_t k[2][KP][W::KW], v[W::LATE ? 1 : 8][W::VW];
   float kscale[2][MX ? KP : 4], vscale[8], most;
 
   __device__ __forceinline__ LdsSource(const AttArgs& args, const W& w, const AttChunk& ch, int head,
@@ -593,9 +605,20 @@ struct LdsSource {
     }
   }
 
+  __device__ __forceinline__ void read_value(const uint8_t* tile, int e, uint32_t* w) const {
+    const uint8_t* p = tile + (e >> 2) * T::kHalf + v_at[e & 3];
+    if constexpr (W::VB == 2) {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    } else {
+      const auto x = *reinterpret_cast<const Pack<uint32_t, W::VW>*>(p);
+#pragma unroll
+      for (int n = 0; n < W::VW; ++n) w[n] = x.v[n];
+    }
+  }
+
   // Reads what has landed in buffer `turn`.
   __device__ __forceinline__ void fetch(int turn) {
-    const uint8_t* at = lds + turn * T::kBytes;
+    at = lds + turn * T::kBytes;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint8_t* half = at + h * T::kHalf;
@@ -608,14 +631,7 @@ struct LdsSource {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t* w = v[h * 4 + i];
-        if constexpr (W::VB == 2) {
-          w[0] = *reinterpret_cast<const uint16_t*>(half + v_at[i]);
-        } else {
-          const auto x = *reinterpret_cast<const Pack<uint32_t, W::VW>*>(half + v_at[i]);
-#pragma unroll
-          for (int n = 0; n < W::VW; ++n) w[n] = x.v[n];
-        }
+        if constexpr (!W::LATE) read_value(at, h * 4 + i, v[h * 4 + i]);
         if constexpr (MX) {
           vscale[h * 4 + i] = mx_operand(
               *reinterpret_cast<const uint32_t*>(half + vs_at + i * (int)a.v_chunks.d * 4));
@@ -638,8 +654,12 @@ struct LdsSource {
   }
   __device__ __forceinline__ float key_scale(int h, int kp) const { return kscale[h][kp]; }
   __device__ __forceinline__ void value(int e, uint32_t* w) const {
+    if constexpr (W::LATE) {
+      read_value(at, e, w);
+    } else {
 #pragma unroll
-    for (int i = 0; i < W::VW; ++i) w[i] = v[e][i];
+      for (int i = 0; i < W::VW; ++i) w[i] = v[e][i];
+    }
   }
   __device__ __forceinline__ float value_scale(int e) const { return vscale[e]; }
   __device__ __forceinline__ float ks(int e) const { return kscale[e >> 2][e & 3]; }
@@ -648,7 +668,7 @@ struct LdsSource {
 };
 
 template <class E, int FMT, int KP, int VD>
-__global__ void __launch_bounds__(kAttWaves * 64, (kResident<E, FMT, KP, VD>))
+__global__ void __launch_bounds__(kAttWaves * 64, (kResident<E, FMT, KP, VD, true>))
 k_kv_attention_lines(AttArgs a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds_bytes[];  // [waves][2] tiles
   using T = LdsTile<FMT, KP, VD>;
@@ -660,8 +680,9 @@ k_kv_attention_lines(AttArgs a) {
   const int rows = min(kTileRows, a.group - block * kTileRows);
   AttWalk walk(a, share, head == 0 && block == 0);
   AttChunk c;
+  using W = AttWave<E, FMT, KP, VD>;
   while (walk.next(&c)) {
-    AttWave<E, FMT, KP, VD> w(a, c, head0, rows);
+    W w(a, c, head0, rows);
     LdsSource<E, FMT, KP, VD> src(
         a, w, c, head, lds_bytes + wave * (2 * T::kBytes),
         (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds_bytes +
@@ -676,9 +697,10 @@ k_kv_attention_lines(AttArgs a) {
         if (t < last) wait_loads<T::kLoads>();
         else wait_loads<0>();
         src.fetch(turn);
+        if constexpr (W::LATE) w.tile(src, t);
         wait_lds();
         if (t + 2 <= last) src.load(t + 2, turn);
-        w.tile(src, t);
+        if constexpr (!W::LATE) w.tile(src, t);
       }
     }
     w.write(c, head0, rows, src.missing);
@@ -698,7 +720,8 @@ struct RegisterSource {
   int v_at;
   uint32_t k_sel[KP], v_sel;
   bool missing;
-  uint32_t k[2][KP][W::KW], v[8][W::VW], kb[2], vb[2];
+  uint32_t k[2][KP][W::KW], v[W::LATE ? 1 : 8][W::VW], kb[2], vb[2];
+  int64_t v_from;          // of position lane % 32
   float k_scale, v_scale;  // of position lane % 32
 
   __device__ __forceinline__ RegisterSource(const AttArgs& args, const W& w, const AttChunk& ch,
@@ -748,10 +771,14 @@ struct RegisterSource {
         load_bytes<W::KW * 4>(k[h][kp], p + (MX ? d / 2 : d));
       }
     }
+    v_from = vo;
+    if constexpr (!W::LATE) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      load_bytes<W::VB>(v[e], v_base + from_lane64(vo, wave.position(e)) + v_at);
+      for (int e = 0; e < 8; ++e) read_value(e, v[e]);
     }
+  }
+  __device__ __forceinline__ void read_value(int e, uint32_t* w) const {
+    load_bytes<W::VB>(w, v_base + from_lane64(v_from, wave.position(e)) + v_at);
   }
 
   __device__ __forceinline__ void key(int h, int kp, uint32_t* w) const {
@@ -765,8 +792,12 @@ struct RegisterSource {
     return scale_operand(b, k_sel[kp]);
   }
   __device__ __forceinline__ void value(int e, uint32_t* w) const {
+    if constexpr (W::LATE) {
+      read_value(e, w);
+    } else {
 #pragma unroll
-    for (int i = 0; i < W::VW; ++i) w[i] = v[e][i];
+      for (int i = 0; i < W::VW; ++i) w[i] = v[e][i];
+    }
   }
   __device__ __forceinline__ float value_scale(int e) const {
     uint32_t b[2];
@@ -780,7 +811,7 @@ struct RegisterSource {
 };
 
 template <class E, int FMT, int KP, int VD>
-__global__ void __launch_bounds__(kAttWaves * 64, (kResident<E, FMT, KP, VD>))
+__global__ void __launch_bounds__(kAttWaves * 64, (kResident<E, FMT, KP, VD, false>))
 k_kv_attention_tiles(AttArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   uint32_t share;
