@@ -358,6 +358,68 @@ int mcop_kv_cache_attention(const mcop_kv_side* key, const mcop_kv_side* value, 
 int64_t mcop_kv_cache_attention_workspace(int64_t num_heads, int64_t query_heads,
                                           int64_t value_head_size);
 
+/* A tensor of pages: page p is page_bytes bytes from base + p * page_stride on (bytes). */
+typedef struct {
+  void* base;
+  int64_t page_bytes, page_stride;
+} mcop_kv_pages;
+
+/* Copies page src[i] to page dst[i] in every tensor (codes and scales of every layer). Pairs with an index
+ * below 0 or past the pages, and pages copied to themselves, are left out. Pages that are written must differ
+ * from each other and from those that are read. The list is read by the call itself; src and dst are device
+ * memory. No counterpart in the reference's path. */
+int mcop_kv_cache_copy_pages(const mcop_kv_pages* tensors, int64_t num_tensors, int64_t num_pages,
+                             const int32_t* src, const int32_t* dst, int64_t num_pairs, void* stream);
+
+/* The bookkeeping of a cache's pages, on the device: ref_counts [num_pages], the sequences that hold each
+ * page (0 or less: free); block_table [num_rows, table_columns], rows table_row_stride elements apart, a
+ * sequence's pages, -1 behind the last; seq_lens [num_rows], its positions. Sequences are rows of the table.
+ * Calls that name a sequence outside the table, or one whose length does not fit its row, leave it alone. */
+typedef struct {
+  int32_t* block_table;
+  int64_t table_row_stride, num_rows, table_columns;
+  int32_t* seq_lens;
+  int32_t* ref_counts;
+  int64_t num_pages, page_size;
+} mcop_kv_pool;
+
+/* Bytes of the workspace of mcop_kv_cache_fork and _extend (num_requests: their sequences) and _compact
+ * (0), or a negative MCOP_E_* code. No counterpart in the reference. */
+int64_t mcop_kv_cache_pages_workspace(int64_t num_requests, int64_t num_pages);
+
+/* Sequence children[i] becomes a copy of parents[i]: its full pages are shared (counted once more), and a
+ * last page that is filled in part is replaced by a free one, the lowest free page for the first fork that
+ * needs one and so on; src[i], dst[i] <- that page of the parent and of the child, for
+ * mcop_kv_cache_copy_pages (-1 where there is none). A fork that no page is left for leaves its child empty;
+ * one with an index outside the table does nothing. Children must be free rows, different from each other and
+ * from all parents. No counterpart in the reference's path. */
+int mcop_kv_cache_fork(const mcop_kv_pool* pool, const int32_t* parents, const int32_t* children,
+                       int64_t num_forks, int32_t* src, int32_t* dst, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/* sequences[i] grows by cu_tokens[i + 1] - cu_tokens[i] tokens, and takes the lowest free pages for them, in
+ * order of i. slots[t], for cu_tokens[i] <= t < cu_tokens[i + 1], <- the slots of its new positions (for
+ * mcop_kv_cache_write_quant), starts[i] <- the first of those positions. Where the free pages end, that
+ * sequence and all behind it that need a page stay as they are, as do those that would not fit their row of
+ * the table: starts[i] and their slots are -1, as are the slots from cu_tokens[num_sequences] to num_tokens.
+ * cu_tokens is non-decreasing from 0. Sequences must differ from each other. No counterpart in the
+ * reference's path. */
+int mcop_kv_cache_extend(const mcop_kv_pool* pool, const int32_t* sequences, const int32_t* cu_tokens,
+                         int64_t num_sequences, int64_t* slots, int64_t num_tokens, int32_t* starts,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gives back the pages of sequences: each is counted once less, the row is -1 and the length 0. A sequence
+ * that is named twice is given back once. No counterpart in the reference's path. */
+int mcop_kv_cache_free(const mcop_kv_pool* pool, const int32_t* sequences, int64_t num_sequences,
+                       void* stream);
+
+/* Moves the pages in use together: used[0] <- their number U; those at U and above go to the free ones below
+ * U, the highest to the lowest. src, dst [num_pages / 2] <- the moves, for mcop_kv_cache_copy_pages, -1 behind
+ * the last; ref_counts and every place of block_table follow (seq_lens is not used). No counterpart in the
+ * reference's path. */
+int mcop_kv_cache_compact(const mcop_kv_pool* pool, int32_t* src, int32_t* dst, int32_t* used,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Message of the last failed call on this host thread ("" if none). Stands in for the
  * reference's TORCH_CHECK messages (c10::Error text), which its entry points raise directly. */
 const char* mcop_last_error(void);

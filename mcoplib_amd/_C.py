@@ -14,7 +14,9 @@ It also registers operators of the same kind that the reference does not have (o
 the ``_C`` namespace, outputs first): ``mxfp4_quant``, ``mxfp4_dequant``, ``rms_norm_mxfp4_quant``
 and ``mxfp4_scaled_mm`` (4-bit blocks of 32 values with a power-of-two scale),
 ``kv_cache_write_quant`` and ``kv_cache_read_dequant`` (a paged key/value cache of int8, fp8 or
-4-bit vectors), and ``kv_cache_attention`` (one new token a sequence over that cache).  None of them has a gradient.
+4-bit vectors), ``kv_cache_attention`` (one new token a sequence over that cache), and
+``kv_cache_copy_pages``, ``kv_cache_fork``, ``kv_cache_extend``, ``kv_cache_free`` and
+``kv_cache_compact`` (the cache's pages).  None of them has a gradient.
 """
 
 from __future__ import annotations
@@ -38,3 +40,8 @@ mxfp4_scaled_mm = _torch_ops.c_mxfp4_scaled_mm
 kv_cache_write_quant = _torch_ops.c_kv_cache_write_quant
 kv_cache_read_dequant = _torch_ops.c_kv_cache_read_dequant
 kv_cache_attention = _torch_ops.c_kv_cache_attention
+kv_cache_copy_pages = _torch_ops.c_kv_cache_copy_pages
+kv_cache_fork = _torch_ops.c_kv_cache_fork
+kv_cache_extend = _torch_ops.c_kv_cache_extend
+kv_cache_free = _torch_ops.c_kv_cache_free
+kv_cache_compact = _torch_ops.c_kv_cache_compact

@@ -34,6 +34,22 @@ class KvSide(ctypes.Structure):
                 + [("head_size", ctypes.c_int64)])
 
 
+class KvPages(ctypes.Structure):
+    """mcop_kv_pages (include/mcop_norm.h)."""
+
+    _fields_ = [("base", ctypes.c_void_p), ("page_bytes", ctypes.c_int64),
+                ("page_stride", ctypes.c_int64)]
+
+
+class KvPool(ctypes.Structure):
+    """mcop_kv_pool (include/mcop_norm.h)."""
+
+    _fields_ = [("block_table", ctypes.c_void_p), ("table_row_stride", ctypes.c_int64),
+                ("num_rows", ctypes.c_int64), ("table_columns", ctypes.c_int64),
+                ("seq_lens", ctypes.c_void_p), ("ref_counts", ctypes.c_void_p),
+                ("num_pages", ctypes.c_int64), ("page_size", ctypes.c_int64)]
+
+
 def _load() -> ctypes.CDLL:
     if not LIB_PATH.exists():
         raise ImportError(
@@ -71,6 +87,14 @@ def _load() -> ctypes.CDLL:
                                             I64, I, P, P, I64, P]
     lib.mcop_kv_cache_attention_workspace.argtypes = [I64, I64, I64]
     lib.mcop_kv_cache_attention_workspace.restype = I64
+    pool = ctypes.POINTER(KvPool)
+    lib.mcop_kv_cache_copy_pages.argtypes = [ctypes.POINTER(KvPages), I64, I64, P, P, I64, P]
+    lib.mcop_kv_cache_fork.argtypes = [pool, P, P, I64, P, P, P, I64, P]
+    lib.mcop_kv_cache_extend.argtypes = [pool, P, P, I64, P, I64, P, P, I64, P]
+    lib.mcop_kv_cache_free.argtypes = [pool, P, I64, P]
+    lib.mcop_kv_cache_compact.argtypes = [pool, P, P, P, P, I64, P]
+    lib.mcop_kv_cache_pages_workspace.argtypes = [I64, I64]
+    lib.mcop_kv_cache_pages_workspace.restype = I64
     lib.mcop_check_row_scalars.argtypes = [P, ctypes.c_uint32, I64, I, F, P]
     lib.mcop_debug_set_launch_override.argtypes = [I, I]
     lib.mcop_debug_set_split_rows.argtypes = [I]
@@ -89,7 +113,9 @@ def _load() -> ctypes.CDLL:
                "mcop_vllm_rms_norm", "mcop_rms_norm_dynamic_per_token_quant_custom",
                "mcop_mxfp4_quant", "mcop_mxfp4_dequant", "mcop_rms_norm_mxfp4_quant",
                "mcop_mxfp4_scaled_mm", "mcop_kv_cache_write_quant",
-               "mcop_kv_cache_read_dequant", "mcop_kv_cache_attention"):
+               "mcop_kv_cache_read_dequant", "mcop_kv_cache_attention",
+               "mcop_kv_cache_copy_pages", "mcop_kv_cache_fork", "mcop_kv_cache_extend",
+               "mcop_kv_cache_free", "mcop_kv_cache_compact"):
         getattr(lib, fn).restype = I
     lib.mcop_last_error.restype = ctypes.c_char_p
     lib.mcop_last_error.argtypes = []

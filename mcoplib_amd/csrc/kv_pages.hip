@@ -1,0 +1,587 @@
+// kv_pages.hip -- the pages of a paged cache between steps: copied, shared with a fork, taken for new tokens,
+// given back, and moved together.
+//
+// The pool is three device tensors: ref_counts[p], the sequences that hold page p (0 or less: free);
+// block_table, a row of pages a sequence, -1 behind the last; seq_lens, the positions of each.  Pages are
+// taken the lowest free one first, in the order of the requests, so that results depend on nothing
+// else.  Bookkeeping is bound by latency: a request's answer needs all requests before it and the counts up to
+// its pages, so one workgroup scans both (a list of the free pages that are asked for, and where each
+// request's begin), and a second launch has a workgroup for every request.  Copies are bound by HBM.
+//
+// Every index that comes from a tensor is checked before it is used: one outside the table, the row or the
+// pool is left out.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/mcop_norm.h"
+#include "launch_trace.h"
+#include "rowkern.h"
+
+namespace mcop {
+
+// ---- Copies: a workgroup moves 16 KiB, a piece of a page or some whole pages.
+constexpr int kCopyLanes = 256, kCopyUnits = 4, kCopyBytes = kCopyLanes * kCopyUnits * 16;
+constexpr int kCopyTensors = 64;  // of a launch; one lane a tensor finds a workgroup's
+
+struct CopyTensor {
+  uint8_t* base;
+  int64_t stride, bytes;  // from page to page; of a page
+};
+struct CopyArgs {
+  CopyTensor t[kCopyTensors];
+  uint32_t first[kCopyTensors];  // the tensor's first workgroup
+  int tensors;
+  const int32_t *src, *dst;
+  int64_t pairs, pages;
+};
+
+__global__ void __launch_bounds__(kCopyLanes) k_kv_copy_pages(CopyArgs a) {
+  const int lane = (int)threadIdx.x & 63;
+  const bool mine = lane < a.tensors && a.first[lane < a.tensors ? lane : 0] <= blockIdx.x;
+  const int i = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(mine)) - 1;
+  const CopyTensor& t = a.t[i];
+  const int64_t block = blockIdx.x - a.first[i];
+  // units of 16 bytes: of a page (the last may be cut short), and of what this workgroup moves
+  const int64_t units = (t.bytes + 15) / 16;
+  int64_t pair, unit;
+  int many = 1;  // pages
+  if (units >= kCopyLanes * kCopyUnits) {
+    const int64_t pieces = (units + kCopyLanes * kCopyUnits - 1) / (kCopyLanes * kCopyUnits);
+    pair = block / pieces;
+    unit = (block - pair * pieces) * (kCopyLanes * kCopyUnits);
+  } else {
+    many = (int)(kCopyLanes * kCopyUnits / units);
+    pair = block * many;
+    unit = 0;
+  }
+  u32x4 v[kCopyUnits];
+  uint8_t* to[kCopyUnits];
+  int left[kCopyUnits];  // bytes
+#pragma unroll
+  for (int k = 0; k < kCopyUnits; ++k) {
+    int64_t p = pair, u = unit + k * kCopyLanes + (int)threadIdx.x;
+    if (many > 1) {
+      const uint32_t q = (uint32_t)u / (uint32_t)units;
+      p += q, u -= (int64_t)q * units;
+      if ((int)q >= many) p = a.pairs;
+    }
+    left[k] = 0;
+    if (p >= a.pairs || u >= units) continue;
+    const int64_t from = a.src[p], where = a.dst[p];
+    if (from < 0 || from >= a.pages || where < 0 || where >= a.pages || from == where) continue;
+    const int64_t at = u * 16;
+    left[k] = (int)min(t.bytes - at, (int64_t)16);
+    to[k] = t.base + where * t.stride + at;
+    const uint8_t* src = t.base + from * t.stride + at;
+    if (left[k] == 16) {
+      typedef u32x4 loose __attribute__((aligned(1)));
+      v[k] = __builtin_nontemporal_load(reinterpret_cast<const loose*>(src));
+    } else {
+      uint8_t b[16];
+#pragma unroll
+      for (int x = 0; x < 16; ++x) b[x] = x < left[k] ? src[x] : 0;
+      v[k] = __builtin_bit_cast(u32x4, *reinterpret_cast<Pack<uint8_t, 16>*>(b));
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kCopyUnits; ++k) {
+    if (left[k] == 16) {
+      typedef u32x4 loose __attribute__((aligned(1)));
+      __builtin_nontemporal_store(v[k], reinterpret_cast<loose*>(to[k]));
+    } else if (left[k] > 0) {
+      const Pack<uint8_t, 16> b = __builtin_bit_cast(Pack<uint8_t, 16>, v[k]);
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        if (x < left[k]) to[k][x] = b.v[x];
+      }
+    }
+  }
+}
+
+// ---- The pool.
+struct Pool {
+  int32_t* table;
+  int64_t stride;
+  int rows, columns;
+  int32_t *lens, *counts;
+  int pages, page_size;
+};
+
+__device__ __forceinline__ int64_t pages_of(int64_t tokens, int page_size) {
+  return (tokens + page_size - 1) / page_size;
+}
+__device__ __forceinline__ bool row_ok(const Pool& p, int row) { return row >= 0 && row < p.rows; }
+__device__ __forceinline__ bool len_ok(const Pool& p, int64_t n) {
+  return n >= 0 && n <= (int64_t)p.columns * p.page_size;
+}
+
+// Exclusive sum over a workgroup of up to 1024 threads; *all: the whole.  The barriers let `lds` (one value a
+// wave) be used again at once.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* lds, int64_t* all) {
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, waves = (int)blockDim.x >> 6;
+  int64_t s = v;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int64_t o = __shfl_up((long long)s, d, 64);
+    if (lane >= d) s += o;
+  }
+  if (lane == 63) lds[wave] = s;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+  for (int w = 0; w < waves; ++w) {
+    const int64_t x = lds[w];
+    if (w < wave) before += x;
+    total += x;
+  }
+  __syncthreads();
+  *all = total;
+  return before + s - v;
+}
+
+// What a request is: a fork of one sequence into another, or new tokens for one.
+struct Requests {
+  const int32_t *from, *to;  // fork: parents, children; extend: sequences, null
+  const int32_t* cu;         // extend: where each one's new tokens begin
+  int count;
+};
+struct Request {
+  bool ok;             // its indexes and lengths are
+  int from, to;
+  int64_t old, now;    // the sequence's length before and after
+  int64_t have, need;  // pages that it has (fork: shares), and needs besides
+};
+template <bool FORK>
+__device__ __forceinline__ Request request_of(const Pool& p, const Requests& r, int i) {
+  Request q = {};
+  q.from = r.from[i];
+  q.to = FORK ? r.to[i] : q.from;
+  q.ok = row_ok(p, q.from) && row_ok(p, q.to);
+  if (!q.ok) return q;
+  q.old = p.lens[q.from];
+  q.now = FORK ? q.old : q.old + (int64_t)r.cu[i + 1] - r.cu[i];
+  q.ok = len_ok(p, q.old) && q.now >= q.old && len_ok(p, q.now);
+  if (!q.ok) return q;
+  q.have = FORK ? q.old / p.page_size : pages_of(q.old, p.page_size);
+  q.need = pages_of(q.now, p.page_size) - q.have;
+  return q;
+}
+
+// Workspace of a fork or an extension: found free pages; then where each request's begin in them; then
+// the pages.
+struct Taken {
+  int32_t *found, *begin, *list;
+  __host__ __device__ Taken(void* ws, int requests)
+      : found(static_cast<int32_t*>(ws)), begin(found + 4), list(begin + requests) {}
+};
+
+constexpr int kScanLanes = 1024, kScanPages = 16;  // pages a lane at a time
+
+// One workgroup: where each request's pages begin in the order of all, and the lowest free pages, as many as
+// are asked for.
+template <bool FORK>
+__global__ void __launch_bounds__(kScanLanes)
+k_kv_pages_take(Pool p, Requests r, Taken t) {
+  __shared__ int64_t lds[kScanLanes / 64];
+  int64_t asked = 0, all;
+  for (int i0 = 0; i0 < r.count; i0 += kScanLanes) {
+    const int i = i0 + (int)threadIdx.x;
+    const int64_t need = i < r.count ? request_of<FORK>(p, r, i).need : 0;
+    const int64_t begin = asked + block_scan(need, lds, &all);
+    if (i < r.count) t.begin[i] = (int32_t)min(begin, (int64_t)INT32_MAX);
+    asked += all;
+  }
+  int64_t found = 0;
+  for (int64_t p0 = 0; p0 < p.pages && found < asked; p0 += kScanLanes * kScanPages) {
+    const int64_t first = p0 + (int64_t)threadIdx.x * kScanPages;
+    uint32_t free = 0;
+    int32_t c[kScanPages];
+    if (first + kScanPages <= p.pages) {
+      __builtin_memcpy(c, p.counts + first, sizeof(c));
+    } else {
+#pragma unroll
+      for (int k = 0; k < kScanPages; ++k) c[k] = p.counts[min(first + k, (int64_t)p.pages - 1)];
+    }
+#pragma unroll
+    for (int k = 0; k < kScanPages; ++k) free |= (uint32_t)(first + k < p.pages && c[k] <= 0) << k;
+    int64_t at = found + block_scan((int64_t)__builtin_popcount(free), lds, &all);
+    while (free != 0 && at < asked) {
+      t.list[at++] = (int32_t)(first + __builtin_ctz(free));
+      free &= free - 1;
+    }
+    found += all;
+  }
+  if (threadIdx.x == 0) t.found[0] = (int32_t)min(found, asked);
+}
+
+// A request's pages, if there are enough; null else.
+__device__ __forceinline__ const int32_t* pages_for(const Taken& t, const Request& q, int i) {
+  const int64_t begin = t.begin[i];
+  return q.need == 0 || begin + q.need <= t.found[0] ? t.list + begin : nullptr;
+}
+
+constexpr int kRowLanes = 256;
+
+// A workgroup a fork: the child's row.
+__global__ void __launch_bounds__(kRowLanes)
+k_kv_pages_fork(Pool p, Requests r, Taken t, int32_t* src, int32_t* dst) {
+  const int i = (int)blockIdx.x;
+  const Request q = request_of<true>(p, r, i);
+  if (!q.ok) {
+    if (threadIdx.x == 0) src[i] = dst[i] = -1;
+    return;
+  }
+  const int32_t* pages = pages_for(t, q, i);
+  const int32_t* from = p.table + q.from * p.stride;
+  int32_t* to = p.table + q.to * p.stride;
+  for (int c = (int)threadIdx.x; c < p.columns; c += kRowLanes) {
+    int32_t page = -1;
+    if (pages != nullptr && c < q.have) {
+      page = from[c];
+      if (page >= 0 && page < p.pages) atomicAdd(&p.counts[page], 1);
+    } else if (pages != nullptr && c < q.have + q.need) {
+      page = pages[0];
+    }
+    to[c] = page;
+  }
+  if (threadIdx.x == 0) {
+    const bool copies = pages != nullptr && q.need > 0;
+    src[i] = copies ? from[q.have] : -1;
+    dst[i] = copies ? pages[0] : -1;
+    if (copies) p.counts[pages[0]] = 1;
+    p.lens[q.to] = pages != nullptr ? (int32_t)q.now : 0;
+  }
+}
+
+// A workgroup a sequence that grows, and one for the slots behind the last: its row, length and slots.
+__global__ void __launch_bounds__(kRowLanes)
+k_kv_pages_extend(Pool p, Requests r, Taken t, int64_t* slots, int64_t tokens, int32_t* starts) {
+  const int i = (int)blockIdx.x;
+  if (i == r.count) {
+    const int64_t last = max(r.cu[r.count], 0);
+    for (int64_t s = last + (int)threadIdx.x; s < tokens; s += kRowLanes) slots[s] = -1;
+    return;
+  }
+  const Request q = request_of<false>(p, r, i);
+  const int32_t* pages = q.ok ? pages_for(t, q, i) : nullptr;
+  const int64_t first = max(r.cu[i], 0), end = min((int64_t)r.cu[i + 1], tokens);
+  int32_t* row = q.ok ? p.table + q.from * p.stride : nullptr;
+  for (int64_t s = first + (int)threadIdx.x; s < end; s += kRowLanes) {
+    int64_t slot = -1;
+    if (pages != nullptr) {
+      const int64_t at = q.old + s - r.cu[i], c = at / p.page_size;
+      const int32_t page = c < q.have ? row[c] : pages[c - q.have];
+      if (page >= 0 && page < p.pages) slot = (int64_t)page * p.page_size + at % p.page_size;
+    }
+    slots[s] = slot;
+  }
+  if (pages != nullptr) {
+    for (int64_t k = (int)threadIdx.x; k < q.need; k += kRowLanes) {
+      row[q.have + k] = pages[k];
+      p.counts[pages[k]] = 1;
+    }
+  }
+  __syncthreads();  // every lane has read the old length
+  if (threadIdx.x == 0) {
+    starts[i] = pages != nullptr ? (int32_t)q.old : -1;
+    if (pages != nullptr) p.lens[q.from] = (int32_t)q.now;
+  }
+}
+
+// A workgroup a sequence that ends.  Its length is taken away first, so that a sequence that is named twice
+// gives its pages back once.
+__global__ void __launch_bounds__(kRowLanes)
+k_kv_pages_free(Pool p, const int32_t* sequences) {
+  __shared__ int32_t len;
+  const int s = sequences[blockIdx.x];
+  if (!row_ok(p, s)) return;
+  if (threadIdx.x == 0) {
+    const int32_t n = p.lens[s];
+    len = n > 0 && len_ok(p, n) && atomicCAS(&p.lens[s], n, 0) == n ? n : 0;
+  }
+  __syncthreads();
+  if (len <= 0) return;
+  const int64_t held = pages_of(len, p.page_size);
+  int32_t* row = p.table + s * p.stride;
+  for (int c = (int)threadIdx.x; c < p.columns; c += kRowLanes) {
+    const int32_t page = row[c];
+    if (c < held && page >= 0 && page < p.pages) atomicSub(&p.counts[page], 1);
+    row[c] = -1;
+  }
+}
+
+// ---- Compaction: U pages are in use.  Those at U and above go to the free ones below it, the highest to the
+// lowest: a page in use with b in use before it is the (U - 1 - b)-th from the end, a free page f with b in use
+// before it the (f - b)-th hole.
+constexpr int kMoveLanes = 1024, kMovePages = 4;  // pages a lane
+
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* lds) {
+  int64_t all;
+  block_scan(v, lds, &all);
+  return all;
+}
+
+// A workgroup 4096 pages.  Each counts the whole pool for itself (twice: all, and those below U): 8192 pages
+// are 32 KiB from L2, where another launch would take longer.
+__global__ void __launch_bounds__(kMoveLanes)
+k_kv_pages_moves(const int32_t* __restrict__ counts, int64_t pages, int32_t* src, int32_t* dst,
+                 int32_t* used, int32_t* moved) {
+  __shared__ int64_t lds[kMoveLanes / 64];
+  const int64_t mine = (int64_t)blockIdx.x * (kMoveLanes * kMovePages), half = pages / 2;
+  int64_t in_use = 0, before = 0;
+  for (int64_t p = (int)threadIdx.x; p < pages; p += kMoveLanes) {
+    const int64_t x = counts[p] > 0;
+    in_use += x;
+    if (p < mine) before += x;
+  }
+  in_use = block_sum(in_use, lds);
+  before = block_sum(before, lds);
+  int64_t below = 0;
+  for (int64_t p = (int)threadIdx.x; p < in_use; p += kMoveLanes) below += counts[p] > 0;
+  const int64_t moves = in_use - block_sum(below, lds);
+  const int64_t first = mine + (int64_t)threadIdx.x * kMovePages;
+  int32_t c[kMovePages];
+  int64_t here = 0, all;
+#pragma unroll
+  for (int k = 0; k < kMovePages; ++k) {
+    c[k] = first + k < pages ? counts[first + k] : 0;
+    here += c[k] > 0;
+  }
+  before += block_scan(here, lds, &all);
+#pragma unroll
+  for (int k = 0; k < kMovePages; ++k) {
+    const int64_t p = first + k;
+    if (p >= pages) break;
+    int64_t rank = -1;
+    if (c[k] > 0) {
+      if (p >= in_use) {
+        rank = in_use - 1 - before;
+        src[rank] = (int32_t)p;
+      }
+      ++before;
+    } else if (p < in_use) {
+      dst[p - before] = (int32_t)p;
+    }
+    moved[p] = (int32_t)rank;
+    // the lists have half as many places as there are pages
+    if (p < half && p >= moves) src[p] = dst[p] = -1;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) used[0] = (int32_t)in_use;
+}
+
+// The table's pages and the counts where they are now.
+__global__ void __launch_bounds__(kRowLanes)
+k_kv_pages_move(Pool p, const int32_t* src, const int32_t* dst, const int32_t* moved, int64_t places) {
+  const int64_t i = (int64_t)blockIdx.x * kRowLanes + threadIdx.x;
+  const int64_t half = p.pages / 2;
+  if (i < half && src[i] >= 0) {
+    p.counts[dst[i]] = p.counts[src[i]];
+    p.counts[src[i]] = 0;
+  }
+  if (i < places) {
+    const int64_t row = i / p.columns;
+    int32_t* at = p.table + row * p.stride + (i - row * p.columns);
+    const int32_t page = *at;
+    if (page >= 0 && page < p.pages && moved[page] >= 0) *at = dst[moved[page]];
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side.
+
+namespace {
+
+// Requests, workgroups of a launch (which takes fewer than 2^32 threads, one request's more among them).
+constexpr int64_t kMostCount = ((int64_t)1 << 24) - 2;
+
+int pool_of(const char* name, const mcop_kv_pool* in, bool lens, Pool* out) {
+  if (!in) return set_error(MCOP_E_INVALID, "%s: null pointer", name);
+  if (in->num_rows < 0 || in->num_rows > INT32_MAX || in->table_columns < 0 ||
+      in->table_columns > INT32_MAX || in->table_row_stride < 0 ||
+      (in->num_rows > 0 && in->table_row_stride > INT64_MAX / 8 / in->num_rows) || in->num_pages < 0 ||
+      in->num_pages > INT32_MAX || in->page_size <= 0 || in->page_size > INT32_MAX) {
+    return set_error(MCOP_E_INVALID, "%s: bad pool: %lld rows of %lld pages, %lld pages of %lld tokens",
+                     name, (long long)in->num_rows, (long long)in->table_columns,
+                     (long long)in->num_pages, (long long)in->page_size);
+  }
+  if ((!in->block_table && in->num_rows > 0 && in->table_columns > 0) ||
+      (lens && !in->seq_lens && in->num_rows > 0) || (!in->ref_counts && in->num_pages > 0)) {
+    return set_error(MCOP_E_INVALID, "%s: null pointer", name);
+  }
+  *out = Pool{in->block_table, in->table_row_stride, (int)in->num_rows, (int)in->table_columns,
+              in->seq_lens, in->ref_counts, (int)in->num_pages, (int)in->page_size};
+  return MCOP_OK;
+}
+
+int count_ok(const char* name, int64_t n) {
+  if (n < 0 || n > kMostCount) {
+    return set_error(MCOP_E_INVALID, "%s: bad number of requests %lld (at most 2^24 - 2)", name,
+                     (long long)n);
+  }
+  return MCOP_OK;
+}
+
+int workspace_ok(const char* name, const void* ws, int64_t bytes, int64_t requests, int64_t pages) {
+  const int64_t need = mcop_kv_cache_pages_workspace(requests, pages);
+  if (!ws || !aligned(16, ws) || bytes < need) {
+    return set_error(MCOP_E_INVALID, "%s: the workspace must be %lld bytes at a multiple of 16", name,
+                     (long long)need);
+  }
+  return MCOP_OK;
+}
+
+}  // namespace
+
+}  // namespace mcop
+
+extern "C" int64_t mcop_kv_cache_pages_workspace(int64_t num_requests, int64_t num_pages) {
+  using namespace mcop;
+  if (num_requests < 0 || num_requests > kMostCount || num_pages < 0 || num_pages > INT32_MAX) {
+    return set_error(MCOP_E_INVALID, "kv_cache_pages_workspace: %lld requests, %lld pages",
+                     (long long)num_requests, (long long)num_pages);
+  }
+  return (4 + num_requests + num_pages) * 4;
+}
+
+extern "C" int mcop_kv_cache_copy_pages(const mcop_kv_pages* tensors, int64_t num_tensors,
+                                        int64_t num_pages, const int32_t* src, const int32_t* dst,
+                                        int64_t num_pairs, void* stream) {
+  using namespace mcop;
+  const char* name = "kv_cache_copy_pages";
+  if (num_tensors < 0 || num_pages < 0 || num_pages > INT32_MAX || num_pairs < 0 ||
+      num_pairs > INT32_MAX) {
+    return set_error(MCOP_E_INVALID, "%s: bad shape num_tensors=%lld num_pages=%lld num_pairs=%lld", name,
+                     (long long)num_tensors, (long long)num_pages, (long long)num_pairs);
+  }
+  if (num_tensors == 0 || num_pairs == 0 || num_pages == 0) return MCOP_OK;
+  if (!tensors || !src || !dst) return set_error(MCOP_E_INVALID, "%s: null pointer", name);
+  for (int64_t i = 0; i < num_tensors; ++i) {
+    const mcop_kv_pages& t = tensors[i];
+    if (!t.base || t.page_bytes <= 0 || t.page_stride < t.page_bytes ||
+        t.page_stride > INT64_MAX / 4 / num_pages) {
+      return set_error(MCOP_E_INVALID, "%s: tensor %lld: null pointer, or bad pages of %lld bytes %lld "
+                       "apart", name, (long long)i, (long long)t.page_bytes, (long long)t.page_stride);
+    }
+  }
+  auto st = static_cast<hipStream_t>(stream);
+  for (int64_t i0 = 0; i0 < num_tensors; i0 += kCopyTensors) {
+    CopyArgs a{};
+    a.tensors = (int)std::min<int64_t>(kCopyTensors, num_tensors - i0);
+    a.src = src, a.dst = dst, a.pairs = num_pairs, a.pages = num_pages;
+    int64_t blocks = 0;
+    constexpr int64_t kUnits = kCopyLanes * kCopyUnits;
+    for (int i = 0; i < a.tensors; ++i) {
+      const mcop_kv_pages& t = tensors[i0 + i];
+      a.t[i] = CopyTensor{static_cast<uint8_t*>(t.base), t.page_stride, t.page_bytes};
+      a.first[i] = (uint32_t)blocks;
+      const int64_t units = (t.page_bytes + 15) / 16;
+      const int64_t per = units >= kUnits ? (units + kUnits - 1) / kUnits : 1;
+      const int64_t pages = units >= kUnits ? 1 : kUnits / units;
+      const int64_t groups = (num_pairs + pages - 1) / pages;
+      if (per > kMostCount || groups > kMostCount / per || blocks + groups * per >= kMostCount) {
+        return set_error(MCOP_E_UNSUPPORTED, "%s: more bytes than one launch takes", name);
+      }
+      blocks += groups * per;
+    }
+    trace_launch(name, "%d tensors, %lld pairs, wgs=%lld", a.tensors, (long long)num_pairs,
+                 (long long)blocks);
+    hipLaunchKernelGGL(k_kv_copy_pages, dim3((unsigned)blocks), dim3(kCopyLanes), 0, st, a);
+    if (int rc = check_launch(name)) return rc;
+  }
+  return MCOP_OK;
+}
+
+extern "C" int mcop_kv_cache_fork(const mcop_kv_pool* pool, const int32_t* parents,
+                                  const int32_t* children, int64_t num_forks, int32_t* src,
+                                  int32_t* dst, void* workspace, int64_t workspace_bytes,
+                                  void* stream) {
+  using namespace mcop;
+  const char* name = "kv_cache_fork";
+  Pool p;
+  if (int rc = count_ok(name, num_forks)) return rc;
+  if (num_forks == 0) return MCOP_OK;
+  if (int rc = pool_of(name, pool, true, &p)) return rc;
+  if (!parents || !children || !src || !dst) return set_error(MCOP_E_INVALID, "%s: null pointer", name);
+  if (int rc = workspace_ok(name, workspace, workspace_bytes, num_forks, p.pages)) return rc;
+  const Requests r{parents, children, nullptr, (int)num_forks};
+  const Taken t(workspace, (int)num_forks);
+  auto st = static_cast<hipStream_t>(stream);
+  trace_launch(name, "%lld forks, %d pages", (long long)num_forks, p.pages);
+  hipLaunchKernelGGL((k_kv_pages_take<true>), dim3(1), dim3(kScanLanes), 0, st, p, r, t);
+  if (int rc = check_launch(name)) return rc;
+  hipLaunchKernelGGL(k_kv_pages_fork, dim3((unsigned)num_forks), dim3(kRowLanes), 0, st, p, r, t, src,
+                     dst);
+  return check_launch(name);
+}
+
+extern "C" int mcop_kv_cache_extend(const mcop_kv_pool* pool, const int32_t* sequences,
+                                    const int32_t* cu_tokens, int64_t num_sequences, int64_t* slots,
+                                    int64_t num_tokens, int32_t* starts, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  using namespace mcop;
+  const char* name = "kv_cache_extend";
+  Pool p;
+  if (int rc = count_ok(name, num_sequences)) return rc;
+  if (num_tokens < 0) return set_error(MCOP_E_INVALID, "%s: bad num_tokens %lld", name, (long long)num_tokens);
+  if (num_sequences == 0 && num_tokens == 0) return MCOP_OK;
+  if (int rc = pool_of(name, pool, true, &p)) return rc;
+  if (!cu_tokens || (num_sequences > 0 && (!sequences || !starts)) || (!slots && num_tokens > 0)) {
+    return set_error(MCOP_E_INVALID, "%s: null pointer", name);
+  }
+  if (int rc = workspace_ok(name, workspace, workspace_bytes, num_sequences, p.pages)) return rc;
+  const Requests r{sequences, nullptr, cu_tokens, (int)num_sequences};
+  const Taken t(workspace, (int)num_sequences);
+  auto st = static_cast<hipStream_t>(stream);
+  trace_launch(name, "%lld sequences, %lld tokens, %d pages", (long long)num_sequences,
+               (long long)num_tokens, p.pages);
+  hipLaunchKernelGGL((k_kv_pages_take<false>), dim3(1), dim3(kScanLanes), 0, st, p, r, t);
+  if (int rc = check_launch(name)) return rc;
+  hipLaunchKernelGGL(k_kv_pages_extend, dim3((unsigned)num_sequences + 1), dim3(kRowLanes), 0, st, p, r,
+                     t, slots, num_tokens, starts);
+  return check_launch(name);
+}
+
+extern "C" int mcop_kv_cache_free(const mcop_kv_pool* pool, const int32_t* sequences,
+                                  int64_t num_sequences, void* stream) {
+  using namespace mcop;
+  const char* name = "kv_cache_free";
+  Pool p;
+  if (int rc = count_ok(name, num_sequences)) return rc;
+  if (num_sequences == 0) return MCOP_OK;
+  if (int rc = pool_of(name, pool, true, &p)) return rc;
+  if (!sequences) return set_error(MCOP_E_INVALID, "%s: null pointer", name);
+  trace_launch(name, "%lld sequences", (long long)num_sequences);
+  hipLaunchKernelGGL(k_kv_pages_free, dim3((unsigned)num_sequences), dim3(kRowLanes), 0,
+                     static_cast<hipStream_t>(stream), p, sequences);
+  return check_launch(name);
+}
+
+extern "C" int mcop_kv_cache_compact(const mcop_kv_pool* pool, int32_t* src, int32_t* dst,
+                                     int32_t* used, void* workspace, int64_t workspace_bytes,
+                                     void* stream) {
+  using namespace mcop;
+  const char* name = "kv_cache_compact";
+  Pool p;
+  if (int rc = pool_of(name, pool, false, &p)) return rc;
+  if (!used || (p.pages > 1 && (!src || !dst))) {
+    return set_error(MCOP_E_INVALID, "%s: null pointer", name);
+  }
+  if (int rc = workspace_ok(name, workspace, workspace_bytes, 0, p.pages)) return rc;
+  const int64_t places = (int64_t)p.rows * p.columns;
+  const int64_t threads = std::max(places, (int64_t)p.pages / 2);
+  if (threads >= ((int64_t)1 << 32) - kRowLanes) {
+    return set_error(MCOP_E_UNSUPPORTED, "%s: a table of %lld places is more than one launch takes", name,
+                     (long long)places);
+  }
+  int32_t* moved = static_cast<int32_t*>(workspace);
+  auto st = static_cast<hipStream_t>(stream);
+  constexpr int kPages = kMoveLanes * kMovePages;
+  trace_launch(name, "%d pages, a table of %d x %d", p.pages, p.rows, p.columns);
+  hipLaunchKernelGGL(k_kv_pages_moves, dim3((unsigned)std::max(1, (int)(((int64_t)p.pages + kPages - 1) / kPages))),
+                     dim3(kMoveLanes), 0, st, p.counts, (int64_t)p.pages, src, dst, used, moved);
+  if (int rc = check_launch(name)) return rc;
+  if (threads == 0) return MCOP_OK;
+  hipLaunchKernelGGL(k_kv_pages_move, dim3((unsigned)((threads + kRowLanes - 1) / kRowLanes)),
+                     dim3(kRowLanes), 0, st, p, src, dst, moved, places);
+  return check_launch(name);
+}

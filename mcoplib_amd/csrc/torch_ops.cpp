@@ -11,7 +11,8 @@
 //     registered by register_vllm_ops() for the CUDA (HIP) key, plus a no-op Meta kernel;
 //     and, of the same kind without a counterpart in the reference, the 4-bit operators
 //     (mxfp4_quant, mxfp4_dequant, rms_norm_mxfp4_quant, mxfp4_scaled_mm) and the quantized
-//     key/value cache (kv_cache_write_quant, kv_cache_read_dequant).
+//     key/value cache (kv_cache_write_quant, kv_cache_read_dequant, kv_cache_attention) with its
+//     pages (kv_cache_copy_pages, kv_cache_fork, kv_cache_extend, kv_cache_free, kv_cache_compact).
 // Every function checks its arguments as the reference does (TORCH_CHECK with the reference's
 // condition text) and, beyond the reference, that every tensor is on the device and that element
 // counts match (the kernels trust them); then it makes the input's device current and enqueues
@@ -889,6 +890,126 @@ void c_kv_cache_attention(Tensor& result, const Tensor& query, const Tensor& key
                                    workspace.data_ptr(), bytes, stream_of(query)));
 }
 
+// The pages of a cache.
+
+// Bytes of a page of t (all but its first dimension), which lie together in some order.
+int64_t page_bytes(const char* name, const Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> dims;  // strides, sizes
+  for (int64_t d = 1; d < t.dim(); ++d) {
+    if (t.size(d) != 1) dims.emplace_back(t.stride(d), t.size(d));
+  }
+  std::sort(dims.begin(), dims.end());
+  int64_t dense = 1;
+  for (const auto& [stride, size] : dims) {
+    TORCH_CHECK(stride == dense, name, ": a page's elements must lie together, got sizes ", t.sizes(),
+                " and strides ", t.strides());
+    dense *= size;
+  }
+  TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= dense, name, ": pages must not overlap, got sizes ",
+              t.sizes(), " and strides ", t.strides());
+  return dense * t.element_size();
+}
+
+void c_kv_cache_copy_pages(at::TensorList caches, const Tensor& src, const Tensor& dst) {
+  const char* name = "kv_cache_copy_pages";
+  const auto* from = ints_ptr(name, "src", src, -1);
+  const auto* to = ints_ptr(name, "dst", dst, src.size(0));
+  if (caches.empty()) return;
+  std::vector<mcop_kv_pages> list;
+  int64_t pages = 0;
+  for (const Tensor& t : caches) {
+    TORCH_CHECK(t.dim() > 0 && t.size(0) == caches[0].size(0), name,
+                ": caches must be [pages, ...] of the same pages, got ", t.sizes(), " beside ",
+                caches[0].sizes());
+    on_device(name, {&src, &dst, &t});
+    pages = t.size(0);
+    if (t.numel() == 0) continue;
+    const int64_t bytes = page_bytes(name, t);
+    list.push_back(mcop_kv_pages{t.data_ptr(), bytes,
+                                 pages > 1 ? t.stride(0) * (int64_t)t.element_size() : bytes});
+  }
+  const DeviceGuard guard(src.device());
+  check_rc(mcop_kv_cache_copy_pages(list.data(), (int64_t)list.size(), pages, from, to, src.size(0),
+                                    stream_of(src)));
+}
+
+// The tables, checked; seq_lens may be absent.
+mcop_kv_pool pool_of(const char* name, const Tensor& block_table, const OptTensor& seq_lens,
+                     const Tensor& ref_counts, int64_t page_size) {
+  auto* table = const_cast<int32_t*>(table_ptr(name, block_table));
+  auto* lens = seq_lens.has_value() ? ints_ptr(name, "seq_lens", *seq_lens, block_table.size(0)) : nullptr;
+  auto* counts = ints_ptr(name, "ref_counts", ref_counts, -1);
+  TORCH_CHECK(page_size > 0, name, ": page_size must be positive, got ", page_size);
+  no_overlap(name, {&block_table});
+  return mcop_kv_pool{table, block_table.size(0) > 1 ? block_table.stride(0) : 0, block_table.size(0),
+                      block_table.size(1), lens, counts, ref_counts.size(0), page_size};
+}
+
+Tensor pages_workspace(const Tensor& like, int64_t requests, int64_t pages) {
+  const int64_t bytes = mcop_kv_cache_pages_workspace(requests, pages);
+  if (bytes < 0) check_rc((int)bytes);
+  return at::empty({bytes}, like.options().dtype(at::kByte));
+}
+
+void c_kv_cache_fork(Tensor& block_table, Tensor& seq_lens, Tensor& ref_counts, const Tensor& parents,
+                     const Tensor& children, Tensor& src, Tensor& dst, int64_t page_size) {
+  const char* name = "kv_cache_fork";
+  const mcop_kv_pool pool = pool_of(name, block_table, seq_lens, ref_counts, page_size);
+  const auto* from = ints_ptr(name, "parents", parents, -1);
+  const int64_t n = parents.size(0);
+  const auto* to = ints_ptr(name, "children", children, n);
+  auto* s = ints_ptr(name, "src", src, n);
+  auto* d = ints_ptr(name, "dst", dst, n);
+  on_device(name, {&block_table, &seq_lens, &ref_counts, &parents, &children, &src, &dst});
+  if (n == 0) return;
+  const DeviceGuard guard(block_table.device());
+  const Tensor ws = pages_workspace(block_table, n, pool.num_pages);
+  check_rc(mcop_kv_cache_fork(&pool, from, to, n, s, d, ws.data_ptr(), ws.numel(),
+                              stream_of(block_table)));
+}
+
+void c_kv_cache_extend(Tensor& block_table, Tensor& seq_lens, Tensor& ref_counts,
+                       const Tensor& sequences, const Tensor& cu_tokens, Tensor& slots, Tensor& starts,
+                       int64_t page_size) {
+  const char* name = "kv_cache_extend";
+  const mcop_kv_pool pool = pool_of(name, block_table, seq_lens, ref_counts, page_size);
+  const auto* who = ints_ptr(name, "sequences", sequences, -1);
+  const int64_t n = sequences.size(0);
+  const auto* cu = ints_ptr(name, "cu_tokens", cu_tokens, n + 1);
+  auto* first = ints_ptr(name, "starts", starts, n);
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous(), name,
+              ": slots must be a contiguous vector of Long, got ", slots.scalar_type(), " ",
+              slots.sizes());
+  on_device(name, {&block_table, &seq_lens, &ref_counts, &sequences, &cu_tokens, &slots, &starts});
+  const DeviceGuard guard(block_table.device());
+  const Tensor ws = pages_workspace(block_table, n, pool.num_pages);
+  check_rc(mcop_kv_cache_extend(&pool, who, cu, n, slots.data_ptr<int64_t>(), slots.size(0), first,
+                                ws.data_ptr(), ws.numel(), stream_of(block_table)));
+}
+
+void c_kv_cache_free(Tensor& block_table, Tensor& seq_lens, Tensor& ref_counts,
+                     const Tensor& sequences, int64_t page_size) {
+  const char* name = "kv_cache_free";
+  const mcop_kv_pool pool = pool_of(name, block_table, seq_lens, ref_counts, page_size);
+  const auto* who = ints_ptr(name, "sequences", sequences, -1);
+  on_device(name, {&block_table, &seq_lens, &ref_counts, &sequences});
+  const DeviceGuard guard(block_table.device());
+  check_rc(mcop_kv_cache_free(&pool, who, sequences.size(0), stream_of(block_table)));
+}
+
+void c_kv_cache_compact(Tensor& block_table, Tensor& ref_counts, Tensor& src, Tensor& dst,
+                        Tensor& used) {
+  const char* name = "kv_cache_compact";
+  const mcop_kv_pool pool = pool_of(name, block_table, std::nullopt, ref_counts, 1);
+  auto* s = ints_ptr(name, "src", src, pool.num_pages / 2);
+  auto* d = ints_ptr(name, "dst", dst, pool.num_pages / 2);
+  auto* u = ints_ptr(name, "used", used, 1);
+  on_device(name, {&block_table, &ref_counts, &src, &dst, &used});
+  const DeviceGuard guard(block_table.device());
+  const Tensor ws = pages_workspace(block_table, 0, pool.num_pages);
+  check_rc(mcop_kv_cache_compact(&pool, s, d, u, ws.data_ptr(), ws.numel(), stream_of(block_table)));
+}
+
 // The allocating forms (custom_ops).
 
 std::vector<int64_t> with_last(const Tensor& t, int64_t last) {
@@ -998,6 +1119,37 @@ std::tuple<Tensor, OptTensor> kv_cache_attention_new(
   return {out, lse};
 }
 
+std::tuple<Tensor, Tensor> kv_cache_fork_new(Tensor& block_table, Tensor& seq_lens,
+                                             Tensor& ref_counts, const Tensor& parents,
+                                             const Tensor& children, int64_t page_size) {
+  const py::gil_scoped_release allocating;
+  Tensor src = at::empty({parents.numel()}, parents.options().dtype(at::kInt));
+  Tensor dst = at::empty_like(src);
+  c_kv_cache_fork(block_table, seq_lens, ref_counts, parents, children, src, dst, page_size);
+  return {src, dst};
+}
+
+std::tuple<Tensor, Tensor> kv_cache_extend_new(Tensor& block_table, Tensor& seq_lens,
+                                               Tensor& ref_counts, const Tensor& sequences,
+                                               const Tensor& cu_tokens, int64_t num_tokens,
+                                               int64_t page_size) {
+  TORCH_CHECK(num_tokens >= 0, "kv_cache_extend: num_tokens must not be negative, got ", num_tokens);
+  const py::gil_scoped_release allocating;
+  Tensor slots = at::empty({num_tokens}, sequences.options().dtype(at::kLong));
+  Tensor starts = at::empty({sequences.numel()}, sequences.options().dtype(at::kInt));
+  c_kv_cache_extend(block_table, seq_lens, ref_counts, sequences, cu_tokens, slots, starts, page_size);
+  return {slots, starts};
+}
+
+std::tuple<Tensor, Tensor, Tensor> kv_cache_compact_new(Tensor& block_table, Tensor& ref_counts) {
+  const py::gil_scoped_release allocating;
+  const auto opts = ref_counts.options().dtype(at::kInt);
+  Tensor src = at::empty({ref_counts.numel() / 2}, opts), dst = at::empty_like(src);
+  Tensor used = at::empty({1}, opts);
+  c_kv_cache_compact(block_table, ref_counts, src, dst, used);
+  return {src, dst, used};
+}
+
 // Meta kernel of the mutating _C ops (no outputs to describe): drop the arguments.
 void meta_noop(const c10::OperatorHandle& op, torch::jit::Stack* stack) {
   torch::jit::drop(*stack, op.schema().arguments().size());
@@ -1042,6 +1194,19 @@ constexpr VllmOp kVllmOps[] = {
      "kv_cache_attention(Tensor! result, Tensor query, Tensor key_cache, Tensor value_cache, "
      "Tensor key_scale, Tensor value_scale, Tensor block_table, Tensor seq_lens, float scale, "
      "int window, Tensor!? lse) -> ()"},
+    {"kv_cache_copy_pages", "kv_cache_copy_pages(Tensor(a!)[] caches, Tensor src, Tensor dst) -> ()"},
+    {"kv_cache_fork",
+     "kv_cache_fork(Tensor! block_table, Tensor! seq_lens, Tensor! ref_counts, Tensor parents, "
+     "Tensor children, Tensor! src, Tensor! dst, int page_size) -> ()"},
+    {"kv_cache_extend",
+     "kv_cache_extend(Tensor! block_table, Tensor! seq_lens, Tensor! ref_counts, Tensor sequences, "
+     "Tensor cu_tokens, Tensor! slots, Tensor! starts, int page_size) -> ()"},
+    {"kv_cache_free",
+     "kv_cache_free(Tensor! block_table, Tensor! seq_lens, Tensor! ref_counts, Tensor sequences, "
+     "int page_size) -> ()"},
+    {"kv_cache_compact",
+     "kv_cache_compact(Tensor! block_table, Tensor! ref_counts, Tensor! src, Tensor! dst, "
+     "Tensor! used) -> ()"},
 };
 
 // Registers the _C schemas (each only if no other library, e.g. vLLM's own _C, defined it) with
@@ -1076,6 +1241,11 @@ void register_vllm_ops() {
   cuda->impl("kv_cache_write_quant", TORCH_FN(c_kv_cache_write_quant));
   cuda->impl("kv_cache_read_dequant", TORCH_FN(c_kv_cache_read_dequant));
   cuda->impl("kv_cache_attention", TORCH_FN(c_kv_cache_attention));
+  cuda->impl("kv_cache_copy_pages", TORCH_FN(c_kv_cache_copy_pages));
+  cuda->impl("kv_cache_fork", TORCH_FN(c_kv_cache_fork));
+  cuda->impl("kv_cache_extend", TORCH_FN(c_kv_cache_extend));
+  cuda->impl("kv_cache_free", TORCH_FN(c_kv_cache_free));
+  cuda->impl("kv_cache_compact", TORCH_FN(c_kv_cache_compact));
   done = true;
 }
 
@@ -1209,6 +1379,38 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("key_scale"), py::arg("value_scale"), py::arg("block_table"), py::arg("seq_lens"),
         py::arg("scale"), py::arg("window") = 0, py::arg("lse") = py::none(),
         py::call_guard<py::gil_scoped_release>());  // it allocates its workspace
+  m.def("c_kv_cache_copy_pages",
+        [](const std::vector<Tensor>& caches, const Tensor& src, const Tensor& dst) {
+          c_kv_cache_copy_pages(caches, src, dst);
+        },
+        "Copies page src[i] to page dst[i] in every tensor [pages, ...] of caches (codes and scales of "
+        "every layer); pairs with a negative index, or one past the pages, are left out. Pages that are "
+        "written must differ from each other and from those that are read.",
+        py::arg("caches"), py::arg("src"), py::arg("dst"));
+  m.def("c_kv_cache_fork", &c_kv_cache_fork,
+        "Sequence (row of block_table) children[i] becomes a copy of parents[i]: full pages are shared, a "
+        "part-filled last page is replaced by the lowest free one; src, dst <- that page of the parent "
+        "and of the child, for kv_cache_copy_pages, -1 where there is none.",
+        py::arg("block_table"), py::arg("seq_lens"), py::arg("ref_counts"), py::arg("parents"),
+        py::arg("children"), py::arg("src"), py::arg("dst"), py::arg("page_size"),
+        py::call_guard<py::gil_scoped_release>());  // it allocates its workspace
+  m.def("c_kv_cache_extend", &c_kv_cache_extend,
+        "sequences[i] grows by cu_tokens[i + 1] - cu_tokens[i] tokens and takes the lowest free pages for "
+        "them; slots <- the new tokens' slots, starts <- their first positions, -1 where the pages do "
+        "not suffice.",
+        py::arg("block_table"), py::arg("seq_lens"), py::arg("ref_counts"), py::arg("sequences"),
+        py::arg("cu_tokens"), py::arg("slots"), py::arg("starts"), py::arg("page_size"),
+        py::call_guard<py::gil_scoped_release>());
+  m.def("c_kv_cache_free", &c_kv_cache_free,
+        "Gives back the pages of sequences: counted once less, the rows -1, the lengths 0.",
+        py::arg("block_table"), py::arg("seq_lens"), py::arg("ref_counts"), py::arg("sequences"),
+        py::arg("page_size"));
+  m.def("c_kv_cache_compact", &c_kv_cache_compact,
+        "Moves the pages in use together: used <- their number U; src, dst [pages / 2] <- the moves from "
+        "U and above to the free pages below, for kv_cache_copy_pages, -1 behind the last; block_table "
+        "and ref_counts follow.",
+        py::arg("block_table"), py::arg("ref_counts"), py::arg("src"), py::arg("dst"), py::arg("used"),
+        py::call_guard<py::gil_scoped_release>());
   // custom_ops: the same into new tensors
   m.def("mxfp4_quant_new", &mxfp4_quant_new, py::arg("input"));
   m.def("mxfp4_dequant_new", &mxfp4_dequant_new, py::arg("codes"), py::arg("scale"),
@@ -1225,4 +1427,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("value_cache"), py::arg("key_scale"), py::arg("value_scale"), py::arg("block_table"),
         py::arg("seq_lens"), py::arg("scale") = py::none(), py::arg("window") = 0,
         py::arg("return_lse") = false);
+  m.def("kv_cache_fork_new", &kv_cache_fork_new, py::arg("block_table"), py::arg("seq_lens"),
+        py::arg("ref_counts"), py::arg("parents"), py::arg("children"), py::arg("page_size"));
+  m.def("kv_cache_extend_new", &kv_cache_extend_new, py::arg("block_table"), py::arg("seq_lens"),
+        py::arg("ref_counts"), py::arg("sequences"), py::arg("cu_tokens"), py::arg("num_tokens"),
+        py::arg("page_size"));
+  m.def("kv_cache_compact_new", &kv_cache_compact_new, py::arg("block_table"), py::arg("ref_counts"));
 }

@@ -5,7 +5,7 @@ key/value cache, which the reference does not have, are here in the same manner.
 
 from __future__ import annotations
 
-from typing import Optional, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -107,3 +107,56 @@ def kv_cache_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache
     out, lse = _torch_ops.kv_cache_attention_new(query, key_cache, value_cache, key_scale, value_scale,
                                                  block_table, seq_lens, scale, window, return_lse)
     return (out, lse) if return_lse else out
+
+
+def kv_cache_copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copies page src[i] to page dst[i] (int32) in every tensor [pages, ...] of caches: the codes and
+    scales of every layer, in one launch for 64 of them.  A page's elements must lie together.  Pairs with
+    a negative index or one past the pages are left out; pages that are written must differ from each
+    other and from those that are read."""
+    _torch_ops.c_kv_cache_copy_pages(caches, src, dst)
+
+
+def kv_cache_fork(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: torch.Tensor,
+                  parents: torch.Tensor, children: torch.Tensor, page_size: int
+                  ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Forks sequences (rows of block_table [sequences, pages], with their lengths seq_lens and the pages'
+    ref_counts [pages], 0 for a free page; all int32, all updated in place): children[i] becomes a copy of
+    parents[i], which it shares the full pages of.  A last page that is filled in part is replaced by a
+    free one, the lowest free page for the first fork that needs one and so on.  Returns (src, dst): that
+    page of the parent and of the child, for kv_cache_copy_pages, -1 where there is none.  A fork that no
+    page is left for leaves its child empty.  Children must be free rows, different from each other and
+    from all parents; a parent may have many."""
+    return _torch_ops.kv_cache_fork_new(block_table, seq_lens, ref_counts, parents, children, page_size)
+
+
+def kv_cache_extend(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: torch.Tensor,
+                    sequences: torch.Tensor, cu_tokens: torch.Tensor, num_tokens: int,
+                    page_size: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Makes room for new tokens: sequences[i] grows by cu_tokens[i + 1] - cu_tokens[i] (int32, from 0),
+    and takes the lowest free pages, in order of i.  num_tokens is the host's count of the new tokens,
+    cu_tokens[-1].  Returns (slots, starts): slots [num_tokens] (int64) is the new tokens' slot_mapping for
+    kv_cache_write_quant, starts [sequences] (int32) the first new position of each.  Where the free pages
+    end, that sequence and those behind it that need a page stay as they are, as does one that would not
+    fit its row: their starts and slots are -1, which kv_cache_write_quant does not write.  The pool's
+    tensors are as in kv_cache_fork; sequences must differ from each other, and a sequence's part-filled
+    last page must be its own (a fork's is)."""
+    return _torch_ops.kv_cache_extend_new(block_table, seq_lens, ref_counts, sequences, cu_tokens,
+                                          num_tokens, page_size)
+
+
+def kv_cache_free(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: torch.Tensor,
+                  sequences: torch.Tensor, page_size: int) -> None:
+    """Gives back the pages of sequences (int32): each page is counted once less, the rows become -1 and
+    the lengths 0.  A sequence that is named twice is given back once.  The pool's tensors are as in
+    kv_cache_fork."""
+    _torch_ops.c_kv_cache_free(block_table, seq_lens, ref_counts, sequences, page_size)
+
+
+def kv_cache_compact(block_table: torch.Tensor, ref_counts: torch.Tensor
+                     ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Moves the pages in use together, so that they are the first ones: those past their number go to the
+    free ones below it, the highest to the lowest.  block_table and ref_counts are updated in place.
+    Returns (src, dst, used): the moves [pages / 2], -1 behind the last, for kv_cache_copy_pages (which
+    must follow, before the cache is used again), and the number of pages in use [1] (int32)."""
+    return _torch_ops.kv_cache_compact_new(block_table, ref_counts)

@@ -111,3 +111,89 @@ def near(got, want, bound, what):
     worst = ((got - want).abs() / room.clamp_min(1e-300))[plain]
     print(f"  {what}: at most {float(worst.max()) if worst.numel() else 0:.3f} of the bound", flush=True)
     assert not worst.numel() or float(over.max()) <= 0, f"{what}: {float(worst.max()):.3f} of the bound"
+
+
+class PagePool:
+    """The page pool as lists, one request after the other."""
+
+    def __init__(self, table, lens, counts, page):
+        self.table, self.lens, self.counts = table.tolist(), lens.tolist(), counts.tolist()
+        self.page, self.columns = page, table.shape[1]
+
+    def _fits(self, n):
+        return 0 <= n <= self.columns * self.page
+
+    def _held(self, n):
+        return -(-n // self.page)
+
+    def fork(self, parents, children):
+        src, dst = [], []
+        free = [p for p, c in enumerate(self.counts) if c <= 0]
+        ended = False  # a fork that needs a page did not get one
+        rows, lens = [list(r) for r in self.table], list(self.lens)
+        for parent, child in zip(parents, children):
+            ok = 0 <= parent < len(rows) and 0 <= child < len(rows) and self._fits(lens[parent])
+            src.append(-1), dst.append(-1)
+            if not ok:
+                continue
+            full, part = divmod(lens[parent], self.page)
+            self.table[child], self.lens[child] = [-1] * self.columns, 0
+            if part and (ended or not free):
+                ended = True
+                continue
+            for c in range(full):
+                page = self.table[child][c] = rows[parent][c]
+                if 0 <= page < len(self.counts):
+                    self.counts[page] += 1
+            if part:
+                src[-1], dst[-1] = rows[parent][full], free.pop(0)
+                self.table[child][full], self.counts[dst[-1]] = dst[-1], 1
+            self.lens[child] = lens[parent]
+        return src, dst
+
+    def extend(self, sequences, cu, num_tokens):
+        slots, starts = [-1] * num_tokens, []
+        free = [p for p, c in enumerate(self.counts) if c <= 0]
+        ended = False
+        for i, s in enumerate(sequences):
+            add = cu[i + 1] - cu[i]
+            starts.append(-1)
+            if not 0 <= s < len(self.table) or add < 0 or not self._fits(self.lens[s]) or not self._fits(
+                    self.lens[s] + add):
+                continue
+            old, have = self.lens[s], self._held(self.lens[s])
+            need = self._held(old + add) - have
+            if need and (ended or need > len(free)):
+                ended = True
+                continue
+            for k in range(need):
+                self.table[s][have + k] = free.pop(0)
+                self.counts[self.table[s][have + k]] = 1
+            self.lens[s], starts[-1] = old + add, old
+            for t in range(add):
+                column, offset = divmod(old + t, self.page)
+                page = self.table[s][column]
+                if 0 <= cu[i] + t < num_tokens and 0 <= page < len(self.counts):
+                    slots[cu[i] + t] = page * self.page + offset
+        return slots, starts
+
+    def free(self, sequences):
+        for s in sequences:
+            if not 0 <= s < len(self.table) or not 0 < self.lens[s] <= self.columns * self.page:
+                continue
+            for page in self.table[s][:self._held(self.lens[s])]:
+                if 0 <= page < len(self.counts):
+                    self.counts[page] -= 1
+            self.table[s], self.lens[s] = [-1] * self.columns, 0
+
+    def compact(self):
+        counts, src, dst = self.counts, [], []
+        used = sum(c > 0 for c in counts)
+        holes = [p for p in range(used) if counts[p] <= 0]
+        for hole, page in zip(holes, [p for p in reversed(range(used, len(counts))) if counts[p] > 0]):
+            src.append(page), dst.append(hole)
+            counts[hole], counts[page] = counts[page], 0
+        place = dict(zip(src, dst))
+        self.table = [[place.get(p, p) for p in row] for row in self.table]
+        behind = [-1] * (len(counts) // 2 - len(src))
+        return src + behind, dst + behind, [used]
