@@ -36,65 +36,81 @@ struct CopyArgs {
   int64_t pairs, pages;
 };
 
-__global__ void __launch_bounds__(kCopyLanes) k_kv_copy_pages(CopyArgs a) {
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+__device__ __forceinline__ u32x4 load_unit(const uint8_t* p) {
+  return *reinterpret_cast<const u32x4_any*>(p);
+}
+__device__ __forceinline__ void store_unit(uint8_t* p, const u32x4& v) {
+  __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(p));
+}
+
+// Each lane's loads go out together: none hangs on a condition, and a lane that has nothing to move reads what
+// another does (with a condition on each, 400 pages of 32 layers took 200 us).
+__global__ void __launch_bounds__(kCopyLanes, 8) k_kv_copy_pages(CopyArgs a) {
   const int lane = (int)threadIdx.x & 63;
   const bool mine = lane < a.tensors && a.first[lane < a.tensors ? lane : 0] <= blockIdx.x;
   const int i = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(mine)) - 1;
-  const CopyTensor& t = a.t[i];
+  const CopyTensor t = a.t[i];
   const int64_t block = blockIdx.x - a.first[i];
-  // units of 16 bytes: of a page (the last may be cut short), and of what this workgroup moves
-  const int64_t units = (t.bytes + 15) / 16;
-  int64_t pair, unit;
-  int many = 1;  // pages
-  if (units >= kCopyLanes * kCopyUnits) {
-    const int64_t pieces = (units + kCopyLanes * kCopyUnits - 1) / (kCopyLanes * kCopyUnits);
-    pair = block / pieces;
-    unit = (block - pair * pieces) * (kCopyLanes * kCopyUnits);
-  } else {
-    many = (int)(kCopyLanes * kCopyUnits / units);
-    pair = block * many;
-    unit = 0;
+  // whole units of 16 bytes of a page, and bytes behind them
+  const int64_t units = t.bytes / 16;
+  const int rest = (int)(t.bytes % 16);
+  constexpr int kUnits = kCopyLanes * kCopyUnits;
+  if (units >= kUnits) {  // a piece of one page
+    const int64_t pieces = (units + kUnits - 1) / kUnits, pair = block / pieces;
+    const int64_t from = a.src[pair], where = a.dst[pair], first = (block - pair * pieces) * kUnits;
+    if (from < 0 || from >= a.pages || where < 0 || where >= a.pages || from == where) return;
+    const uint8_t* src = t.base + from * t.stride;
+    uint8_t* dst = t.base + where * t.stride;
+    u32x4 v[kCopyUnits];
+#pragma unroll
+    for (int k = 0; k < kCopyUnits; ++k) {
+      v[k] = load_unit(src + min(first + k * kCopyLanes + (int)threadIdx.x, units - 1) * 16);
+    }
+#pragma unroll
+    for (int k = 0; k < kCopyUnits; ++k) {
+      const int64_t u = first + k * kCopyLanes + (int)threadIdx.x;
+      if (u < units) store_unit(dst + u * 16, v[k]);
+    }
+    if (first + kUnits >= units && (int)threadIdx.x < rest) {
+      dst[units * 16 + threadIdx.x] = src[units * 16 + threadIdx.x];
+    }
+    return;
+  }
+  // some whole pages, a unit (or what is behind the last) a lane at a time
+  const uint32_t each = (uint32_t)units + (rest > 0 ? 1 : 0);
+  const int many = kUnits / (int)each;
+  const int64_t pair0 = block * many;
+  int64_t from[kCopyUnits], where[kCopyUnits];
+  uint32_t unit[kCopyUnits];
+  bool moves[kCopyUnits];
+#pragma unroll
+  for (int k = 0; k < kCopyUnits; ++k) {
+    const uint32_t x = (uint32_t)(k * kCopyLanes) + threadIdx.x, q = x / each;
+    unit[k] = x - q * each;
+    const int64_t pair = pair0 + q;
+    moves[k] = (int)q < many && pair < a.pairs;
+    from[k] = a.src[min(pair, a.pairs - 1)], where[k] = a.dst[min(pair, a.pairs - 1)];
   }
   u32x4 v[kCopyUnits];
-  uint8_t* to[kCopyUnits];
-  int left[kCopyUnits];  // bytes
 #pragma unroll
   for (int k = 0; k < kCopyUnits; ++k) {
-    int64_t p = pair, u = unit + k * kCopyLanes + (int)threadIdx.x;
-    if (many > 1) {
-      const uint32_t q = (uint32_t)u / (uint32_t)units;
-      p += q, u -= (int64_t)q * units;
-      if ((int)q >= many) p = a.pairs;
-    }
-    left[k] = 0;
-    if (p >= a.pairs || u >= units) continue;
-    const int64_t from = a.src[p], where = a.dst[p];
-    if (from < 0 || from >= a.pages || where < 0 || where >= a.pages || from == where) continue;
-    const int64_t at = u * 16;
-    left[k] = (int)min(t.bytes - at, (int64_t)16);
-    to[k] = t.base + where * t.stride + at;
-    const uint8_t* src = t.base + from * t.stride + at;
-    if (left[k] == 16) {
-      typedef u32x4 loose __attribute__((aligned(1)));
-      v[k] = __builtin_nontemporal_load(reinterpret_cast<const loose*>(src));
-    } else {
-      uint8_t b[16];
-#pragma unroll
-      for (int x = 0; x < 16; ++x) b[x] = x < left[k] ? src[x] : 0;
-      v[k] = __builtin_bit_cast(u32x4, *reinterpret_cast<Pack<uint8_t, 16>*>(b));
+    moves[k] = moves[k] && from[k] >= 0 && from[k] < a.pages && where[k] >= 0 && where[k] < a.pages &&
+               from[k] != where[k];
+    if (units > 0) {
+      v[k] = load_unit(t.base + (moves[k] ? from[k] : 0) * t.stride +
+                       min((int64_t)unit[k], units - 1) * 16);
     }
   }
 #pragma unroll
   for (int k = 0; k < kCopyUnits; ++k) {
-    if (left[k] == 16) {
-      typedef u32x4 loose __attribute__((aligned(1)));
-      __builtin_nontemporal_store(v[k], reinterpret_cast<loose*>(to[k]));
-    } else if (left[k] > 0) {
-      const Pack<uint8_t, 16> b = __builtin_bit_cast(Pack<uint8_t, 16>, v[k]);
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        if (x < left[k]) to[k][x] = b.v[x];
-      }
+    if (!moves[k]) continue;
+    const uint8_t* src = t.base + from[k] * t.stride;
+    uint8_t* dst = t.base + where[k] * t.stride;
+    if (unit[k] < units) {
+      store_unit(dst + unit[k] * 16, v[k]);
+    } else {
+      for (int x = 0; x < rest; ++x) dst[units * 16 + x] = src[units * 16 + x];
     }
   }
 }
@@ -177,12 +193,40 @@ struct Taken {
 
 constexpr int kScanLanes = 1024, kScanPages = 16;  // pages a lane at a time
 
+// The counts of sixteen pages from `first` on, and which of them are in use.
+struct PageCounts {
+  int32_t c[kScanPages];
+  __device__ __forceinline__ void load(const int32_t* counts, int64_t first, int64_t pages) {
+    if (first + kScanPages <= pages) {
+      __builtin_memcpy(c, counts + first, sizeof(c));
+    } else {
+#pragma unroll
+      for (int k = 0; k < kScanPages; ++k) c[k] = first + k < pages ? counts[first + k] : 0;
+    }
+  }
+  __device__ __forceinline__ uint32_t used() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < kScanPages; ++k) m |= (uint32_t)(c[k] > 0) << k;
+    return m;
+  }
+};
+// The low bits that stand for pages below `end`, of sixteen from `first` on.
+__device__ __forceinline__ uint32_t pages_below(int64_t first, int64_t end) {
+  const int64_t n = end - first;
+  return n <= 0 ? 0u : n >= kScanPages ? 0xffffu : (1u << (int)n) - 1;
+}
+
 // One workgroup: where each request's pages begin in the order of all, and the lowest free pages, as many as
 // are asked for.
 template <bool FORK>
 __global__ void __launch_bounds__(kScanLanes)
 k_kv_pages_take(Pool p, Requests r, Taken t) {
   __shared__ int64_t lds[kScanLanes / 64];
+  // the first counts are on their way while the requests are read
+  const int64_t lane_first = (int64_t)threadIdx.x * kScanPages;
+  PageCounts c;
+  c.load(p.counts, lane_first, p.pages);
   int64_t asked = 0, all;
   for (int i0 = 0; i0 < r.count; i0 += kScanLanes) {
     const int i = i0 + (int)threadIdx.x;
@@ -193,17 +237,9 @@ k_kv_pages_take(Pool p, Requests r, Taken t) {
   }
   int64_t found = 0;
   for (int64_t p0 = 0; p0 < p.pages && found < asked; p0 += kScanLanes * kScanPages) {
-    const int64_t first = p0 + (int64_t)threadIdx.x * kScanPages;
-    uint32_t free = 0;
-    int32_t c[kScanPages];
-    if (first + kScanPages <= p.pages) {
-      __builtin_memcpy(c, p.counts + first, sizeof(c));
-    } else {
-#pragma unroll
-      for (int k = 0; k < kScanPages; ++k) c[k] = p.counts[min(first + k, (int64_t)p.pages - 1)];
-    }
-#pragma unroll
-    for (int k = 0; k < kScanPages; ++k) free |= (uint32_t)(first + k < p.pages && c[k] <= 0) << k;
+    const int64_t first = p0 + lane_first;
+    if (p0 > 0) c.load(p.counts, first, p.pages);
+    uint32_t free = ~c.used() & pages_below(first, p.pages);
     int64_t at = found + block_scan((int64_t)__builtin_popcount(free), lds, &all);
     while (free != 0 && at < asked) {
       t.list[at++] = (int32_t)(first + __builtin_ctz(free));
@@ -321,23 +357,47 @@ __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* lds) {
   return all;
 }
 
-// A workgroup 4096 pages.  Each counts the whole pool for itself (twice: all, and those below U): 8192 pages
-// are 32 KiB from L2, where another launch would take longer.
+// A workgroup 4096 pages.  Each counts the whole pool for itself (twice: all, and those below U; the first
+// 65536 pages stay in registers): 8192 pages are 32 KiB from L2, where another launch would take longer.
 __global__ void __launch_bounds__(kMoveLanes)
 k_kv_pages_moves(const int32_t* __restrict__ counts, int64_t pages, int32_t* src, int32_t* dst,
                  int32_t* used, int32_t* moved) {
   __shared__ int64_t lds[kMoveLanes / 64];
+  constexpr int kKept = 4;
+  constexpr int64_t kRound = kMoveLanes * kScanPages;
   const int64_t mine = (int64_t)blockIdx.x * (kMoveLanes * kMovePages), half = pages / 2;
-  int64_t in_use = 0, before = 0;
-  for (int64_t p = (int)threadIdx.x; p < pages; p += kMoveLanes) {
-    const int64_t x = counts[p] > 0;
-    in_use += x;
-    if (p < mine) before += x;
+  const int64_t lane_first = (int64_t)threadIdx.x * kScanPages;
+  uint32_t kept[kKept];
+  int64_t sums = 0;  // in use before this workgroup's pages; in the high half all in use
+#pragma unroll
+  for (int r = 0; r < kKept; ++r) {
+    kept[r] = 0;
+    if (r * kRound >= pages) continue;
+    PageCounts c;
+    c.load(counts, r * kRound + lane_first, pages);
+    kept[r] = c.used();
+    const int64_t n = __builtin_popcount(kept[r]);
+    sums += n << 32 | (r * kRound + lane_first < mine ? n : 0);
   }
-  in_use = block_sum(in_use, lds);
-  before = block_sum(before, lds);
+  for (int64_t p0 = kKept * kRound; p0 < pages; p0 += kRound) {
+    PageCounts c;
+    c.load(counts, p0 + lane_first, pages);
+    const int64_t n = __builtin_popcount(c.used());
+    sums += n << 32 | (p0 + lane_first < mine ? n : 0);
+  }
+  sums = block_sum(sums, lds);
+  const int64_t in_use = sums >> 32;
+  int64_t before = sums & 0xffffffff;
   int64_t below = 0;
-  for (int64_t p = (int)threadIdx.x; p < in_use; p += kMoveLanes) below += counts[p] > 0;
+#pragma unroll
+  for (int r = 0; r < kKept; ++r) {
+    below += __builtin_popcount(kept[r] & pages_below(r * kRound + lane_first, in_use));
+  }
+  for (int64_t p0 = kKept * kRound; p0 < in_use; p0 += kRound) {
+    PageCounts c;
+    c.load(counts, p0 + lane_first, pages);
+    below += __builtin_popcount(c.used() & pages_below(p0 + lane_first, in_use));
+  }
   const int64_t moves = in_use - block_sum(below, lds);
   const int64_t first = mine + (int64_t)threadIdx.x * kMovePages;
   int32_t c[kMovePages];
@@ -474,9 +534,9 @@ extern "C" int mcop_kv_cache_copy_pages(const mcop_kv_pages* tensors, int64_t nu
       const mcop_kv_pages& t = tensors[i0 + i];
       a.t[i] = CopyTensor{static_cast<uint8_t*>(t.base), t.page_stride, t.page_bytes};
       a.first[i] = (uint32_t)blocks;
-      const int64_t units = (t.page_bytes + 15) / 16;
+      const int64_t units = t.page_bytes / 16;
       const int64_t per = units >= kUnits ? (units + kUnits - 1) / kUnits : 1;
-      const int64_t pages = units >= kUnits ? 1 : kUnits / units;
+      const int64_t pages = units >= kUnits ? 1 : kUnits / ((t.page_bytes + 15) / 16);
       const int64_t groups = (num_pairs + pages - 1) / pages;
       if (per > kMostCount || groups > kMostCount / per || blocks + groups * per >= kMostCount) {
         return set_error(MCOP_E_UNSUPPORTED, "%s: more bytes than one launch takes", name);
