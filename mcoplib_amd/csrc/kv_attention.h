@@ -23,6 +23,7 @@
 
 #include "kv_side.h"
 #include "rowkern.h"
+#include "wave_scan.h"
 
 namespace mcop {
 
@@ -76,19 +77,6 @@ __device__ __forceinline__ uint32_t att_tiles(const AttArgs& a, int n) {
   return ((uint32_t)n + kAttTile - 1) / kAttTile - (uint32_t)att_first(a, n) / kAttTile;
 }
 
-// Inclusive sums over the wave's lanes, by register moves: within rows of 16, then across them.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // row_shr:1
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row_bcast:15
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // row_bcast:31
-  return v;
-}
-__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(v), 63);
-}
 // Walks the sequences of share `share`; a wave works together, 64 sequences at a time.
 struct AttWalk {
   const AttArgs& a;

@@ -17,6 +17,7 @@
 #include "../../include/mcop_norm.h"
 #include "launch_trace.h"
 #include "rowkern.h"
+#include "wave_scan.h"
 
 namespace mcop {
 
@@ -132,27 +133,22 @@ __device__ __forceinline__ bool len_ok(const Pool& p, int64_t n) {
   return n >= 0 && n <= (int64_t)p.columns * p.page_size;
 }
 
-// Exclusive sum over a workgroup of up to 1024 threads; *all: the whole.  The barriers let `lds` (one value a
-// wave) be used again at once.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* lds, int64_t* all) {
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, waves = (int)blockDim.x >> 6;
-  int64_t s = v;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t o = __shfl_up((long long)s, d, 64);
-    if (lane >= d) s += o;
-  }
-  if (lane == 63) lds[wave] = s;
+// Exclusive sum over a workgroup of 1024 threads, of values up to 2^31 - 1, where it stops; *all: the whole.
+// The barriers let `lds` be used again at once.
+constexpr int kScanLanes = 1024, kScanWaves = kScanLanes / 64;
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* lds, uint32_t* all) {
+  const ScanAddUpTo31 op;
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const uint32_t upto = wave_scan<ScanAddUpTo31>(v);
+  uint32_t before = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)upto, 0x138, 0xf, 0xf, false);  // wave_shr:1
+  if (lane == 63) lds[wave] = upto;
   __syncthreads();
-  int64_t before = 0, total = 0;
-  for (int w = 0; w < waves; ++w) {
-    const int64_t x = lds[w];
-    if (w < wave) before += x;
-    total += x;
-  }
+  // every wave sums the waves for itself
+  const uint32_t sums = wave_scan<ScanAddUpTo31>(lane < kScanWaves ? lds[lane] : 0);
   __syncthreads();
-  *all = total;
-  return before + s - v;
+  *all = (uint32_t)__builtin_amdgcn_readlane((int)sums, kScanWaves - 1);
+  const uint32_t earlier = (uint32_t)__builtin_amdgcn_readlane((int)sums, wave > 0 ? wave - 1 : 0);
+  return op(before, wave > 0 ? earlier : 0);
 }
 
 // What a request is: a fork of one sequence into another, or new tokens for one.
@@ -191,7 +187,7 @@ struct Taken {
       : found(static_cast<int32_t*>(ws)), begin(found + 4), list(begin + requests) {}
 };
 
-constexpr int kScanLanes = 1024, kScanPages = 16;  // pages a lane at a time
+constexpr int kScanPages = 16;  // pages a lane at a time
 
 // The counts of sixteen pages from `first` on, and which of them are in use.
 struct PageCounts {
@@ -222,25 +218,26 @@ __device__ __forceinline__ uint32_t pages_below(int64_t first, int64_t end) {
 template <bool FORK>
 __global__ void __launch_bounds__(kScanLanes)
 k_kv_pages_take(Pool p, Requests r, Taken t) {
-  __shared__ int64_t lds[kScanLanes / 64];
+  __shared__ uint32_t lds[kScanWaves];
   // the first counts are on their way while the requests are read
   const int64_t lane_first = (int64_t)threadIdx.x * kScanPages;
   PageCounts c;
   c.load(p.counts, lane_first, p.pages);
-  int64_t asked = 0, all;
+  const ScanAddUpTo31 add;  // no pool has 2^31 pages: what is past that is not there
+  uint32_t asked = 0, all;
   for (int i0 = 0; i0 < r.count; i0 += kScanLanes) {
     const int i = i0 + (int)threadIdx.x;
-    const int64_t need = i < r.count ? request_of<FORK>(p, r, i).need : 0;
-    const int64_t begin = asked + block_scan(need, lds, &all);
-    if (i < r.count) t.begin[i] = (int32_t)min(begin, (int64_t)INT32_MAX);
-    asked += all;
+    const uint32_t need = i < r.count ? (uint32_t)request_of<FORK>(p, r, i).need : 0;
+    const uint32_t begin = add(asked, block_scan(need, lds, &all));
+    if (i < r.count) t.begin[i] = (int32_t)begin;
+    asked = add(asked, all);
   }
-  int64_t found = 0;
+  uint32_t found = 0;
   for (int64_t p0 = 0; p0 < p.pages && found < asked; p0 += kScanLanes * kScanPages) {
     const int64_t first = p0 + lane_first;
     if (p0 > 0) c.load(p.counts, first, p.pages);
     uint32_t free = ~c.used() & pages_below(first, p.pages);
-    int64_t at = found + block_scan((int64_t)__builtin_popcount(free), lds, &all);
+    uint32_t at = found + block_scan((uint32_t)__builtin_popcount(free), lds, &all);
     while (free != 0 && at < asked) {
       t.list[at++] = (int32_t)(first + __builtin_ctz(free));
       free &= free - 1;
@@ -349,26 +346,20 @@ k_kv_pages_free(Pool p, const int32_t* sequences) {
 // ---- Compaction: U pages are in use.  Those at U and above go to the free ones below it, the highest to the
 // lowest: a page in use with b in use before it is the (U - 1 - b)-th from the end, a free page f with b in use
 // before it the (f - b)-th hole.
-constexpr int kMoveLanes = 1024, kMovePages = 4;  // pages a lane
-
-__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* lds) {
-  int64_t all;
-  block_scan(v, lds, &all);
-  return all;
-}
+constexpr int kMoveLanes = kScanLanes, kMovePages = 4;  // pages a lane
 
 // A workgroup 4096 pages.  Each counts the whole pool for itself (twice: all, and those below U; the first
 // 65536 pages stay in registers): 8192 pages are 32 KiB from L2, where another launch would take longer.
 __global__ void __launch_bounds__(kMoveLanes)
 k_kv_pages_moves(const int32_t* __restrict__ counts, int64_t pages, int32_t* src, int32_t* dst,
                  int32_t* used, int32_t* moved) {
-  __shared__ int64_t lds[kMoveLanes / 64];
+  __shared__ uint32_t lds[kScanWaves];
   constexpr int kKept = 4;
   constexpr int64_t kRound = kMoveLanes * kScanPages;
   const int64_t mine = (int64_t)blockIdx.x * (kMoveLanes * kMovePages), half = pages / 2;
   const int64_t lane_first = (int64_t)threadIdx.x * kScanPages;
   uint32_t kept[kKept];
-  int64_t sums = 0;  // in use before this workgroup's pages; in the high half all in use
+  uint32_t in_use = 0, before = 0;  // before this workgroup's pages
 #pragma unroll
   for (int r = 0; r < kKept; ++r) {
     kept[r] = 0;
@@ -376,19 +367,20 @@ k_kv_pages_moves(const int32_t* __restrict__ counts, int64_t pages, int32_t* src
     PageCounts c;
     c.load(counts, r * kRound + lane_first, pages);
     kept[r] = c.used();
-    const int64_t n = __builtin_popcount(kept[r]);
-    sums += n << 32 | (r * kRound + lane_first < mine ? n : 0);
+    const uint32_t n = (uint32_t)__builtin_popcount(kept[r]);
+    in_use += n;
+    if (r * kRound + lane_first < mine) before += n;
   }
   for (int64_t p0 = kKept * kRound; p0 < pages; p0 += kRound) {
     PageCounts c;
     c.load(counts, p0 + lane_first, pages);
-    const int64_t n = __builtin_popcount(c.used());
-    sums += n << 32 | (p0 + lane_first < mine ? n : 0);
+    const uint32_t n = (uint32_t)__builtin_popcount(c.used());
+    in_use += n;
+    if (p0 + lane_first < mine) before += n;
   }
-  sums = block_sum(sums, lds);
-  const int64_t in_use = sums >> 32;
-  int64_t before = sums & 0xffffffff;
-  int64_t below = 0;
+  block_scan(in_use, lds, &in_use);
+  block_scan(before, lds, &before);
+  uint32_t below = 0;
 #pragma unroll
   for (int r = 0; r < kKept; ++r) {
     below += __builtin_popcount(kept[r] & pages_below(r * kRound + lane_first, in_use));
@@ -398,10 +390,11 @@ k_kv_pages_moves(const int32_t* __restrict__ counts, int64_t pages, int32_t* src
     c.load(counts, p0 + lane_first, pages);
     below += __builtin_popcount(c.used() & pages_below(p0 + lane_first, in_use));
   }
-  const int64_t moves = in_use - block_sum(below, lds);
+  block_scan(below, lds, &below);
+  const int64_t moves = in_use - below;
   const int64_t first = mine + (int64_t)threadIdx.x * kMovePages;
   int32_t c[kMovePages];
-  int64_t here = 0, all;
+  uint32_t here = 0, all;
 #pragma unroll
   for (int k = 0; k < kMovePages; ++k) {
     c[k] = first + k < pages ? counts[first + k] : 0;
@@ -415,7 +408,7 @@ k_kv_pages_moves(const int32_t* __restrict__ counts, int64_t pages, int32_t* src
     int64_t rank = -1;
     if (c[k] > 0) {
       if (p >= in_use) {
-        rank = in_use - 1 - before;
+        rank = (int64_t)in_use - 1 - before;
         src[rank] = (int32_t)p;
       }
       ++before;
