@@ -194,37 +194,44 @@ struct AttWave {
   const AttArgs& a;
   const int lane, c, g;
   int first, end;
+  Pack<typename E::S, 8> raw[KP][2];  // the queries as they were loaded
   bf16x8 q[KP][2][TQ];
   f32x4 o[VD];
   float m, l;
   int unit;
 
   __device__ __forceinline__ AttWave(const AttArgs& args, const AttChunk& chunk, int head0, int rows)
-      : a(args), lane((int)threadIdx.x & 63), c(lane & 15), g(lane >> 4), first(chunk.first),
-        end(chunk.end) {
+      : a(args), lane((int)threadIdx.x & 63), c(lane & 15), g(lane >> 4),
+        first(__builtin_amdgcn_readfirstlane(chunk.first)),
+        end(__builtin_amdgcn_readfirstlane(chunk.end)) {
     const typename E::S* src = static_cast<const typename E::S*>(a.key.plain) +
                                chunk.sequence * a.key.p_token +
                                (head0 + min(c, rows - 1)) * a.key.p_head;
-    Pack<typename E::S, 8> x[KP][2];
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) x[kp][j] = load8<typename E::S, true, false>(src + key_at(kp) + j * 8);
+      for (int j = 0; j < 2; ++j) raw[kp][j] = load8<typename E::S, true, false>(src + key_at(kp) + j * 8);
     }
-    // the loads as they are, before what the elements' conditions would make of them
+  }
+  // Waits for the queries as they were loaded, before what the elements' conditions would make of the loads.
+  __device__ __forceinline__ void settle() {
+    constexpr int W = sizeof(raw[0][0]) / 4;
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        constexpr int W = sizeof(x[0][0]) / 4;
-        Pack<uint32_t, W> w = __builtin_bit_cast(Pack<uint32_t, W>, x[kp][j]);
+        Pack<uint32_t, W> w = __builtin_bit_cast(Pack<uint32_t, W>, raw[kp][j]);
 #pragma unroll
         for (int i = 0; i < W; ++i) asm volatile("" : "+v"(w.v[i]));
-        x[kp][j] = __builtin_bit_cast(Pack<typename E::S, 8>, w);
+        raw[kp][j] = __builtin_bit_cast(Pack<typename E::S, 8>, w);
       }
     }
+  }
+  // Takes them apart into their terms, and starts with nothing.
+  __device__ __forceinline__ void begin(int rows) {
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
+      if constexpr (VD == 16) __builtin_amdgcn_sched_barrier(0);
       const int nominal = kp * 64 + g * 16, at = key_at(kp);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -234,7 +241,7 @@ struct AttWave {
           float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            f[e] = E::to_f(x[kp][j].v[i * 2 + e]) * (a.scale < 0.0f ? -1.0f : 1.0f);
+            f[e] = E::to_f(raw[kp][j].v[i * 2 + e]) * (a.scale < 0.0f ? -1.0f : 1.0f);
             if (at + j * 8 + i * 2 + e < nominal || c >= rows) f[e] = 0.0f;
           }
 #pragma unroll
@@ -250,6 +257,7 @@ struct AttWave {
     for (int n = 0; n < VD; ++n) o[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     m = -__builtin_inff(), l = 0.0f;
     unit = MX ? 0 : kAttNoUnit;
+    if constexpr (VD == 16) __builtin_amdgcn_sched_barrier(0);
   }
 
   // The first of the lane's sixteen elements of pair kp of a key; of column r's unit of a value.
@@ -266,6 +274,10 @@ struct AttWave {
   }
   template <bool EDGE, class Src>
   __device__ __forceinline__ void tile_of(Src& src, int t) {
+    // The two forms begin differently, and take keys as values of their own: else the compiler puts their
+    // conversions in front of the branch, all at once, which spills the widest kernels.
+    if constexpr (EDGE) asm volatile("; edge" ::: "memory");
+    else asm volatile("; inside" ::: "memory");
     bool live[8];
     if constexpr (EDGE) {
 #pragma unroll
@@ -283,6 +295,8 @@ struct AttWave {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         src.key(h, kp, w[h]);
+#pragma unroll
+        for (int i = 0; i < KW; ++i) asm volatile("" : "+v"(w[h][i]));
         if constexpr (MX) scale[h] = src.key_scale(h, kp);
       }
 #pragma unroll
@@ -428,18 +442,26 @@ struct AttWave {
         a.lse[(int64_t)ch.sequence * a.query_heads + query] = att_lse(m, sum);
       }
     }
+    // one division a row; an element's rounding of its product is 2^-24 of it
+    const float share = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int d = value_at(g * 4 + i);
       if (ch.part >= 0) {
         float* dst = a.parts + ((int64_t)ch.part * a.query_heads + query) * a.value.dim + d;
+        float v[VD];
 #pragma unroll
-        for (int n = 0; n < VD; ++n) dst[n] = o[n][i];
+        for (int n = 0; n < VD; ++n) v[n] = o[n][i];
+        __builtin_memcpy(dst, v, sizeof(v));
       } else {
-        typename E::S* dst = static_cast<typename E::S*>(a.value.plain) +
-                             ch.sequence * a.value.p_token + query * a.value.p_head + d;
+        typename E::S v[VD];
 #pragma unroll
-        for (int n = 0; n < VD; ++n) dst[n] = E::from_f(att_value(o[n][i], sum, unit));
+        for (int n = 0; n < VD; ++n) {
+          const float x = o[n][i] * share;
+          v[n] = E::from_f(MX || unit == 0 ? x : __builtin_ldexpf(x, unit));
+        }
+        __builtin_memcpy(static_cast<typename E::S*>(a.value.plain) + ch.sequence * a.value.p_token +
+                             query * a.value.p_head + d, v, sizeof(v));
       }
     }
   }
@@ -687,11 +709,14 @@ k_kv_attention_lines(AttArgs a) {
         a, w, c, head, lds_bytes + wave * (2 * T::kBytes),
         (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds_bytes +
             wave * (2 * T::kBytes));
+    // queries and pages are on their way together; the queries are taken apart while tiles are
+    if (c.tiles > 0) src.look_up(c.tile);
+    w.settle();
+    if (c.tiles > 0) src.load(c.tile, 0);
+    if (c.tiles > 1) src.load(c.tile + 1, 1);
+    w.begin(rows);
     if (c.tiles > 0) {
       const int last = c.tile + c.tiles - 1;
-      src.look_up(c.tile);
-      src.load(c.tile, 0);
-      if (c.tiles > 1) src.load(c.tile + 1, 1);
       for (int t = c.tile, turn = 0; t <= last; ++t, turn ^= 1) {
         // a tile is taken to registers whole, so that the loads of the one after the next follow at once
         if (t < last) wait_loads<T::kLoads>();
@@ -824,6 +849,8 @@ k_kv_attention_tiles(AttArgs a) {
   while (walk.next(&c)) {
     AttWave<E, FMT, KP, VD> w(a, c, head0, rows);
     RegisterSource<E, FMT, KP, VD> src(a, w, c, head);
+    w.settle();
+    w.begin(rows);
     for (int t = c.tile; t < c.tile + c.tiles; ++t) {
       src.load(t);
       w.tile(src, t);
