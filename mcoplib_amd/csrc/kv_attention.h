@@ -27,9 +27,8 @@
 
 namespace mcop {
 
-constexpr int kAttTile = 32;      // positions of a tile
-constexpr int kAttWaves = 4;      // of a workgroup, which share out a chunk's tiles
-constexpr int kAttLeastTiles = 1; // of a share
+constexpr int kAttTile = 32;  // positions of a tile
+constexpr int kAttWaves = 4;  // of a workgroup
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttArgs {
@@ -97,7 +96,7 @@ struct AttWalk {
       if (i + lane < a.sequences) t += max(att_tiles(a, a.lens[i + lane]), 1u);
     }
     total = wave_total(t);
-    per = max((total - 1) / (uint32_t)a.target + 1, (uint32_t)kAttLeastTiles);
+    per = (total - 1) / (uint32_t)a.target + 1;
     at = share < (uint32_t)a.target ? share * per : total;
     to = min(at + per, total);
     block = 0, splits = 0;
@@ -180,61 +179,6 @@ __device__ __forceinline__ float att_value(float o, float l, int e) {
 }
 __device__ __forceinline__ float att_lse(float m, float l) {
   return l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
-}
-
-// Joins the waves' parts of `rows` query heads from LDS (m, l [kAttWaves][most], e [kAttWaves], o
-// [kAttWaves][most][value.dim]) and writes the outputs of query heads head0.. (or, of a split sequence,
-// its part).
-template <class E>
-__device__ __forceinline__ void att_write(const AttArgs& a, const AttChunk& c, int head0, int rows,
-                                          int most, const float* m, const float* l, const int* e,
-                                          const float* o) {
-  int unit = e[0];
-#pragma unroll
-  for (int w = 1; w < kAttWaves; ++w) unit = max(unit, e[w]);
-  for (int r = 0; r < rows; ++r) {
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int w = 0; w < kAttWaves; ++w) top = __builtin_fmaxf(top, m[w * most + r]);
-    float f[kAttWaves], sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kAttWaves; ++w) {
-      f[w] = att_weight(m[w * most + r], top);
-      sum += l[w * most + r] * f[w];
-      f[w] *= att_power(e[w] - unit);
-    }
-    if (c.missing) sum = __builtin_nanf("");
-    const int head = head0 + r;
-    for (int d = (int)threadIdx.x; d < a.value.dim; d += kAttWaves * 64) {
-      float v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kAttWaves; ++w) v += o[(w * most + r) * a.value.dim + d] * f[w];
-      if (c.part >= 0) {
-        a.parts[((int64_t)c.part * a.query_heads + head) * a.value.dim + d] = v;
-      } else {
-        static_cast<typename E::S*>(a.value.plain)[c.sequence * a.value.p_token +
-                                                   head * a.value.p_head + d] =
-            E::from_f(att_value(v, sum, unit));
-      }
-    }
-    if (threadIdx.x == 0) {
-      if (c.part >= 0) {
-        float* s = a.sums + ((int64_t)c.part * a.query_heads + head) * 4;
-        s[0] = top, s[1] = sum, s[2] = (float)unit;
-      } else if (a.lse != nullptr) {
-        a.lse[(int64_t)c.sequence * a.query_heads + head] = att_lse(top, sum);
-      }
-    }
-  }
-}
-
-// The page of position p, or -1.
-__device__ __forceinline__ int att_page(const AttArgs& a, int sequence, uint32_t p, uint32_t* off) {
-  const uint32_t column = a.by_page.quotient(p);
-  *off = p - column * (uint32_t)a.page_size;
-  if (column >= (uint32_t)a.columns) return -1;
-  const int g = a.table[sequence * a.table_stride + column];
-  return g < 0 || g >= a.pages ? -1 : g;
 }
 
 }  // namespace mcop

@@ -25,6 +25,61 @@ __device__ __forceinline__ float code_value(const uint8_t* v, int d) {
   }
 }
 
+// Joins the waves' parts of `rows` query heads from LDS (m, l [kAttWaves][kAttRows], e [kAttWaves], o
+// [kAttWaves][kAttRows][value.dim]) and writes the outputs of query heads head0.. (or, of a split sequence,
+// its part).
+template <class E>
+__device__ __forceinline__ void att_write(const AttArgs& a, const AttChunk& c, int head0, int rows,
+                                          const float* m, const float* l, const int* e,
+                                          const float* o) {
+  int unit = e[0];
+#pragma unroll
+  for (int w = 1; w < kAttWaves; ++w) unit = max(unit, e[w]);
+  for (int r = 0; r < rows; ++r) {
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < kAttWaves; ++w) top = __builtin_fmaxf(top, m[w * kAttRows + r]);
+    float f[kAttWaves], sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kAttWaves; ++w) {
+      f[w] = att_weight(m[w * kAttRows + r], top);
+      sum += l[w * kAttRows + r] * f[w];
+      f[w] *= att_power(e[w] - unit);
+    }
+    if (c.missing) sum = __builtin_nanf("");
+    const int head = head0 + r;
+    for (int d = (int)threadIdx.x; d < a.value.dim; d += kAttWaves * 64) {
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kAttWaves; ++w) v += o[(w * kAttRows + r) * a.value.dim + d] * f[w];
+      if (c.part >= 0) {
+        a.parts[((int64_t)c.part * a.query_heads + head) * a.value.dim + d] = v;
+      } else {
+        static_cast<typename E::S*>(a.value.plain)[c.sequence * a.value.p_token +
+                                                   head * a.value.p_head + d] =
+            E::from_f(att_value(v, sum, unit));
+      }
+    }
+    if (threadIdx.x == 0) {
+      if (c.part >= 0) {
+        float* s = a.sums + ((int64_t)c.part * a.query_heads + head) * 4;
+        s[0] = top, s[1] = sum, s[2] = (float)unit;
+      } else if (a.lse != nullptr) {
+        a.lse[(int64_t)c.sequence * a.query_heads + head] = att_lse(top, sum);
+      }
+    }
+  }
+}
+
+// The page of position p, or -1.
+__device__ __forceinline__ int att_page(const AttArgs& a, int sequence, uint32_t p, uint32_t* off) {
+  const uint32_t column = a.by_page.quotient(p);
+  *off = p - column * (uint32_t)a.page_size;
+  if (column >= (uint32_t)a.columns) return -1;
+  const int g = a.table[sequence * a.table_stride + column];
+  return g < 0 || g >= a.pages ? -1 : g;
+}
+
 // Vector arithmetic: a wave walks every fourth position, its lanes the elements, and every query head's
 // product is a sum over the wave.  For head sizes that the matrix kernels are not built for.
 template <class E, int FMT, int N>
@@ -135,7 +190,7 @@ k_kv_attention_rows(AttArgs a) {
       }
     }
     __syncthreads();
-    att_write<E>(a, c, head0, rows, kAttRows, ms, ls, es, os);
+    att_write<E>(a, c, head0, rows, ms, ls, es, os);
     __syncthreads();  // LDS is free again
   }
 }
@@ -271,7 +326,7 @@ bool whole_lines(const AttArgs& a, int fmt) {
       return false;
     }
   }
-  return a.page_size % 16 == 0;
+  return a.page_size % (kAttTile / 2) == 0;
 }
 
 template <class E, int FMT>
@@ -293,13 +348,12 @@ int launch_of(const char* name, AttArgs a, mcop_dtype dtype, hipStream_t st) {
   const int packed = FMT == KV_MXFP4 ? 32 : 16;
   a.k_chunks = Divisor((uint32_t)std::max(1, a.key.dim / packed));
   a.v_chunks = Divisor((uint32_t)std::max(1, a.value.dim / packed));
-  const size_t lds =
-      sizeof(float) * kAttWaves *
-      (shape >= 0 ? 0
-                  : 2 * kAttRows + 1 + (size_t)kAttRows * a.value.dim);
+  // of the vector kernel: maximum, sum and outputs of each row, the outputs' unit
+  const size_t lds = sizeof(float) * kAttWaves * (kAttRows * (2 + (size_t)a.value.dim) + 1);
   trace_launch(name, "sequences=%d heads=%d of %d head sizes %d and %d: %s kernel, wgs=%lld, %d "
                "shares%s", a.sequences, a.heads, a.query_heads, a.key.dim, a.value.dim,
-               lines ? "matrix, through LDS," : shape >= 0 ? "matrix" : "vector", (long long)blocks, a.target, joins ? "" : ", none split");
+               lines ? "matrix, through LDS," : shape >= 0 ? "matrix" : "vector", (long long)blocks,
+               a.target, joins ? "" : ", none split");
   const dim3 grid((unsigned)blocks), block(kAttWaves * 64);
   if (shape >= 0) {
     int rc;

@@ -27,15 +27,11 @@ namespace mcop {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// Workgroups a CU that a kernel's registers are held to: two where that spills none of them.
+// Workgroups a CU that a kernel's registers are held to: two, where that spills none of them (16 x 131072
+// positions of 8 x 192 and 128 mxfp4: 48 us with two, 52 with one).
 template <class E, int FMT, int KP, int VD, bool LINES>
 constexpr int kResident =
-    VD == 4 ? 2
-    : VD == 16 ? 1
-    : LINES ? (std::is_same_v<E, F32> ? 1
-               : KP == 2              ? (FMT != KV_INT8 || std::is_same_v<E, BF16> ? 2 : 1)
-                                      : (FMT == KV_MXFP4 || (FMT == KV_FP8 && std::is_same_v<E, BF16>) ? 2 : 1))
-            : (KP == 2 || FMT == KV_MXFP4 || (FMT == KV_FP8 && !std::is_same_v<E, F32>) ? 2 : 1);
+    VD == 16 || (LINES && KP == 3 && FMT != KV_MXFP4 && std::is_same_v<E, F32>) ? 1 : 2;
 
 constexpr int kTileRows = 16;    // query heads of a wave
 constexpr float kAttSlack = 8.0f;  // weights are at most 2^8
@@ -712,6 +708,7 @@ k_kv_attention_lines(AttArgs a) {
     // queries and pages are on their way together; the queries are taken apart while tiles are
     if (c.tiles > 0) src.look_up(c.tile);
     w.settle();
+    wait_lds();  // of the segment before: nothing of it is in flight when its buffers are filled again
     if (c.tiles > 0) src.load(c.tile, 0);
     if (c.tiles > 1) src.load(c.tile + 1, 1);
     w.begin(rows);
@@ -744,6 +741,7 @@ struct RegisterSource {
   const void *ks_base, *vs_base;
   int v_at;
   uint32_t k_sel[KP], v_sel;
+  int base, found;  // columns [base, base + 64) of the table's row: lane i knows the page of base + i
   bool missing;
   uint32_t k[2][KP][W::KW], v[W::LATE ? 1 : 8][W::VW], kb[2], vb[2];
   int64_t v_from;          // of position lane % 32
@@ -768,14 +766,20 @@ struct RegisterSource {
     missing = false;
   }
 
+  __device__ __forceinline__ void look_up(uint32_t column) {
+    base = __builtin_amdgcn_readfirstlane((int)column);
+    found = row[min(base + wave.lane, (int)a.by_page.quotient((uint32_t)wave.end - 1))];
+    if (found >= a.pages) found = -1;
+  }
+
   // Loads tile t; positions before the first or behind the last stand for those.
   __device__ __forceinline__ void load(int t) {
     const int p = min(max(t * kAttTile + (wave.lane & 31), wave.first), wave.end - 1);
     const uint32_t column = a.by_page.quotient((uint32_t)p);
-    const int found = row[column];
-    const bool none = found < 0 || found >= a.pages;
-    missing |= __builtin_amdgcn_ballot_w64(none) != 0;
-    const int64_t page = none ? 0 : found, off = (uint32_t)p - column * (uint32_t)a.page_size;
+    if (__builtin_amdgcn_readlane((int)column, 31) >= base + 64) look_up(column);
+    const int g = (int)from_lane((uint32_t)found, (int)column - base);
+    missing |= __builtin_amdgcn_ballot_w64(g < 0) != 0;
+    const int64_t page = max(g, 0), off = (uint32_t)p - column * (uint32_t)a.page_size;
     const int64_t ko = page * a.key.c_page + off * a.key.c_token;
     const int64_t vo = page * a.value.c_page + off * a.value.c_token;
     const int64_t kso = page * a.key.s_page + off * a.key.s_token;
@@ -849,6 +853,8 @@ k_kv_attention_tiles(AttArgs a) {
   while (walk.next(&c)) {
     AttWave<E, FMT, KP, VD> w(a, c, head0, rows);
     RegisterSource<E, FMT, KP, VD> src(a, w, c, head);
+    // queries and pages are on their way together
+    if (c.tiles > 0) src.look_up(a.by_page.quotient((uint32_t)max(c.tile * kAttTile, c.first)));
     w.settle();
     w.begin(rows);
     for (int t = c.tile; t < c.tile + c.tiles; ++t) {
