@@ -159,7 +159,7 @@ __device__ __forceinline__ void att_place(const AttArgs& a, uint32_t i, uint32_t
   *block = (int)(inner - (uint32_t)*head * (uint32_t)a.row_blocks);
 }
 
-// 2^(m - top), 1 where both are -inf.
+// 2^(m - top), 0 where both are -inf.
 __device__ __forceinline__ float att_weight(float m, float top) {
   return __builtin_amdgcn_exp2f(m - (top == -__builtin_inff() ? 0.0f : top));
 }

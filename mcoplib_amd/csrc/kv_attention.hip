@@ -195,86 +195,115 @@ k_kv_attention_rows(AttArgs a) {
   }
 }
 
-// Joins the parts of split sequence blockIdx.y of the plan, a query head a workgroup: a group of 32 lanes
-// takes every eighth part, four elements a lane, with maximum and sum of its own, and the groups are
-// joined in LDS.
-constexpr int kJoinLanes = 32, kJoinGroups = 8;
+// Joins the parts of split sequence blockIdx.y of the plan, a query head in WAVES waves, each with every
+// WAVES-th part.  Lane i knows maximum, sum and unit of part i, all of a wave's at once, and what its weights
+// become; then the parts' elements are added up, four a lane and of kJoinBatch parts on their way together
+// (vectors of up to 128 elements: each half of the wave every second part).  The code is kept short: it is
+// fetched from memory after a kernel whose reads have passed through the whole L2.
+constexpr int kJoinWaves = 4, kJoinBatch = 4;  // waves of a workgroup; parts that a wave has on their way
 
-template <class E>
-__global__ void __launch_bounds__(kJoinLanes * kJoinGroups)
+template <class E, int WAVES>
+__global__ void __launch_bounds__(kJoinWaves * 64)
 k_kv_attention_join(AttArgs a) {
-  __shared__ float ms[kJoinGroups], ls[kJoinGroups], os[kJoinGroups][kJoinLanes * 4];
-  __shared__ int es[kJoinGroups];
   // all of the plan at once, also where it says that there is no such entry
   const int32_t* plan = a.plan + 2 + 3 * blockIdx.y;
   const int splits = a.plan[0], sequence = plan[0];
   const uint32_t per = (uint32_t)a.plan[1], begin = (uint32_t)plan[1], end = (uint32_t)plan[2];
   if ((int)blockIdx.y >= splits) return;
-  const int share = (int)(begin / per), count = (int)((end - 1) / per) - share + 1;
-  const int head = (int)blockIdx.x, lane = (int)threadIdx.x & (kJoinLanes - 1),
-            g = (int)threadIdx.x / kJoinLanes, dim = a.value.dim;
-  typename E::S* out = static_cast<typename E::S*>(a.value.plain) + sequence * a.value.p_token +
-                       head * a.value.p_head;
-  for (int d0 = 0; d0 < dim; d0 += kJoinLanes * 4) {
-    // the last four overlap those before them where there are not four more
-    const int d = min(d0 + lane * 4, max(dim - 4, 0));
-    float m = -__builtin_inff(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    int unit = -252;  // below any part's
-#pragma unroll 4
-    for (int i = g; i < count; i += kJoinGroups) {
-      // the first share's part is its second one where the share begins with another sequence
-      const int part = 2 * (share + i) + (i == 0 && begin > (uint32_t)share * per ? 1 : 0);
-      const int64_t row = (int64_t)part * a.query_heads + head;
-      const Pack<float, 4> s = ld<float, 4>(a.sums + row * 4);
-      const float mi = s.v[0], li = s.v[1];
-      const int ei = (int)s.v[2];
-      const float* src = a.parts + row * dim;
-      float v[4];
-      if (dim >= 4) {
-        __builtin_memcpy(v, src + d, sizeof(v));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = src[min(e, dim - 1)];
-      }
-      const float top = __builtin_fmaxf(m, mi);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  const int head = (int)blockIdx.x * (kJoinWaves / WAVES) + (WAVES == 1 ? wave : 0);
+  if (WAVES == 1 && head >= a.query_heads) return;
+  const int share = (int)(begin / per), count = (int)((end - 1) / per) - share + 1, dim = a.value.dim;
+  // the first share's part is its second one where the share begins with another sequence
+  const int shift = begin > (uint32_t)share * per ? 1 : 0;
+  auto row_of = [&](int i) {
+    return (int64_t)(2 * (share + i) + (i == 0 ? shift : 0)) * a.query_heads + head;
+  };
+  auto larger = [](float x, float y) { return __builtin_fmaxf(x, y); };
+  auto sum_of = [](float x, float y) { return x + y; };
+  const int by = WAVES == 1 ? 1 : WAVES, from = WAVES == 1 ? 0 : wave;
+  const int mine = (count - from + by - 1) / by;  // parts from, from + by, ...
+  const bool halves = dim <= 128;
+  const int step = halves ? 2 : 1, half = halves ? lane >> 5 : 0;
+  for (int d0 = 0; d0 < dim; d0 += 256) {
+    // the last four overlap those before them where there are not four more; of less than four the rest is
+    // what lies behind them in the workspace, and is not written
+    const int d = min(d0 + (halves ? lane & 31 : lane) * 4, max(dim - 4, 0));
+    float m = -__builtin_inff(), l = 0.0f, unit = -252.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j0 = 0; j0 < mine; j0 += 64) {
+      const bool is = j0 + lane < mine;
+      const Pack<float, 4> s = ld<float, 4>(a.sums + row_of(from + by * min(j0 + lane, mine - 1)) * 4);
+      const float mi = is ? s.v[0] : -__builtin_inff(), ui = is ? s.v[2] : -252.0f;
+      const float top = larger(m, wave_reduce(mi, larger)), high = larger(unit, wave_reduce(ui, larger));
       const float keep = att_weight(m, top), w = att_weight(mi, top);
-      m = top;
-      l = l * keep + li * w;
-      const int high = max(unit, ei);
-      const float keep_o = keep * att_power(unit - high), w_o = w * att_power(ei - high);
-      unit = high;
+      l = l * keep + wave_reduce(is ? s.v[1] * w : 0.0f, sum_of);
+      const float keep_o = keep * att_power((int)(unit - high));
+      const float f = is ? w * att_power((int)(ui - high)) : 0.0f;
+      m = top, unit = high;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = o[e] * keep_o + v[e] * w_o;
-    }
-    if (lane == 0) ms[g] = m, ls[g] = l, es[g] = unit;
+      for (int e = 0; e < 4; ++e) o[e] *= keep_o;
+      const int n = min(mine - j0, 64);
+      for (int j = 0; j < n; j += kJoinBatch * step) {
+        Pack<float, 4> v[kJoinBatch];
+        float g[kJoinBatch];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) os[g][lane * 4 + e] = o[e];
-    __syncthreads();
-    float top = -__builtin_inff(), sum = 0.0f;
-    int high = -252;
+        for (int b = 0; b < kJoinBatch; ++b) {
+          const int x = j + b * step + half;
+          const float* src = a.parts + row_of(from + by * (j0 + min(x, n - 1))) * dim + d;
+          __builtin_memcpy(v[b].v, src, sizeof(v[b].v));
+          g[b] = from_lane_f(f, x & 63);
+          // behind the last: that one once more, without weight
+          if (x >= n) g[b] = 0.0f, v[b] = {};
+        }
 #pragma unroll
-    for (int i = 0; i < kJoinGroups; ++i) {
-      top = __builtin_fmaxf(top, ms[i]);
-      high = max(high, es[i]);
-    }
-    float f[kJoinGroups];
+        for (int b = 0; b < kJoinBatch; ++b) {
 #pragma unroll
-    for (int i = 0; i < kJoinGroups; ++i) {
-      f[i] = att_weight(ms[i], top);
-      sum += ls[i] * f[i];
-      f[i] *= att_power(es[i] - high);
+          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(v[b].v[e], g[b], o[e]);
+        }
+      }
     }
-    const int x = (int)threadIdx.x, at = min(d0 + (x & ~3), max(dim - 4, 0)) + (x & 3);
-    if (x < kJoinLanes * 4 && d0 + (x & ~3) < dim && at < dim) {
-      float v = 0.0f;
+    if (halves) {
 #pragma unroll
-      for (int i = 0; i < kJoinGroups; ++i) v += os[i][x] * f[i];
-      out[at] = E::from_f(att_value(v, sum, high));
+      for (int e = 0; e < 4; ++e) {
+        float x, y;
+        swap_halves(o[e], &x, &y);
+        o[e] = x + y;
+      }
     }
-    if (a.lse != nullptr && d0 == 0 && threadIdx.x == 0) {
-      a.lse[(int64_t)sequence * a.query_heads + head] = att_lse(top, sum);
+    if constexpr (WAVES > 1) {
+      __shared__ float sums[WAVES][3];
+      __shared__ Pack<float, 4> os[WAVES][64];
+      if (lane == 0) sums[wave][0] = m, sums[wave][1] = l, sums[wave][2] = unit;
+      os[wave][lane] = Pack<float, 4>{o[0], o[1], o[2], o[3]};
+      __syncthreads();
+      m = -__builtin_inff(), unit = -252.0f, l = 0.0f;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) m = larger(m, sums[i][0]), unit = larger(unit, sums[i][2]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) {
+        const float w = att_weight(sums[i][0], m), f = w * att_power((int)(sums[i][2] - unit));
+        l += sums[i][1] * w;
+        const Pack<float, 4> v = os[i][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += v.v[e] * f;
+      }
+      __syncthreads();
+      if (wave > 0) continue;
     }
-    __syncthreads();
+    typename E::S* out = static_cast<typename E::S*>(a.value.plain) + sequence * a.value.p_token +
+                         head * a.value.p_head + d;
+    const float part = l == 0.0f ? 0.0f : 1.0f / l;
+    if (half == 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (e < dim) out[e] = E::from_f(__builtin_ldexpf(o[e] * part, (int)unit));
+      }
+    }
+    if (a.lse != nullptr && d0 == 0 && lane == 0) {
+      a.lse[(int64_t)sequence * a.query_heads + head] = att_lse(m, l);
+    }
   }
 }
 
@@ -368,9 +397,17 @@ int launch_of(const char* name, AttArgs a, mcop_dtype dtype, hipStream_t st) {
   }
   if (int rc = check_launch(name)) return rc;
   if (!joins) return MCOP_OK;
-  // each cut between two shares splits one sequence
-  const dim3 pairs((unsigned)a.query_heads, (unsigned)std::min(a.sequences, a.target - 1));
-  hipLaunchKernelGGL((k_kv_attention_join<E>), pairs, dim3(kJoinLanes * kJoinGroups), 0, st, a);
+  // each cut between two shares splits one sequence; a query head in one wave while an even split has no
+  // more parts than two of its batches
+  const dim3 lanes(kJoinWaves * 64);
+  const unsigned splits = (unsigned)std::min(a.sequences, a.target - 1);
+  if (a.target / a.sequences < 2 * kJoinBatch) {
+    const dim3 grid((unsigned)((a.query_heads + kJoinWaves - 1) / kJoinWaves), splits);
+    hipLaunchKernelGGL((k_kv_attention_join<E, 1>), grid, lanes, 0, st, a);
+  } else {
+    hipLaunchKernelGGL((k_kv_attention_join<E, kJoinWaves>), dim3((unsigned)a.query_heads, splits), lanes, 0,
+                       st, a);
+  }
   return check_launch(name);
 }
 

@@ -129,14 +129,29 @@ __device__ __forceinline__ float scale_operand(const uint32_t* w, uint32_t selec
   return __builtin_bit_cast(float, __builtin_amdgcn_perm(w[1], w[0], selector) >> 1);
 }
 
-// The larger, the sum over the four lanes of a query head.
+// The larger, the sum over the four lanes of a query head.  The swaps put rows 0 and 2 of a value's four
+// rows of sixteen lanes into one register and rows 1 and 3 into the other; the lower and upper halves.
+__device__ __forceinline__ void swap_rows(float v, float* x, float* y) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  *x = __builtin_bit_cast(float, (uint32_t)r[0]), *y = __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+__device__ __forceinline__ void swap_halves(float v, float* x, float* y) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  *x = __builtin_bit_cast(float, (uint32_t)r[0]), *y = __builtin_bit_cast(float, (uint32_t)r[1]);
+}
 __device__ __forceinline__ float column_max(float v) {
-  v = __builtin_fmaxf(v, __shfl_xor(v, 16, 64));
-  return __builtin_fmaxf(v, __shfl_xor(v, 32, 64));
+  float x, y;
+  swap_rows(v, &x, &y);
+  swap_halves(__builtin_fmaxf(x, y), &x, &y);
+  return __builtin_fmaxf(x, y);
 }
 __device__ __forceinline__ float column_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+  float x, y;
+  swap_rows(v, &x, &y);
+  swap_halves(x + y, &x, &y);
+  return x + y;
 }
 
 // 16, 4 bytes, or one as a dword, a lane from its address to LDS at `to` + 16, 4 * lane, which the instruction
