@@ -57,7 +57,7 @@ FOUR_WAVE_KERNELS = (
 EXACT_KERNELS = (r"^void mcop::k_(rms_norm_quant|fused_add_rms_norm|rms_norm|rms_norm_smooth_quant|"
                  r"add_rms_norm_quant_padded|per_token_quant|rms_norm_group_quant)<.*, (true|1)>\(")
 # Kernels of the 4-bit operators and the quantized cache that a launch takes by shape alone.
-SHAPE_KERNELS = r"^void mcop::k_(mxfp4_(quant|dequant|mm_rows|mm_tile)|kv_cache_(write|read)(_tokens)?|kv_attention_\w+)<"
+SHAPE_KERNELS = r"^(void )?mcop::k_(mxfp4_(quant|dequant|mm_rows|mm_tile)|kv_cache_(write|read)(_tokens)?|kv_attention_\w+|kv_copy_pages|kv_pages_\w+)[<(]"
 RESOURCES = "resource_usage.json"
 
 

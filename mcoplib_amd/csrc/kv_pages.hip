@@ -6,13 +6,15 @@
 // taken the lowest free one first, in the order of the requests, so that results depend on nothing
 // else.  Bookkeeping is bound by latency: a request's answer needs all requests before it and the counts up to
 // its pages, so one workgroup scans both (a list of the free pages that are asked for, and where each
-// request's begin), and a second launch has a workgroup for every request.  Copies are bound by HBM.
+// request's begin), and writes the requests' rows itself where they are few and short; else a second launch
+// has a workgroup for every request.  Copies are bound by HBM.
 //
 // Every index that comes from a tensor is checked before it is used: one outside the table, the row or the
 // pool is left out.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/mcop_norm.h"
 #include "launch_trace.h"
@@ -135,7 +137,7 @@ __device__ __forceinline__ bool len_ok(const Pool& p, int64_t n) {
 
 // Exclusive sum over a workgroup of 1024 threads, of values up to 2^31 - 1, where it stops; *all: the whole.
 // The barriers let `lds` be used again at once.
-constexpr int kScanLanes = 1024, kScanWaves = kScanLanes / 64;
+constexpr int kScanLanes = 1 << 10, kScanWaves = kScanLanes / 64;
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* lds, uint32_t* all) {
   const ScanAddUpTo31 op;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
@@ -213,11 +215,93 @@ __device__ __forceinline__ uint32_t pages_below(int64_t first, int64_t end) {
   return n <= 0 ? 0u : n >= kScanPages ? 0xffffu : (1u << (int)n) - 1;
 }
 
+// A request's pages, if there are enough; null else.
+__device__ __forceinline__ const int32_t* pages_for(const Taken& t, const Request& q, int i) {
+  const int64_t begin = t.begin[i];
+  return q.need == 0 || begin + q.need <= t.found[0] ? t.list + begin : nullptr;
+}
+
+// What a request's lanes do (of a wave, some waves, or a part of one).
+struct Lanes {
+  int lane, all;
+};
+
+// Fork i: the child's row.
+struct ForkTo {
+  int32_t *src, *dst;
+};
+__device__ __forceinline__ void fork_row(const Pool& p, const Requests& r, const Taken& t, const ForkTo& to,
+                                         int i, Lanes me) {
+  const Request q = request_of<true>(p, r, i);
+  if (!q.ok) {
+    if (me.lane == 0) to.src[i] = to.dst[i] = -1;
+    return;
+  }
+  const int32_t* pages = pages_for(t, q, i);
+  const int32_t* from = p.table + q.from * p.stride;
+  int32_t* row = p.table + q.to * p.stride;
+  for (int c = me.lane; c < p.columns; c += me.all) {
+    int32_t page = -1;
+    if (pages != nullptr && c < q.have) {
+      page = from[c];
+      if (page >= 0 && page < p.pages) atomicAdd(&p.counts[page], 1);
+    } else if (pages != nullptr && c < q.have + q.need) {
+      page = pages[0];
+    }
+    row[c] = page;
+  }
+  if (me.lane == 0) {
+    const bool copies = pages != nullptr && q.need > 0;
+    to.src[i] = copies ? from[q.have] : -1;
+    to.dst[i] = copies ? pages[0] : -1;
+    if (copies) p.counts[pages[0]] = 1;
+    p.lens[q.to] = pages != nullptr ? (int32_t)q.now : 0;
+  }
+}
+
+// Sequence i that grows: its row and slots, and what lane 0 writes as its length when every lane has read the
+// old one (-1: nothing); i == r.count: the slots behind the last.
+struct ExtendTo {
+  int64_t* slots;
+  int64_t tokens;
+  int32_t* starts;
+};
+__device__ __forceinline__ int extend_row(const Pool& p, const Requests& r, const Taken& t,
+                                          const ExtendTo& to, int i, Lanes me) {
+  if (i == r.count) {
+    const int64_t last = max(r.cu[r.count], 0);
+    for (int64_t s = last + me.lane; s < to.tokens; s += me.all) to.slots[s] = -1;
+    return -1;
+  }
+  const Request q = request_of<false>(p, r, i);
+  const int32_t* pages = q.ok ? pages_for(t, q, i) : nullptr;
+  const int64_t first = max(r.cu[i], 0), end = min((int64_t)r.cu[i + 1], to.tokens);
+  int32_t* row = q.ok ? p.table + q.from * p.stride : nullptr;
+  for (int64_t s = first + me.lane; s < end; s += me.all) {
+    int64_t slot = -1;
+    if (pages != nullptr) {
+      const int64_t at = q.old + s - r.cu[i], c = at / p.page_size;
+      const int32_t page = c < q.have ? row[c] : pages[c - q.have];
+      if (page >= 0 && page < p.pages) slot = (int64_t)page * p.page_size + at % p.page_size;
+    }
+    to.slots[s] = slot;
+  }
+  if (pages != nullptr) {
+    for (int64_t k = me.lane; k < q.need; k += me.all) {
+      row[q.have + k] = pages[k];
+      p.counts[pages[k]] = 1;
+    }
+  }
+  if (me.lane == 0) to.starts[i] = pages != nullptr ? (int32_t)q.old : -1;
+  return pages != nullptr ? (int)q.now : -1;
+}
+
 // One workgroup: where each request's pages begin in the order of all, and the lowest free pages, as many as
-// are asked for.
-template <bool FORK>
+// are asked for.  With ALONE also the rows, 2^log_lanes lanes a request, where a second launch would take longer.
+template <class To, bool ALONE>
 __global__ void __launch_bounds__(kScanLanes)
-k_kv_pages_take(Pool p, Requests r, Taken t) {
+k_kv_pages_take(Pool p, Requests r, Taken t, To to, int log_lanes) {
+  constexpr bool FORK = std::is_same_v<To, ForkTo>;
   __shared__ uint32_t lds[kScanWaves];
   // the first counts are on their way while the requests are read
   const int64_t lane_first = (int64_t)threadIdx.x * kScanPages;
@@ -245,82 +329,33 @@ k_kv_pages_take(Pool p, Requests r, Taken t) {
     found += all;
   }
   if (threadIdx.x == 0) t.found[0] = (int32_t)min(found, asked);
-}
-
-// A request's pages, if there are enough; null else.
-__device__ __forceinline__ const int32_t* pages_for(const Taken& t, const Request& q, int i) {
-  const int64_t begin = t.begin[i];
-  return q.need == 0 || begin + q.need <= t.found[0] ? t.list + begin : nullptr;
+  if constexpr (ALONE) {
+    __syncthreads();  // the lists are whole
+    const Lanes me{(int)threadIdx.x & ((1 << log_lanes) - 1), 1 << log_lanes};
+    const int i = (int)threadIdx.x >> log_lanes;
+    if constexpr (FORK) {
+      if (i < r.count) fork_row(p, r, t, to, i, me);
+    } else {
+      const int now = i <= r.count ? extend_row(p, r, t, to, i, me) : -1;
+      __syncthreads();
+      if (now >= 0 && me.lane == 0) p.lens[r.from[i]] = now;
+    }
+  }
 }
 
 constexpr int kRowLanes = 256;
 
-// A workgroup a fork: the child's row.
+// A workgroup a request (an extension's last one: the slots behind the last).
 __global__ void __launch_bounds__(kRowLanes)
-k_kv_pages_fork(Pool p, Requests r, Taken t, int32_t* src, int32_t* dst) {
-  const int i = (int)blockIdx.x;
-  const Request q = request_of<true>(p, r, i);
-  if (!q.ok) {
-    if (threadIdx.x == 0) src[i] = dst[i] = -1;
-    return;
-  }
-  const int32_t* pages = pages_for(t, q, i);
-  const int32_t* from = p.table + q.from * p.stride;
-  int32_t* to = p.table + q.to * p.stride;
-  for (int c = (int)threadIdx.x; c < p.columns; c += kRowLanes) {
-    int32_t page = -1;
-    if (pages != nullptr && c < q.have) {
-      page = from[c];
-      if (page >= 0 && page < p.pages) atomicAdd(&p.counts[page], 1);
-    } else if (pages != nullptr && c < q.have + q.need) {
-      page = pages[0];
-    }
-    to[c] = page;
-  }
-  if (threadIdx.x == 0) {
-    const bool copies = pages != nullptr && q.need > 0;
-    src[i] = copies ? from[q.have] : -1;
-    dst[i] = copies ? pages[0] : -1;
-    if (copies) p.counts[pages[0]] = 1;
-    p.lens[q.to] = pages != nullptr ? (int32_t)q.now : 0;
-  }
+k_kv_pages_fork(Pool p, Requests r, Taken t, ForkTo to) {
+  fork_row(p, r, t, to, (int)blockIdx.x, {(int)threadIdx.x, kRowLanes});
 }
-
-// A workgroup a sequence that grows, and one for the slots behind the last: its row, length and slots.
 __global__ void __launch_bounds__(kRowLanes)
-k_kv_pages_extend(Pool p, Requests r, Taken t, int64_t* slots, int64_t tokens, int32_t* starts) {
-  const int i = (int)blockIdx.x;
-  if (i == r.count) {
-    const int64_t last = max(r.cu[r.count], 0);
-    for (int64_t s = last + (int)threadIdx.x; s < tokens; s += kRowLanes) slots[s] = -1;
-    return;
-  }
-  const Request q = request_of<false>(p, r, i);
-  const int32_t* pages = q.ok ? pages_for(t, q, i) : nullptr;
-  const int64_t first = max(r.cu[i], 0), end = min((int64_t)r.cu[i + 1], tokens);
-  int32_t* row = q.ok ? p.table + q.from * p.stride : nullptr;
-  for (int64_t s = first + (int)threadIdx.x; s < end; s += kRowLanes) {
-    int64_t slot = -1;
-    if (pages != nullptr) {
-      const int64_t at = q.old + s - r.cu[i], c = at / p.page_size;
-      const int32_t page = c < q.have ? row[c] : pages[c - q.have];
-      if (page >= 0 && page < p.pages) slot = (int64_t)page * p.page_size + at % p.page_size;
-    }
-    slots[s] = slot;
-  }
-  if (pages != nullptr) {
-    for (int64_t k = (int)threadIdx.x; k < q.need; k += kRowLanes) {
-      row[q.have + k] = pages[k];
-      p.counts[pages[k]] = 1;
-    }
-  }
-  __syncthreads();  // every lane has read the old length
-  if (threadIdx.x == 0) {
-    starts[i] = pages != nullptr ? (int32_t)q.old : -1;
-    if (pages != nullptr) p.lens[q.from] = (int32_t)q.now;
-  }
+k_kv_pages_extend(Pool p, Requests r, Taken t, ExtendTo to) {
+  const int now = extend_row(p, r, t, to, (int)blockIdx.x, {(int)threadIdx.x, kRowLanes});
+  __syncthreads();
+  if (now >= 0 && threadIdx.x == 0) p.lens[r.from[blockIdx.x]] = now;
 }
-
 // A workgroup a sequence that ends.  Its length is taken away first, so that a sequence that is named twice
 // gives its pages back once.
 __global__ void __launch_bounds__(kRowLanes)
@@ -483,6 +518,17 @@ int workspace_ok(const char* name, const void* ws, int64_t bytes, int64_t reques
   return MCOP_OK;
 }
 
+// Log of the lanes a request where the workgroup that takes the pages writes `requests` rows of at most
+// `elements` too, kAloneSteps a lane; -1: another launch does.  Replayed from a graph, one launch against two:
+// one token for each of 16 sequences 5.3 and 7.0 us, of 60 6.1 and 7.4; four forks of rows of 256 pages 5.3 and
+// 6.5, of 1000 (four steps a lane) 7.3 and 8.2; 16 of 250, also four steps, 7.6 and 7.1.
+constexpr int kAloneSteps = 4;
+int lanes_alone(int64_t requests, int64_t elements) {
+  int log_lanes = 10;
+  while (log_lanes >= 0 && requests << log_lanes > kScanLanes) --log_lanes;
+  return log_lanes >= 0 && elements <= (int64_t)kAloneSteps << log_lanes ? log_lanes : -1;
+}
+
 }  // namespace
 
 }  // namespace mcop
@@ -559,11 +605,18 @@ extern "C" int mcop_kv_cache_fork(const mcop_kv_pool* pool, const int32_t* paren
   const Requests r{parents, children, nullptr, (int)num_forks};
   const Taken t(workspace, (int)num_forks);
   auto st = static_cast<hipStream_t>(stream);
-  trace_launch(name, "%lld forks, %d pages", (long long)num_forks, p.pages);
-  hipLaunchKernelGGL((k_kv_pages_take<true>), dim3(1), dim3(kScanLanes), 0, st, p, r, t);
+  const ForkTo to{src, dst};
+  const int log_lanes = lanes_alone(num_forks, p.columns);
+  trace_launch(name, "%lld forks, %d pages, %s", (long long)num_forks, p.pages,
+               log_lanes >= 0 ? "one launch" : "two launches");
+  if (log_lanes >= 0) {
+    hipLaunchKernelGGL((k_kv_pages_take<ForkTo, true>), dim3(1), dim3(kScanLanes), 0, st, p, r, t, to,
+                       log_lanes);
+    return check_launch(name);
+  }
+  hipLaunchKernelGGL((k_kv_pages_take<ForkTo, false>), dim3(1), dim3(kScanLanes), 0, st, p, r, t, to, 0);
   if (int rc = check_launch(name)) return rc;
-  hipLaunchKernelGGL(k_kv_pages_fork, dim3((unsigned)num_forks), dim3(kRowLanes), 0, st, p, r, t, src,
-                     dst);
+  hipLaunchKernelGGL(k_kv_pages_fork, dim3((unsigned)num_forks), dim3(kRowLanes), 0, st, p, r, t, to);
   return check_launch(name);
 }
 
@@ -585,12 +638,19 @@ extern "C" int mcop_kv_cache_extend(const mcop_kv_pool* pool, const int32_t* seq
   const Requests r{sequences, nullptr, cu_tokens, (int)num_sequences};
   const Taken t(workspace, (int)num_sequences);
   auto st = static_cast<hipStream_t>(stream);
-  trace_launch(name, "%lld sequences, %lld tokens, %d pages", (long long)num_sequences,
-               (long long)num_tokens, p.pages);
-  hipLaunchKernelGGL((k_kv_pages_take<false>), dim3(1), dim3(kScanLanes), 0, st, p, r, t);
+  const ExtendTo to{slots, num_tokens, starts};
+  const int log_lanes = lanes_alone(num_sequences + 1, num_tokens);
+  trace_launch(name, "%lld sequences, %lld tokens, %d pages, %s", (long long)num_sequences,
+               (long long)num_tokens, p.pages, log_lanes >= 0 ? "one launch" : "two launches");
+  if (log_lanes >= 0) {
+    hipLaunchKernelGGL((k_kv_pages_take<ExtendTo, true>), dim3(1), dim3(kScanLanes), 0, st, p, r, t, to,
+                       log_lanes);
+    return check_launch(name);
+  }
+  hipLaunchKernelGGL((k_kv_pages_take<ExtendTo, false>), dim3(1), dim3(kScanLanes), 0, st, p, r, t, to, 0);
   if (int rc = check_launch(name)) return rc;
   hipLaunchKernelGGL(k_kv_pages_extend, dim3((unsigned)num_sequences + 1), dim3(kRowLanes), 0, st, p, r,
-                     t, slots, num_tokens, starts);
+                     t, to);
   return check_launch(name);
 }
 

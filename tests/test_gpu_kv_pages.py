@@ -216,6 +216,30 @@ def test_decreasing_token_counts_grow_nothing():
     assert both.lens.tolist()[:3] == [7, 6, 4]
 
 
+# Few requests of short rows are written by the workgroup that takes their pages, in parts of a wave, waves or
+# several of them; more or longer ones by a launch of their own.
+@pytest.mark.parametrize("forks,columns", [(1, 5), (1, 4096), (1, 4097), (2, 2048), (2, 2049), (3, 1024), (5, 513),
+                                           (16, 256), (17, 128), (17, 129), (64, 64), (100, 32), (1000, 4),
+                                           (1024, 4), (1024, 5), (1025, 4)])
+def test_forks_of_few_and_of_many(forks, columns):
+    lens = [columns * 3, columns * 3 - 2, 1, 0]
+    both = Both(2 * columns + 1 + forks - forks // 3, 4 + forks, columns, 3, lens)  # some get none
+    both.fork([i % 4 for i in range(forks)], [4 + (i * 7 + 3) % forks if forks % 7 else 4 + i
+                                              for i in range(forks)])
+
+
+@pytest.mark.parametrize("sequences,tokens", [(1, 1), (1, 2048), (1, 2049), (2, 1024), (2, 1025), (3, 1025),
+                                              (7, 512), (7, 513), (31, 128), (31, 129), (32, 100), (63, 64),
+                                              (127, 127), (255, 255), (500, 500), (1023, 1023), (1024, 1024)])
+def test_extensions_of_few_and_of_many(sequences, tokens):
+    """All tokens in one sequence, then spread over all; other entries of the table lie behind."""
+    both = Both(3 * sequences + tokens // 3, sequences + 2, tokens // 2 + 3, 4, [i % 6 for i in range(sequences)])
+    order = [(i * 5 + 1) % sequences for i in range(sequences)] if sequences % 5 else list(range(sequences))
+    both.extend(order, [tokens if i == sequences // 2 else 0 for i in range(sequences)])
+    both.extend(order, [tokens // sequences] * sequences, behind=3)
+    both.extend(order, [1] * sequences)
+
+
 @pytest.mark.parametrize("page", [1, 16])
 def test_ends_of_sequences(page):
     both = Both(100, 12, 8, page, [5 * page, 1, 0, 3 * page + 1, 8 * page])
