@@ -16,7 +16,8 @@ Surfaces (same names, argument order and in-place conventions as the reference):
 
 Beyond the reference, in _C and custom_ops: mxfp4_quant, mxfp4_dequant, rms_norm_mxfp4_quant and
 mxfp4_scaled_mm (4-bit microscaled operands), kv_cache_write_quant and kv_cache_read_dequant (a
-paged key/value cache quantized as it is written).
+paged key/value cache quantized as it is written), kv_cache_attention (decode steps over it), and
+kv_cache_copy_pages, kv_cache_fork, kv_cache_extend, kv_cache_free and kv_cache_compact (its pages).
 
 op and _C are C++ (csrc/torch_ops.cpp, built into _torch_ops.so) and custom_ops is Python, as
 in the reference; all of them call libmcop_norm.so (hand-written HIP kernels, C ABI in

@@ -1,7 +1,8 @@
 """``mcoplib.custom_ops`` wrappers of the fused norm/quant path (reference
 mcoplib/custom_ops.py:7-45): allocate the outputs the way the reference does and call the
-``op`` entry point, both in the _torch_ops extension.  The 4-bit operators and the quantized
-key/value cache, which the reference does not have, are here in the same manner."""
+``op`` entry point, both in the _torch_ops extension.  The 4-bit operators, the quantized
+key/value cache, attention over it and its pages, which the reference does not have, are here in the
+same manner."""
 
 from __future__ import annotations
 
