@@ -9,10 +9,16 @@
 //       the second one's operand, whose eight positions a lane are taken in this order
 //   V   those eight positions, VD elements from VD c: its rows for VD products, one element of each
 //   O   query head c, elements VD (4 g + i) + n
-// so codes go from memory to the matrix units in registers: no LDS, no barrier, and a transposition of V
-// that is half an instruction an element (two positions' elements to a dword).  Vectors that are not
-// whole units of 16 (K) or VD (V) elements end in a unit that overlaps the one before: its queries are zero
-// where it repeats elements, and outputs that come twice are the same.
+// so neither the weights nor V change lanes between the products (V's transposition is half an instruction an
+// element: two positions' elements to a dword), and no wave waits for another.  Codes come through LDS, where
+// they are whole lines, or straight to registers.  Vectors that are not whole units of 16 (K) or VD (V)
+// elements end in a unit that overlaps the one before: its queries are zero where it repeats elements, and
+// outputs that come twice are the same.
+//
+// What bounds it: reading the cache, and behind that one wave a SIMD that loads, converts and multiplies in
+// turn.  2 x 131072 positions of 8 x 128 fp8 for 8 query heads each (554 MB) take 109 us with the join, 5.1
+// TB/s, the same reads alone 90-94; 64 ragged sequences of 131072 in all, int8 (279 MB), 71 us; 16 of 4-bit
+// keys of 192 and values of 128 (179 MB), 47 us.  Vector units are 32-38% busy, the matrix units 7-13%.
 //
 // Every code (int8, e4m3, e2m1 with its block's power of two) is a bf16 value.  fp32 scales stay out of
 // the products: a key's multiplies its logit, a value's its weight.  Queries enter as the sum of one bf16

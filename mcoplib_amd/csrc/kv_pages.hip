@@ -48,7 +48,8 @@ __device__ __forceinline__ void store_unit(uint8_t* p, const u32x4& v) {
 }
 
 // Each lane's loads go out together: none hangs on a condition, and a lane that has nothing to move reads what
-// another does (with a condition on each, 400 pages of 32 layers took 200 us).
+// another does (with a condition on each, 400 pages of 32 layers took 200 us; so 167, 5.2 TB/s of what is read and
+// written).  Bound by HBM in both directions.
 __global__ void __launch_bounds__(kCopyLanes, 8) k_kv_copy_pages(CopyArgs a) {
   const int lane = (int)threadIdx.x & 63;
   const bool mine = lane < a.tensors && a.first[lane < a.tensors ? lane : 0] <= blockIdx.x;
@@ -297,7 +298,8 @@ __device__ __forceinline__ int extend_row(const Pool& p, const Requests& r, cons
 }
 
 // One workgroup: where each request's pages begin in the order of all, and the lowest free pages, as many as
-// are asked for.  With ALONE also the rows, 2^log_lanes lanes a request, where a second launch would take longer.
+// are asked for.  With ALONE also the rows, 2^log_lanes lanes a request, where a second launch would take
+// longer (lanes_alone).
 template <class To, bool ALONE>
 __global__ void __launch_bounds__(kScanLanes)
 k_kv_pages_take(Pool p, Requests r, Taken t, To to, int log_lanes) {
@@ -520,8 +522,8 @@ int workspace_ok(const char* name, const void* ws, int64_t bytes, int64_t reques
 
 // Log of the lanes a request where the workgroup that takes the pages writes `requests` rows of at most
 // `elements` too, kAloneSteps a lane; -1: another launch does.  Replayed from a graph, one launch against two:
-// one token for each of 16 sequences 5.3 and 7.0 us, of 60 6.1 and 7.4; four forks of rows of 256 pages 5.3 and
-// 6.5, of 1000 (four steps a lane) 7.3 and 8.2; 16 of 250, also four steps, 7.6 and 7.1.
+// one token for each of 16 sequences 5.3 and 7.0 us, of 60 6.1 and 7.4; four forks of rows of 256 pages 5.3
+// and 6.5, of 1000 (four steps a lane) 7.3 and 8.2; 16 of 250, also four steps, 7.6 and 7.1.
 constexpr int kAloneSteps = 4;
 int lanes_alone(int64_t requests, int64_t elements) {
   int log_lanes = 10;
@@ -690,8 +692,9 @@ extern "C" int mcop_kv_cache_compact(const mcop_kv_pool* pool, int32_t* src, int
   auto st = static_cast<hipStream_t>(stream);
   constexpr int kPages = kMoveLanes * kMovePages;
   trace_launch(name, "%d pages, a table of %d x %d", p.pages, p.rows, p.columns);
-  hipLaunchKernelGGL(k_kv_pages_moves, dim3((unsigned)std::max(1, (int)(((int64_t)p.pages + kPages - 1) / kPages))),
-                     dim3(kMoveLanes), 0, st, p.counts, (int64_t)p.pages, src, dst, used, moved);
+  const unsigned blocks = (unsigned)std::max<int64_t>(1, ((int64_t)p.pages + kPages - 1) / kPages);
+  hipLaunchKernelGGL(k_kv_pages_moves, dim3(blocks), dim3(kMoveLanes), 0, st, p.counts, (int64_t)p.pages, src,
+                     dst, used, moved);
   if (int rc = check_launch(name)) return rc;
   if (threads == 0) return MCOP_OK;
   hipLaunchKernelGGL(k_kv_pages_move, dim3((unsigned)((threads + kRowLanes - 1) / kRowLanes)),
