@@ -35,9 +35,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Workgroups a CU that a kernel's registers are held to: two, where that spills none of them (16 x 131072
 // positions of 8 x 192 and 128 mxfp4: 48 us with two, 52 with one).
-template <class E, int FMT, int KP, int VD, bool LINES>
-constexpr int kResident =
-    VD == 16 || (LINES && KP == 3 && FMT != KV_MXFP4 && std::is_same_v<E, F32>) ? 1 : 2;
+constexpr int att_resident(bool fp32, int fmt, int kp, int vd, bool lines) {
+  return vd == 16 || (lines && kp == 3 && fmt != KV_MXFP4 && fp32) ? 1 : 2;
+}
 
 constexpr int kTileRows = 16;    // query heads of a wave
 constexpr float kAttSlack = 8.0f;  // weights are at most 2^8
@@ -518,6 +518,7 @@ struct LdsTile {  // loads of a half's keys, values and 4-bit blocks' scales; by
   static constexpr int kScales = 1024 * (KN + VN), kHalf = kScales + 256 * (KS + VS);
   static constexpr int kBytes = 2 * kHalf + (MX ? 0 : 256);
   static constexpr int kLoads = 2 * (KN + VN + KS + VS) + (MX ? 0 : 1);
+  static constexpr int kGroup = kAttWaves * 2 * kBytes;  // a workgroup's
 };
 
 template <class E, int FMT, int KP, int VD>
@@ -707,7 +708,7 @@ struct LdsSource {
 };
 
 template <class E, int FMT, int KP, int VD>
-__global__ void __launch_bounds__(kAttWaves * 64, (kResident<E, FMT, KP, VD, true>))
+__global__ void __launch_bounds__(kAttWaves * 64, att_resident(std::is_same_v<E, F32>, FMT, KP, VD, true))
 k_kv_attention_lines(AttArgs a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds_bytes[];  // [waves][2] tiles
   using T = LdsTile<FMT, KP, VD>;
@@ -861,7 +862,7 @@ struct RegisterSource {
 };
 
 template <class E, int FMT, int KP, int VD>
-__global__ void __launch_bounds__(kAttWaves * 64, (kResident<E, FMT, KP, VD, false>))
+__global__ void __launch_bounds__(kAttWaves * 64, att_resident(std::is_same_v<E, F32>, FMT, KP, VD, false))
 k_kv_attention_tiles(AttArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   uint32_t share;
@@ -891,6 +892,11 @@ struct TileShape {
   int kp, vd;
 };
 constexpr TileShape kTileShapes[] = {{1, 4}, {2, 8}, {3, 8}, {4, 16}};
+// Whether a CU holds two workgroups of the kernel through LDS, by registers and LDS.
+template <class E, int FMT, int I>
+constexpr bool kTwoResident =
+    att_resident(std::is_same_v<E, F32>, FMT, kTileShapes[I].kp, kTileShapes[I].vd, true) == 2 &&
+    2 * LdsTile<FMT, kTileShapes[I].kp, kTileShapes[I].vd>::kGroup <= 160 * 1024;
 
 // Launches the kernel of shape `shape` (an index above) on the sequences' chunks.
 int attention_tiles_int8(int shape, bool lines, mcop_dtype dtype, const AttArgs& a, dim3 grid,
@@ -904,8 +910,8 @@ template <int FMT, class E, int KP, int VD>
 void attention_tiles_of(bool lines, const AttArgs& a, dim3 grid, hipStream_t st) {
   const dim3 block(kAttWaves * 64);
   if (lines) {
-    constexpr size_t kLds = (size_t)kAttWaves * 2 * LdsTile<FMT, KP, VD>::kBytes;
-    hipLaunchKernelGGL((k_kv_attention_lines<E, FMT, KP, VD>), grid, block, kLds, st, a);
+    hipLaunchKernelGGL((k_kv_attention_lines<E, FMT, KP, VD>), grid, block, (LdsTile<FMT, KP, VD>::kGroup), st,
+                       a);
   } else {
     hipLaunchKernelGGL((k_kv_attention_tiles<E, FMT, KP, VD>), grid, block, 0, st, a);
   }

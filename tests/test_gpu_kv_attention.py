@@ -116,6 +116,16 @@ def test_split_lengths(lens, dtype, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("sequences", [127, 255, 256, 400])
+def test_more_sequences_than_shares(sequences, dtype, kind):
+    """On both sides of two sequences a share, some of them cut."""
+    say(f"attention {kind} {dtype} {sequences} sequences")
+    lens = [(i * 37) % 90 if i % 50 else 400 for i in range(sequences)]
+    Case(kind, dtype, lens, 8, 2, 96, 128, 16).check()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("window", [1, 2, 31, 32, 33, 100, 128, 129, 5000])
 def test_windows(window, kind):
     """Only the window's positions are read: those before it read as NaN, and have no pages."""
