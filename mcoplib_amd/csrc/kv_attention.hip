@@ -361,18 +361,17 @@ bool whole_lines(const AttArgs& a, int fmt) {
   return a.page_size % (kAttTile / 2) == 0;
 }
 
-// Codes through LDS with eight waves a CU: where two workgroups are resident, and either the tiles are small
-// (64 sequences of 4000 of 8 x 64 fp8: 58 us, 66 with four) or shares have two sequences or more each, whose
-// starts overlap then while few are cut (1024 of 128 of 8 x 128: 65 us and 74; 512 of 100: 37 and 41; with one
-// sequence a share, 128 of 1000, 58 and 49).
-template <class E, int FMT>
-bool two_resident(int shape) {
-  switch (shape) {
-    case 0: return kTwoResident<E, FMT, 0>;
-    case 1: return kTwoResident<E, FMT, 1>;
-    case 2: return kTwoResident<E, FMT, 2>;
-    default: return kTwoResident<E, FMT, 3>;
-  }
+// Codes through LDS with eight waves a CU: where two workgroups are resident, and either tiles are small (64
+// sequences of 4000 of 8 x 64 fp8: 58 us, 66 with four; of 2000 of 8 x 128 4-bit, tiles of 5 KiB: 38 and 45) or
+// shares have two sequences or more each, whose starts overlap then while few are cut (1024 of 128 of 8 x 128
+// fp8: 65 us and 74; 512 of 100 int8: 37 and 41; with one sequence a share, 128 of 1000, 58 and 49).  Keys of 192
+// and values of 128, 4-bit, tiles of 7.5 KiB, run the same with either.
+constexpr int kSmallTile = 6 * 1024;
+template <class E, int FMT, int I = 0>
+bool eight_waves(int shape, bool many) {
+  if (shape == I) return kTwoResident<E, FMT, I> && (many || kTileBytes<FMT, I> <= kSmallTile);
+  if constexpr (I < 3) return eight_waves<E, FMT, I + 1>(shape, many);
+  return false;
 }
 
 template <class E, int FMT>
@@ -382,7 +381,7 @@ int launch_of(const char* name, AttArgs a, mcop_dtype dtype, hipStream_t st) {
   a.target = (int)target_of(kAttShares, a.heads, a.group);
   if (lines) {
     const int four = (int)target_of(kLineShares, a.heads, a.group);
-    if (!two_resident<E, FMT>(shape) || (kTileShapes[shape].vd > 4 && a.sequences < 2 * four)) a.target = four;
+    if (!eight_waves<E, FMT>(shape, a.sequences >= 2 * four)) a.target = four;
   }
   const bool joins = a.target > 1;  // one share splits nothing
   a.row_blocks = (a.group + rows - 1) / rows;

@@ -897,6 +897,8 @@ template <class E, int FMT, int I>
 constexpr bool kTwoResident =
     att_resident(std::is_same_v<E, F32>, FMT, kTileShapes[I].kp, kTileShapes[I].vd, true) == 2 &&
     2 * LdsTile<FMT, kTileShapes[I].kp, kTileShapes[I].vd>::kGroup <= 160 * 1024;
+template <int FMT, int I>
+constexpr int kTileBytes = LdsTile<FMT, kTileShapes[I].kp, kTileShapes[I].vd>::kBytes;
 
 // Launches the kernel of shape `shape` (an index above) on the sequences' chunks.
 int attention_tiles_int8(int shape, bool lines, mcop_dtype dtype, const AttArgs& a, dim3 grid,
