@@ -318,10 +318,13 @@ namespace {
 // Shares: waves for the card over all of a share's key heads and blocks of sixteen query heads.  Codes
 // through LDS: four waves a CU, which have two tiles each in flight (2 x 131072 positions of 8 x 128 fp8: 109
 // us, 113 with eight waves and twice the parts; 48 windows of 1024 of 4 x 256: 37 and 57); else eight (37
-// ragged sequences of 5 x 80 and 96 int8 to fp32: 33 us with four, 28 so).
+// ragged sequences of 5 x 80 and 96 int8 to fp32: 33 us with four, 28 so), while two workgroups are resident (83
+// of 12338 in all, 7 x 129 fp8 to fp32, one workgroup a CU: 40 us with four waves a CU, 49 with eight).
 constexpr int kLineShares = 1024, kAttShares = 2048;
 int64_t target_of(int64_t shares, int64_t heads, int64_t group) {
-  return std::max<int64_t>(1, shares / (heads * ((group + 15) / 16)));
+  const int64_t n = shares / (heads * ((group + 15) / 16));
+  // the same for every die: 68 shares of 15 heads would be 34 workgroups for some dies' 32 CUs
+  return n >= 8 ? n / 8 * 8 : std::max<int64_t>(1, n);
 }
 
 struct Workspace {
@@ -363,9 +366,9 @@ bool whole_lines(const AttArgs& a, int fmt) {
 
 // Codes through LDS with eight waves a CU: where two workgroups are resident, and either tiles are small (64
 // sequences of 4000 of 8 x 64 fp8: 58 us, 66 with four; of 2000 of 8 x 128 4-bit, tiles of 5 KiB: 38 and 45) or
-// shares have two sequences or more each, whose starts overlap then while few are cut (1024 of 128 of 8 x 128
-// fp8: 65 us and 74; 512 of 100 int8: 37 and 41; with one sequence a share, 128 of 1000, 58 and 49).  Keys of 192
-// and values of 128, 4-bit, tiles of 7.5 KiB, run the same with either.
+// shares have three sequences for two or more, whose starts overlap then while few are cut (1024 of 128 of 8 x
+// 128 fp8: 65 us and 74; 512 of 100 int8: 37 and 41; 200 of 333 fp8, 1.6 a share, 36.6 and 38.2; 150 of 600, 1.2,
+// 44 and 42).  Keys of 192 and values of 128, 4-bit, tiles of 7.5 KiB, run the same with either.
 constexpr int kSmallTile = 6 * 1024;
 template <class E, int FMT, int I = 0>
 bool eight_waves(int shape, bool many) {
@@ -379,9 +382,11 @@ int launch_of(const char* name, AttArgs a, mcop_dtype dtype, hipStream_t st) {
   const int shape = tile_shape(a), rows = shape >= 0 ? kTileRows : kAttRows;
   const bool lines = shape >= 0 && whole_lines(a, FMT);
   a.target = (int)target_of(kAttShares, a.heads, a.group);
-  if (lines) {
+  if (shape >= 0) {
     const int four = (int)target_of(kLineShares, a.heads, a.group);
-    if (!eight_waves<E, FMT>(shape, a.sequences >= 2 * four)) a.target = four;
+    if (lines ? !eight_waves<E, FMT>(shape, 2 * a.sequences >= 3 * four) : kTileShapes[shape].vd == 16) {
+      a.target = four;
+    }
   }
   const bool joins = a.target > 1;  // one share splits nothing
   a.row_blocks = (a.group + rows - 1) / rows;
