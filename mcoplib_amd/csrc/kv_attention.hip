@@ -82,8 +82,8 @@ __device__ __forceinline__ int att_page(const AttArgs& a, int sequence, uint32_t
 
 // Vector arithmetic: a wave walks every fourth position, its lanes the elements, and every query head's
 // product is a sum over the wave.  For head sizes that the matrix kernels are not built for; where they are, they
-// are two to twenty times as fast (37 ragged sequences of 5 x 80 and 96 int8 to fp32: 28 us, 199 so; 64 of
-// 8 x 128 int8: 71 and 1477; one of 1000 positions: 11 and 23).  A position's sums over the wave bound it.
+// are two to twenty times as fast (37 ragged sequences of 5 x 80 and 96 int8 to fp32: 25 us, 198 so; 64 of
+// 8 x 128 int8: 66 and 1461; one of 1000 positions: 11 and 23).  A position's sums over the wave bound it.
 template <class E, int FMT, int N>
 __global__ void __launch_bounds__(kAttWaves * 64)
 k_kv_attention_rows(AttArgs a) {
@@ -316,10 +316,10 @@ k_kv_attention_join(AttArgs a) {
 namespace {
 
 // Shares: waves for the card over all of a share's key heads and blocks of sixteen query heads.  Codes
-// through LDS: four waves a CU, which have two tiles each in flight (2 x 131072 positions of 8 x 128 fp8: 109
-// us, 113 with eight waves and twice the parts; 48 windows of 1024 of 4 x 256: 37 and 57); else eight (37
-// ragged sequences of 5 x 80 and 96 int8 to fp32: 33 us with four, 28 so), while two workgroups are resident (83
-// of 12338 in all, 7 x 129 fp8 to fp32, one workgroup a CU: 40 us with four waves a CU, 49 with eight).
+// through LDS: four waves a CU, which have two tiles each in flight (2 x 131072 positions of 8 x 128 fp8: 107
+// us, 115 with eight waves and twice the parts; 48 windows of 1024 of 4 x 256: 35 and 49); else eight (37
+// ragged sequences of 5 x 80 and 96 int8 to fp32: 29 us with four, 25 so), while two workgroups are resident (83
+// of 12338 in all, 7 x 129 fp8 to fp32, one workgroup a CU: 36 us with four waves a CU, 48 with eight).
 constexpr int kLineShares = 1024, kAttShares = 2048;
 int64_t target_of(int64_t shares, int64_t heads, int64_t group) {
   const int64_t n = shares / (heads * ((group + 15) / 16));
@@ -365,10 +365,10 @@ bool whole_lines(const AttArgs& a, int fmt) {
 }
 
 // Codes through LDS with eight waves a CU: where two workgroups are resident, and either tiles are small (64
-// sequences of 4000 of 8 x 64 fp8: 58 us, 66 with four; of 2000 of 8 x 128 4-bit, tiles of 5 KiB: 38 and 45) or
-// shares have three sequences for two or more, whose starts overlap then while few are cut (1024 of 128 of 8 x
-// 128 fp8: 65 us and 74; 512 of 100 int8: 37 and 41; 200 of 333 fp8, 1.6 a share, 36.6 and 38.2; 150 of 600, 1.2,
-// 44 and 42).  Keys of 192 and values of 128, 4-bit, tiles of 7.5 KiB, run the same with either.
+// sequences of 4000 of 8 x 64 fp8: 57 us, 68 with four; of 2000 of 8 x 128 4-bit, tiles of 5 KiB: 38 and 45) or
+// shares have two sequences or more each, whose starts overlap then while few are cut (1024 of 128 of 8 x 128
+// fp8: 62 us and 72; 512 of 100 int8: 36 and 41; 200 of 333 fp8, 1.6 a share, the same; 150 of 600, 1.2 a share,
+// 43 and 40).  Keys of 192 and values of 128, 4-bit, tiles of 7.5 KiB: 50.5 and 49.5.
 constexpr int kSmallTile = 6 * 1024;
 template <class E, int FMT, int I = 0>
 bool eight_waves(int shape, bool many) {
@@ -384,7 +384,7 @@ int launch_of(const char* name, AttArgs a, mcop_dtype dtype, hipStream_t st) {
   a.target = (int)target_of(kAttShares, a.heads, a.group);
   if (shape >= 0) {
     const int four = (int)target_of(kLineShares, a.heads, a.group);
-    if (lines ? !eight_waves<E, FMT>(shape, 2 * a.sequences >= 3 * four) : kTileShapes[shape].vd == 16) {
+    if (lines ? !eight_waves<E, FMT>(shape, a.sequences >= 2 * four) : kTileShapes[shape].vd == 16) {
       a.target = four;
     }
   }
@@ -423,8 +423,8 @@ int launch_of(const char* name, AttArgs a, mcop_dtype dtype, hipStream_t st) {
   if (int rc = check_launch(name)) return rc;
   if (!joins) return MCOP_OK;
   // each cut between two shares splits one sequence; a query head in one wave while an even split has fewer
-  // parts than two of its batches (a call over 64 sequences, two parts each: 71 us, 75 with four waves; over
-  // 48 windows, five: 37 and 39; 37 ragged sequences with eleven: 28, 29.5 with one wave)
+  // parts than two of its batches (a call over 64 sequences, two parts each: 66 us, 70 with four waves; over
+  // 48 windows, five: 35 and 37; 37 ragged sequences with eleven: 25, 27 with one wave)
   const dim3 lanes(kJoinWaves * 64);
   const unsigned splits = (unsigned)std::min(a.sequences, a.target - 1);
   if (a.target / a.sequences < 2 * kJoinBatch) {
@@ -490,7 +490,7 @@ extern "C" int mcop_kv_cache_attention(const mcop_kv_side* key, const mcop_kv_si
   }
   // the kernels count tiles in 32 bits; a sequence has as many as its row of the table holds
   const int64_t capacity = std::min<int64_t>(table_columns * page_size, INT32_MAX);
-  if ((capacity / kAttTile + 2) * num_sequences > INT32_MAX) {
+  if ((capacity / kAttTile + 2 + kAttStart) * num_sequences > INT32_MAX) {
     return set_error(MCOP_E_UNSUPPORTED, "%s: %lld sequences of up to %lld positions are 2^31 tiles of 32 "
                      "or more", name, (long long)num_sequences, (long long)capacity);
   }

@@ -15,10 +15,10 @@
 // elements end in a unit that overlaps the one before: its queries are zero where it repeats elements, and
 // outputs that come twice are the same.
 //
-// What bounds it: reading the cache, and behind that one wave a SIMD that loads, converts and multiplies in
-// turn.  2 x 131072 positions of 8 x 128 fp8 for 8 query heads each (554 MB) take 109 us with the join, 5.1
-// TB/s, the same reads alone 90-94; 64 ragged sequences of 131072 in all, int8 (279 MB), 71 us; 16 of 4-bit
-// keys of 192 and values of 128 (179 MB), 47 us.  Vector units are 32-38% busy, the matrix units 7-13%.
+// What bounds it: reading the cache, for 4-bit ones also the vector units (with every tile masked, a tenth more
+// instructions, 4-bit codes take 5% longer, int8 and fp8 the same).  2 x 131072 positions of 8 x 128 fp8 for 8 query heads each (554 MB) take 107-111 us with the join, 5.1
+// TB/s, the same reads alone 90-94; 64 ragged sequences of 131072 in all, int8 (279 MB), 66 us; 16 of 4-bit
+// keys of 192 and values of 128 (179 MB), 49 us.  Vector units are 32-38% busy, the matrix units 7-13%.
 //
 // Every code (int8, e4m3, e2m1 with its block's power of two) is a bf16 value.  fp32 scales stay out of
 // the products: a key's multiplies its logit, a value's its weight.  Queries enter as the sum of one bf16
@@ -34,7 +34,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Workgroups a CU that a kernel's registers are held to: two, where that spills none of them (16 x 131072
-// positions of 8 x 192 and 128 mxfp4: 48 us with two, 52 with one).
+// positions in all of 8 x 192 and 128 mxfp4: 49 us with two, 52 with one).
 constexpr int att_resident(bool fp32, int fmt, int kp, int vd, bool lines) {
   return vd == 16 || (lines && kp == 3 && fmt != KV_MXFP4 && fp32) ? 1 : 2;
 }
