@@ -202,7 +202,7 @@ k_kv_attention_rows(AttArgs a) {
 // become; then the parts' elements are added up, four a lane and of kJoinBatch parts on their way together
 // (vectors of up to 128 elements: each half of the wave every second part).  The code is kept short: it is
 // fetched from memory after a kernel whose reads have passed through the whole L2 (64 sequences' 128 cuts of 64
-// query heads: 5.4 us; a workgroup a head with more code 7.0).
+// query heads: 5.3 us; a workgroup a head with more code 7.0).
 constexpr int kJoinWaves = 4, kJoinBatch = 4;  // waves of a workgroup; parts that a wave has on their way
 
 template <class E, int WAVES>

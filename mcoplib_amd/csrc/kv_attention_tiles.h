@@ -18,7 +18,7 @@
 // What bounds it: reading the cache, for 4-bit ones also the vector units (with every tile masked, a tenth more
 // instructions, 4-bit codes take 5% longer, int8 and fp8 the same).  2 x 131072 positions of 8 x 128 fp8 for 8 query heads each (554 MB) take 107-111 us with the join, 5.1
 // TB/s, the same reads alone 90-94; 64 ragged sequences of 131072 in all, int8 (279 MB), 66 us; 16 of 4-bit
-// keys of 192 and values of 128 (179 MB), 49 us.  Vector units are 32-38% busy, the matrix units 7-13%.
+// keys of 192 and values of 128 (179 MB), 49 us.  Vector units are 32-37% busy, the matrix units 8-12%.
 //
 // Every code (int8, e4m3, e2m1 with its block's power of two) is a bf16 value.  fp32 scales stay out of
 // the products: a key's multiplies its logit, a value's its weight.  Queries enter as the sum of one bf16
