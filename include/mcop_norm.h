@@ -339,12 +339,14 @@ int mcop_kv_cache_read_dequant(const mcop_kv_side* key, const mcop_kv_side* valu
  * positions j of sequence b from max(0, n - window) (window 0: from 0) to n - 1, n = seq_lens[b], with page
  * i of the sequence in block_table[b * table_row_stride + i]:
  *   s_j = scale * <q, k_j>,  out = sum_j e^(s_j) v_j / sum_j e^(s_j),  lse = log sum_j e^(s_j)
- * in fp32 (queries and weights enter the matrix units without loss beyond 2^-26 of a weight;
- * fp32 queries that bf16 rounds to infinity, from 3.39e38 on, count as that), rounded once. lse is [num_sequences, query_heads] or NULL. A sequence of no positions gives 0 and -inf; one
- * with a position that has no page of the cache (past the columns, or a page outside the cache) NaN.
- * Slots behind a sequence's last position are not read. The order of the sums depends on the shapes and the
- * lengths only. workspace: mcop_kv_cache_attention_workspace() bytes at a multiple of 16, used by this call
- * alone until it ends on the stream. At most 2^24 sequences. No counterpart in the reference's path. */
+ * in fp32 (queries and weights enter the matrix units with all their bits; queries are multiplied with a
+ * key's codes, 4-bit ones in their block's scale, and added up, then with its fp32 scale), rounded once. A query
+ * with an infinity gives NaN, or, where all its logits are -infinity, may give what no positions give. lse is [num_sequences, query_heads] or NULL. A
+ * sequence of no positions gives 0 and -inf; one with a position that has no page of the cache (past the
+ * columns, or a page outside the cache) NaN. Slots behind a sequence's last position are not read. The order of
+ * the sums depends on the shapes and the lengths only. workspace: mcop_kv_cache_attention_workspace() bytes at a
+ * multiple of 16, used by this call alone until it ends on the stream. At most 2^24 sequences. No counterpart in
+ * the reference's path. */
 int mcop_kv_cache_attention(const mcop_kv_side* key, const mcop_kv_side* value, mcop_dtype cache_dtype,
                             int64_t num_pages, int64_t page_size, int64_t num_heads,
                             int64_t query_heads, const int32_t* block_table,

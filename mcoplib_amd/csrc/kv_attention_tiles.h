@@ -22,9 +22,10 @@
 //
 // Every code (int8, e4m3, e2m1 with its block's power of two) is a bf16 value.  fp32 scales stay out of
 // the products: a key's multiplies its logit, a value's its weight.  Queries enter as the sum of one bf16
-// (bf16), two (fp16) or three (fp32), which is exact; weights as three, to 2^-27 of themselves.  Weights of two terms,
-// 2^-18 off, changed the last bit of one 16-bit output in 400; the third is a product more for each of two, and takes
-// 1-2 us of a 4-bit cache's 50 and of the widest heads' 35, nothing else.
+// (bf16), two (fp16) or three (fp32), weights as three: both exact.  Weights of two terms, 2^-17 off, changed the last
+// bit of one 16-bit output in 400; the third is a product more for each of two, and takes 1-2 us of a 4-bit cache's
+// 50 and of the widest heads' 35, nothing else.  Terms are cut off, not rounded, which takes as long: rounded ones
+// would be infinite for the largest fp32 queries.
 #pragma once
 
 #include "kv_attention.h"
@@ -52,22 +53,20 @@ struct AttTerms {  // bf16 terms of a query, of a weight
   static constexpr int P = 3;
 };
 
-// Two fp32 values as bf16 in a dword, and what that leaves of them.
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
-}
-__device__ __forceinline__ uint32_t take_bf16(float& a, float& b) {
-  const uint32_t u = pack_bf16(a, b);
-  a -= __builtin_bit_cast(float, u << 16);
-  b -= __builtin_bit_cast(float, u & 0xffff0000u);
-  return u;
-}
 // The high halves of two dwords, the low halves.
 __device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) {
   return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
 }
 __device__ __forceinline__ uint32_t low_halves(uint32_t lo, uint32_t hi) {
   return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
+// The leading eight bits of two values' significands as bf16 in a dword, and what that leaves of them, exactly:
+// three such terms hold a binary32 value, two a binary16 one.  (Of an infinity it leaves NaN.)
+__device__ __forceinline__ uint32_t take_bf16(float& a, float& b) {
+  const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+  a -= __builtin_bit_cast(float, x & 0xffff0000u);
+  b -= __builtin_bit_cast(float, y & 0xffff0000u);
+  return high_halves(x, y);
 }
 __device__ __forceinline__ uint32_t i8_bits(uint32_t w, int byte) {  // as binary32
   return __builtin_bit_cast(uint32_t, (float)(int8_t)(w >> (8 * byte)));

@@ -1,5 +1,5 @@
 """kv_cache_attention where its numbers end, on the GPU against the formula in 64 bits: weights whose every bit
-shows."""
+shows, queries next to fp32's largest."""
 
 import math
 
@@ -9,7 +9,7 @@ import torch
 import kv_plain
 import mcoplib_amd._C  # noqa: F401
 import mx_plain
-from gpu_util import DEV, say
+from gpu_util import DEV, gen, say
 from mcoplib import custom_ops
 
 pytestmark = pytest.mark.gpu
@@ -40,9 +40,9 @@ def test_weights_keep_their_bits(n, dk, dv, page, dtype, kind):
 
     The other positions have values of zero and weights of e^-39, which neither sum sees.  The bound, in u =
     2^-24 of |2| + |-3| w = 4: w's exponent is one product of three fp32 factors (scale, log2 e, their product)
-    and a rounding, 2.25 u of 0.59, so 0.9 u of w, and its own 2 u; two products, in three terms each (to
-    2^-26, u / 4), added up in steps of 2 u of the largest, 2: 3 u of 4 at most; w's errors reach half of the 4.
-    3 u + (2.9 + 0.25) u / 2 < 5 u; a weight of 17 bits is 2^-19 = 32 u of 4 off.
+    and a rounding, 2.25 u of 0.59, so 0.9 u of w, and its own 2 u; two products, in three terms each, added
+    up in steps of 2 u of the largest, 2: 3 u of 4 at most; w's errors reach half of the 4.
+    3 u + 2.9 u / 2 < 5 u; a weight of 17 bits is 2^-19 = 32 u of 4 off.
     The sum of the weights is 5/3, and the result's own rounding is of almost nothing."""
     k, v = torch.zeros(n, 1, dk), torch.zeros(n, 1, dv)
     a, b = n // 2 - 1, n // 2
@@ -71,3 +71,54 @@ def test_weights_keep_their_bits(n, dk, dv, page, dtype, kind):
     off = float((out - want).abs().max()) * (1 + w) / (4 * U)
     print(f"  {off:.2f} u", flush=True)
     assert off <= 5.0 + 2.0 ** -8 * abs(want) / U
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dk,dv,page", [(64, 64, 16), (128, 128, 16), (256, 256, 16), (96, 64, 7),
+                                        (512, 32, 16)])
+def test_fp32_queries_up_to_the_largest(dk, dv, page, kind):
+    """Queries that bf16 rounds to infinity (from 3.39e38 on), of one element, beside keys of tiny scales: no sum
+    of products leaves fp32's range, and the logits are ordinary ones."""
+    n, g, most = 100, gen(dk), torch.finfo(torch.float32).max
+    pages = -(-n // page)
+    kc, ks = kv_plain.empty_cache(kind, pages, page, 2, dk, poison=False)
+    vc, vs = kv_plain.empty_cache(kind, pages, page, 2, dv)
+    p = torch.arange(n)
+    k = torch.zeros(n, 2, dk)
+    k[..., 5] = torch.randint(-1, 2, (n, 2), generator=g).float()
+    kc.view(torch.uint8)[p // page, p % page] = exact_codes(k, kind)[0].view(torch.uint8)
+    ks[p // page, p % page] = 4 if kind == "mxfp4" else 1e-37
+    kv_plain.put(vc, vs, kind, p // page, p % page, torch.randn(n, 2, dv, generator=g))
+    query = torch.zeros(1, 8, dk)
+    query[0, :, 5] = torch.tensor([most, -most, most * 0.9985, -1e38, most, 3.39e38, 1.0, 0.0])
+    table = torch.arange(pages, dtype=torch.int32)[None]
+    lens = torch.tensor([n], dtype=torch.int32)
+    scale = float(torch.tensor(0.0625))
+    say(f"attention {kind} {dk}/{dv} pages of {page}: queries of 3.4e38")
+    out, lse = custom_ops.kv_cache_attention(*(t.to(DEV) for t in (query, kc, vc, ks, vs, table, lens)), scale,
+                                             return_lse=True)
+    o, z, ob, zb = kv_plain.attention(query, kc, vc, ks, vs, kind, table, lens, scale)
+    kv_plain.near(lse, z, zb, "lse")
+    kv_plain.near(out, o, ob, "out")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dk", [64, 512])
+def test_infinite_queries_spoil_their_own_row(dk, dtype):
+    n, g = 100, gen(dk)
+    kc, ks = kv_plain.empty_cache("int8", 7, 16, 1, dk, poison=False)
+    vc, vs = kv_plain.empty_cache("int8", 7, 16, 1, 64)
+    p = torch.arange(n)
+    kc[p // 16, p % 16, 0, 5], ks[p // 16, p % 16] = 1, 0.5
+    kv_plain.put(vc, vs, "int8", p // 16, p % 16, torch.randn(n, 1, 64, generator=g))
+    query = torch.zeros(1, 4, dk, dtype=dtype)
+    query[0, :, 5] = torch.tensor([math.inf, 2.0, -math.inf, -1.0], dtype=dtype)
+    table, lens = torch.arange(7, dtype=torch.int32)[None], torch.tensor([n], dtype=torch.int32)
+    say(f"attention {dtype} {dk}: infinite queries")
+    out, lse = custom_ops.kv_cache_attention(*(t.to(DEV) for t in (query, kc, vc, ks, vs, table, lens)), 1.0,
+                                             return_lse=True)
+    assert torch.isnan(out[0, 0]).all() and not torch.isfinite(lse[0, 0])
+    assert torch.isnan(out[0, 2]).all() or ((out[0, 2] == 0).all() and lse[0, 2] == -math.inf)  # all are -inf
+    o, z, ob, zb = kv_plain.attention(query[:, 1::2], kc, vc, ks, vs, "int8", table, lens, 1.0)
+    kv_plain.near(lse[:, 1::2], z, zb, "lse")
+    kv_plain.near(out[:, 1::2], o, ob, "out")
