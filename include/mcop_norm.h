@@ -392,8 +392,9 @@ int64_t mcop_kv_cache_pages_workspace(int64_t num_requests, int64_t num_pages);
 /* Sequence children[i] becomes a copy of parents[i]: its full pages are shared (counted once more), and a
  * last page that is filled in part is replaced by a free one, the lowest free page for the first fork that
  * needs one and so on; src[i], dst[i] <- that page of the parent and of the child, for
- * mcop_kv_cache_copy_pages (-1 where there is none). A fork that no page is left for leaves its child empty;
- * one with an index outside the table does nothing. Children must be free rows, different from each other and
+ * mcop_kv_cache_copy_pages (-1 where there is none). Pages that the parent has not (outside the pool), the
+ * child has not either. A fork that no page is left for leaves its child empty; one with an index outside the
+ * table does nothing. Children must be free rows, different from each other and
  * from all parents. No counterpart in the reference's path. */
 int mcop_kv_cache_fork(const mcop_kv_pool* pool, const int32_t* parents, const int32_t* children,
                        int64_t num_forks, int32_t* src, int32_t* dst, void* workspace,

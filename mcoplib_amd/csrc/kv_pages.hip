@@ -179,6 +179,10 @@ __device__ __forceinline__ Request request_of(const Pool& p, const Requests& r, 
   if (!q.ok) return q;
   q.have = FORK ? q.old / p.page_size : pages_of(q.old, p.page_size);
   q.need = pages_of(q.now, p.page_size) - q.have;
+  if (FORK && q.need > 0) {  // a part-filled page that the parent has not: the child has none either
+    const int32_t page = p.table[q.from * p.stride + q.have];
+    if (page < 0 || page >= p.pages) q.need = 0;
+  }
   return q;
 }
 

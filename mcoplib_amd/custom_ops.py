@@ -125,9 +125,9 @@ def kv_cache_fork(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts:
     ref_counts [pages], 0 for a free page; all int32, all updated in place): children[i] becomes a copy of
     parents[i], which it shares the full pages of.  A last page that is filled in part is replaced by a
     free one, the lowest free page for the first fork that needs one and so on.  Returns (src, dst): that
-    page of the parent and of the child, for kv_cache_copy_pages, -1 where there is none.  A fork that no
-    page is left for leaves its child empty.  Children must be free rows, different from each other and
-    from all parents; a parent may have many."""
+    page of the parent and of the child, for kv_cache_copy_pages, -1 where there is none.  A page that the
+    parent has not, the child has not either.  A fork that no page is left for leaves its child empty.
+    Children must be free rows, different from each other and from all parents; a parent may have many."""
     return _torch_ops.kv_cache_fork_new(block_table, seq_lens, ref_counts, parents, children, page_size)
 
 
