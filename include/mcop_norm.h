@@ -404,8 +404,8 @@ int mcop_kv_cache_fork(const mcop_kv_pool* pool, const int32_t* parents, const i
  * order of i. slots[t], for cu_tokens[i] <= t < cu_tokens[i + 1], <- the slots of its new positions (for
  * mcop_kv_cache_write_quant), starts[i] <- the first of those positions. Where the free pages end, that
  * sequence and all behind it that need a page stay as they are, as do those that would not fit their row of
- * the table: starts[i] and their slots are -1, as are the slots from cu_tokens[num_sequences] to num_tokens.
- * cu_tokens is non-decreasing from 0. Sequences must differ from each other. No counterpart in the
+ * the table or whose length would pass 2^31 - 1: starts[i] and their slots are -1, as are the slots from
+ * cu_tokens[num_sequences] to num_tokens. cu_tokens is non-decreasing from 0. Sequences must differ from each other. No counterpart in the
  * reference's path. */
 int mcop_kv_cache_extend(const mcop_kv_pool* pool, const int32_t* sequences, const int32_t* cu_tokens,
                          int64_t num_sequences, int64_t* slots, int64_t num_tokens, int32_t* starts,

@@ -132,8 +132,8 @@ __device__ __forceinline__ int64_t pages_of(int64_t tokens, int page_size) {
   return (tokens + page_size - 1) / page_size;
 }
 __device__ __forceinline__ bool row_ok(const Pool& p, int row) { return row >= 0 && row < p.rows; }
-__device__ __forceinline__ bool len_ok(const Pool& p, int64_t n) {
-  return n >= 0 && n <= (int64_t)p.columns * p.page_size;
+__device__ __forceinline__ bool len_ok(const Pool& p, int64_t n) {  // of a row of the table, and of lens
+  return n >= 0 && n <= INT32_MAX && n <= (int64_t)p.columns * p.page_size;
 }
 
 // Exclusive sum over a workgroup of 1024 threads, of values up to 2^31 - 1, where it stops; *all: the whole.

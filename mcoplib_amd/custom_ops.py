@@ -139,8 +139,8 @@ def kv_cache_extend(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_count
     cu_tokens[-1].  Returns (slots, starts): slots [num_tokens] (int64) is the new tokens' slot_mapping for
     kv_cache_write_quant, starts [sequences] (int32) the first new position of each.  Where the free pages
     end, that sequence and those behind it that need a page stay as they are, as does one that would not
-    fit its row: their starts and slots are -1, which kv_cache_write_quant does not write.  The pool's
-    tensors are as in kv_cache_fork; sequences must differ from each other, and a sequence's part-filled
+    fit its row or 32 bits: their starts and slots are -1, which kv_cache_write_quant does not write.  The
+    pool's tensors are as in kv_cache_fork; sequences must differ from each other, and a sequence's part-filled
     last page must be its own (a fork's is)."""
     return _torch_ops.kv_cache_extend_new(block_table, seq_lens, ref_counts, sequences, cu_tokens,
                                           num_tokens, page_size)

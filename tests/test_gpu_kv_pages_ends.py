@@ -1,5 +1,5 @@
 """The page operators of the cache on the GPU where the pool's numbers end: forks of sequences whose last page is
-missing."""
+missing, lengths next to 2^31."""
 
 import pytest
 import torch
@@ -67,3 +67,26 @@ def test_a_child_of_a_missing_last_page_reads_as_its_parent(bad):
     slots, starts = custom_ops.kv_cache_extend(*pool, _i32([1]), _i32([0, 5]), 5, 8)
     assert starts.tolist() == [21] and slots.tolist() == [-1, -1, -1, 0, 1]
     assert pool[0].tolist() == [[3, 7, bad, -1], [3, 7, -1, 0]]
+
+
+@pytest.mark.parametrize("columns", [3, 4])
+@pytest.mark.parametrize("behind", [0, 5000])  # in one launch, in two
+def test_lengths_end_at_32_bits(behind, columns):
+    """A sequence whose new length is no int32 stays as it was, though its row and the pool have room."""
+    say(f"lengths up to 2^31, rows of {columns}, {behind} tokens behind")
+    most, page = (1 << 31) - 1, 1 << 30
+    pool = _pool([[1, 4], [], []], [most - 1, 0, 0], 6, columns)
+    before = [t.tolist() for t in pool]
+    for add in (2, 4, most):
+        slots, starts = custom_ops.kv_cache_extend(*pool, _i32([0]), _i32([0, add]), 4 + behind, page)
+        assert starts.tolist() == [-1] and (slots == -1).all()
+        assert [t.tolist() for t in pool] == before
+    slots, starts = custom_ops.kv_cache_extend(*pool, _i32([0, 1]), _i32([0, 4, 6]), 6 + behind, page)
+    assert starts.tolist() == [-1, 0] and slots.tolist() == [-1] * 4 + [0, 1] + [-1] * behind
+    slots, starts = custom_ops.kv_cache_extend(*pool, _i32([0]), _i32([0, 1]), 1 + behind, page)
+    assert starts.tolist() == [most - 1] and slots.tolist() == [4 * page + page - 2] + [-1] * behind
+    none = [-1] * columns
+    assert pool[0].tolist() == [[1, 4, *none[2:]], [0, *none[1:]], none]
+    assert pool[1].tolist() == [most, 2, 0] and pool[2].tolist() == [1, 1, 0, 0, 1, 0]
+    custom_ops.kv_cache_free(*pool, _i32([0, 1]), page)
+    assert pool[0].tolist() == [none] * 3 and pool[1].tolist() == [0, 0, 0] and pool[2].tolist() == [0] * 6
