@@ -110,12 +110,14 @@ k_kv_attention_rows(AttArgs a) {
       }
       m[r] = -__builtin_inff(), l[r] = 0.0f;
     }
-    const int from = max(c.first, c.tile * kAttTile), to = min(c.end, (c.tile + c.tiles) * kAttTile);
+    // the end of the last tile of 2^31 - 1 positions, and the position after a wave's last, are no ints
+    const uint32_t from = (uint32_t)max(c.first, c.tile * kAttTile);
+    const uint32_t to = min((uint32_t)c.end, (uint32_t)(c.tile + c.tiles) * kAttTile);
     bool missing = false;
     int unit = FMT == KV_MXFP4 ? 0 : kAttNoUnit;
-    for (int p = from + wave; p < to; p += kAttWaves) {
+    for (uint32_t p = from + wave; p < to; p += kAttWaves) {
       uint32_t off;
-      const int page = att_page(a, c.sequence, (uint32_t)p, &off);
+      const int page = att_page(a, c.sequence, p, &off);
       if (page < 0) {
         missing = true;
         continue;

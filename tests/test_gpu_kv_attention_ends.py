@@ -1,5 +1,5 @@
 """kv_cache_attention where its numbers end, on the GPU against the formula in 64 bits: weights whose every bit
-shows, queries next to fp32's largest."""
+shows, queries next to fp32's largest, lengths next to 2^31."""
 
 import math
 
@@ -122,3 +122,26 @@ def test_infinite_queries_spoil_their_own_row(dk, dtype):
     o, z, ob, zb = kv_plain.attention(query[:, 1::2], kc, vc, ks, vs, "int8", table, lens, 1.0)
     kv_plain.near(lse[:, 1::2], z, zb, "lse")
     kv_plain.near(out[:, 1::2], o, ob, "out")
+
+
+@pytest.mark.parametrize("window", [3, 40, 100])
+@pytest.mark.parametrize("kind,dk,dv", [("int8", 8, 8), ("fp8", 320, 16), ("mxfp4", 32, 288), ("int8", 64, 64),
+                                        ("fp8", 61, 64), ("mxfp4", 128, 128), ("int8", 256, 200)])
+def test_lengths_up_to_the_largest_int32(kind, dk, dv, window):
+    """Windows at the end of sequences whose rows of the table name one page again and again: positions and
+    the ends of tiles next to 2^31."""
+    page, g = 1 << 16, gen(dk + window)
+    lens = torch.tensor([(1 << 31) - 1 - x for x in (0, 1, 30, 31, 32, 33, 64)] + [50], dtype=torch.int32)
+    kc, ks = kv_plain.empty_cache(kind, 1, page, 2, dk)
+    vc, vs = kv_plain.empty_cache(kind, 1, page, 2, dv)
+    off = torch.cat([torch.arange(50), torch.arange(page - 200, page)])
+    for codes, scales, d in ((kc, ks, dk), (vc, vs, dv)):
+        kv_plain.put(codes, scales, kind, torch.zeros_like(off), off, torch.randn(250, 2, d, generator=g))
+    query = torch.randn(len(lens), 6, dk, generator=g)
+    table = torch.zeros(len(lens), 1 << 15, dtype=torch.int32)
+    say(f"attention {kind} {dk}/{dv}, windows of {window} at 2^31")
+    out, lse = custom_ops.kv_cache_attention(*(t.to(DEV) for t in (query, kc, vc, ks, vs, table, lens)), 0.1, window,
+                                             return_lse=True)
+    o, z, ob, zb = kv_plain.attention(query, kc, vc, ks, vs, kind, table, lens, float(torch.tensor(0.1)), window)
+    kv_plain.near(lse, z, zb, "lse")
+    kv_plain.near(out, o, ob, "out")
