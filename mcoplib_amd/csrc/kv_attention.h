@@ -8,7 +8,8 @@
 // log2 e).  Parts of P that were walked apart are joined by  m = max m_i,  l = sum l_i 2^(m_i - m),
 // o = sum o_i 2^(m_i - m).  The o_i of int8 and fp8 caches are held in units of 2^e, the exponent of the
 // largest value scale seen, so that neither a weight times a scale nor their sum leaves fp32's range where
-// the values themselves do not.  An empty P gives o = 0 and lse = -inf; a position of P without a page of the
+// the values themselves do not; those of 4-bit caches in units of 2^48 from the first block scale of 2^65 or more
+// on (kMxUnit).  An empty P gives o = 0 and lse = -inf; a position of P without a page of the
 // cache makes the sequence's rows NaN.
 //
 // Work is split by tiles of 32 positions.  The lengths are on the device, so every wave finds its own
@@ -176,6 +177,11 @@ __device__ __forceinline__ int att_unit(float scale) {
   const int e = (int)((__builtin_bit_cast(uint32_t, scale) >> 23) & 255) - 127;
   return e < kAttNoUnit ? kAttNoUnit : (e > 126 ? 126 : e);
 }
+// 4-bit values: up to 6 times a block scale of 2^127, weights of at most 2^8, fewer than 2^31 of them.  Sums of scales
+// below 2^65 stay below 2^107; in units of 2^48 those of any scale below 2^121, and a weight that counts beside
+// others, of 2^-48 and more, keeps all terms of its products.
+constexpr int kMxUnit = 48;
+constexpr uint32_t kMxFarByte = 127 + 65;  // the two leading bits of a scale byte
 // 2^e for e of 0 down to -252.
 __device__ __forceinline__ float att_power(int e) { return __builtin_ldexpf(1.0f, e); }
 

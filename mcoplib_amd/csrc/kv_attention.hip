@@ -128,6 +128,7 @@ k_kv_attention_rows(AttArgs a) {
       const int64_t ks = page * a.key.s_page + off * a.key.s_token + head * a.key.s_head;
       const int64_t vs = page * a.value.s_page + off * a.value.s_token + head * a.value.s_head;
       float kf[N], vf[N];
+      bool far = false;  // of the lane's 4-bit values
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         const int d = lane + n * 64;
@@ -141,26 +142,29 @@ k_kv_attention_rows(AttArgs a) {
         if (d < a.value.dim) {
           vf[n] = code_value<FMT>(v, d);
           if constexpr (FMT == KV_MXFP4) {
-            vf[n] *= mx_value(static_cast<const uint8_t*>(a.value.scales)[vs + (d >> 5)]);
+            const uint32_t byte = static_cast<const uint8_t*>(a.value.scales)[vs + (d >> 5)];
+            vf[n] *= mx_value(byte);
+            far = far || byte >= kMxFarByte;
           }
         }
       }
       float k_scale = a.scale, v_scale = 1.0f;
+      int e = FMT == KV_MXFP4 && __builtin_amdgcn_ballot_w64(far) != 0 ? kMxUnit : unit;
       if constexpr (FMT != KV_MXFP4) {
         k_scale *= static_cast<const float*>(a.key.scales)[ks];
         v_scale = static_cast<const float*>(a.value.scales)[vs];
-        const int e = att_unit(v_scale);
-        if (e > unit) {
-          const float down = att_power(unit - e);
-#pragma unroll
-          for (int r = 0; r < kAttRows; ++r) {
-#pragma unroll
-            for (int n = 0; n < N; ++n) o[r][n] *= down;
-          }
-          unit = e;
-        }
-        v_scale = __builtin_ldexpf(v_scale, -unit);
+        e = att_unit(v_scale);
       }
+      if (e > unit) {
+        const float down = att_power(unit - e);
+#pragma unroll
+        for (int r = 0; r < kAttRows; ++r) {
+#pragma unroll
+          for (int n = 0; n < N; ++n) o[r][n] *= down;
+        }
+        unit = e;
+      }
+      v_scale = __builtin_ldexpf(v_scale, -unit);
 #pragma unroll
       for (int r = 0; r < kAttRows; ++r) {
         float s = 0.0f;

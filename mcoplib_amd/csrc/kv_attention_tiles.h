@@ -199,6 +199,7 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 //   value(e, w)        VD codes of position(e), and value_scale(e) of 4-bit ones
 //   ks(e), vs(e)       fp32 scales of position(e)
 //   most_vs()          the lane's part of the tile's value scales
+//   far(live)          whether a 4-bit one of its part is kMxFarByte or more (live: which of value_scale(e) count)
 template <class E, int FMT, int KP, int VD>
 struct AttWave {
   static constexpr int TQ = AttTerms<E>::Q, TP = AttTerms<E>::P;
@@ -362,9 +363,13 @@ struct AttWave {
         if (e_max >= -kAttUnitSlack && e_max <= kAttUnitSlack) e_max = 0;
       }
     }
-    // the reference of the weights moves when a logit is 2^kAttSlack past it, not with every new maximum:
-    // of sixteen query heads one has a new one in nearly every tile
-    if (wider || __builtin_amdgcn_ballot_w64(top > m + kAttSlack) != 0) {
+    // The reference of the weights moves when a logit is more than kAttSlack past it, a weight of 2^kAttSlack, not
+    // with every new maximum: of sixteen query heads one has a new one in nearly every tile.  4-bit values of
+    // any size are looked for in the same branch (1-2% of a 4-bit cache's time, 2-3% with a branch of their own).
+    bool far = false;
+    if constexpr (MX) far = src.template far<EDGE>(live);
+    if (wider || __builtin_amdgcn_ballot_w64(top > m + kAttSlack || far) != 0) {
+      if (MX && __builtin_amdgcn_ballot_w64(far) != 0) e_max = kMxUnit;
       const float keep = att_weight(m, top);
       const float keep_o = keep * att_power(unit - e_max);
       l *= keep;
@@ -383,12 +388,16 @@ struct AttWave {
       w[e] = MX ? p : p * src.vs(e);
       if (!MX && EDGE) w[e] = live[e] ? w[e] : 0.0f;  // no 0 times a scale that is no number
     }
-    if (!MX && unit != 0) {
+    if (unit != 0) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        w[e] = EDGE && !live[e] ? 0.0f
-                                : __builtin_amdgcn_exp2f(__builtin_fmaf(f[e], by, -at)) *
-                                      __builtin_ldexpf(src.vs(e), -unit);
+        if constexpr (MX) {
+          w[e] *= att_power(-kMxUnit);
+        } else {
+          w[e] = EDGE && !live[e] ? 0.0f
+                                  : __builtin_amdgcn_exp2f(__builtin_fmaf(f[e], by, -at)) *
+                                        __builtin_ldexpf(src.vs(e), -unit);
+        }
       }
     }
     if constexpr (VD == 16) __builtin_amdgcn_sched_barrier(0);
@@ -475,7 +484,7 @@ struct AttWave {
 #pragma unroll
         for (int n = 0; n < VD; ++n) {
           const float x = o[n][i] * share;
-          v[n] = E::from_f(MX || unit == 0 ? x : __builtin_ldexpf(x, unit));
+          v[n] = E::from_f(unit == 0 ? x : __builtin_ldexpf(x, unit));
         }
         __builtin_memcpy(static_cast<typename E::S*>(a.value.plain) + ch.sequence * a.value.p_token +
                              query * a.value.p_head + d, v, sizeof(v));
@@ -702,6 +711,15 @@ struct LdsSource {
     }
   }
   __device__ __forceinline__ float value_scale(int e) const { return vscale[e]; }
+  template <bool EDGE>
+  __device__ __forceinline__ bool far(const bool* live) const {  // slots that are not live hold anything
+    uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      most = max(most, EDGE && !live[e] ? 0u : __builtin_bit_cast(uint32_t, vscale[e]));
+    }
+    return most >= kMxFarByte << 23;
+  }
   __device__ __forceinline__ float ks(int e) const { return kscale[e >> 2][e & 3]; }
   __device__ __forceinline__ float vs(int e) const { return vscale[e]; }
   __device__ __forceinline__ float most_vs() const { return most; }
@@ -855,6 +873,11 @@ struct RegisterSource {
     b[0] = from_lane(vb[0], wave.position(e));
     b[1] = VD > 8 ? from_lane(vb[1], wave.position(e)) : 0;
     return scale_operand(b, v_sel);
+  }
+  template <bool EDGE>
+  __device__ __forceinline__ bool far(const bool*) const {  // of position lane % 32, a live one
+    const uint32_t top = vb[0] & vb[0] << 1, next = VD > 8 ? vb[1] & vb[1] << 1 : 0;
+    return ((top | next) & 0x80808080u) != 0;
   }
   __device__ __forceinline__ float ks(int e) const { return from_lane_f(k_scale, wave.position(e)); }
   __device__ __forceinline__ float vs(int e) const { return from_lane_f(v_scale, wave.position(e)); }

@@ -1,5 +1,5 @@
 """kv_cache_attention where its numbers end, on the GPU against the formula in 64 bits: weights whose every bit
-shows, queries next to fp32's largest, lengths next to 2^31."""
+shows, queries and 4-bit values next to fp32's largest, lengths next to 2^31."""
 
 import math
 
@@ -143,5 +143,40 @@ def test_lengths_up_to_the_largest_int32(kind, dk, dv, window):
     out, lse = custom_ops.kv_cache_attention(*(t.to(DEV) for t in (query, kc, vc, ks, vs, table, lens)), 0.1, window,
                                              return_lse=True)
     o, z, ob, zb = kv_plain.attention(query, kc, vc, ks, vs, kind, table, lens, float(torch.tensor(0.1)), window)
+    kv_plain.near(lse, z, zb, "lse")
+    kv_plain.near(out, o, ob, "out")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (256, 256), (32, 1024)])
+@pytest.mark.parametrize("page", [16, 7])
+@pytest.mark.parametrize("late", [False, True])
+def test_4bit_values_at_the_end_of_the_range(late, page, dk, dv, dtype):
+    """Values next to fp32's largest, in all positions or in the last third only, under logits that rise by
+    less than a factor of 2^8 of weight: neither a weight times a value nor their sum leaves fp32's range
+    where the result does not."""
+    lens, g = [300, 3], gen(dk + page)
+    pages = sum(-(-n // page) for n in lens)
+    kc, ks = kv_plain.empty_cache("mxfp4", pages, page, 2, dk)
+    vc, vs = kv_plain.empty_cache("mxfp4", pages, page, 2, dv)
+    table = torch.full((2, -(-300 // page)), -1, dtype=torch.int32)
+    table[0], table[1, :-(-3 // page)] = torch.arange(table.shape[1]), pages - 1
+    for b, n in enumerate(lens):
+        p = torch.arange(n)
+        at, off = table[b].long()[p // page], p % page
+        k = torch.zeros(n, 2, dk)
+        k[..., 0] = (5.0 * p / n)[:, None]
+        kv_plain.put(kc, ks, "mxfp4", at, off, k)
+        v = 1 + torch.rand(n, 2, dv, generator=g)
+        kv_plain.put(vc, vs, "mxfp4", at, off, v)
+        vs[at, off] = torch.where((p >= 2 * n // 3)[:, None, None] | torch.tensor(not late),
+                                  torch.tensor(250, dtype=torch.uint8), vs[at, off])
+    query = torch.zeros(2, 4, dk, dtype=dtype)
+    query[..., 0] = 1.0
+    say(f"attention mxfp4 {dtype} {dk}/{dv} pages of {page}: values of 2^125")
+    out, lse = custom_ops.kv_cache_attention(
+        query.to(DEV), kc.to(DEV), vc.to(DEV), ks.to(DEV), vs.to(DEV), table.to(DEV),
+        torch.tensor(lens, dtype=torch.int32, device=DEV), 1.0, return_lse=True)
+    o, z, ob, zb = kv_plain.attention(query, kc, vc, ks, vs, "mxfp4", table, torch.tensor(lens), 1.0)
     kv_plain.near(lse, z, zb, "lse")
     kv_plain.near(out, o, ob, "out")
