@@ -343,10 +343,10 @@ int mcop_kv_cache_read_dequant(const mcop_kv_side* key, const mcop_kv_side* valu
  * key's codes, 4-bit ones in their block's scale, and added up, then with its fp32 scale), rounded once. A query
  * with an infinity gives NaN, or, where all its logits are -infinity, may give what no positions give. lse is [num_sequences, query_heads] or NULL. A
  * sequence of no positions gives 0 and -inf; one with a position that has no page of the cache (past the
- * columns, or a page outside the cache) NaN. Slots behind a sequence's last position are not read. The order of
- * the sums depends on the shapes and the lengths only. workspace: mcop_kv_cache_attention_workspace() bytes at a
- * multiple of 16, used by this call alone until it ends on the stream. At most 2^24 sequences. No counterpart in
- * the reference's path. */
+ * columns, or a page outside the cache) NaN. What slots that are not attended to hold has no effect. The order of
+ * the sums depends on the shapes and the lengths only. seq_lens and block_table are read throughout the call and
+ * must not change before it ends on the stream. workspace: mcop_kv_cache_attention_workspace() bytes at a multiple
+ * of 16, used by this call alone until then. At most 2^24 sequences. No counterpart in the reference's path. */
 int mcop_kv_cache_attention(const mcop_kv_side* key, const mcop_kv_side* value, mcop_dtype cache_dtype,
                             int64_t num_pages, int64_t page_size, int64_t num_heads,
                             int64_t query_heads, const int32_t* block_table,

@@ -16,8 +16,8 @@
 // share: the tiles of all sequences one after the other, cut into `target` equal shares, whatever the
 // sequences' lengths (one tile at least for each, also an empty one).  A sequence's start, where a wave waits for
 // its queries, its pages and its first tile in turn, counts as kAttStart tiles more: 64 ragged sequences of 131072
-// in all took 70 us without, 66 so, sorted by length 78 and 66, 300 of 30 beside 64 of 1500 86 and 67; 16 equal
-// ones of 8192, whose shares were whole eighths, 47 and 49.  A share may end one sequence, hold
+// in all took 71 us without, 66 so, sorted by length 81 and 66, 300 of 30 beside 64 of 1500 87 and 68; 16 equal
+// ones of 8192 of a 4-bit cache, whose shares were whole eighths, 51 and 53.  A share may end one sequence, hold
 // some whole and begin another: whole ones are written at once, the others as parts, of which a share has
 // two at most.  A second kernel joins each sequence's parts in order: results do not depend on timing.
 #pragma once

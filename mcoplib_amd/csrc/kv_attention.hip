@@ -82,8 +82,8 @@ __device__ __forceinline__ int att_page(const AttArgs& a, int sequence, uint32_t
 
 // Vector arithmetic: a wave walks every fourth position, its lanes the elements, and every query head's
 // product is a sum over the wave.  For head sizes that the matrix kernels are not built for; where they are, they
-// are two to twenty times as fast (37 ragged sequences of 5 x 80 and 96 int8 to fp32: 25 us, 198 so; 64 of
-// 8 x 128 int8: 66 and 1461; one of 1000 positions: 11 and 23).  A position's sums over the wave bound it.
+// are two to twenty times as fast (37 ragged sequences of 5 x 80 and 96 int8 to fp32: 25 us, 199 so; 64 of
+// 8 x 128 int8: 66 and 1468; one of 1000 positions: 11 and 23).  A position's sums over the wave bound it.
 template <class E, int FMT, int N>
 __global__ void __launch_bounds__(kAttWaves * 64)
 k_kv_attention_rows(AttArgs a) {
@@ -322,8 +322,8 @@ k_kv_attention_join(AttArgs a) {
 namespace {
 
 // Shares: waves for the card over all of a share's key heads and blocks of sixteen query heads.  Codes
-// through LDS: four waves a CU, which have two tiles each in flight (2 x 131072 positions of 8 x 128 fp8: 107
-// us, 115 with eight waves and twice the parts; 48 windows of 1024 of 4 x 256: 35 and 49); else eight (37
+// through LDS: four waves a CU, which have two tiles each in flight (2 x 131072 positions of 8 x 128 fp8: 109
+// us, 115 with eight waves and twice the parts; 48 windows of 1024 of 4 x 256: 35 and 50); else eight (37
 // ragged sequences of 5 x 80 and 96 int8 to fp32: 29 us with four, 25 so), while two workgroups are resident (83
 // of 12338 in all, 7 x 129 fp8 to fp32, one workgroup a CU: 36 us with four waves a CU, 48 with eight).
 constexpr int kLineShares = 1024, kAttShares = 2048;
@@ -371,10 +371,10 @@ bool whole_lines(const AttArgs& a, int fmt) {
 }
 
 // Codes through LDS with eight waves a CU: where two workgroups are resident, and either tiles are small (64
-// sequences of 4000 of 8 x 64 fp8: 57 us, 68 with four; of 2000 of 8 x 128 4-bit, tiles of 5 KiB: 38 and 45) or
+// sequences of 4000 of 8 x 64 fp8: 58 us, 71 with four; of 2000 of 8 x 128 4-bit, tiles of 5 KiB: 42 and 49) or
 // shares have two sequences or more each, whose starts overlap then while few are cut (1024 of 128 of 8 x 128
-// fp8: 62 us and 72; 512 of 100 int8: 36 and 41; 200 of 333 fp8, 1.6 a share, the same; 150 of 600, 1.2 a share,
-// 43 and 40).  Keys of 192 and values of 128, 4-bit, tiles of 7.5 KiB: 50.5 and 49.5.
+// fp8: 64 us and 74; 512 of 100 int8: 37 and 43; 200 of 333 fp8, 1.6 a share, the same; 150 of 600, 1.2 a share,
+// 44 and 42).  Keys of 192 and values of 128, 4-bit, tiles of 7.5 KiB: 52 and 53.
 constexpr int kSmallTile = 6 * 1024;
 template <class E, int FMT, int I = 0>
 bool eight_waves(int shape, bool many) {

@@ -16,16 +16,17 @@
 // outputs that come twice are the same.
 //
 // What bounds it: reading the cache, for 4-bit ones also the vector units (with every tile masked, a tenth more
-// instructions, 4-bit codes take 5% longer, int8 and fp8 the same).  2 x 131072 positions of 8 x 128 fp8 for 8 query heads each (554 MB) take 107-111 us with the join, 5.1
-// TB/s, the same reads alone 90-94; 64 ragged sequences of 131072 in all, int8 (279 MB), 66 us; 16 of 4-bit
-// keys of 192 and values of 128 (179 MB), 49 us.  Vector units are 32-37% busy, the matrix units 8-12%.
+// instructions, 4-bit codes take 4% longer, int8 3%, fp8 the same).  2 x 131072 positions of 8 x 128 fp8 for 8
+// query heads each (554 MB) take 107-114 us by card with the join, 5 TB/s, the same reads alone 90-94; 64 ragged
+// sequences of 131072 in all, int8 (279 MB), 66 us; 16 of 4-bit keys of 192 and values of 128 (179 MB), 52 us.
+// Vector units are 35-39% busy, the matrix units 11-16%.
 //
-// Every code (int8, e4m3, e2m1 with its block's power of two) is a bf16 value.  fp32 scales stay out of
-// the products: a key's multiplies its logit, a value's its weight.  Queries enter as the sum of one bf16
-// (bf16), two (fp16) or three (fp32), weights as three: both exact.  Weights of two terms, 2^-17 off, changed the last
-// bit of one 16-bit output in 400; the third is a product more for each of two, and takes 1-2 us of a 4-bit cache's
-// 50 and of the widest heads' 35, nothing else.  Terms are cut off, not rounded, which takes as long: rounded ones
-// would be infinite for the largest fp32 queries.
+// Every code (int8, e4m3, e2m1 with its block's power of two) is a bf16 value.  fp32 scales stay out of the
+// products: a key's multiplies its logit, a value's its weight.  Queries enter as the sum of one bf16 (bf16),
+// two (fp16) or three (fp32), weights as three: both exact.  Weights of two rounded terms, 2^-18 off, changed
+// the last bit of one 16-bit output in 400; the third is a product more for each of two, and takes 1-2 us of a
+// 4-bit cache's 52 and one of the widest heads' 35, nothing else.  Terms are cut off, not rounded, which takes
+// as long: rounded ones would be infinite for the largest fp32 queries.
 #pragma once
 
 #include "kv_attention.h"
@@ -36,7 +37,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Workgroups a CU that a kernel's registers are held to: two, where that spills none of them (16 x 131072
-// positions in all of 8 x 192 and 128 mxfp4: 49 us with two, 52 with one).
+// positions in all of 8 x 192 and 128 mxfp4: 53 us with two, 57 with one).
 constexpr int att_resident(bool fp32, int fmt, int kp, int vd, bool lines) {
   return vd == 16 || (lines && kp == 3 && fmt != KV_MXFP4 && fp32) ? 1 : 2;
 }
